@@ -330,6 +330,158 @@ int spmm_csr_cpu(int32_t M, const int32_t* rowptr, const int32_t* col,
                  const float* val, const float* B, int32_t O, float* C,
                  int32_t nthreads);
 
+/* -------------------------------------------------- dense operators */
+/* What stands next to the sparse product in a layer: the RMS norm of its
+ * output and the layer's input, a dense (linear) layer, their gradients, and
+ * the optimizer's step.  No counterpart in the reference, which has the sparse
+ * product alone.
+ *
+ * Matrices are row-major on the device with any row stride `ld*` in elements
+ * (>= the row length; 0 = rows back to back) and any alignment of their
+ * element type; 16-byte aligned rows are the fastest.  A call enqueues kernels
+ * on `stream` and nothing else (no allocation, copy or synchronisation), so it
+ * can be captured into a HIP graph; with a non-NULL `ms` it waits and stores
+ * the kernels' time, as the SpMM calls do.  Calls that overlap in time need
+ * workspaces of their own.  Bad arguments are VCSR_EINVAL, sizes or strides
+ * past what a kernel addresses VCSR_ERANGE, before any launch.  Results do not
+ * vary from call to call: no atomics. */
+enum {
+    VCSR_F32 = 0,
+    VCSR_BF16 = 1,
+    VCSR_FP8 = 2 /* OCP e4m3 (largest value 448, no infinities) */
+};
+enum {
+    VCSR_ACT_NONE = 0,
+    VCSR_ACT_RELU = 1,
+    VCSR_ACT_GELU = 2, /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+    VCSR_ACT_SILU = 3  /* z / (1 + exp(-z))                               */
+};
+
+/* t = x + residual;  y = t / sqrt(mean(t^2) + eps) * weight, row by row, in
+ * FP32.  For y of VCSR_FP8, y_scale[m] = max(max_c |y|, 1e-30) / 448 and the
+ * codes are y / y_scale[m] rounded to e4m3.  A row with a NaN or an infinity
+ * gives NaN for all of y or for what it multiplies, and no other row does. */
+typedef struct {
+    int64_t M;           /* rows; 0 is no work                               */
+    int32_t C;           /* columns, >= 1                                    */
+    int32_t x_type;      /* x, residual, sum: VCSR_F32 or VCSR_BF16          */
+    int32_t y_type;      /* VCSR_F32, VCSR_BF16 or VCSR_FP8                  */
+    float eps;           /* >= 0                                             */
+    const void* x;       int64_t ldx;
+    const void* residual; int64_t ldr;  /* NULL: t = x                       */
+    const float* weight; /* C                                                */
+    void* sum;           int64_t ldsum; /* NULL, or t rounded to x_type; may
+                                           be x or residual itself           */
+    void* y;             int64_t ldy;
+    float* y_scale;      /* M, for VCSR_FP8 (NULL otherwise)                 */
+    float* rstd;         /* NULL, or M: 1 / sqrt(mean(t^2) + eps)            */
+} vcsr_rmsnorm_args;
+int vcsr_rmsnorm(const vcsr_rmsnorm_args* args, void* stream, float* ms);
+
+/* Gradients of vcsr_rmsnorm: with s the saved sum (or x), h = s * rstd and
+ * g = dy * weight:  dx = dsum + rstd * (g - h * mean(g * h)),
+ * dweight = sum over rows of dy * h.  dx is the gradient of x and of the
+ * residual alike. */
+typedef struct {
+    int64_t M;
+    int32_t C;
+    int32_t x_type;      /* s, dsum, dx: VCSR_F32 or VCSR_BF16               */
+    int32_t y_type;      /* dy: VCSR_F32 or VCSR_BF16                        */
+    const void* dy;      int64_t lddy;
+    const void* s;       int64_t lds;
+    const float* weight; /* C                                                */
+    const float* rstd;   /* M                                                */
+    const void* dsum;    int64_t lddsum; /* NULL, or what flows into `sum`   */
+    void* dx;            int64_t lddx;   /* may be dsum itself               */
+    float* dweight;      /* C (zeros for M = 0), or NULL                     */
+    void* workspace;     size_t workspace_bytes;
+} vcsr_rmsnorm_grad_args;
+/* Bytes of workspace for the sizes and types of `args` (its pointers are not
+ * read, except which of them are NULL). */
+int vcsr_rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args* args, size_t* bytes);
+int vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args* args, void* stream, float* ms);
+
+/* z = x W^T + bias;  y = act(z) + residual.  W has one row per output column.
+ * Products are summed in FP32 (FP32 operands on the FP32 matrix cores); VCSR_FP8
+ * operands carry a scale per row: z[m][n] = x_scale[m] * w_scale[n] * (x W^T)
+ * + bias[n].  y and z are rounded once. */
+typedef struct {
+    int64_t M;           /* rows of x and y; 0 is no work                    */
+    int32_t N, K;        /* outputs and inputs of a row, >= 1                */
+    int32_t x_type;      /* x and w: VCSR_F32, VCSR_BF16 or VCSR_FP8         */
+    int32_t y_type;      /* y, z, residual: VCSR_F32 or VCSR_BF16            */
+    int32_t act;         /* VCSR_ACT_*                                       */
+    const void* x;       int64_t ldx;
+    const void* w;       int64_t ldw;   /* N x K                             */
+    const float* x_scale; /* M, for VCSR_FP8 (NULL otherwise)                */
+    const float* w_scale; /* N, for VCSR_FP8 (NULL otherwise)                */
+    const float* bias;   /* N or NULL                                        */
+    const void* residual; int64_t ldr;  /* NULL, or M x N; may be y itself   */
+    void* z;             int64_t ldz;   /* NULL, or z for the gradient       */
+    void* y;             int64_t ldy;
+    void* workspace;     size_t workspace_bytes;
+} vcsr_linear_args;
+int vcsr_linear_workspace(const vcsr_linear_args* args, size_t* bytes);
+int vcsr_linear(const vcsr_linear_args* args, void* stream, float* ms);
+
+/* Gradients of vcsr_linear on VCSR_F32 or VCSR_BF16 operands: dz = dy *
+ * act'(z), dx = dz W, dw = dz^T x, dbias = sum over rows of dz (the residual's
+ * gradient is dy).  For VCSR_BF16 operands dz is rounded to bf16 before the two
+ * products (the matrix cores' operand type); dbias sums the unrounded dz. */
+typedef struct {
+    int64_t M;
+    int32_t N, K;
+    int32_t x_type;      /* x, w, dx, dw: VCSR_F32 or VCSR_BF16              */
+    int32_t y_type;      /* dy, z: VCSR_F32 or VCSR_BF16                     */
+    int32_t act;
+    const void* dy;      int64_t lddy;
+    const void* z;       int64_t ldz;   /* may be NULL for VCSR_ACT_NONE     */
+    const void* x;       int64_t ldx;   /* needed for dw                     */
+    const void* w;       int64_t ldw;   /* needed for dx                     */
+    void* dx;            int64_t lddx;  /* M x K, or NULL                    */
+    void* dw;            int64_t lddw;  /* N x K (zeros for M = 0), or NULL  */
+    float* dbias;        /* N (zeros for M = 0), or NULL                     */
+    void* workspace;     size_t workspace_bytes;
+} vcsr_linear_grad_args;
+int vcsr_linear_grad_workspace(const vcsr_linear_grad_args* args, size_t* bytes);
+int vcsr_linear_grad(const vcsr_linear_grad_args* args, void* stream, float* ms);
+
+/* AdamW over all tensors of a model in one launch.  With g = grad_scale *
+ * grad:  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ * param = param (1 - lr weight_decay)
+ *         - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps).
+ * States are FP32, or VCSR_FP8 with one FP32 scale per block of 256
+ * consecutive values of a tensor (the last block may be shorter): m holds
+ * m / m_scale, v holds sqrt(v) / v_scale, each scale is max(largest magnitude
+ * of the block, 1e-30) / 448, and a nonzero sqrt(v) is stored as the smallest
+ * code (2^-9) where it would round to zero, so that no step divides by a lost
+ * v.  All zero bytes are a valid fresh state of either type. */
+typedef struct {
+    int64_t n;           /* values; 0 is allowed                             */
+    int32_t grad_type;   /* VCSR_F32 or VCSR_BF16                            */
+    int32_t state_type;  /* VCSR_F32 or VCSR_FP8                             */
+    float* param;
+    const void* grad;
+    void *m, *v;
+    float *m_scale, *v_scale; /* ceil(n / 256) each, for VCSR_FP8            */
+    void* copy;          /* NULL, or n values: param rounded to bf16         */
+    double weight_decay;
+} vcsr_adamw_tensor;
+/* Held in 64 bits until the step's FP32 constants (1 - beta1, lr / (1 -
+ * beta1^step), ...) are formed from them, each rounded once. */
+typedef struct {
+    double lr, beta1, beta2, eps, grad_scale;
+    int64_t step;        /* 1 for the first */
+} vcsr_adamw_hyper;
+typedef struct vcsr_adamw vcsr_adamw;
+/* Binds the tensors' addresses (they stay the caller's) to a plan on the
+ * current device; tensors must not overlap.  A step only enqueues its kernel. */
+int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* stream,
+                      vcsr_adamw** out);
+int vcsr_adamw_step(const vcsr_adamw* plan, const vcsr_adamw_hyper* hyper, void* stream,
+                    float* ms);
+void vcsr_adamw_free(vcsr_adamw* plan);
+
 /* --------------------------------------------------- device plumbing */
 /* Minimal HIP helpers so hosts (ctypes, the CLI) need no other GPU runtime. */
 int vcsr_device_count(int32_t* n);

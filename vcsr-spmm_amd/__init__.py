@@ -35,6 +35,10 @@ CLI_PATH = os.path.join(_HERE, "bin", "spmm_vcsr")
 VCSR_OK, VCSR_EINVAL, VCSR_EIO, VCSR_ENOMEM, VCSR_EDEVICE, VCSR_ERANGE, VCSR_ESTATE = range(7)
 LAYOUT_H, LAYOUT_S, LAYOUT_TC = 0, 1, 2
 KERNEL_AUTO, KERNEL_SEGMENT, KERNEL_MFMA, KERNEL_ROW, KERNEL_TILE = 0, 1, 2, 3, 4
+# Value types of the dense operators as buffers carry them: float32, bf16 as
+# 16-bit patterns, e4m3 as 8-bit patterns (VCSR_F32, VCSR_BF16, VCSR_FP8).
+F32, BF16, FP8 = np.dtype(np.float32), np.dtype(np.uint16), np.dtype(np.uint8)
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 
 # Every symbol include/vcsr_spmm.h declares (checked by the CPU test suite).
 EXPORTS = (
@@ -48,7 +52,9 @@ EXPORTS = (
     "vcsr_device_count vcsr_device_name vcsr_dev_malloc vcsr_dev_free vcsr_memcpy_h2d "
     "vcsr_memcpy_d2h vcsr_memcpy_d2d vcsr_memset_d vcsr_stream_create vcsr_stream_destroy "
     "vcsr_stream_sync vcsr_device_sync vcsr_event_create vcsr_event_destroy "
-    "vcsr_event_record vcsr_event_elapsed"
+    "vcsr_event_record vcsr_event_elapsed "
+    "vcsr_rmsnorm vcsr_rmsnorm_grad_workspace vcsr_rmsnorm_grad vcsr_linear_workspace vcsr_linear "
+    "vcsr_linear_grad_workspace vcsr_linear_grad vcsr_adamw_create vcsr_adamw_step vcsr_adamw_free"
 ).split()
 
 
@@ -88,6 +94,53 @@ class _Arrays(C.Structure):
                 ("segment_group_start", C.POINTER(C.c_int32))]
 
 
+class _RmsnormArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("C", C.c_int32), ("x_type", C.c_int32), ("y_type", C.c_int32),
+                ("eps", C.c_float), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("weight", C.c_void_p),
+                ("sum", C.c_void_p), ("ldsum", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("y_scale", C.c_void_p), ("rstd", C.c_void_p)]
+
+
+class _RmsnormGradArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("C", C.c_int32), ("x_type", C.c_int32), ("y_type", C.c_int32),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("s", C.c_void_p), ("lds", C.c_int64),
+                ("weight", C.c_void_p), ("rstd", C.c_void_p), ("dsum", C.c_void_p),
+                ("lddsum", C.c_int64), ("dx", C.c_void_p), ("lddx", C.c_int64),
+                ("dweight", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class _LinearArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("x_type", C.c_int32),
+                ("y_type", C.c_int32), ("act", C.c_int32), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("w", C.c_void_p), ("ldw", C.c_int64), ("x_scale", C.c_void_p),
+                ("w_scale", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p),
+                ("ldr", C.c_int64), ("z", C.c_void_p), ("ldz", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class _LinearGradArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("x_type", C.c_int32),
+                ("y_type", C.c_int32), ("act", C.c_int32), ("dy", C.c_void_p),
+                ("lddy", C.c_int64), ("z", C.c_void_p), ("ldz", C.c_int64), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64), ("dx", C.c_void_p),
+                ("lddx", C.c_int64), ("dw", C.c_void_p), ("lddw", C.c_int64),
+                ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class _AdamwTensor(C.Structure):
+    _fields_ = [("n", C.c_int64), ("grad_type", C.c_int32), ("state_type", C.c_int32),
+                ("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p),
+                ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("copy", C.c_void_p), ("weight_decay", C.c_double)]
+
+
+class _AdamwHyper(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("grad_scale", C.c_double), ("step", C.c_int64)]
+
+
 _lib = None
 
 
@@ -101,6 +154,7 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
     lib = C.CDLL(path)
     P, I32, I64, U64, F = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
     pI, pF, pP = C.POINTER(C.c_int32), C.POINTER(C.c_float), C.POINTER(C.c_void_p)
+    pS = C.POINTER(C.c_size_t)
     sig = {
         "vcsr_last_error": (C.c_char_p, []),
         "vcsr_version": (C.c_char_p, []),
@@ -154,6 +208,16 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "vcsr_event_destroy": (C.c_int, [P]),
         "vcsr_event_record": (C.c_int, [P, P]),
         "vcsr_event_elapsed": (C.c_int, [P, P, pF]),
+        "vcsr_rmsnorm": (C.c_int, [C.POINTER(_RmsnormArgs), P, pF]),
+        "vcsr_rmsnorm_grad_workspace": (C.c_int, [C.POINTER(_RmsnormGradArgs), pS]),
+        "vcsr_rmsnorm_grad": (C.c_int, [C.POINTER(_RmsnormGradArgs), P, pF]),
+        "vcsr_linear_workspace": (C.c_int, [C.POINTER(_LinearArgs), pS]),
+        "vcsr_linear": (C.c_int, [C.POINTER(_LinearArgs), P, pF]),
+        "vcsr_linear_grad_workspace": (C.c_int, [C.POINTER(_LinearGradArgs), pS]),
+        "vcsr_linear_grad": (C.c_int, [C.POINTER(_LinearGradArgs), P, pF]),
+        "vcsr_adamw_create": (C.c_int, [C.POINTER(_AdamwTensor), I32, P, pP]),
+        "vcsr_adamw_step": (C.c_int, [P, C.POINTER(_AdamwHyper), P, pF]),
+        "vcsr_adamw_free": (None, [P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -603,3 +667,229 @@ def run_vcsr_spmm_gpu_noalloc(fmt: Vcsr, dB, O, dC, stream=None, accumulate=Fals
     _need_bc(fmt.N, fmt.M, O, dB, dC)
     _check(load_library().spmm_vcsr_noalloc(fmt._h, dB.ptr, O, dC.ptr, _sp(stream),
                                             1 if accumulate else 0))
+
+
+# ----------------------------------------------------------- dense operators
+class DeviceView:
+    """A matrix or vector in device memory that another object owns (`owner`
+    is kept alive): its address, shape, dtype (F32, BF16 or FP8) and, for a
+    matrix, the elements from one row to the next."""
+
+    def __init__(self, ptr, shape, dtype, ld=None, owner=None):
+        self.ptr = C.c_void_p(int(getattr(ptr, "value", ptr) or 0))
+        self.shape = tuple(shape) if isinstance(shape, (tuple, list)) else (int(shape),)
+        self.dtype = np.dtype(dtype)
+        self.ld = int(ld) if ld is not None else (self.shape[-1] if self.shape else 1)
+        rows = int(np.prod(self.shape[:-1])) if len(self.shape) > 1 else 1
+        elems = (rows - 1) * self.ld + self.shape[-1] if rows and self.shape else 0
+        self.nbytes = elems * self.dtype.itemsize
+        self.owner = owner
+
+
+_TYPE = {F32: 0, BF16: 1, FP8: 2}
+
+
+def _type(arr, what):
+    t = _TYPE.get(arr.dtype)
+    if t is None:
+        raise VcsrError(VCSR_EINVAL, f"{what}: dtype {arr.dtype}; float32, bf16 (uint16) or "
+                                     "e4m3 (uint8) patterns are expected")
+    return t
+
+
+def _mat(arr, rows, cols, what, dtype=None):
+    """(address, row stride) of a matrix argument after checking its shape,
+    type and size; (None, 0) for None."""
+    if arr is None:
+        return None, 0
+    if arr.shape != (rows, cols):
+        raise VcsrError(VCSR_EINVAL, f"{what}: shape {arr.shape}, expected {(rows, cols)}")
+    if dtype is not None and arr.dtype != dtype:
+        raise VcsrError(VCSR_EINVAL, f"{what}: dtype {arr.dtype}, expected {dtype}")
+    ld = getattr(arr, "ld", cols)
+    if rows and arr.nbytes < ((rows - 1) * ld + cols) * arr.dtype.itemsize:
+        raise VcsrError(VCSR_EINVAL, f"{what}: {arr.nbytes} bytes are too few")
+    return arr.ptr, ld
+
+
+def _vec(arr, n, what):
+    if arr is None:
+        return None
+    if arr.dtype != F32 or arr.nbytes < 4 * n:
+        raise VcsrError(VCSR_EINVAL, f"{what}: {arr.dtype}, {arr.nbytes} bytes; "
+                                     f"{n} float32 values are expected")
+    return arr.ptr
+
+
+def _shape2(arr, what):
+    if len(arr.shape) != 2:
+        raise VcsrError(VCSR_EINVAL, f"{what}: shape {arr.shape}, a matrix is expected")
+    return arr.shape
+
+
+_workspaces = {}  # stream handle -> DeviceArray
+
+
+def workspace(nbytes, stream=None):
+    """The binding's workspace of a stream, at least nbytes large: grown (after
+    the stream's work is done) when a call needs more, kept until
+    release_workspaces().  Calls on one stream run one after the other, so they
+    share it; for a call that is captured into a graph pass a DeviceArray of
+    its own, or make the same call once before the capture."""
+    key = stream.h.value if stream is not None else None
+    have = _workspaces.get(key)
+    if have is None or have.nbytes < nbytes:
+        if have is not None:
+            _check(load_library().vcsr_stream_sync(_sp(stream)))
+        have = _workspaces[key] = DeviceArray((max(int(nbytes), 1 << 20),), np.uint8)
+    return have
+
+
+def release_workspaces():
+    """Frees the workspaces of all streams once the device is idle."""
+    if _workspaces:
+        _check(load_library().vcsr_device_sync())
+        _workspaces.clear()
+
+
+def _with_workspace(args, query, given, stream):
+    need = C.c_size_t(0)
+    _check(query(C.byref(args), C.byref(need)))
+    if need.value:
+        ws = given if given is not None else workspace(need.value, stream)
+        args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+
+
+def _call(fn, args, stream, timed):
+    if not timed:
+        rc = fn(C.byref(args), _sp(stream), None)
+        if rc:
+            _check(rc)
+        return None
+    ms = C.c_float(0)
+    _check(fn(C.byref(args), _sp(stream), C.byref(ms)))
+    return ms.value
+
+
+def run_rmsnorm_gpu(x, weight, y, residual=None, sum=None, y_scale=None, rstd=None, eps=1e-6,
+                    stream=None, timed=False):
+    """y = t / sqrt(mean(t^2) + eps) * weight for t = x + residual, row by row
+    (vcsr_rmsnorm).  x, residual, sum: float32 or BF16; y: float32, BF16 or FP8
+    with y_scale, one scale a row.  sum receives t, rstd each row's factor."""
+    M, N = _shape2(x, "x")
+    (xp, ldx), (rp, ldr) = _mat(x, M, N, "x"), _mat(residual, M, N, "residual", x.dtype)
+    (sp, lds), (yp, ldy) = _mat(sum, M, N, "sum", x.dtype), _mat(y, M, N, "y")
+    args = _RmsnormArgs(M, N, _type(x, "x"), _type(y, "y"), eps, xp, ldx, rp, ldr,
+                        _vec(weight, N, "weight"), sp, lds, yp, ldy,
+                        _vec(y_scale, M, "y_scale"), _vec(rstd, M, "rstd"))
+    return _call(load_library().vcsr_rmsnorm, args, stream, timed)
+
+
+def run_rmsnorm_grad_gpu(dy, s, weight, rstd, dx, dweight=None, dsum=None, workspace=None,
+                         stream=None, timed=False):
+    """Gradients of run_rmsnorm_gpu (vcsr_rmsnorm_grad): s is the saved sum (x
+    without a residual), dsum what flows into it from elsewhere; dx is the
+    gradient of x and of the residual."""
+    M, N = _shape2(s, "s")
+    (dp, lddy), (sp, lds) = _mat(dy, M, N, "dy"), _mat(s, M, N, "s")
+    (up, ldu), (xp, ldx) = _mat(dsum, M, N, "dsum", s.dtype), _mat(dx, M, N, "dx", s.dtype)
+    args = _RmsnormGradArgs(M, N, _type(s, "s"), _type(dy, "dy"), dp, lddy, sp, lds,
+                            _vec(weight, N, "weight"), _vec(rstd, M, "rstd"), up, ldu, xp, ldx,
+                            _vec(dweight, N, "dweight"))
+    lib = load_library()
+    _with_workspace(args, lib.vcsr_rmsnorm_grad_workspace, workspace, stream)
+    return _call(lib.vcsr_rmsnorm_grad, args, stream, timed)
+
+
+def _act(act):
+    a = ACTIVATIONS.get(act)
+    if a is None:
+        raise VcsrError(VCSR_EINVAL, f"act: {act!r}, one of {sorted(ACTIVATIONS)} is expected")
+    return a
+
+
+def run_linear_gpu(x, w, y, bias=None, residual=None, act="none", z=None, x_scale=None,
+                   w_scale=None, workspace=None, stream=None, timed=False):
+    """y = act(x W^T + bias) + residual (vcsr_linear); w has one row per output
+    column.  x, w: float32, BF16, or FP8 with x_scale and w_scale, one scale a
+    row; y, z, residual: float32 or BF16.  z receives the activation's input."""
+    (M, K), N = _shape2(x, "x"), _shape2(w, "w")[0]
+    (xp, ldx), (wp, ldw) = _mat(x, M, K, "x"), _mat(w, N, K, "w", x.dtype)
+    (yp, ldy), (rp, ldr) = _mat(y, M, N, "y"), _mat(residual, M, N, "residual", y.dtype)
+    zp, ldz = _mat(z, M, N, "z", y.dtype)
+    args = _LinearArgs(M, N, K, _type(x, "x"), _type(y, "y"), _act(act), xp, ldx, wp, ldw,
+                       _vec(x_scale, M, "x_scale"), _vec(w_scale, N, "w_scale"),
+                       _vec(bias, N, "bias"), rp, ldr, zp, ldz, yp, ldy)
+    lib = load_library()
+    _with_workspace(args, lib.vcsr_linear_workspace, workspace, stream)
+    return _call(lib.vcsr_linear, args, stream, timed)
+
+
+def run_linear_grad_gpu(dy, x, w, z=None, act="none", dx=None, dw=None, dbias=None,
+                        workspace=None, stream=None, timed=False):
+    """Gradients of run_linear_gpu (vcsr_linear_grad) from dy and the saved z
+    (not needed for act "none"): those of dx, dw and dbias that are given.  The
+    residual's gradient is dy."""
+    (M, K), N = _shape2(x, "x"), _shape2(w, "w")[0]
+    (xp, ldx), (wp, ldw) = _mat(x, M, K, "x"), _mat(w, N, K, "w", x.dtype)
+    (dp, lddy), (zp, ldz) = _mat(dy, M, N, "dy"), _mat(z, M, N, "z", dy.dtype)
+    (xg, lddx), (wg, lddw) = _mat(dx, M, K, "dx", x.dtype), _mat(dw, N, K, "dw", x.dtype)
+    args = _LinearGradArgs(M, N, K, _type(x, "x"), _type(dy, "dy"), _act(act), dp, lddy, zp, ldz,
+                           xp, ldx, wp, ldw, xg, lddx, wg, lddw, _vec(dbias, N, "dbias"))
+    lib = load_library()
+    _with_workspace(args, lib.vcsr_linear_grad_workspace, workspace, stream)
+    return _call(lib.vcsr_linear_grad, args, stream, timed)
+
+
+class AdamW:
+    """One AdamW step over all tensors of a model (vcsr_adamw_create / _step).
+
+    `tensors`: dicts of device buffers `param` (float32), `grad` (float32 or
+    BF16), `m` and `v` (float32, or FP8 with `m_scale` and `v_scale`, one
+    float32 per 256 values), optionally `copy` (BF16, receives the parameter)
+    and a number `weight_decay`.  Zeroed states start a run."""
+
+    def __init__(self, tensors, stream=None):
+        table = (_AdamwTensor * max(len(tensors), 1))()
+        for i, t in enumerate(tensors):
+            n = int(np.prod(t["param"].shape))
+            fp8 = t["m"].dtype == FP8
+            blocks = -(-n // 256)
+            for name, dtypes, count in (("param", (F32,), n), ("grad", (F32, BF16), n),
+                                        ("m", (F32, FP8), n), ("v", (t["m"].dtype,), n),
+                                        ("m_scale", (F32,), blocks), ("v_scale", (F32,), blocks),
+                                        ("copy", (BF16,), n)):
+                b = t.get(name)
+                if b is None:
+                    if name == "copy" or (not fp8 and name in ("m_scale", "v_scale")):
+                        continue
+                    raise VcsrError(VCSR_EINVAL, f"tensor {i}: {name} is missing")
+                if b.dtype not in dtypes or b.nbytes < count * b.dtype.itemsize or \
+                        getattr(b, "ld", b.shape[-1] if b.shape else 1) != \
+                        (b.shape[-1] if b.shape else 1):
+                    raise VcsrError(VCSR_EINVAL, f"tensor {i}: {name}: {b.dtype}, {b.nbytes} "
+                                                 f"bytes; {count} contiguous values are expected")
+            ptr = {k: t[k].ptr if t.get(k) is not None else None for k in
+                   ("param", "grad", "m", "v", "m_scale", "v_scale", "copy")}
+            table[i] = _AdamwTensor(n, _TYPE[t["grad"].dtype], _TYPE[t["m"].dtype], ptr["param"],
+                                    ptr["grad"], ptr["m"], ptr["v"], ptr["m_scale"],
+                                    ptr["v_scale"], ptr["copy"], t.get("weight_decay", 0.0))
+        self._keep = [dict(t) for t in tensors]
+        self._h = C.c_void_p()
+        _check(load_library().vcsr_adamw_create(table, len(tensors), _sp(stream),
+                                                C.byref(self._h)))
+
+    def step(self, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, stream=None,
+             timed=False):
+        """The step numbered `step` (1 for the first); gradients are multiplied
+        by grad_scale first.  Enqueued only, unless timed."""
+        ms = C.c_float(0)
+        hyper = _AdamwHyper(lr, beta1, beta2, eps, grad_scale, step)
+        _check(load_library().vcsr_adamw_step(self._h, C.byref(hyper), _sp(stream),
+                                              C.byref(ms) if timed else None))
+        return ms.value if timed else None
+
+    def __del__(self):
+        if getattr(self, "_h", None) and _lib is not None and self._h.value:
+            _lib.vcsr_adamw_free(self._h)
+            self._h = C.c_void_p()

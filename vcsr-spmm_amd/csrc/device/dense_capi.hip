@@ -1,0 +1,432 @@
+// dense_capi.hip - extern "C" entry points of the dense operators: argument
+// checks, workspaces and launches.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <memory>
+#include <string>
+#include <vector>
+
+#include "dense.hpp"
+#include "entry.hpp"
+
+namespace {
+
+using namespace vcsr::entry;
+
+bool is_wide(int32_t t) { return t == VCSR_F32 || t == VCSR_BF16; }
+size_t size_of(int32_t t) { return t == VCSR_F32 ? 4 : t == VCSR_BF16 ? 2 : 1; }
+
+void range(bool ok, const char* what) {
+    if (!ok) throw vcsr::Error(VCSR_ERANGE, what);
+}
+
+// Rows are launched as a grid dimension, and a tile's rows are addressed with
+// 32-bit offsets.
+constexpr int64_t kMaxRows = (int64_t)1 << 31, kMaxLd = (int64_t)1 << 22;
+
+void check_rows(int64_t M) {
+    need(M >= 0, "negative M");
+    range(M < kMaxRows, "M over 2^31 - 1");
+}
+// A matrix argument of `cols` columns; resolves a stride of 0.
+void check_matrix(const void* p, int64_t& ld, int64_t cols, int32_t type, const char* what,
+                  bool optional, int64_t rows) {
+    if (!p) {
+        need(optional || rows == 0, what);
+        if (ld == 0) ld = cols;
+        return;
+    }
+    if (ld == 0) ld = cols;
+    need(ld >= cols, what);
+    range(ld <= kMaxLd, what);
+    need((uintptr_t)p % size_of(type) == 0, what);
+}
+void check_vector(const void* p, const char* what, bool optional = false) {
+    need(p || optional, what);
+    need((uintptr_t)p % 4 == 0, what);
+}
+void check_workspace(const void* p, size_t have, size_t want) {
+    if (!want) return;
+    need(p && have >= want, "workspace: too small (see the _workspace function)");
+    need((uintptr_t)p % 16 == 0, "workspace: not 16-byte aligned");
+}
+
+vcsr_rmsnorm_args checked(const vcsr_rmsnorm_args* args) {
+    need(args, "null argument");
+    vcsr_rmsnorm_args a = *args;
+    check_rows(a.M);
+    need(a.C >= 1, "C: at least 1");
+    need(is_wide(a.x_type), "x_type: VCSR_F32 or VCSR_BF16");
+    need(is_wide(a.y_type) || a.y_type == VCSR_FP8, "y_type: VCSR_F32, VCSR_BF16 or VCSR_FP8");
+    need(a.eps >= 0.f && std::isfinite(a.eps), "eps: a finite number, at least 0");
+    check_matrix(a.x, a.ldx, a.C, a.x_type, "x: pointer, alignment or stride", false, a.M);
+    check_matrix(a.residual, a.ldr, a.C, a.x_type, "residual: alignment or stride", true, a.M);
+    check_vector(a.weight, "weight: pointer or alignment");
+    check_matrix(a.sum, a.ldsum, a.C, a.x_type, "sum: alignment or stride", true, a.M);
+    check_matrix(a.y, a.ldy, a.C, a.y_type, "y: pointer, alignment or stride", false, a.M);
+    need((a.y_scale != nullptr) == (a.y_type == VCSR_FP8) || a.M == 0,
+         "y_scale: given for VCSR_FP8 and only then");
+    check_vector(a.y_scale, "y_scale: alignment", true);
+    check_vector(a.rstd, "rstd: alignment", true);
+    need(a.y != a.x || a.M == 0 || (a.y_type == a.x_type && a.ldy == a.ldx),
+         "y over x: of another type or stride");
+    return a;
+}
+
+vcsr_rmsnorm_grad_args checked_sizes(const vcsr_rmsnorm_grad_args* args) {
+    need(args, "null argument");
+    vcsr_rmsnorm_grad_args a = *args;
+    check_rows(a.M);
+    need(a.C >= 1, "C: at least 1");
+    need(is_wide(a.x_type), "x_type: VCSR_F32 or VCSR_BF16");
+    need(is_wide(a.y_type), "y_type: VCSR_F32 or VCSR_BF16");
+    return a;
+}
+vcsr_rmsnorm_grad_args checked(const vcsr_rmsnorm_grad_args* args) {
+    vcsr_rmsnorm_grad_args a = checked_sizes(args);
+    check_matrix(a.dy, a.lddy, a.C, a.y_type, "dy: pointer, alignment or stride", false, a.M);
+    check_matrix(a.s, a.lds, a.C, a.x_type, "s: pointer, alignment or stride", false, a.M);
+    check_vector(a.weight, "weight: pointer or alignment");
+    check_vector(a.rstd, "rstd: pointer or alignment", a.M == 0);
+    check_matrix(a.dsum, a.lddsum, a.C, a.x_type, "dsum: alignment or stride", true, a.M);
+    check_matrix(a.dx, a.lddx, a.C, a.x_type, "dx: pointer, alignment or stride", false, a.M);
+    check_vector(a.dweight, "dweight: alignment", true);
+    check_workspace(a.workspace, a.workspace_bytes, vcsr::rmsnorm_grad_workspace(a));
+    return a;
+}
+
+void check_act(int32_t act) {
+    need(act >= VCSR_ACT_NONE && act <= VCSR_ACT_SILU, "act: one of VCSR_ACT_*");
+}
+
+vcsr_linear_args checked_sizes(const vcsr_linear_args* args) {
+    need(args, "null argument");
+    vcsr_linear_args a = *args;
+    check_rows(a.M);
+    need(a.N >= 1 && a.K >= 1, "N, K: at least 1");
+    need(is_wide(a.x_type) || a.x_type == VCSR_FP8, "x_type: VCSR_F32, VCSR_BF16 or VCSR_FP8");
+    need(is_wide(a.y_type), "y_type: VCSR_F32 or VCSR_BF16");
+    check_act(a.act);
+    if (a.ldx == 0) a.ldx = a.K;
+    if (a.ldw == 0) a.ldw = a.K;
+    if (a.ldy == 0) a.ldy = a.N;
+    return a;
+}
+vcsr::Gemm gemm_of(const vcsr_linear_args& a) {
+    vcsr::Gemm g;
+    g.I = a.M;
+    g.J = a.N;
+    g.R = a.K;
+    g.type = a.x_type;
+    g.out_type = a.y_type;
+    g.act = a.act;
+    g.p = a.x;
+    g.ldp = a.ldx;
+    g.q = a.w;
+    g.ldq = a.ldw;
+    g.p_scale = a.x_scale;
+    g.q_scale = a.w_scale;
+    g.bias = a.bias;
+    g.residual = a.residual;
+    g.ldr = a.ldr;
+    g.z = a.z;
+    g.ldz = a.ldz;
+    g.out = a.y;
+    g.ldo = a.ldy;
+    g.part = (float*)a.workspace;
+    return g;
+}
+vcsr_linear_args checked(const vcsr_linear_args* args) {
+    vcsr_linear_args a = checked_sizes(args);
+    check_matrix(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", false, a.M);
+    check_matrix(a.w, a.ldw, a.K, a.x_type, "w: pointer, alignment or stride", false, a.M);
+    const bool scaled = a.x_type == VCSR_FP8;
+    need(a.M == 0 || ((a.x_scale != nullptr) == scaled && (a.w_scale != nullptr) == scaled),
+         "x_scale, w_scale: given for VCSR_FP8 and only then");
+    check_vector(a.x_scale, "x_scale: alignment", true);
+    check_vector(a.w_scale, "w_scale: alignment", true);
+    check_vector(a.bias, "bias: alignment", true);
+    check_matrix(a.residual, a.ldr, a.N, a.y_type, "residual: alignment or stride", true, a.M);
+    check_matrix(a.z, a.ldz, a.N, a.y_type, "z: alignment or stride", true, a.M);
+    check_matrix(a.y, a.ldy, a.N, a.y_type, "y: pointer, alignment or stride", false, a.M);
+    need(!a.z || a.z != a.y, "z: another matrix than y");
+    check_workspace(a.workspace, a.workspace_bytes, vcsr::gemm_workspace(gemm_of(a)));
+    return a;
+}
+
+// The gradient's work: dz (unless dy serves as it is), dbias' partial rows,
+// and the two products, whose partial sums share what is behind.
+struct LinearGrad {
+    vcsr_linear_grad_args a;
+    bool own_dz = false;  // dz lies in the workspace
+    int64_t lddz = 0;
+    size_t dz_bytes = 0, bias_bytes = 0, part_bytes = 0;
+    vcsr::Gemm dx, dw;
+    size_t bytes() const { return dz_bytes + bias_bytes + part_bytes; }
+};
+
+size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
+
+LinearGrad grad_of(const vcsr_linear_grad_args* args) {
+    need(args, "null argument");
+    LinearGrad w;
+    vcsr_linear_grad_args& a = w.a;
+    a = *args;
+    check_rows(a.M);
+    need(a.N >= 1 && a.K >= 1, "N, K: at least 1");
+    need(is_wide(a.x_type), "x_type: VCSR_F32 or VCSR_BF16");
+    need(is_wide(a.y_type), "y_type: VCSR_F32 or VCSR_BF16");
+    check_act(a.act);
+    need(a.z || a.act == VCSR_ACT_NONE || a.M == 0, "z: needed for an activation");
+    auto stride = [](int64_t& ld, int64_t cols) {
+        if (ld == 0) ld = cols;
+    };
+    stride(a.lddy, a.N);
+    stride(a.ldz, a.N);
+    stride(a.ldx, a.K);
+    stride(a.ldw, a.K);
+    stride(a.lddx, a.K);
+    stride(a.lddw, a.K);
+    if (a.M == 0) return w;
+    const bool products = a.dx || a.dw;
+    w.own_dz = products && (a.act != VCSR_ACT_NONE || a.x_type != a.y_type);
+    // Rows of dz on 16-byte boundaries.
+    w.lddz = w.own_dz ? ((int64_t)a.N + 7) / 8 * 8 : a.lddy;
+    if (w.own_dz) w.dz_bytes = round_up((size_t)a.M * (size_t)w.lddz * size_of(a.x_type));
+    if (a.dbias)
+        w.bias_bytes = round_up((size_t)vcsr::dz_row_blocks(a.M, a.N) * (size_t)a.N * 4);
+    char* base = (char*)a.workspace;
+    const void* dz = w.own_dz ? (const void*)base : a.dy;
+    float* part = (float*)(base + w.dz_bytes + w.bias_bytes);
+    vcsr::Gemm& x = w.dx;
+    x.type = x.out_type = a.x_type;
+    x.I = a.M;
+    x.J = a.K;
+    x.R = a.N;
+    x.p = dz;
+    x.ldp = w.lddz;
+    x.q = a.w;
+    x.ldq = a.ldw;
+    x.q_cols = true;
+    x.out = a.dx;
+    x.ldo = a.lddx;
+    x.part = part;
+    vcsr::Gemm& g = w.dw;
+    g.type = g.out_type = a.x_type;
+    g.I = a.N;
+    g.J = a.K;
+    g.R = a.M;
+    g.p = dz;
+    g.ldp = w.lddz;
+    g.p_cols = true;
+    g.q = a.x;
+    g.ldq = a.ldx;
+    g.q_cols = true;
+    g.out = a.dw;
+    g.ldo = a.lddw;
+    g.part = part;
+    if (a.dx) w.part_bytes = vcsr::gemm_workspace(x);
+    if (a.dw) w.part_bytes = std::max(w.part_bytes, vcsr::gemm_workspace(g));
+    return w;
+}
+
+LinearGrad checked(const vcsr_linear_grad_args* args) {
+    LinearGrad w = grad_of(args);
+    vcsr_linear_grad_args& a = w.a;
+    check_matrix(a.dy, a.lddy, a.N, a.y_type, "dy: pointer, alignment or stride", false, a.M);
+    check_matrix(a.z, a.ldz, a.N, a.y_type, "z: pointer, alignment or stride",
+                 a.act == VCSR_ACT_NONE, a.M);
+    check_matrix(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", !a.dw, a.M);
+    check_matrix(a.w, a.ldw, a.K, a.x_type, "w: pointer, alignment or stride", !a.dx, a.M);
+    check_matrix(a.dx, a.lddx, a.K, a.x_type, "dx: alignment or stride", true, a.M);
+    check_matrix(a.dw, a.lddw, a.K, a.x_type, "dw: alignment or stride", true, a.M);
+    check_vector(a.dbias, "dbias: alignment", true);
+    check_workspace(a.workspace, a.workspace_bytes, w.bytes());
+    return w;
+}
+
+hipError_t zero_matrix(void* p, int64_t ld, int64_t rows, int64_t row_bytes, int64_t size,
+                       hipStream_t st) {
+    if (ld * size == row_bytes) return vcsr::launch_zero(p, rows * row_bytes, st);
+    for (int64_t r = 0; r < rows; ++r) {
+        hipError_t e = vcsr::launch_zero((char*)p + r * ld * size, row_bytes, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t run_grad(const LinearGrad& w, hipStream_t st) {
+    const vcsr_linear_grad_args& a = w.a;
+    hipError_t e = hipSuccess;
+    if (a.M == 0) {
+        const int64_t size = (int64_t)size_of(a.x_type);
+        if (a.dw) e = zero_matrix(a.dw, a.lddw, a.N, a.K * size, size, st);
+        if (e == hipSuccess && a.dbias) e = vcsr::launch_zero(a.dbias, (int64_t)a.N * 4, st);
+        return e;
+    }
+    char* base = (char*)a.workspace;
+    float* bias_part = a.dbias ? (float*)(base + w.dz_bytes) : nullptr;
+    if (w.own_dz || bias_part) {
+        e = vcsr::launch_dz(a, w.own_dz ? base : nullptr, w.lddz, bias_part, st);
+        if (e == hipSuccess && bias_part)
+            e = vcsr::launch_sum_rows(bias_part, vcsr::dz_row_blocks(a.M, a.N), a.N, a.N, a.dbias,
+                                      st);
+    }
+    if (e == hipSuccess && a.dx) e = vcsr::launch_gemm(w.dx, st);
+    if (e == hipSuccess && a.dw) e = vcsr::launch_gemm(w.dw, st);
+    return e;
+}
+
+}  // namespace
+
+struct vcsr_adamw {
+    int device = -1;
+    vcsr_adamw_tensor* tensors = nullptr;  // on the device
+    int2* chunks = nullptr;                // {tensor, chunk of it}
+    int32_t n_chunks = 0;
+    ~vcsr_adamw() {
+        if (tensors) (void)hipFree(tensors);
+        if (chunks) (void)hipFree(chunks);
+    }
+};
+
+extern "C" {
+
+int vcsr_rmsnorm(const vcsr_rmsnorm_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_rmsnorm_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return vcsr::launch_rmsnorm(a, st); });
+    });
+}
+
+int vcsr_rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args* args, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = vcsr::rmsnorm_grad_workspace(checked_sizes(args));
+    });
+}
+
+int vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_rmsnorm_grad_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return vcsr::launch_rmsnorm_grad(a, st); });
+    });
+}
+
+int vcsr_linear_workspace(const vcsr_linear_args* args, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        const vcsr_linear_args a = checked_sizes(args);
+        *bytes = a.M > 0 ? vcsr::gemm_workspace(gemm_of(a)) : 0;
+    });
+}
+
+int vcsr_linear(const vcsr_linear_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_linear_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        const vcsr::Gemm g = gemm_of(a);
+        run_timed(st, ms, [&] { return vcsr::launch_gemm(g, st); });
+    });
+}
+
+int vcsr_linear_grad_workspace(const vcsr_linear_grad_args* args, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = grad_of(args).bytes();
+    });
+}
+
+int vcsr_linear_grad(const vcsr_linear_grad_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const LinearGrad w = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return run_grad(w, st); });
+    });
+}
+
+int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* stream,
+                      vcsr_adamw** out) {
+    return guarded([&] {
+        need(out, "null argument");
+        *out = nullptr;
+        need(count >= 0 && (tensors || count == 0), "tensors: null or a negative count");
+        std::vector<vcsr_adamw_tensor> list(tensors, tensors + count);
+        std::vector<int2> chunks;
+        for (int32_t i = 0; i < count; ++i) {
+            const vcsr_adamw_tensor& t = list[i];
+            const std::string who = "tensor " + std::to_string(i) + ": ";
+            auto must = [&](bool ok, const char* what) { need(ok, (who + what).c_str()); };
+            must(t.n >= 0, "negative n");
+            range(t.n < kMaxRows * vcsr::kAdamwChunk, (who + "n over 2^43").c_str());
+            must(is_wide(t.grad_type), "grad_type: VCSR_F32 or VCSR_BF16");
+            must(t.state_type == VCSR_F32 || t.state_type == VCSR_FP8,
+                 "state_type: VCSR_F32 or VCSR_FP8");
+            must(std::isfinite(t.weight_decay), "weight_decay: not finite");
+            if (t.n == 0) continue;
+            const bool f8 = t.state_type == VCSR_FP8;
+            must(t.param && t.grad && t.m && t.v, "param, grad, m or v: null");
+            must(!f8 || (t.m_scale && t.v_scale), "m_scale, v_scale: needed for VCSR_FP8");
+            must(((uintptr_t)t.param | (uintptr_t)t.m_scale | (uintptr_t)t.v_scale) % 4 == 0 &&
+                     (uintptr_t)t.grad % size_of(t.grad_type) == 0 &&
+                     ((uintptr_t)t.m | (uintptr_t)t.v) % size_of(t.state_type) == 0 &&
+                     (uintptr_t)t.copy % 2 == 0,
+                 "a pointer is not aligned to its type");
+            const int64_t n = (t.n + vcsr::kAdamwChunk - 1) / vcsr::kAdamwChunk;
+            range((int64_t)chunks.size() + n < kMaxRows, "tensors: over 2^31 chunks of 4096");
+            for (int64_t k = 0; k < n; ++k) chunks.push_back(make_int2(i, (int)k));
+        }
+        need_device();
+        std::unique_ptr<vcsr_adamw> h(new vcsr_adamw);
+        hip_check(hipGetDevice(&h->device), "hipGetDevice");
+        hipStream_t st = (hipStream_t)stream;
+        h->tensors = upload_array(list, st, "AdamW tensors");
+        h->chunks = upload_array(chunks, st, "AdamW chunks");
+        h->n_chunks = (int32_t)chunks.size();
+        hip_check(hipStreamSynchronize(st), "hipStreamSynchronize");  // the host arrays end here
+        *out = h.release();
+    });
+}
+
+int vcsr_adamw_step(const vcsr_adamw* plan, const vcsr_adamw_hyper* hyper, void* stream,
+                    float* ms) {
+    return guarded([&] {
+        need(plan && hyper, "null argument");
+        const vcsr_adamw_hyper& y = *hyper;
+        need(std::isfinite(y.lr) && std::isfinite(y.grad_scale), "lr, grad_scale: not finite");
+        need(y.beta1 >= 0.0 && y.beta1 < 1.0 && y.beta2 >= 0.0 && y.beta2 < 1.0,
+             "beta1, beta2: in [0, 1)");
+        need(y.eps >= 0.0 && std::isfinite(y.eps), "eps: a finite number, at least 0");
+        need(y.step >= 1, "step: at least 1");
+        int device = -1;
+        hip_check(hipGetDevice(&device), "hipGetDevice");
+        if (device != plan->device)
+            throw vcsr::Error(VCSR_ESTATE, "the plan is another device's");
+        vcsr::AdamwStep s;
+        s.beta1 = (float)y.beta1;
+        s.beta2 = (float)y.beta2;
+        s.one_minus_beta1 = (float)(1.0 - y.beta1);
+        s.one_minus_beta2 = (float)(1.0 - y.beta2);
+        s.lr = y.lr;
+        s.lr_over_bias1 = (float)(y.lr / (1.0 - std::pow(y.beta1, (double)y.step)));
+        s.inv_root_bias2 =
+            (float)(1.0 / std::sqrt(1.0 - std::pow(y.beta2, (double)y.step)));
+        s.eps = (float)y.eps;
+        s.grad_scale = (float)y.grad_scale;
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] {
+            return vcsr::launch_adamw(plan->tensors, plan->chunks, plan->n_chunks, s, st);
+        });
+    });
+}
+
+void vcsr_adamw_free(vcsr_adamw* plan) { delete plan; }
+
+}  // extern "C"

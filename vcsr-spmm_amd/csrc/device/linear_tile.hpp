@@ -1,0 +1,388 @@
+// linear_tile.hpp - the dense product on the matrix cores, for linear_f32.hip,
+// linear_bf16.hip and linear_fp8.hip.
+//
+// out[i][j] = epilogue(sum_k P(i, k) Q(j, k)).  A block computes a TI x TJ tile
+// of out; its WI x WJ waves take equal parts.  The sum goes in steps of 128
+// bytes of k: both operands' tiles are brought to LDS (two buffers: the next
+// step's tiles arrive while this one's are multiplied), and a wave multiplies
+// 16 x 16 blocks with v_mfma_f32_16x16x4_f32 or _16x16x32_bf16.
+//
+// LDS tiles are TI (or TJ) x 128 bytes in 16-byte granules:
+//   by rows     row r at r * 128, granule g of its k at slot g ^ key(r);
+//   by columns  k-row k at k * TI * size, granule c of its i at slot c ^ key(k).
+// The keys spread the granules that 16 lanes read together over all banks.
+// A lane of the matrix instruction holds row (lane & 15) and, of each step, k in
+// 16-byte granules (lane >> 4) + 4 s; any assignment of k to lanes is right as
+// long as both operands use it.
+//
+// The matrix instruction's rows are out's columns: a lane then holds 4
+// consecutive j of one i.  Within 32 columns, row a of block b stands for
+// column (a >> 2) * 8 + b * 4 + (a & 3), so that two blocks give a lane 8
+// consecutive j, a 16-byte store of bf16.
+#pragma once
+
+#include "common.hpp"
+#include "dense.hpp"
+
+namespace vcsr {
+namespace tile {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+
+constexpr int kStepBytes = 128;
+
+// Granule keys of tiles by rows, for 16 consecutive rows (P) and for the rows
+// that a block of Q stands for.
+__device__ __forceinline__ int key_p(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int key_q(int r) { return ((r >> 1) & 1) | ((r >> 2) & 6); }
+template <bool Q>
+__device__ __forceinline__ int key_rows(int r) {
+    return Q ? key_q(r) : key_p(r);
+}
+// Key of k-row k of a tile by columns with `gran` granules a k-row.
+template <class T, int GRAN>
+__device__ __forceinline__ int key_cols(int k) {
+    if (sizeof(T) == 2) return (((k & 3) | ((k >> 1) & 4)) << 1) & (GRAN - 1);
+    return ((k >> 2) & 3) << 2 & (GRAN - 1);
+}
+
+struct Operand {
+    const uint8_t* p;
+    int64_t ld;     // bytes
+    int64_t n;      // rows of the operand (i or j)
+    int64_t first;  // of the tile
+};
+
+// One operand's tile loader: NT threads bring ROWS x 128 bytes.  `GR` granules a
+// thread; granule e = it * NT + tid of the tile lies at e * 16 in LDS.
+template <class T, int ROWS, int NT, bool COLS, bool Q>
+struct Loader {
+    static constexpr int GR = ROWS * 8 / NT;
+    static constexpr int EPG = 16 / (int)sizeof(T);
+    static constexpr int BK = kStepBytes / (int)sizeof(T);
+    static constexpr int KGRAN = ROWS * (int)sizeof(T) / 16;  // granules of a k-row (by columns)
+    static_assert(ROWS * 8 % NT == 0, "whole granules");
+
+    // k (relative to the step) and row of the first element of granule e.
+    __device__ static void place(int e, int& row, int& k) {
+        if (COLS) {
+            k = e / KGRAN;
+            row = ((e % KGRAN) ^ key_cols<T, KGRAN>(k)) * EPG;
+        } else {
+            row = e >> 3;
+            k = ((e & 7) ^ key_rows<Q>(row)) * EPG;
+        }
+    }
+
+    // Through registers, any alignment and tail: elements past the operand's
+    // rows or past k_end are zeros.
+    __device__ static void fetch(const Operand& o, int64_t k0, int64_t k_end, u32x4 (&v)[GR]) {
+#pragma unroll
+        for (int it = 0; it < GR; ++it) {
+            int row, k;
+            place(it * NT + (int)threadIdx.x, row, k);
+            const int64_t kk = k0 + k, r = o.first + row;
+            const T* p = (const T*)(o.p + (COLS ? kk * o.ld : r * o.ld)) + (COLS ? r : kk);
+            int64_t have = COLS ? o.n - r : k_end - kk;  // elements along the granule
+            if (COLS ? kk >= k_end : r >= o.n) have = 0;
+            if (have >= EPG) {
+                const Mem<T, EPG> m = *(const Mem<T, EPG>*)p;
+                __builtin_memcpy(&v[it], &m, 16);
+            } else {
+                T t[EPG];
+                __builtin_memset(t, 0, 16);
+#pragma unroll
+                for (int i = 0; i < EPG; ++i)
+                    if (i < have) t[i] = p[i];
+                __builtin_memcpy(&v[it], t, 16);
+            }
+        }
+    }
+    __device__ static void put(uint8_t* lds, const u32x4 (&v)[GR]) {
+#pragma unroll
+        for (int it = 0; it < GR; ++it)
+            *(u32x4*)(lds + (it * NT + (int)threadIdx.x) * 16) = v[it];
+    }
+};
+
+// The operand block of one matrix step: 16 rows (of wave-tile block `b`, first
+// row `r0` of the wave's part) and granule step s.
+template <class T, int ROWS, bool COLS, bool Q>
+struct Reader;
+
+// Row of the tile that lane row a of block b stands for.
+template <bool Q>
+__device__ __forceinline__ int tile_row(int r0, int b, int a) {
+    return Q ? r0 + (b >> 1) * 32 + (a >> 2) * 8 + (b & 1) * 4 + (a & 3) : r0 + b * 16 + a;
+}
+
+template <class T, int ROWS, bool Q>
+struct Reader<T, ROWS, false, Q> {
+    __device__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
+        const int lane = threadIdx.x & 63;
+        const int r = tile_row<Q>(r0, b, lane & 15);
+        const int g = (lane >> 4) + 4 * s;
+        return *(const u32x4*)(lds + r * kStepBytes + ((g ^ key_rows<Q>(r)) << 4));
+    }
+};
+// bf16 by columns: the transposing read gives lane t of 16 lanes element t of 4
+// k-rows (lane t addresses 4 consecutive i of k-row t / 4).
+template <int ROWS, bool Q>
+struct Reader<bf16, ROWS, true, Q> {
+    __device__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
+        constexpr int GRAN = ROWS * 2 / 16;
+        const int lane = threadIdx.x & 63, t = lane & 15;
+        const int col = tile_row<Q>(r0, b, (t & 3) * 4);  // 4 consecutive ones from here
+        u32x2 half[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = s * 32 + (lane >> 4) * 8 + h * 4 + (t >> 2);
+            const int at = k * ROWS * 2 + (((col >> 3) ^ key_cols<bf16, GRAN>(k)) << 4) +
+                           (col & 7) * 2;
+            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(lds + at));
+            __builtin_memcpy(&half[h], &v, 8);
+        }
+        return u32x4{half[0].x, half[0].y, half[1].x, half[1].y};
+    }
+};
+template <int ROWS, bool Q>
+struct Reader<float, ROWS, true, Q> {
+    __device__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
+        constexpr int GRAN = ROWS * 4 / 16;
+        const int lane = threadIdx.x & 63;
+        const int col = tile_row<Q>(r0, b, lane & 15);
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = s * 16 + (lane >> 4) * 4 + j;
+            const int at = k * ROWS * 4 + (((col >> 2) ^ key_cols<float, GRAN>(k)) << 4) +
+                           (col & 3) * 4;
+            v[j] = *(const uint32_t*)(lds + at);
+        }
+        return v;
+    }
+};
+
+// acc (rows: Q's block, columns: P's block) += Q P^T over the k of one granule.
+template <class T>
+__device__ __forceinline__ f32x4 mma(const u32x4& q, const u32x4& p, f32x4 acc);
+template <>
+__device__ __forceinline__ f32x4 mma<bf16>(const u32x4& q, const u32x4& p, f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, q),
+                                                   __builtin_bit_cast(bf16x8, p), acc, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma<float>(const u32x4& q, const u32x4& p, f32x4 acc) {
+    const f32x4 a = __builtin_bit_cast(f32x4, q), b = __builtin_bit_cast(f32x4, p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc, 0, 0, 0);
+    return acc;
+}
+// e4m3: the values become bf16 exactly and go through the bf16 instruction,
+// whose sums are FP32.  The e4m3 instructions (16x16x32 and 16x16x128) align
+// their products to the largest and drop bits: up to 2^-12 of the largest product
+// was measured over 128 random terms, far more than FP32's rounding.
+__device__ __forceinline__ void widen(const u32x4& v, bf16x8 (&o)[2]) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.f, false);
+        const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.f, true);
+        o[i >> 1][(i & 1) * 4 + 0] = a[0];
+        o[i >> 1][(i & 1) * 4 + 1] = a[1];
+        o[i >> 1][(i & 1) * 4 + 2] = b[0];
+        o[i >> 1][(i & 1) * 4 + 3] = b[1];
+    }
+}
+// One granule of each operand, as the matrix instruction takes it.
+template <class T>
+struct Frag {
+    u32x4 v;
+    __device__ __forceinline__ void set(const u32x4& x) { v = x; }
+};
+template <>
+struct Frag<fp8> {
+    bf16x8 v[2];
+    __device__ __forceinline__ void set(const u32x4& x) { widen(x, v); }
+};
+template <class T>
+__device__ __forceinline__ f32x4 mma(const Frag<T>& q, const Frag<T>& p, f32x4 acc) {
+    return mma<T>(q.v, p.v, acc);
+}
+template <>
+__device__ __forceinline__ f32x4 mma<fp8>(const Frag<fp8>& q, const Frag<fp8>& p, f32x4 acc) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q.v[h], p.v[h], acc, 0, 0, 0);
+    return acc;
+}
+
+// y, z and the residual of 8 consecutive columns from j of row i.
+template <class O>
+__device__ __forceinline__ void finish(const Gemm& g, int64_t i, int j, float (&v)[8]) {
+    const int n = g.J - j;
+    if (g.p_scale) {
+        const float ps = g.p_scale[i];
+        float qs[8];
+        load_vec(g.q_scale + j, n, qs);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= ps * qs[k];
+    }
+    if (g.bias) {
+        float b[8];
+        load_vec(g.bias + j, n, b);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += b[k];
+    }
+    if (g.z) store_vec((O*)g.z + i * g.ldz + j, n, v);
+    if (g.act != VCSR_ACT_NONE) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = act_f32(g.act, v[k]);
+    }
+    if (g.residual) {
+        float r[8];
+        load_vec((const O*)g.residual + i * g.ldr + j, n, r);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += r[k];
+    }
+    store_vec((O*)g.out + i * g.ldo + j, n, v);
+}
+
+// Row length of the partial sums: whole vectors of 8.
+__host__ __device__ inline int64_t part_ld(int32_t J) { return ((int64_t)J + 7) / 8 * 8; }
+
+template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
+__global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, int64_t steps) {
+    constexpr int NT = 64 * WI * WJ;
+    constexpr int FI = TI / WI / 16, FJ = TJ / WJ / 16;
+    constexpr int BK = kStepBytes / (int)sizeof(T);
+    static_assert(FJ % 2 == 0, "column blocks go in pairs");
+    using LP = Loader<T, TI, NT, PCOLS, false>;
+    using LQ = Loader<T, TJ, NT, QCOLS, true>;
+    using RP = Reader<T, TI, PCOLS, false>;
+    using RQ = Reader<T, TJ, QCOLS, true>;
+    __shared__ __attribute__((aligned(128))) uint8_t lds[2][(TI + TJ) * kStepBytes];
+
+    // Blocks of one XCD take neighbouring tiles, down a column of tiles first,
+    // so that they share Q's rows and a few of P's.
+    const int64_t ti = (g.I + TI - 1) / TI;
+    const uint32_t tj = (uint32_t)(((int64_t)g.J + TJ - 1) / TJ);
+    const uint32_t b = xcd_remap(blockIdx.x, gridDim.x);
+    const uint32_t split = b % (uint32_t)splits, t = b / (uint32_t)splits;
+    constexpr uint32_t kBand = 4;  // tile columns taken together
+    const uint32_t band = t / (uint32_t)(kBand * ti), in_band = t - band * (uint32_t)(kBand * ti);
+    const uint32_t width = tj - band * kBand < kBand ? tj - band * kBand : kBand;
+    const int64_t i0 = (int64_t)(in_band / width) * TI;
+    const int64_t j0 = (int64_t)(band * kBand + in_band % width) * TJ;
+
+    const Operand P{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, i0};
+    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, j0};
+    const int64_t k_first = (int64_t)split * steps * BK;
+    const int64_t k_end = k_first + steps * BK < g.R ? k_first + steps * BK : g.R;
+
+    const int wave = uniform((int)(threadIdx.x >> 6));
+    const int ri = (wave / WJ) * (TI / WI), rj = (wave % WJ) * (TJ / WJ);
+    f32x4 acc[FI][FJ];
+#pragma unroll
+    for (int x = 0; x < FI; ++x)
+#pragma unroll
+        for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    u32x4 vp[LP::GR], vq[LQ::GR];
+    LP::fetch(P, k_first, k_end, vp);
+    LQ::fetch(Q, k_first, k_end, vq);
+    int buf = 0;
+    for (int64_t k = k_first; k < k_end; k += BK, buf ^= 1) {
+        uint8_t* lp = lds[buf];
+        uint8_t* lq = lp + TI * kStepBytes;
+        LP::put(lp, vp);
+        LQ::put(lq, vq);
+        __syncthreads();
+        if (k + BK < k_end) {
+            LP::fetch(P, k + BK, k_end, vp);
+            LQ::fetch(Q, k + BK, k_end, vq);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            Frag<T> p[FI];
+#pragma unroll
+            for (int x = 0; x < FI; ++x) p[x].set(RP::get(lp, ri, x, s));
+#pragma unroll
+            for (int y = 0; y < FJ; ++y) {
+                Frag<T> q;
+                q.set(RQ::get(lq, rj, y, s));
+#pragma unroll
+                for (int x = 0; x < FI; ++x) acc[x][y] = mma<T>(q, p[x], acc[x][y]);
+            }
+        }
+        // The other buffer is written next; all waves have read it before the
+        // barrier above.
+    }
+
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int x = 0; x < FI; ++x) {
+        const int64_t i = i0 + ri + x * 16 + (lane & 15);
+        if (i >= g.I) continue;
+#pragma unroll
+        for (int y = 0; y < FJ; y += 2) {
+            const int64_t j = j0 + rj + (y >> 1) * 32 + (lane >> 4) * 8;
+            if (j >= g.J) continue;
+            float v[8] = {acc[x][y][0],     acc[x][y][1],     acc[x][y][2],     acc[x][y][3],
+                          acc[x][y + 1][0], acc[x][y + 1][1], acc[x][y + 1][2], acc[x][y + 1][3]};
+            if (splits > 1)
+                store_vec(g.part + ((int64_t)split * g.I + i) * part_ld(g.J) + j, 8, v);
+            else if (g.out_type == VCSR_BF16)
+                finish<bf16>(g, i, (int)j, v);
+            else
+                finish<float>(g, i, (int)j, v);
+        }
+    }
+}
+
+// The partial sums of a split product, added in order, and the epilogue.
+template <class O>
+__global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
+    const int64_t ld = part_ld(g.J), e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = e / (ld / 8);
+    const int j = (int)(e % (ld / 8)) * 8;
+    if (i >= g.I) return;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        float p[8];
+        load_vec(g.part + ((int64_t)s * g.I + i) * ld + j, 8, p);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += p[k];
+    }
+    finish<O>(g, i, j, v);
+}
+
+template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
+hipError_t launch_shape(const Gemm& g, const GemmPlan& p, hipStream_t st) {
+    const int64_t blocks =
+        (g.I + TI - 1) / TI * (((int64_t)g.J + TJ - 1) / TJ) * (int64_t)p.splits;
+    gemm_kernel<T, TI, TJ, WI, WJ, PCOLS, QCOLS>
+        <<<(unsigned)blocks, 64 * WI * WJ, 0, st>>>(g, p.splits, p.steps);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits <= 1) return e;
+    const unsigned join = (unsigned)((g.I * (part_ld(g.J) / 8) + 255) / 256);
+    if (g.out_type == VCSR_BF16)
+        gemm_join_kernel<bf16><<<join, 256, 0, st>>>(g, p.splits);
+    else
+        gemm_join_kernel<float><<<join, 256, 0, st>>>(g, p.splits);
+    return hipGetLastError();
+}
+
+template <class T, bool PCOLS, bool QCOLS>
+hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
+    if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS>(g, p, st);
+    return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS>(g, p, st);
+}
+
+}  // namespace tile
+}  // namespace vcsr
