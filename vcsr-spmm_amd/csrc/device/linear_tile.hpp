@@ -33,6 +33,9 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 
 constexpr int kStepBytes = 128;
+// Bytes a buffer descriptor covers, and an offset past them.
+constexpr int kRange = 0x7fffffff;
+constexpr uint32_t kPast = 0x80000000u;
 
 // Granule keys of tiles by rows, for 16 consecutive rows (P) and for the rows
 // that a block of Q stands for.
@@ -99,6 +102,44 @@ struct Loader {
                     if (i < have) t[i] = p[i];
                 __builtin_memcpy(&v[it], t, 16);
             }
+        }
+    }
+    // Straight to LDS: rows on 16-byte boundaries and whole granules.  off: byte
+    // offset of each of the thread's granules from the tile's first k; a granule
+    // past k_end is asked for beyond the buffer's range, which gives zeros.
+    __device__ static void offsets(const Operand& o, uint32_t (&off)[GR]) {
+#pragma unroll
+        for (int it = 0; it < GR; ++it) {
+            int row, k;
+            place(it * NT + (int)threadIdx.x, row, k);
+            if (COLS) {
+                off[it] = o.first + row < o.n ? (uint32_t)(k * o.ld) + row * (int)sizeof(T) : kPast;
+            } else {  // rows past the last one read it again; their sums go nowhere
+                const int64_t last = o.n - 1 - o.first;
+                off[it] = (uint32_t)((row < last ? row : last) * o.ld) + k * (int)sizeof(T);
+            }
+        }
+    }
+    __device__ static void copy(const Operand& o, const uint32_t (&off)[GR], int64_t k0,
+                                int64_t k_end, lds_byte* lds) {
+        const uint8_t* base =
+            o.p + (COLS ? k0 * o.ld + o.first * (int64_t)sizeof(T)
+                        : o.first * o.ld + k0 * (int64_t)sizeof(T));
+        const __amdgpu_buffer_rsrc_t rsrc =
+            __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kRange, 0x00020000);
+        const int wave = uniform((int)(threadIdx.x >> 6));
+        const int left = k_end - k0 < BK ? (int)(k_end - k0) : BK;
+#pragma unroll
+        for (int it = 0; it < GR; ++it) {
+            uint32_t at = off[it];
+            if (left < BK) {
+                int row, k;
+                place(it * NT + (int)threadIdx.x, row, k);
+                if (k >= left) at = kPast;
+            }
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rsrc, (__attribute__((address_space(3))) void*)(lds + (it * NT + wave * 64) * 16),
+                16, at, 0, 0, 0);
         }
     }
     __device__ static void put(uint8_t* lds, const u32x4 (&v)[GR]) {
@@ -222,41 +263,57 @@ __device__ __forceinline__ f32x4 mma<fp8>(const Frag<fp8>& q, const Frag<fp8>& p
     return acc;
 }
 
-// y, z and the residual of 8 consecutive columns from j of row i.
-template <class O>
-__device__ __forceinline__ void finish(const Gemm& g, int64_t i, int j, float (&v)[8]) {
-    const int n = g.J - j;
+// The epilogue of N consecutive columns from j of row i: scales, bias, z, act,
+// residual, out.
+template <class O, int N>
+__device__ __forceinline__ void finish(const Gemm& g, int64_t i, int j, float (&v)[N]) {
     if (g.p_scale) {
         const float ps = g.p_scale[i];
-        float qs[8];
-        load_vec(g.q_scale + j, n, qs);
+        float qs[N];
+        load_vec(g.q_scale + j, N, qs);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] *= ps * qs[k];
+        for (int k = 0; k < N; ++k) v[k] *= ps * qs[k];
     }
     if (g.bias) {
-        float b[8];
-        load_vec(g.bias + j, n, b);
+        float b[N];
+        load_vec(g.bias + j, N, b);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += b[k];
+        for (int k = 0; k < N; ++k) v[k] += b[k];
     }
-    if (g.z) store_vec((O*)g.z + i * g.ldz + j, n, v);
+    if (g.z) store_vec((O*)g.z + i * g.ldz + j, N, v);
     if (g.act != VCSR_ACT_NONE) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = act_f32(g.act, v[k]);
+        for (int k = 0; k < N; ++k) v[k] = act_f32(g.act, v[k]);
     }
     if (g.residual) {
-        float r[8];
-        load_vec((const O*)g.residual + i * g.ldr + j, n, r);
+        float r[N];
+        load_vec((const O*)g.residual + i * g.ldr + j, N, r);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += r[k];
+        for (int k = 0; k < N; ++k) v[k] += r[k];
     }
-    store_vec((O*)g.out + i * g.ldo + j, n, v);
+    store_vec((O*)g.out + i * g.ldo + j, N, v);
+}
+// Up to 8 columns whose sums lie in LDS or memory.
+template <class O>
+__device__ __forceinline__ void finish_from(const Gemm& g, int64_t i, int j, const float* sums) {
+    if (g.J - j >= 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = sums[k];
+        finish<O>(g, i, j, v);
+    } else {
+#pragma unroll 1
+        for (int k = 0; j + k < g.J; ++k) {
+            float v[1] = {sums[k]};
+            finish<O>(g, i, j + k, v);
+        }
+    }
 }
 
 // Row length of the partial sums: whole vectors of 8.
 __host__ __device__ inline int64_t part_ld(int32_t J) { return ((int64_t)J + 7) / 8 * 8; }
 
-template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
+template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS, bool DMA>
 __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, int64_t steps) {
     constexpr int NT = 64 * WI * WJ;
     constexpr int FI = TI / WI / 16, FJ = TJ / WJ / 16;
@@ -293,20 +350,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
 #pragma unroll
         for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    u32x4 vp[LP::GR], vq[LQ::GR];
-    LP::fetch(P, k_first, k_end, vp);
-    LQ::fetch(Q, k_first, k_end, vq);
-    int buf = 0;
-    for (int64_t k = k_first; k < k_end; k += BK, buf ^= 1) {
-        uint8_t* lp = lds[buf];
-        uint8_t* lq = lp + TI * kStepBytes;
-        LP::put(lp, vp);
-        LQ::put(lq, vq);
-        __syncthreads();
-        if (k + BK < k_end) {
-            LP::fetch(P, k + BK, k_end, vp);
-            LQ::fetch(Q, k + BK, k_end, vq);
-        }
+    auto multiply = [&](const uint8_t* lp, const uint8_t* lq) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             Frag<T> p[FI];
@@ -320,28 +364,83 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
                 for (int x = 0; x < FI; ++x) acc[x][y] = mma<T>(q, p[x], acc[x][y]);
             }
         }
-        // The other buffer is written next; all waves have read it before the
-        // barrier above.
+    };
+    int buf = 0;
+    if constexpr (DMA) {
+        uint32_t op[LP::GR], oq[LQ::GR];
+        LP::offsets(P, op);
+        LQ::offsets(Q, oq);
+        lds_byte* const to = (lds_byte*)&lds[0][0];
+        LP::copy(P, op, k_first, k_end, to);
+        LQ::copy(Q, oq, k_first, k_end, to + TI * kStepBytes);
+        for (int64_t k = k_first; k < k_end; k += BK, buf ^= 1) {
+            // This step's tiles are in LDS, and all waves are done with the
+            // other buffer.
+            __builtin_amdgcn_s_waitcnt(0);
+            __builtin_amdgcn_s_barrier();
+            if (k + BK < k_end) {
+                lds_byte* const next = to + (buf ^ 1) * (TI + TJ) * kStepBytes;
+                LP::copy(P, op, k + BK, k_end, next);
+                LQ::copy(Q, oq, k + BK, k_end, next + TI * kStepBytes);
+            }
+            multiply(lds[buf], lds[buf] + TI * kStepBytes);
+        }
+    } else {
+        u32x4 vp[LP::GR], vq[LQ::GR];
+        LP::fetch(P, k_first, k_end, vp);
+        LQ::fetch(Q, k_first, k_end, vq);
+        for (int64_t k = k_first; k < k_end; k += BK, buf ^= 1) {
+            uint8_t* lp = lds[buf];
+            uint8_t* lq = lp + TI * kStepBytes;
+            LP::put(lp, vp);
+            LQ::put(lq, vq);
+            // All waves have read the buffer that is written next.
+            __syncthreads();
+            if (k + BK < k_end) {
+                LP::fetch(P, k + BK, k_end, vp);
+                LQ::fetch(Q, k + BK, k_end, vq);
+            }
+            multiply(lp, lq);
+        }
     }
 
+    // Epilogue: each wave turns its part round in LDS, a few blocks of rows at a
+    // time, so that its lanes go along rows of out.
+    constexpr int CW = TJ / WJ, LD = CW + 4;  // 4 floats on: rows start in other banks
+    constexpr int ROOM = (int)sizeof(lds) / (WI * WJ) / (16 * LD * 4);  // blocks of 16 rows
+    constexpr int XB = ROOM >= FI ? FI : ROOM >= FI / 2 ? FI / 2 : FI / 4;
+    static_assert(XB >= 1 && FI % XB == 0, "rounds of whole blocks");
     const int lane = threadIdx.x & 63;
+    float* const mine = (float*)&lds[0][0] + wave * (XB * 16 * LD);
+    __syncthreads();
 #pragma unroll
-    for (int x = 0; x < FI; ++x) {
-        const int64_t i = i0 + ri + x * 16 + (lane & 15);
-        if (i >= g.I) continue;
+    for (int r = 0; r < FI; r += XB) {
 #pragma unroll
-        for (int y = 0; y < FJ; y += 2) {
-            const int64_t j = j0 + rj + (y >> 1) * 32 + (lane >> 4) * 8;
-            if (j >= g.J) continue;
-            float v[8] = {acc[x][y][0],     acc[x][y][1],     acc[x][y][2],     acc[x][y][3],
-                          acc[x][y + 1][0], acc[x][y + 1][1], acc[x][y + 1][2], acc[x][y + 1][3]};
-            if (splits > 1)
+        for (int x = 0; x < XB; ++x)
+#pragma unroll
+            for (int y = 0; y < FJ; ++y)
+                *(f32x4*)(mine + (x * 16 + (lane & 15)) * LD + (y >> 1) * 32 + (lane >> 4) * 8 +
+                          (y & 1) * 4) = acc[r + x][y];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int e = lane; e < XB * 16 * (CW / 8); e += 64) {
+            const int row = e / (CW / 8), col = e % (CW / 8) * 8;
+            const int64_t i = i0 + ri + r * 16 + row;
+            const int j = (int)j0 + rj + col;
+            if (i >= g.I || j >= g.J) continue;
+            const float* sums = mine + row * LD + col;
+            if (splits > 1) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = sums[k];
                 store_vec(g.part + ((int64_t)split * g.I + i) * part_ld(g.J) + j, 8, v);
-            else if (g.out_type == VCSR_BF16)
-                finish<bf16>(g, i, (int)j, v);
-            else
-                finish<float>(g, i, (int)j, v);
+            } else if (g.out_type == VCSR_BF16) {
+                finish_from<bf16>(g, i, j, sums);
+            } else {
+                finish_from<float>(g, i, j, sums);
+            }
         }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -359,14 +458,22 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] += p[k];
     }
-    finish<O>(g, i, j, v);
+    if (g.J - j >= 8) {
+        finish<O>(g, i, j, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float one[1] = {v[k]};
+            if (j + k < g.J) finish<O>(g, i, j + k, one);
+        }
+    }
 }
 
-template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
+template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS, bool DMA>
 hipError_t launch_shape(const Gemm& g, const GemmPlan& p, hipStream_t st) {
     const int64_t blocks =
         (g.I + TI - 1) / TI * (((int64_t)g.J + TJ - 1) / TJ) * (int64_t)p.splits;
-    gemm_kernel<T, TI, TJ, WI, WJ, PCOLS, QCOLS>
+    gemm_kernel<T, TI, TJ, WI, WJ, PCOLS, QCOLS, DMA>
         <<<(unsigned)blocks, 64 * WI * WJ, 0, st>>>(g, p.splits, p.steps);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
@@ -380,8 +487,13 @@ hipError_t launch_shape(const Gemm& g, const GemmPlan& p, hipStream_t st) {
 
 template <class T, bool PCOLS, bool QCOLS>
 hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
-    if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS>(g, p, st);
-    return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS>(g, p, st);
+    if (p.dma) {
+        if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS, true>(g, p, st);
+        if (p.tile_i == 128) return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS, true>(g, p, st);
+        return launch_shape<T, 256, 256, 2, 4, PCOLS, QCOLS, true>(g, p, st);
+    }
+    if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS, false>(g, p, st);
+    return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS, false>(g, p, st);
 }
 
 }  // namespace tile
