@@ -183,7 +183,6 @@ size_t gemm_workspace(const Gemm& g);
 // The shapes one kernel takes (chosen by launch_gemm).
 struct GemmPlan {
     int tile_i, tile_j;
-    bool dma;        // operands go from memory to LDS without registers
     int32_t splits;  // of the sum; each writes partial sums
     int64_t steps;   // tile steps of a split
 };

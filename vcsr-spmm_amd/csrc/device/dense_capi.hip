@@ -21,9 +21,9 @@ void range(bool ok, const char* what) {
     if (!ok) throw vcsr::Error(VCSR_ERANGE, what);
 }
 
-// Rows are launched as a grid dimension, and a tile's rows are addressed with
-// 32-bit offsets.
-constexpr int64_t kMaxRows = (int64_t)1 << 31, kMaxLd = (int64_t)1 << 22;
+// Rows are launched as a grid dimension; a product's operand tile, at most 256
+// rows, is addressed with 31-bit byte offsets.
+constexpr int64_t kMaxRows = (int64_t)1 << 31, kOperandLd = (int64_t)1 << 20;
 
 void check_rows(int64_t M) {
     need(M >= 0, "negative M");
@@ -39,8 +39,13 @@ void check_matrix(const void* p, int64_t& ld, int64_t cols, int32_t type, const 
     }
     if (ld == 0) ld = cols;
     need(ld >= cols, what);
-    range(ld <= kMaxLd, what);
+    range(ld <= ((int64_t)1 << 40), what);
     need((uintptr_t)p % size_of(type) == 0, what);
+}
+void check_operand(const void* p, int64_t& ld, int64_t cols, int32_t type, const char* what,
+                   bool optional, int64_t rows) {
+    check_matrix(p, ld, cols, type, what, optional, rows);
+    range(ld <= kOperandLd, what);
 }
 void check_vector(const void* p, const char* what, bool optional = false) {
     need(p || optional, what);
@@ -139,8 +144,8 @@ vcsr::Gemm gemm_of(const vcsr_linear_args& a) {
 }
 vcsr_linear_args checked(const vcsr_linear_args* args) {
     vcsr_linear_args a = checked_sizes(args);
-    check_matrix(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", false, a.M);
-    check_matrix(a.w, a.ldw, a.K, a.x_type, "w: pointer, alignment or stride", false, a.M);
+    check_operand(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", false, a.M);
+    check_operand(a.w, a.ldw, a.K, a.x_type, "w: pointer, alignment or stride", false, a.M);
     const bool scaled = a.x_type == VCSR_FP8;
     need(a.M == 0 || ((a.x_scale != nullptr) == scaled && (a.w_scale != nullptr) == scaled),
          "x_scale, w_scale: given for VCSR_FP8 and only then");
@@ -189,6 +194,7 @@ LinearGrad grad_of(const vcsr_linear_grad_args* args) {
     stride(a.lddx, a.K);
     stride(a.lddw, a.K);
     if (a.M == 0) return w;
+    range(a.N <= kOperandLd && a.K <= kOperandLd, "N, K over 2^20");
     const bool products = a.dx || a.dw;
     w.own_dz = products && (a.act != VCSR_ACT_NONE || a.x_type != a.y_type);
     // Rows of dz on 16-byte boundaries.
@@ -234,11 +240,11 @@ LinearGrad grad_of(const vcsr_linear_grad_args* args) {
 LinearGrad checked(const vcsr_linear_grad_args* args) {
     LinearGrad w = grad_of(args);
     vcsr_linear_grad_args& a = w.a;
-    check_matrix(a.dy, a.lddy, a.N, a.y_type, "dy: pointer, alignment or stride", false, a.M);
+    check_operand(a.dy, a.lddy, a.N, a.y_type, "dy: pointer, alignment or stride", false, a.M);
     check_matrix(a.z, a.ldz, a.N, a.y_type, "z: pointer, alignment or stride",
                  a.act == VCSR_ACT_NONE, a.M);
-    check_matrix(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", !a.dw, a.M);
-    check_matrix(a.w, a.ldw, a.K, a.x_type, "w: pointer, alignment or stride", !a.dx, a.M);
+    check_operand(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", !a.dw, a.M);
+    check_operand(a.w, a.ldw, a.K, a.x_type, "w: pointer, alignment or stride", !a.dx, a.M);
     check_matrix(a.dx, a.lddx, a.K, a.x_type, "dx: alignment or stride", true, a.M);
     check_matrix(a.dw, a.lddw, a.K, a.x_type, "dw: alignment or stride", true, a.M);
     check_vector(a.dbias, "dbias: alignment", true);

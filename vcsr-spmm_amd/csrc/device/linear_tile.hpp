@@ -57,6 +57,7 @@ struct Operand {
     int64_t ld;     // bytes
     int64_t n;      // rows of the operand (i or j)
     int64_t first;  // of the tile
+    int64_t bytes;  // from p to the end of its last row
 };
 
 // One operand's tile loader: NT threads bring ROWS x 128 bytes.  `GR` granules a
@@ -80,8 +81,8 @@ struct Loader {
         }
     }
 
-    // Through registers, any alignment and tail: elements past the operand's
-    // rows or past k_end are zeros.
+    // Through registers, for a step that ends inside its 128 bytes or with the
+    // operand: elements past the operand's rows or past k_end are zeros.
     __device__ static void fetch(const Operand& o, int64_t k0, int64_t k_end, u32x4 (&v)[GR]) {
 #pragma unroll
         for (int it = 0; it < GR; ++it) {
@@ -104,9 +105,10 @@ struct Loader {
             }
         }
     }
-    // Straight to LDS: rows on 16-byte boundaries and whole granules.  off: byte
-    // offset of each of the thread's granules from the tile's first k; a granule
-    // past k_end is asked for beyond the buffer's range, which gives zeros.
+    // Straight to LDS, whole steps only.  The hardware takes any byte address and
+    // checks the range dword by dword.  off: byte offset of each of the thread's
+    // granules from the tile's first k.  By columns, a granule that crosses the
+    // last i goes on into the next k-row: its sums go nowhere.
     __device__ static void offsets(const Operand& o, uint32_t (&off)[GR]) {
 #pragma unroll
         for (int it = 0; it < GR; ++it) {
@@ -114,33 +116,25 @@ struct Loader {
             place(it * NT + (int)threadIdx.x, row, k);
             if (COLS) {
                 off[it] = o.first + row < o.n ? (uint32_t)(k * o.ld) + row * (int)sizeof(T) : kPast;
-            } else {  // rows past the last one read it again; their sums go nowhere
+            } else {  // rows past the last one read it again
                 const int64_t last = o.n - 1 - o.first;
                 off[it] = (uint32_t)((row < last ? row : last) * o.ld) + k * (int)sizeof(T);
             }
         }
     }
     __device__ static void copy(const Operand& o, const uint32_t (&off)[GR], int64_t k0,
-                                int64_t k_end, lds_byte* lds) {
-        const uint8_t* base =
-            o.p + (COLS ? k0 * o.ld + o.first * (int64_t)sizeof(T)
-                        : o.first * o.ld + k0 * (int64_t)sizeof(T));
-        const __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kRange, 0x00020000);
+                                lds_byte* lds) {
+        const int64_t at = COLS ? k0 * o.ld + o.first * (int64_t)sizeof(T)
+                                : o.first * o.ld + k0 * (int64_t)sizeof(T);
+        const int64_t left = o.bytes - at;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(o.p + at), 0, left < kRange ? (int)left : kRange, 0x00020000);
         const int wave = uniform((int)(threadIdx.x >> 6));
-        const int left = k_end - k0 < BK ? (int)(k_end - k0) : BK;
 #pragma unroll
-        for (int it = 0; it < GR; ++it) {
-            uint32_t at = off[it];
-            if (left < BK) {
-                int row, k;
-                place(it * NT + (int)threadIdx.x, row, k);
-                if (k >= left) at = kPast;
-            }
+        for (int it = 0; it < GR; ++it)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 rsrc, (__attribute__((address_space(3))) void*)(lds + (it * NT + wave * 64) * 16),
-                16, at, 0, 0, 0);
-        }
+                16, off[it], 0, 0, 0);
     }
     __device__ static void put(uint8_t* lds, const u32x4 (&v)[GR]) {
 #pragma unroll
@@ -313,7 +307,7 @@ __device__ __forceinline__ void finish_from(const Gemm& g, int64_t i, int j, con
 // Row length of the partial sums: whole vectors of 8.
 __host__ __device__ inline int64_t part_ld(int32_t J) { return ((int64_t)J + 7) / 8 * 8; }
 
-template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS, bool DMA>
+template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
 __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, int64_t steps) {
     constexpr int NT = 64 * WI * WJ;
     constexpr int FI = TI / WI / 16, FJ = TJ / WJ / 16;
@@ -337,8 +331,13 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
     const int64_t i0 = (int64_t)(in_band / width) * TI;
     const int64_t j0 = (int64_t)(band * kBand + in_band % width) * TJ;
 
-    const Operand P{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, i0};
-    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, j0};
+    auto extent = [&](int64_t ld, bool cols, int64_t n) {
+        return ((cols ? g.R - 1 : n - 1) * ld + (cols ? n : g.R)) * (int64_t)sizeof(T);
+    };
+    const Operand P{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, i0,
+                    extent(g.ldp, PCOLS, g.I)};
+    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, j0,
+                    extent(g.ldq, QCOLS, g.J)};
     const int64_t k_first = (int64_t)split * steps * BK;
     const int64_t k_end = k_first + steps * BK < g.R ? k_first + steps * BK : g.R;
 
@@ -365,43 +364,39 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
             }
         }
     };
+    // The sum's last step goes through registers unless its granules are whole.
+    const bool ragged = k_end == g.R && ((g.R % BK) != 0 || (PCOLS && g.I % LP::EPG != 0) ||
+                                         (QCOLS && g.J % LQ::EPG != 0));
+    const int64_t k_full = ragged ? k_first + (k_end - k_first - 1) / BK * BK : k_end;
+    uint32_t op[LP::GR], oq[LQ::GR];
+    LP::offsets(P, op);
+    LQ::offsets(Q, oq);
+    lds_byte* const to = (lds_byte*)&lds[0][0];
     int buf = 0;
-    if constexpr (DMA) {
-        uint32_t op[LP::GR], oq[LQ::GR];
-        LP::offsets(P, op);
-        LQ::offsets(Q, oq);
-        lds_byte* const to = (lds_byte*)&lds[0][0];
-        LP::copy(P, op, k_first, k_end, to);
-        LQ::copy(Q, oq, k_first, k_end, to + TI * kStepBytes);
-        for (int64_t k = k_first; k < k_end; k += BK, buf ^= 1) {
-            // This step's tiles are in LDS, and all waves are done with the
-            // other buffer.
-            __builtin_amdgcn_s_waitcnt(0);
-            __builtin_amdgcn_s_barrier();
-            if (k + BK < k_end) {
-                lds_byte* const next = to + (buf ^ 1) * (TI + TJ) * kStepBytes;
-                LP::copy(P, op, k + BK, k_end, next);
-                LQ::copy(Q, oq, k + BK, k_end, next + TI * kStepBytes);
-            }
-            multiply(lds[buf], lds[buf] + TI * kStepBytes);
+    if (k_first < k_full) {
+        LP::copy(P, op, k_first, to);
+        LQ::copy(Q, oq, k_first, to + TI * kStepBytes);
+    }
+    for (int64_t k = k_first; k < k_full; k += BK, buf ^= 1) {
+        // This step's tiles are in LDS, and all waves are done with the other
+        // buffer.
+        __builtin_amdgcn_s_waitcnt(0);
+        __builtin_amdgcn_s_barrier();
+        if (k + BK < k_full) {
+            lds_byte* const next = to + (buf ^ 1) * (TI + TJ) * kStepBytes;
+            LP::copy(P, op, k + BK, next);
+            LQ::copy(Q, oq, k + BK, next + TI * kStepBytes);
         }
-    } else {
+        multiply(lds[buf], lds[buf] + TI * kStepBytes);
+    }
+    if (ragged) {
         u32x4 vp[LP::GR], vq[LQ::GR];
-        LP::fetch(P, k_first, k_end, vp);
-        LQ::fetch(Q, k_first, k_end, vq);
-        for (int64_t k = k_first; k < k_end; k += BK, buf ^= 1) {
-            uint8_t* lp = lds[buf];
-            uint8_t* lq = lp + TI * kStepBytes;
-            LP::put(lp, vp);
-            LQ::put(lq, vq);
-            // All waves have read the buffer that is written next.
-            __syncthreads();
-            if (k + BK < k_end) {
-                LP::fetch(P, k + BK, k_end, vp);
-                LQ::fetch(Q, k + BK, k_end, vq);
-            }
-            multiply(lp, lq);
-        }
+        LP::fetch(P, k_full, k_end, vp);
+        LQ::fetch(Q, k_full, k_end, vq);
+        LP::put(lds[buf], vp);
+        LQ::put(lds[buf] + TI * kStepBytes, vq);
+        __syncthreads();
+        multiply(lds[buf], lds[buf] + TI * kStepBytes);
     }
 
     // Epilogue: each wave turns its part round in LDS, a few blocks of rows at a
@@ -469,11 +464,11 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
     }
 }
 
-template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS, bool DMA>
+template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
 hipError_t launch_shape(const Gemm& g, const GemmPlan& p, hipStream_t st) {
     const int64_t blocks =
         (g.I + TI - 1) / TI * (((int64_t)g.J + TJ - 1) / TJ) * (int64_t)p.splits;
-    gemm_kernel<T, TI, TJ, WI, WJ, PCOLS, QCOLS, DMA>
+    gemm_kernel<T, TI, TJ, WI, WJ, PCOLS, QCOLS>
         <<<(unsigned)blocks, 64 * WI * WJ, 0, st>>>(g, p.splits, p.steps);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
@@ -487,13 +482,9 @@ hipError_t launch_shape(const Gemm& g, const GemmPlan& p, hipStream_t st) {
 
 template <class T, bool PCOLS, bool QCOLS>
 hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
-    if (p.dma) {
-        if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS, true>(g, p, st);
-        if (p.tile_i == 128) return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS, true>(g, p, st);
-        return launch_shape<T, 256, 256, 2, 4, PCOLS, QCOLS, true>(g, p, st);
-    }
-    if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS, false>(g, p, st);
-    return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS, false>(g, p, st);
+    if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS>(g, p, st);
+    if (p.tile_i == 128) return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS>(g, p, st);
+    return launch_shape<T, 256, 256, 2, 4, PCOLS, QCOLS>(g, p, st);
 }
 
 }  // namespace tile
