@@ -12,7 +12,7 @@ GemmPlan plan_of(const Gemm& g) {
     const int size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
     GemmPlan p{};
     auto tiles = [&](int64_t t) { return (g.I + t - 1) / t * (((int64_t)g.J + t - 1) / t); };
-    p.tile_i = p.tile_j = tiles(256) >= kCus * 3 / 4 ? 256 : tiles(128) >= kCus ? 128 : 64;
+    p.tile_i = p.tile_j = g.type != VCSR_F32 && tiles(256) >= kCus * 3 / 4 ? 256 : tiles(128) >= kCus ? 128 : 64;
     const int64_t all = (g.R * size + tile::kStepBytes - 1) / tile::kStepBytes;
     // Few tiles: the sum is split until the chip has two blocks a compute unit,
     // at least 4 steps each.

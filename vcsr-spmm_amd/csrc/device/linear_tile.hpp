@@ -61,8 +61,9 @@ struct Operand {
 };
 
 // One operand's tile loader: NT threads bring ROWS x 128 bytes.  `GR` granules a
-// thread; granule e = it * NT + tid of the tile lies at e * 16 in LDS.
-template <class T, int ROWS, int NT, bool COLS, bool Q>
+// thread; granule e = it * NT + tid of the tile lies at e * 16 in LDS.  SEG > 0:
+// the tile's rows are runs of SEG rows, 2 * SEG apart.
+template <class T, int ROWS, int NT, bool COLS, bool Q, int SEG = 0>
 struct Loader {
     static constexpr int GR = ROWS * 8 / NT;
     static constexpr int EPG = 16 / (int)sizeof(T);
@@ -79,6 +80,7 @@ struct Loader {
             row = e >> 3;
             k = ((e & 7) ^ key_rows<Q>(row)) * EPG;
         }
+        if (SEG) row += row / (SEG ? SEG : 1) * SEG;
     }
 
     // Through registers, for a step that ends inside its 128 bytes or with the
@@ -307,6 +309,101 @@ __device__ __forceinline__ void finish_from(const Gemm& g, int64_t i, int j, con
 // Row length of the partial sums: whole vectors of 8.
 __host__ __device__ inline int64_t part_ld(int32_t J) { return ((int64_t)J + 7) / 8 * 8; }
 
+// Waits and barriers that nothing is moved across.
+__device__ __forceinline__ void barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// All but the N newest of the wave's loads have arrived (and its LDS writes).
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    if (N == 0)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+constexpr int kAhead = 8;  // loads a wave of gemm_turns_kernel has under way at a wait
+
+// Where block b of a launch works: tile and part of the sum.  Blocks of one XCD
+// take neighbouring tiles, `band` columns of tiles at a time, so that those that
+// run together share Q's rows and a few of P's in its L2.
+struct Place {
+    int64_t i0, j0;
+    uint32_t split;
+};
+template <int TI, int TJ>
+__device__ __forceinline__ Place place_of(const Gemm& g, uint32_t block, uint32_t splits) {
+    constexpr uint32_t kBand = 4;
+    const uint32_t ti = (uint32_t)((g.I + TI - 1) / TI);
+    const uint32_t tj = (uint32_t)(((int64_t)g.J + TJ - 1) / TJ);
+    const uint32_t b = xcd_remap(block, gridDim.x);
+    const uint32_t split = b % splits, t = b / splits;
+    const uint32_t band = t / (kBand * ti), in_band = t - band * (kBand * ti);
+    const uint32_t width = tj - band * kBand < kBand ? tj - band * kBand : kBand;
+    return Place{(int64_t)(in_band / width) * TI, (int64_t)(band * kBand + in_band % width) * TJ,
+                 split};
+}
+
+template <class T>
+__device__ __forceinline__ int64_t extent(int64_t n, int64_t r, int64_t ld, bool cols) {
+    return ((cols ? r - 1 : n - 1) * ld + (cols ? n : r)) * (int64_t)sizeof(T);
+}
+
+// acc of a wave -> out.  Each wave turns its part round in its own LDS room, a
+// few blocks of rows at a time, so that its lanes go along rows of out.
+template <int FI, int FJ, int ROOM>
+__device__ __forceinline__ void write_out(const Gemm& g, f32x4 (&acc)[FI][FJ], float* mine,
+                                          int64_t i_first, int64_t j_first, int splits,
+                                          uint32_t split) {
+    constexpr int CW = FJ * 16, LD = CW + 4;  // 4 floats on: rows start in other banks
+    constexpr int BLOCKS = ROOM / (16 * LD * 4);
+    constexpr int XB = BLOCKS >= FI ? FI : BLOCKS >= FI / 2 ? FI / 2 : BLOCKS >= FI / 4 ? FI / 4 : 1;
+    static_assert(BLOCKS >= 1 && FI % XB == 0, "rounds of whole blocks");
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int r = 0; r < FI; r += XB) {
+#pragma unroll
+        for (int x = 0; x < XB; ++x)
+#pragma unroll
+            for (int y = 0; y < FJ; ++y)
+                *(f32x4*)(mine + (x * 16 + (lane & 15)) * LD + (y >> 1) * 32 + (lane >> 4) * 8 +
+                          (y & 1) * 4) = acc[r + x][y];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int e = lane; e < XB * 16 * (CW / 8); e += 64) {
+            const int row = e / (CW / 8), col = e % (CW / 8) * 8;
+            const int64_t i = i_first + r * 16 + row;
+            const int j = (int)j_first + col;
+            if (i >= g.I || j >= g.J) continue;
+            const float* sums = mine + row * LD + col;
+            if (splits > 1) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = sums[k];
+                store_vec(g.part + ((int64_t)split * g.I + i) * part_ld(g.J) + j, 8, v);
+            } else if (g.out_type == VCSR_BF16) {
+                finish_from<bf16>(g, i, j, sums);
+            } else {
+                finish_from<float>(g, i, j, sums);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Whether the sum's last step goes through registers: its granules are not all
+// whole.
+template <class T>
+__device__ __forceinline__ bool ragged_end(const Gemm& g, int64_t k_end, bool p_cols, bool q_cols) {
+    constexpr int EPG = 16 / (int)sizeof(T), BK = kStepBytes / (int)sizeof(T);
+    return k_end == g.R && ((g.R % BK) != 0 || (p_cols && g.I % EPG != 0) ||
+                            (q_cols && g.J % EPG != 0));
+}
+
+// Tiles whose blocks share a compute unit: a step's loads run under the other
+// blocks' work as well as under the block's own.
 template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
 __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, int64_t steps) {
     constexpr int NT = 64 * WI * WJ;
@@ -319,26 +416,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
     using RQ = Reader<T, TJ, QCOLS, true>;
     __shared__ __attribute__((aligned(128))) uint8_t lds[2][(TI + TJ) * kStepBytes];
 
-    // Blocks of one XCD take neighbouring tiles, down a column of tiles first,
-    // so that they share Q's rows and a few of P's.
-    const int64_t ti = (g.I + TI - 1) / TI;
-    const uint32_t tj = (uint32_t)(((int64_t)g.J + TJ - 1) / TJ);
-    const uint32_t b = xcd_remap(blockIdx.x, gridDim.x);
-    const uint32_t split = b % (uint32_t)splits, t = b / (uint32_t)splits;
-    constexpr uint32_t kBand = 4;  // tile columns taken together
-    const uint32_t band = t / (uint32_t)(kBand * ti), in_band = t - band * (uint32_t)(kBand * ti);
-    const uint32_t width = tj - band * kBand < kBand ? tj - band * kBand : kBand;
-    const int64_t i0 = (int64_t)(in_band / width) * TI;
-    const int64_t j0 = (int64_t)(band * kBand + in_band % width) * TJ;
-
-    auto extent = [&](int64_t ld, bool cols, int64_t n) {
-        return ((cols ? g.R - 1 : n - 1) * ld + (cols ? n : g.R)) * (int64_t)sizeof(T);
-    };
-    const Operand P{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, i0,
-                    extent(g.ldp, PCOLS, g.I)};
-    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, j0,
-                    extent(g.ldq, QCOLS, g.J)};
-    const int64_t k_first = (int64_t)split * steps * BK;
+    const Place at = place_of<TI, TJ>(g, blockIdx.x, (uint32_t)splits);
+    const Operand P{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, at.i0,
+                    extent<T>(g.I, g.R, g.ldp, PCOLS)};
+    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, at.j0,
+                    extent<T>(g.J, g.R, g.ldq, QCOLS)};
+    const int64_t k_first = (int64_t)at.split * steps * BK;
     const int64_t k_end = k_first + steps * BK < g.R ? k_first + steps * BK : g.R;
 
     const int wave = uniform((int)(threadIdx.x >> 6));
@@ -364,9 +447,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
             }
         }
     };
-    // The sum's last step goes through registers unless its granules are whole.
-    const bool ragged = k_end == g.R && ((g.R % BK) != 0 || (PCOLS && g.I % LP::EPG != 0) ||
-                                         (QCOLS && g.J % LQ::EPG != 0));
+    const bool ragged = ragged_end<T>(g, k_end, PCOLS, QCOLS);
     const int64_t k_full = ragged ? k_first + (k_end - k_first - 1) / BK * BK : k_end;
     uint32_t op[LP::GR], oq[LQ::GR];
     LP::offsets(P, op);
@@ -380,8 +461,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
     for (int64_t k = k_first; k < k_full; k += BK, buf ^= 1) {
         // This step's tiles are in LDS, and all waves are done with the other
         // buffer.
-        __builtin_amdgcn_s_waitcnt(0);
-        __builtin_amdgcn_s_barrier();
+        wait_loads<0>();
+        barrier();
         if (k + BK < k_full) {
             lds_byte* const next = to + (buf ^ 1) * (TI + TJ) * kStepBytes;
             LP::copy(P, op, k + BK, next);
@@ -398,45 +479,143 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
         __syncthreads();
         multiply(lds[buf], lds[buf] + TI * kStepBytes);
     }
-
-    // Epilogue: each wave turns its part round in LDS, a few blocks of rows at a
-    // time, so that its lanes go along rows of out.
-    constexpr int CW = TJ / WJ, LD = CW + 4;  // 4 floats on: rows start in other banks
-    constexpr int ROOM = (int)sizeof(lds) / (WI * WJ) / (16 * LD * 4);  // blocks of 16 rows
-    constexpr int XB = ROOM >= FI ? FI : ROOM >= FI / 2 ? FI / 2 : FI / 4;
-    static_assert(XB >= 1 && FI % XB == 0, "rounds of whole blocks");
-    const int lane = threadIdx.x & 63;
-    float* const mine = (float*)&lds[0][0] + wave * (XB * 16 * LD);
     __syncthreads();
+    constexpr int ROOM = (int)sizeof(lds) / (WI * WJ) / 16 * 16;
+    write_out<FI, FJ, ROOM>(g, acc, (float*)(&lds[0][0] + wave * ROOM), at.i0 + ri, at.j0 + rj,
+                            splits, at.split);
+}
+
+// 256 x 256 tiles, eight waves of 128 x 64, one block a compute unit.
+//
+// Two waves a SIMD take turns: while one multiplies, the other brings its next
+// operands from LDS.  A step is four turns of 4 x 4 blocks: the upper 64 rows of
+// the wave's part with both halves of k, then the lower 64.  The barrier before
+// the loop puts waves 4 to 7 half a turn behind, and each half turn ends at a
+// barrier of all waves.
+//
+// LDS holds two steps, each in three pieces: P's upper rows, P's lower rows and
+// Q.  A step's Q and upper P have been read by all waves when those in front
+// begin its third turn, and are asked for again there, two steps on; its lower P
+// at the first turn of the next step.  So every load has six turns (some 3,000
+// clocks of matrix work) to arrive, which covers a miss of L2: asking a step ahead for
+// all of it left 58 of 468 us waiting at 8192 x 8192 x 4096.  Loads end in order:
+// a wave waits until all but the 8 newest have, before its half turn that ends
+// at the barrier behind which the first wave reads them.
+template <class T, bool PCOLS, bool QCOLS>
+__global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int64_t steps) {
+    constexpr int TI = 256, TJ = 256, NT = 512, WJ = 4, FI = 8, FJ = 4, H = 4;
+    constexpr int BK = kStepBytes / (int)sizeof(T);
+    constexpr int kP = TI / 2 * kStepBytes, kStage = (TI + TJ) * kStepBytes;
+    using LP = Loader<T, TI / 2, NT, PCOLS, false, 64>;
+    using LQ = Loader<T, TJ, NT, QCOLS, true>;
+    using RP = Reader<T, TI / 2, PCOLS, false>;
+    using RQ = Reader<T, TJ, QCOLS, true>;
+    __shared__ __attribute__((aligned(128))) uint8_t lds[2 * kStage];
+
+    const Place at = place_of<TI, TJ>(g, blockIdx.x, (uint32_t)splits);
+    Operand P[2];
 #pragma unroll
-    for (int r = 0; r < FI; r += XB) {
+    for (int h = 0; h < 2; ++h)
+        P[h] = Operand{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, at.i0 + h * 64,
+                       extent<T>(g.I, g.R, g.ldp, PCOLS)};
+    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, at.j0,
+                    extent<T>(g.J, g.R, g.ldq, QCOLS)};
+    const int64_t k_first = (int64_t)at.split * steps * BK;
+    const int64_t k_end = k_first + steps * BK < g.R ? k_first + steps * BK : g.R;
+    const bool ragged = ragged_end<T>(g, k_end, PCOLS, QCOLS);
+    const int n = (int)((k_end - k_first - (ragged ? 1 : 0)) / BK);  // whole steps
+
+    const int wave = uniform((int)(threadIdx.x >> 6));
+    const int wi = wave / WJ, wj = wave % WJ;
+    f32x4 acc[FI][FJ];
 #pragma unroll
-        for (int x = 0; x < XB; ++x)
+    for (int x = 0; x < FI; ++x)
 #pragma unroll
-            for (int y = 0; y < FJ; ++y)
-                *(f32x4*)(mine + (x * 16 + (lane & 15)) * LD + (y >> 1) * 32 + (lane >> 4) * 8 +
-                          (y & 1) * 4) = acc[r + x][y];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int e = lane; e < XB * 16 * (CW / 8); e += 64) {
-            const int row = e / (CW / 8), col = e % (CW / 8) * 8;
-            const int64_t i = i0 + ri + r * 16 + row;
-            const int j = (int)j0 + rj + col;
-            if (i >= g.I || j >= g.J) continue;
-            const float* sums = mine + row * LD + col;
-            if (splits > 1) {
-                float v[8];
+        for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    uint32_t op[2][LP::GR], oq[LQ::GR];
+    LP::offsets(P[0], op[0]);
+    LP::offsets(P[1], op[1]);
+    LQ::offsets(Q, oq);
+    lds_byte* const to = (lds_byte*)&lds[0];
+    auto ask_front = [&](int t) {  // Q and upper P of step t
+        lds_byte* const into = to + (t & 1) * kStage;
+        LQ::copy(Q, oq, k_first + (int64_t)t * BK, into + 2 * kP);
+        LP::copy(P[0], op[0], k_first + (int64_t)t * BK, into);
+    };
+    auto ask_back = [&](int t) {  // lower P
+        LP::copy(P[1], op[1], k_first + (int64_t)t * BK, to + (t & 1) * kStage + kP);
+    };
+    if (n > 0) ask_front(0), ask_back(0);
+    if (n > 1) ask_front(1);
+    wait_loads<0>();
+    barrier();
+    if (wi) barrier();
+    for (int t = 0; t < n; ++t) {
+        const uint8_t* const stage = lds + (t & 1) * kStage;
+        Frag<T> p[H], q[2][FJ];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = sums[k];
-                store_vec(g.part + ((int64_t)split * g.I + i) * part_ld(g.J) + j, 8, v);
-            } else if (g.out_type == VCSR_BF16) {
-                finish_from<bf16>(g, i, j, sums);
-            } else {
-                finish_from<float>(g, i, j, sums);
+        for (int turn = 0; turn < 4; ++turn) {
+            const int h = turn >> 1, s = turn & 1;
+            if (h == 0)
+#pragma unroll
+                for (int y = 0; y < FJ; ++y) q[s][y].set(RQ::get(stage + 2 * kP, wj * 64, y, s));
+#pragma unroll
+            for (int x = 0; x < H; ++x) p[x].set(RP::get(stage + h * kP, wi * 64, x, s));
+            if (turn == 0 && t + 1 < n) ask_back(t + 1);
+            if (turn == 2 && t + 2 < n) ask_front(t + 2);
+            if (turn == 1) {  // lower P of this step
+                if (t + 1 < n) wait_loads<kAhead>();
+                else wait_loads<0>();
+            }
+            if (turn == 3) {  // Q and upper P of the next
+                if (t + 2 < n) wait_loads<kAhead>();
+                else wait_loads<0>();
+            }
+            wait_lds();
+            barrier();
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int x = 0; x < H; ++x)
+#pragma unroll
+                for (int y = 0; y < FJ; ++y)
+                    acc[h * H + x][y] = mma<T>(q[s][y], p[x], acc[h * H + x][y]);
+            __builtin_amdgcn_s_setprio(0);
+            barrier();
+        }
+    }
+    if (!wi) barrier();
+    if (ragged) {
+        uint8_t* const stage = lds + (n & 1) * kStage;
+        const int64_t k = k_first + (int64_t)n * BK;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 v[LP::GR];
+            LP::fetch(P[h], k, k_end, v);
+            LP::put(stage + h * kP, v);
+        }
+        u32x4 v[LQ::GR];
+        LQ::fetch(Q, k, k_end, v);
+        LQ::put(stage + 2 * kP, v);
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            Frag<T> q[FJ];
+#pragma unroll
+            for (int y = 0; y < FJ; ++y) q[y].set(RQ::get(stage + 2 * kP, wj * 64, y, s));
+#pragma unroll
+            for (int x = 0; x < FI; ++x) {
+                Frag<T> p;
+                p.set(RP::get(stage + x / H * kP, wi * 64, x % H, s));
+#pragma unroll
+                for (int y = 0; y < FJ; ++y) acc[x][y] = mma<T>(q[y], p, acc[x][y]);
             }
         }
-        __builtin_amdgcn_wave_barrier();
     }
+    __syncthreads();
+    constexpr int ROOM = (int)sizeof(lds) / 8;
+    write_out<FI, FJ, ROOM>(g, acc, (float*)(lds + wave * ROOM), at.i0 + wi * 128, at.j0 + wj * 64,
+                            splits, at.split);
 }
 
 // The partial sums of a split product, added in order, and the epilogue.
@@ -464,12 +643,18 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
     }
 }
 
-template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
-hipError_t launch_shape(const Gemm& g, const GemmPlan& p, hipStream_t st) {
-    const int64_t blocks =
-        (g.I + TI - 1) / TI * (((int64_t)g.J + TJ - 1) / TJ) * (int64_t)p.splits;
-    gemm_kernel<T, TI, TJ, WI, WJ, PCOLS, QCOLS>
-        <<<(unsigned)blocks, 64 * WI * WJ, 0, st>>>(g, p.splits, p.steps);
+template <class T, bool PCOLS, bool QCOLS>
+hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
+    const int64_t blocks = (g.I + p.tile_i - 1) / p.tile_i *
+                           (((int64_t)g.J + p.tile_j - 1) / p.tile_j) * (int64_t)p.splits;
+    if (blocks >= ((int64_t)1 << 31)) return hipErrorInvalidConfiguration;
+    const unsigned n = (unsigned)blocks;
+    if (p.tile_i == 64)
+        gemm_kernel<T, 64, 64, 2, 2, PCOLS, QCOLS><<<n, 256, 0, st>>>(g, p.splits, p.steps);
+    else if (p.tile_i == 128)
+        gemm_kernel<T, 128, 128, 2, 2, PCOLS, QCOLS><<<n, 256, 0, st>>>(g, p.splits, p.steps);
+    else if constexpr (sizeof(T) < 4)
+        gemm_turns_kernel<T, PCOLS, QCOLS><<<n, 512, 0, st>>>(g, p.splits, p.steps);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
     const unsigned join = (unsigned)((g.I * (part_ld(g.J) / 8) + 255) / 256);
@@ -478,13 +663,6 @@ hipError_t launch_shape(const Gemm& g, const GemmPlan& p, hipStream_t st) {
     else
         gemm_join_kernel<float><<<join, 256, 0, st>>>(g, p.splits);
     return hipGetLastError();
-}
-
-template <class T, bool PCOLS, bool QCOLS>
-hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
-    if (p.tile_i == 64) return launch_shape<T, 64, 64, 2, 2, PCOLS, QCOLS>(g, p, st);
-    if (p.tile_i == 128) return launch_shape<T, 128, 128, 2, 2, PCOLS, QCOLS>(g, p, st);
-    return launch_shape<T, 256, 256, 2, 4, PCOLS, QCOLS>(g, p, st);
 }
 
 }  // namespace tile
