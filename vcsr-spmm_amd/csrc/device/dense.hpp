@@ -104,7 +104,11 @@ constexpr float kGelu2 = 1.5957691216f;  // 2 sqrt(2 / pi)
 template <int ACT>
 __device__ __forceinline__ float act_f32(float z) {
     if (ACT == VCSR_ACT_RELU) return z < 0.f ? 0.f : z;  // a NaN stays one
-    if (ACT == VCSR_ACT_GELU) return z * sigmoid_f32(kGelu2 * (z + 0.044715f * z * z * z));
+    if (ACT == VCSR_ACT_GELU)  // -log2(e) kGelu2 (z + 0.044715 z^3) in three operations
+        return z * __builtin_amdgcn_rcpf(
+                       1.f + __builtin_amdgcn_exp2f(
+                                 z * __builtin_fmaf(z * z, -1.44269504f * kGelu2 * 0.044715f,
+                                                    -1.44269504f * kGelu2)));
     if (ACT == VCSR_ACT_SILU) return z * sigmoid_f32(z);
     return z;
 }

@@ -60,6 +60,15 @@ struct Operand {
     int64_t bytes;  // from p to the end of its last row
 };
 
+// v moved down by `bytes` (0 to 15), zeros behind.
+__device__ __forceinline__ u32x4 shift_down(u32x4 v, int bytes) {
+    if (bytes & 8) v = u32x4{v.z, v.w, 0, 0};
+    if (bytes & 4) v = u32x4{v.y, v.z, v.w, 0};
+    const uint32_t b = bytes & 3;
+    return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, b), __builtin_amdgcn_alignbyte(v.z, v.y, b),
+                 __builtin_amdgcn_alignbyte(v.w, v.z, b), __builtin_amdgcn_alignbyte(0, v.w, b)};
+}
+
 // One operand's tile loader: NT threads bring ROWS x 128 bytes.  `GR` granules a
 // thread; granule e = it * NT + tid of the tile lies at e * 16 in LDS.  SEG > 0:
 // the tile's rows are runs of SEG rows, 2 * SEG apart.
@@ -72,7 +81,7 @@ struct Loader {
     static_assert(ROWS * 8 % NT == 0, "whole granules");
 
     // k (relative to the step) and row of the first element of granule e.
-    __device__ static void place(int e, int& row, int& k) {
+    __device__ __forceinline__ static void place(int e, int& row, int& k) {
         if (COLS) {
             k = e / KGRAN;
             row = ((e % KGRAN) ^ key_cols<T, KGRAN>(k)) * EPG;
@@ -84,34 +93,51 @@ struct Loader {
     }
 
     // Through registers, for a step that ends inside its 128 bytes or with the
-    // operand: elements past the operand's rows or past k_end are zeros.
-    __device__ static void fetch(const Operand& o, int64_t k0, int64_t k_end, u32x4 (&v)[GR]) {
+    // operand: elements past the operand's rows or past k_end are zeros.  A
+    // granule that ends outside is read ending at the last element, and shifted;
+    // rows shorter than a granule go element by element.
+    __device__ __forceinline__ static void fetch(const Operand& o, int64_t k0, int64_t k_end,
+                                                 uint8_t* lds) {
+        const int64_t total = COLS ? o.n : k_end;  // elements of a run
+        u32x4 v[GR];
 #pragma unroll
         for (int it = 0; it < GR; ++it) {
             int row, k;
             place(it * NT + (int)threadIdx.x, row, k);
             const int64_t kk = k0 + k, r = o.first + row;
-            const T* p = (const T*)(o.p + (COLS ? kk * o.ld : r * o.ld)) + (COLS ? r : kk);
-            int64_t have = COLS ? o.n - r : k_end - kk;  // elements along the granule
-            if (COLS ? kk >= k_end : r >= o.n) have = 0;
-            if (have >= EPG) {
-                const Mem<T, EPG> m = *(const Mem<T, EPG>*)p;
+            const int64_t run = COLS ? kk : r, pos = COLS ? r : kk;
+            const bool in = (COLS ? kk < k_end : r < o.n) && pos < total;
+            v[it] = u32x4{0, 0, 0, 0};
+            if (in && total >= EPG) {
+                const int back = total - pos < EPG ? (int)(EPG - (total - pos)) : 0;
+                const Mem<T, EPG> m =
+                    *(const Mem<T, EPG>*)((const T*)(o.p + run * o.ld) + (pos - back));
                 __builtin_memcpy(&v[it], &m, 16);
-            } else {
-                T t[EPG];
-                __builtin_memset(t, 0, 16);
-#pragma unroll
-                for (int i = 0; i < EPG; ++i)
-                    if (i < have) t[i] = p[i];
-                __builtin_memcpy(&v[it], t, 16);
+                v[it] = shift_down(v[it], back * (int)sizeof(T));
             }
+        }
+#pragma unroll
+        for (int it = 0; it < GR; ++it)
+            *(u32x4*)(lds + (it * NT + (int)threadIdx.x) * 16) = v[it];
+        if (total >= EPG) return;
+#pragma unroll 1
+        for (int it = 0; it < GR; ++it) {
+            int row, k;
+            place(it * NT + (int)threadIdx.x, row, k);
+            const int64_t kk = k0 + k, r = o.first + row;
+            const int64_t run = COLS ? kk : r, pos = COLS ? r : kk;
+            if (COLS ? kk >= k_end : r >= o.n) continue;
+#pragma unroll 1
+            for (int i = 0; pos + i < total; ++i)
+                ((T*)(lds + (it * NT + (int)threadIdx.x) * 16))[i] =
+                    ((const T*)(o.p + run * o.ld))[pos + i];
         }
     }
     // Straight to LDS, whole steps only.  The hardware takes any byte address and
     // checks the range dword by dword.  off: byte offset of each of the thread's
     // granules from the tile's first k.  By columns, a granule that crosses the
     // last i goes on into the next k-row: its sums go nowhere.
-    __device__ static void offsets(const Operand& o, uint32_t (&off)[GR]) {
+    __device__ __forceinline__ static void offsets(const Operand& o, uint32_t (&off)[GR]) {
 #pragma unroll
         for (int it = 0; it < GR; ++it) {
             int row, k;
@@ -124,8 +150,8 @@ struct Loader {
             }
         }
     }
-    __device__ static void copy(const Operand& o, const uint32_t (&off)[GR], int64_t k0,
-                                lds_byte* lds) {
+    __device__ __forceinline__ static void copy(const Operand& o, const uint32_t (&off)[GR],
+                                                int64_t k0, lds_byte* lds) {
         const int64_t at = COLS ? k0 * o.ld + o.first * (int64_t)sizeof(T)
                                 : o.first * o.ld + k0 * (int64_t)sizeof(T);
         const int64_t left = o.bytes - at;
@@ -137,11 +163,6 @@ struct Loader {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 rsrc, (__attribute__((address_space(3))) void*)(lds + (it * NT + wave * 64) * 16),
                 16, off[it], 0, 0, 0);
-    }
-    __device__ static void put(uint8_t* lds, const u32x4 (&v)[GR]) {
-#pragma unroll
-        for (int it = 0; it < GR; ++it)
-            *(u32x4*)(lds + (it * NT + (int)threadIdx.x) * 16) = v[it];
     }
 };
 
@@ -158,7 +179,7 @@ __device__ __forceinline__ int tile_row(int r0, int b, int a) {
 
 template <class T, int ROWS, bool Q>
 struct Reader<T, ROWS, false, Q> {
-    __device__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
+    __device__ __forceinline__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
         const int lane = threadIdx.x & 63;
         const int r = tile_row<Q>(r0, b, lane & 15);
         const int g = (lane >> 4) + 4 * s;
@@ -169,7 +190,7 @@ struct Reader<T, ROWS, false, Q> {
 // k-rows (lane t addresses 4 consecutive i of k-row t / 4).
 template <int ROWS, bool Q>
 struct Reader<bf16, ROWS, true, Q> {
-    __device__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
+    __device__ __forceinline__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
         constexpr int GRAN = ROWS * 2 / 16;
         const int lane = threadIdx.x & 63, t = lane & 15;
         const int col = tile_row<Q>(r0, b, (t & 3) * 4);  // 4 consecutive ones from here
@@ -188,7 +209,7 @@ struct Reader<bf16, ROWS, true, Q> {
 };
 template <int ROWS, bool Q>
 struct Reader<float, ROWS, true, Q> {
-    __device__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
+    __device__ __forceinline__ static u32x4 get(const uint8_t* lds, int r0, int b, int s) {
         constexpr int GRAN = ROWS * 4 / 16;
         const int lane = threadIdx.x & 63;
         const int col = tile_row<Q>(r0, b, lane & 15);
@@ -289,20 +310,13 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t i, int j, float (&
     }
     store_vec((O*)g.out + i * g.ldo + j, N, v);
 }
-// Up to 8 columns whose sums lie in LDS or memory.
+// The last columns of row i, fewer than 8 from j, whose sums lie in LDS.
 template <class O>
-__device__ __forceinline__ void finish_from(const Gemm& g, int64_t i, int j, const float* sums) {
-    if (g.J - j >= 8) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = sums[k];
-        finish<O>(g, i, j, v);
-    } else {
+__device__ __forceinline__ void finish_tail(const Gemm& g, int64_t i, int j, const float* sums) {
 #pragma unroll 1
-        for (int k = 0; j + k < g.J; ++k) {
-            float v[1] = {sums[k]};
-            finish<O>(g, i, j + k, v);
-        }
+    for (int k = 0; j + k < g.J; ++k) {
+        float v[1] = {sums[k]};
+        finish<O>(g, i, j + k, v);
     }
 }
 
@@ -352,16 +366,27 @@ __device__ __forceinline__ int64_t extent(int64_t n, int64_t r, int64_t ld, bool
 }
 
 // acc of a wave -> out.  Each wave turns its part round in its own LDS room, a
-// few blocks of rows at a time, so that its lanes go along rows of out.
-template <int FI, int FJ, int ROOM>
-__device__ __forceinline__ void write_out(const Gemm& g, f32x4 (&acc)[FI][FJ], float* mine,
-                                          int64_t i_first, int64_t j_first, int splits,
-                                          uint32_t split) {
+// few blocks of rows at a time, so that its lanes go along rows of out: 8
+// consecutive columns a lane, the same ones in every row.  (Stores straight from
+// the matrix layout write half lines: 70 against 65 us for 8192 x 8192 at K = 128.)
+// PLAIN: out alone, as the gradients need it.
+template <class O, int ACT, bool PLAIN, bool PART, int FI, int FJ, int ROOM>
+__device__ __forceinline__ void write_rows(const Gemm& g, const f32x4 (&acc)[FI][FJ], float* mine,
+                                           int64_t i_first, int64_t j_first, uint32_t split) {
     constexpr int CW = FJ * 16, LD = CW + 4;  // 4 floats on: rows start in other banks
     constexpr int BLOCKS = ROOM / (16 * LD * 4);
     constexpr int XB = BLOCKS >= FI ? FI : BLOCKS >= FI / 2 ? FI / 2 : BLOCKS >= FI / 4 ? FI / 4 : 1;
-    static_assert(BLOCKS >= 1 && FI % XB == 0, "rounds of whole blocks");
+    constexpr int LANES = CW / 8;  // of a row
+    static_assert(BLOCKS >= 1 && FI % XB == 0 && 64 % LANES == 0, "rounds of whole blocks");
     const int lane = threadIdx.x & 63;
+    const int col = lane % LANES * 8;
+    const int64_t j = j_first + col;
+    const int n = g.J - j < 8 ? (int)(g.J - j) : 8;
+    float bias[8], scale[8];
+    if (!PLAIN && !PART && n == 8) {
+        if (g.bias) load_vec(g.bias + j, 8, bias);
+        if (g.q_scale) load_vec(g.q_scale + j, 8, scale);
+    }
 #pragma unroll
     for (int r = 0; r < FI; r += XB) {
 #pragma unroll
@@ -371,26 +396,73 @@ __device__ __forceinline__ void write_out(const Gemm& g, f32x4 (&acc)[FI][FJ], f
                 *(f32x4*)(mine + (x * 16 + (lane & 15)) * LD + (y >> 1) * 32 + (lane >> 4) * 8 +
                           (y & 1) * 4) = acc[r + x][y];
         __builtin_amdgcn_wave_barrier();
+        if (!PART && n > 0 && n < 8) {
 #pragma unroll 1
-        for (int e = lane; e < XB * 16 * (CW / 8); e += 64) {
-            const int row = e / (CW / 8), col = e % (CW / 8) * 8;
-            const int64_t i = i_first + r * 16 + row;
-            const int j = (int)j_first + col;
-            if (i >= g.I || j >= g.J) continue;
-            const float* sums = mine + row * LD + col;
-            if (splits > 1) {
+            for (int row = lane / LANES; row < XB * 16; row += 64 / LANES) {
+                const int64_t i = i_first + r * 16 + row;
+                if (i < g.I) finish_tail<O>(g, i, (int)j, mine + row * LD + col);
+            }
+        } else if (n > 0) {
+#pragma unroll
+            for (int step = 0; step < XB * 16 * LANES / 64; ++step) {
+                const int row = step * (64 / LANES) + lane / LANES;
+                const int64_t i = i_first + r * 16 + row;
+                if (i >= g.I) continue;
+                const float* sums = mine + row * LD + col;
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = sums[k];
-                store_vec(g.part + ((int64_t)split * g.I + i) * part_ld(g.J) + j, 8, v);
-            } else if (g.out_type == VCSR_BF16) {
-                finish_from<bf16>(g, i, j, sums);
-            } else {
-                finish_from<float>(g, i, j, sums);
+                if (PART) {
+                    store_vec(g.part + ((int64_t)split * g.I + i) * part_ld(g.J) + j, 8, v);
+                    continue;
+                }
+                if (!PLAIN) {
+                    if (g.p_scale) {
+                        const float ps = g.p_scale[i];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] *= ps * scale[k];
+                    }
+                    if (g.bias) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] += bias[k];
+                    }
+                    if (g.z) store_vec((O*)g.z + i * g.ldz + j, 8, v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = act_f32<ACT>(v[k]);
+                    if (g.residual) {
+                        float res[8];
+                        load_vec((const O*)g.residual + i * g.ldr + j, 8, res);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] += res[k];
+                    }
+                }
+                store_vec((O*)g.out + i * g.ldo + j, 8, v);
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
+}
+template <class O, bool PLAIN, int ROOM, int FI, int FJ>
+__device__ __forceinline__ void write_typed(const Gemm& g, const f32x4 (&acc)[FI][FJ], float* mine,
+                                            int64_t i, int64_t j) {
+    if (PLAIN || g.act == VCSR_ACT_NONE)
+        write_rows<O, VCSR_ACT_NONE, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+    else if (g.act == VCSR_ACT_RELU)
+        write_rows<O, VCSR_ACT_RELU, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+    else if (g.act == VCSR_ACT_GELU)
+        write_rows<O, VCSR_ACT_GELU, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+    else
+        write_rows<O, VCSR_ACT_SILU, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+}
+template <bool PLAIN, int ROOM, int FI, int FJ>
+__device__ __forceinline__ void write_out(const Gemm& g, const f32x4 (&acc)[FI][FJ], float* mine,
+                                          int64_t i, int64_t j, int splits, uint32_t split) {
+    if (splits > 1)
+        write_rows<float, VCSR_ACT_NONE, true, true, FI, FJ, ROOM>(g, acc, mine, i, j, split);
+    else if (g.out_type == VCSR_BF16)
+        write_typed<bf16, PLAIN, ROOM>(g, acc, mine, i, j);
+    else
+        write_typed<float, PLAIN, ROOM>(g, acc, mine, i, j);
 }
 
 // Whether the sum's last step goes through registers: its granules are not all
@@ -471,18 +543,15 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
         multiply(lds[buf], lds[buf] + TI * kStepBytes);
     }
     if (ragged) {
-        u32x4 vp[LP::GR], vq[LQ::GR];
-        LP::fetch(P, k_full, k_end, vp);
-        LQ::fetch(Q, k_full, k_end, vq);
-        LP::put(lds[buf], vp);
-        LQ::put(lds[buf] + TI * kStepBytes, vq);
+        LP::fetch(P, k_full, k_end, lds[buf]);
+        LQ::fetch(Q, k_full, k_end, lds[buf] + TI * kStepBytes);
         __syncthreads();
         multiply(lds[buf], lds[buf] + TI * kStepBytes);
     }
     __syncthreads();
     constexpr int ROOM = (int)sizeof(lds) / (WI * WJ) / 16 * 16;
-    write_out<FI, FJ, ROOM>(g, acc, (float*)(&lds[0][0] + wave * ROOM), at.i0 + ri, at.j0 + rj,
-                            splits, at.split);
+    write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(&lds[0][0] + wave * ROOM), at.i0 + ri,
+                                    at.j0 + rj, splits, at.split);
 }
 
 // 256 x 256 tiles, eight waves of 128 x 64, one block a compute unit.
@@ -588,15 +657,9 @@ __global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int
     if (ragged) {
         uint8_t* const stage = lds + (n & 1) * kStage;
         const int64_t k = k_first + (int64_t)n * BK;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4 v[LP::GR];
-            LP::fetch(P[h], k, k_end, v);
-            LP::put(stage + h * kP, v);
-        }
-        u32x4 v[LQ::GR];
-        LQ::fetch(Q, k, k_end, v);
-        LQ::put(stage + 2 * kP, v);
+        LP::fetch(P[0], k, k_end, stage);
+        LP::fetch(P[1], k, k_end, stage + kP);
+        LQ::fetch(Q, k, k_end, stage + 2 * kP);
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -614,8 +677,8 @@ __global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int
     }
     __syncthreads();
     constexpr int ROOM = (int)sizeof(lds) / 8;
-    write_out<FI, FJ, ROOM>(g, acc, (float*)(lds + wave * ROOM), at.i0 + wi * 128, at.j0 + wj * 64,
-                            splits, at.split);
+    write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(lds + wave * ROOM), at.i0 + wi * 128,
+                                    at.j0 + wj * 64, splits, at.split);
 }
 
 // The partial sums of a split product, added in order, and the epilogue.
