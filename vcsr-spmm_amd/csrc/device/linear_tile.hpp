@@ -33,6 +33,7 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 
 constexpr int kStepBytes = 128;
+constexpr int64_t kCus = 256;  // compute units
 // Bytes a buffer descriptor covers, and an offset past them.
 constexpr int kRange = 0x7fffffff;
 constexpr uint32_t kPast = 0x80000000u;
@@ -144,9 +145,11 @@ struct Loader {
             place(it * NT + (int)threadIdx.x, row, k);
             if (COLS) {
                 off[it] = o.first + row < o.n ? (uint32_t)(k * o.ld) + row * (int)sizeof(T) : kPast;
-            } else {  // rows past the last one read it again
+            } else {  // rows past the last one read it again, or zeros where the tile has none
                 const int64_t last = o.n - 1 - o.first;
-                off[it] = (uint32_t)((row < last ? row : last) * o.ld) + k * (int)sizeof(T);
+                off[it] = last < 0 ? kPast
+                                   : (uint32_t)((row < last ? row : last) * o.ld) +
+                                         k * (int)sizeof(T);
             }
         }
     }
@@ -154,9 +157,9 @@ struct Loader {
                                                 int64_t k0, lds_byte* lds) {
         const int64_t at = COLS ? k0 * o.ld + o.first * (int64_t)sizeof(T)
                                 : o.first * o.ld + k0 * (int64_t)sizeof(T);
-        const int64_t left = o.bytes - at;
+        const int64_t left = o.bytes - at;  // the descriptor's range is unsigned: none is 0
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(o.p + at), 0, left < kRange ? (int)left : kRange, 0x00020000);
+            (void*)(o.p + at), 0, left < 0 ? 0 : left < kRange ? (int)left : kRange, 0x00020000);
         const int wave = uniform((int)(threadIdx.x >> 6));
 #pragma unroll
         for (int it = 0; it < GR; ++it)
