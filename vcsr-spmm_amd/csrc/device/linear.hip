@@ -37,6 +37,11 @@ GemmPlan plan_of(const Gemm& g) {
     const TileCost* costs = g.type == VCSR_F32 ? kF32 : g.type == VCSR_BF16 ? kBf16 : kFp8;
     const int n_costs = g.type == VCSR_F32 ? 2 : 3;
     const int64_t all = (g.R * size + tile::kStepBytes - 1) / tile::kStepBytes;
+    // Up to 8 rows: W is read straight into the matrix layout, 6 to 9 us up to 32 MB of
+    // it against 10 of the tiles (their join is a launch of its own).  Not where
+    // few blocks would read long rows alone: 512 x 8000 bf16 16 us against 10.
+    if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || 16 * g.R * size <= 192 << 10))
+        return GemmPlan{16, 16, 1, all};
     GemmPlan best{};
     float best_us = 0.f;
     for (int c = 0; c < n_costs; ++c) {

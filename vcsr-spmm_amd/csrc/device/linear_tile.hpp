@@ -684,14 +684,18 @@ __global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int
                                     at.j0 + wj * 64, splits, at.split);
 }
 
-// The partial sums of a split product, added in order, and the epilogue.
+// The partial sums of a split product and the epilogue, for few parts: a thread
+// adds those of 8 columns in order.
 template <class O>
-__global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
-    const int64_t ld = part_ld(g.J), e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t i = e / (ld / 8);
-    const int j = (int)(e % (ld / 8)) * 8;
+__global__ __launch_bounds__(256) void gemm_join_few_kernel(Gemm g, int splits) {
+    const int64_t ld = part_ld(g.J);
+    const uint32_t per_row = (uint32_t)(ld / 8);
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = e / per_row;
+    const int j = (int)(e - i * per_row) * 8;
     if (i >= g.I) return;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
         float p[8];
         load_vec(g.part + ((int64_t)s * g.I + i) * ld + j, 8, p);
@@ -709,8 +713,153 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
     }
 }
 
+// For many parts (from 8): a block takes 32 vectors of 8 columns; 8 threads a vector add every eighth part, then LDS adds the
+// eight in order: with few columns of out the parts' loads are what there is to
+// run at once.
+template <class O>
+__global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
+    __shared__ float lds[8][32][9];
+    const int64_t ld = part_ld(g.J);
+    const uint32_t per_row = (uint32_t)(ld / 8);
+    const int at = threadIdx.x & 31, grp = threadIdx.x >> 5;
+    const int64_t e = (int64_t)blockIdx.x * 32 + at;
+    const int64_t i = e / per_row;
+    const int j = (int)(e - i * per_row) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (i < g.I) {
+#pragma unroll 4
+        for (int s = grp; s < splits; s += 8) {
+            float p[8];
+            load_vec(g.part + ((int64_t)s * g.I + i) * ld + j, 8, p);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] += p[k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) lds[grp][at][k] = v[k];
+    __syncthreads();
+    // One column a thread from here.
+    const int col = threadIdx.x & 7;
+    const int64_t f = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+    const int64_t row = f / per_row;
+    const int c = (int)(f - row * per_row) * 8 + col;
+    if (row >= g.I || c >= g.J) return;
+    float sum[1] = {lds[0][threadIdx.x >> 3][col]};
+#pragma unroll
+    for (int q = 1; q < 8; ++q) sum[0] += lds[q][threadIdx.x >> 3][col];
+    finish<O>(g, row, c, sum);
+}
+
+// One granule of a run of `total` elements from `pos`, zeros past its end; every
+// element by itself where the run is shorter than a granule.
+template <class T>
+__device__ __forceinline__ u32x4 load_granule(const T* run, int64_t pos, int64_t total) {
+    constexpr int EPG = 16 / (int)sizeof(T);
+    u32x4 v{0, 0, 0, 0};
+    if (pos >= total) return v;
+    if (total >= EPG) {
+        const int back = total - pos < EPG ? (int)(EPG - (total - pos)) : 0;
+        const Mem<T, EPG> m = *(const Mem<T, EPG>*)(run + (pos - back));
+        __builtin_memcpy(&v, &m, 16);
+        return shift_down(v, back * (int)sizeof(T));
+    }
+    T t[EPG];
+    __builtin_memset(t, 0, 16);
+#pragma unroll
+    for (int i = 0; i < EPG; ++i)
+        if (pos + i < total) t[i] = run[pos + i];
+    __builtin_memcpy(&v, t, 16);
+    return v;
+}
+
+// Few rows of x (at most 16): what takes time is reading W once.  A block takes
+// 16 rows of W; its 8 waves take its 128-byte lines in turn, UN lines of every
+// row asked for at once and straight from memory into the matrix layout (all of a
+// 4096-wide bf16 row, so that the chip has the whole W under way).  The waves'
+// sums meet in LDS and are added in order: one launch, no partial sums in memory.
+template <class T, class O, int UN>
+__global__ __launch_bounds__(512) void gemm_rows_kernel(Gemm g) {
+    constexpr int EPG = 16 / (int)sizeof(T), WAVES = 8;
+    __shared__ __attribute__((aligned(16))) float lds[WAVES][16][20];
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    const int64_t j0 = (int64_t)blockIdx.x * 16;
+    const int64_t jr = j0 + (lane & 15) < g.J ? j0 + (lane & 15) : g.J - 1;
+    const int64_t i = lane & 15;
+    const T* const w = (const T*)g.q + jr * g.ldq;
+    const T* const x = (const T*)g.p + (i < g.I ? i : 0) * g.ldp;
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    const int64_t lines = (g.R + EPG * 8 - 1) / (EPG * 8);
+    for (int64_t l0 = wave; l0 < lines; l0 += WAVES * UN) {
+        u32x4 q[UN][2], p[UN][2];
+        auto at = [&](int u, int h) { return ((l0 + WAVES * u) * 8 + h * 4 + (lane >> 4)) * EPG; };
+        if ((l0 + WAVES * (UN - 1) + 1) * EPG * 8 <= g.R) {
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const Mem<T, EPG> m = *(const Mem<T, EPG>*)(w + at(u, h));
+                    __builtin_memcpy(&q[u][h], &m, 16);
+                }
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    p[u][h] = u32x4{0, 0, 0, 0};
+                    if (i < g.I) {
+                        const Mem<T, EPG> m = *(const Mem<T, EPG>*)(x + at(u, h));
+                        __builtin_memcpy(&p[u][h], &m, 16);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    q[u][h] = load_granule(w, at(u, h), g.R);
+                    p[u][h] = u32x4{0, 0, 0, 0};
+                    if (i < g.I) p[u][h] = load_granule(x, at(u, h), g.R);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                Frag<T> a, b;
+                a.set(q[u][h]);
+                b.set(p[u][h]);
+                acc = mma<T>(a, b, acc);
+            }
+    }
+    *(f32x4*)&lds[wave][lane & 15][(lane >> 4) * 4] = acc;
+    __syncthreads();
+    const int row = threadIdx.x >> 4, col = threadIdx.x & 15;
+    if (row >= 16 || row >= g.I || j0 + col >= g.J) return;
+    float sum[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) sum[0] += lds[k][row][col];
+    finish<O>(g, row, (int)j0 + col, sum);
+}
+
+template <class T, class O>
+hipError_t launch_rows(const Gemm& g, hipStream_t st) {
+    const unsigned blocks = (unsigned)(((int64_t)g.J + 15) / 16);
+    const int64_t lines = (g.R * (int64_t)sizeof(T) + 127) / 128;
+    if (lines <= 16)
+        gemm_rows_kernel<T, O, 2><<<blocks, 512, 0, st>>>(g);
+    else if (lines <= 32)
+        gemm_rows_kernel<T, O, 4><<<blocks, 512, 0, st>>>(g);
+    else
+        gemm_rows_kernel<T, O, 8><<<blocks, 512, 0, st>>>(g);
+    return hipGetLastError();
+}
+
 template <class T, bool PCOLS, bool QCOLS>
 hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
+    if constexpr (!PCOLS && !QCOLS) {
+        if (p.tile_i == 16)
+            return g.out_type == VCSR_BF16 ? launch_rows<T, bf16>(g, st)
+                                           : launch_rows<T, float>(g, st);
+    }
     const int64_t blocks = (g.I + p.tile_i - 1) / p.tile_i *
                            (((int64_t)g.J + p.tile_j - 1) / p.tile_j) * (int64_t)p.splits;
     if (blocks >= ((int64_t)1 << 31)) return hipErrorInvalidConfiguration;
@@ -723,11 +872,19 @@ hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
         gemm_turns_kernel<T, PCOLS, QCOLS><<<n, 512, 0, st>>>(g, p.splits, p.steps);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits <= 1) return e;
-    const unsigned join = (unsigned)((g.I * (part_ld(g.J) / 8) + 255) / 256);
-    if (g.out_type == VCSR_BF16)
-        gemm_join_kernel<bf16><<<join, 256, 0, st>>>(g, p.splits);
-    else
-        gemm_join_kernel<float><<<join, 256, 0, st>>>(g, p.splits);
+    const int64_t vectors = g.I * (part_ld(g.J) / 8);
+    const unsigned few = (unsigned)((vectors + 255) / 256), many = (unsigned)((vectors + 31) / 32);
+    if (g.out_type == VCSR_BF16) {
+        if (p.splits < 8)
+            gemm_join_few_kernel<bf16><<<few, 256, 0, st>>>(g, p.splits);
+        else
+            gemm_join_kernel<bf16><<<many, 256, 0, st>>>(g, p.splits);
+    } else {
+        if (p.splits < 8)
+            gemm_join_few_kernel<float><<<few, 256, 0, st>>>(g, p.splits);
+        else
+            gemm_join_kernel<float><<<many, 256, 0, st>>>(g, p.splits);
+    }
     return hipGetLastError();
 }
 
