@@ -61,6 +61,32 @@ __device__ __forceinline__ void load_vec(const T* p, int n, float (&v)[N]) {
         for (int i = 0; i < N; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
     }
 }
+// The same for the values [c, c + N) of a row of C >= N values, without branches
+// that would keep loads from being under way together: past the row's end, the
+// row's last N values moved down (none for c >= C).
+template <class T, int N>
+__device__ __forceinline__ void load_tail(const T* row, int c, int C, float (&v)[N]) {
+    const int back = c + N > C ? c + N - C : 0;
+    const Mem<T, N> m = *(const Mem<T, N>*)(row + (back < N ? c - back : 0));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32(m.v[i]);
+#pragma unroll
+    for (int s = 1; s < N; s <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float next = i + s < N ? v[i + s < N ? i + s : i] : 0.f;
+            v[i] = back & s ? next : v[i];
+        }
+    if (back >= N)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.f;
+}
+template <class T, int N>
+__device__ __forceinline__ void load_full(const T* p, float (&v)[N]) {
+    const Mem<T, N> m = *(const Mem<T, N>*)p;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32(m.v[i]);
+}
 // The first n <= N values of v to p, rounded to nearest even.
 template <class T, int N>
 __device__ __forceinline__ void store_vec(T* p, int n, const float (&v)[N]) {
@@ -197,7 +223,7 @@ hipError_t launch_gemm_fp8(const Gemm& g, const GemmPlan& p, hipStream_t st);
 // --------------------------------------------------------------- adamw.hip
 // One chunk of a tensor is kAdamwChunk values, a block's work.
 constexpr int32_t kAdamwBlock = 256;
-constexpr int32_t kAdamwChunk = 4096;
+constexpr int32_t kAdamwChunk = 2048;
 struct AdamwStep {  // a step's constants, rounded once from 64 bits
     float beta1, one_minus_beta1, beta2, one_minus_beta2, lr_over_bias1, inv_root_bias2, eps,
         grad_scale;

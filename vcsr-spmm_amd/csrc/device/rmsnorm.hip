@@ -8,6 +8,8 @@
 // h)); again one pass, the row's s and dy in registers.  dweight sums dy * h
 // over the rows a block takes in registers, then over the blocks (colsum.hip),
 // in a fixed order.  All of it is bound by memory.
+#include <type_traits>
+
 #include "dense.hpp"
 #include "launch.hpp"
 
@@ -61,8 +63,7 @@ __device__ __forceinline__ float row_factor(float rstd, float top, float* y_scal
     return scale;
 }
 
-// y's values of one vector.  8 bits: t * rstd * w / scale, where the largest
-// magnitude may come out a rounding over 448 and still rounds to it.
+// y's values of one vector.
 template <class Y, int V>
 __device__ __forceinline__ void write_y(Y* p, int n, const float (&t)[V], const float (&w)[V],
                                         float rstd, float scale) {
@@ -75,78 +76,82 @@ __device__ __forceinline__ void write_y(Y* p, int n, const float (&t)[V], const 
     store_vec(p, n, y);
 }
 
-// Rows of at most NV * LANES vectors, held in registers.  WAVES = 1: groups of
-// `lanes` <= 64 lanes take a row each; WAVES > 1: a block takes a row.
-template <class X, class Y, int WAVES, int NV>
-__global__ __launch_bounds__(256) void rmsnorm_kernel(vcsr_rmsnorm_args a, int lanes) {
-    constexpr int V = kVec<X>;
-    __shared__ float lds[2 * WAVES];
-    const int tid = threadIdx.x;
-    const int lane = WAVES > 1 ? tid : tid & (lanes - 1);
-    const int stride = WAVES > 1 ? 64 * WAVES : lanes;
-    const int64_t row = WAVES > 1 ? (int64_t)blockIdx.x
-                                  : (int64_t)blockIdx.x * (256 / lanes) + tid / lanes;
-    const bool live = row < a.M;  // lanes past the last row still take part in the shuffles
-    float t[NV][V];
-    float sum = 0.f, top = 0.f;
-    if (live) {
-        const X* x = (const X*)a.x + row * a.ldx;
+// A lane's NV vectors of a row of C >= V values: all but the last are whole.
+template <class T, int NV, int V>
+__device__ __forceinline__ void load_row(const T* row, int lane, int stride, int C,
+                                         float (&v)[NV][V]) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * stride + lane) * V;
-            load_vec(x + c, c < a.C ? a.C - c : 0, t[k]);
-        }
-        if (a.residual) {
-            const X* r = (const X*)a.residual + row * a.ldr;
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c = (k * stride + lane) * V;
-                float v[V];
-                load_vec(r + c, c < a.C ? a.C - c : 0, v);
-#pragma unroll
-                for (int i = 0; i < V; ++i) t[k][i] += v[i];
-            }
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int i = 0; i < V; ++i) t[k][i] = 0.f;
-    }
-    float w[NV][V];
+    for (int k = 0; k + 1 < NV; ++k) load_full(row + (k * stride + lane) * V, v[k]);
+    load_tail(row, ((NV - 1) * stride + lane) * V, C, v[NV - 1]);
+}
+template <class T, int NV, int V>
+__device__ __forceinline__ void store_row(T* row, int lane, int stride, int C,
+                                          const float (&v)[NV][V]) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = (k * stride + lane) * V;
-        load_vec(a.weight + c, c < a.C ? a.C - c : 0, w[k]);
+        if (k + 1 < NV)
+            store_vec(row + c, V, v[k]);
+        else if (c < C)
+            store_vec(row + c, C - c, v[k]);
+    }
+}
+
+// Rows of at most NV * 64 * WPR vectors, held in registers.  WPR = 1: groups of
+// `lanes` (a power of two <= 64) lanes of a 256-thread block take a row each; WPR >
+// 1: a block of WPR waves takes a row.
+template <class X, class Y, int WPR, int NV>
+__global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_kernel(vcsr_rmsnorm_args a,
+                                                                           int lanes) {
+    constexpr int V = kVec<X>;
+    __shared__ float lds[2 * WPR];
+    const int tid = threadIdx.x;
+    const int lane = WPR > 1 ? tid : tid & (lanes - 1);
+    const int stride = WPR > 1 ? 64 * WPR : lanes;
+    const int64_t row = WPR > 1 ? (int64_t)blockIdx.x
+                                : (int64_t)blockIdx.x * (256 / lanes) + tid / lanes;
+    const bool live = row < a.M;  // lanes past the last row still take part in the shuffles
+    const int64_t at = live ? row : 0;
+    float t[NV][V], w[NV][V];
+    float sum = 0.f, top = 0.f;
+    load_row((const X*)a.x + at * a.ldx, lane, stride, a.C, t);
+    load_row(a.weight, lane, stride, a.C, w);
+    if (a.residual) {
+        float v[NV][V];
+        load_row((const X*)a.residual + at * a.ldr, lane, stride, a.C, v);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) t[k][i] += v[k][i];
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             sum = __builtin_fmaf(t[k][i], t[k][i], sum);
             if (sizeof(Y) == 1) top = max_nan(top, __builtin_fabsf(t[k][i] * w[k][i]));
         }
-    }
-    reduce_lanes(WAVES > 1 ? 64 : lanes, sum, top);
-    if (WAVES > 1) reduce_waves<WAVES>(lds, sum, top);
+    reduce_lanes(WPR > 1 ? 64 : lanes, sum, top);
+    if (WPR > 1) reduce_waves<WPR>(lds, sum, top);
     if (!live) return;
     const float rstd = 1.f / __builtin_sqrtf(sum / (float)a.C + a.eps);
     if (a.rstd && lane == 0) a.rstd[row] = rstd;
     const float scale = row_factor<Y>(rstd, top, a.y_scale, row, lane == 0);
-    if (a.sum) {
-        X* s = (X*)a.sum + row * a.ldsum;
+    if (a.sum) store_row((X*)a.sum + row * a.ldsum, lane, stride, a.C, t);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * stride + lane) * V;
-            if (c < a.C) store_vec(s + c, a.C - c, t[k]);
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            // 8 bits: the largest magnitude may come out a rounding over 448 and
+            // still rounds to it.
+            t[k][i] = t[k][i] * rstd * w[k][i];
+            if (sizeof(Y) == 1) t[k][i] = t[k][i] / scale;
         }
-    }
-    Y* y = (Y*)a.y + row * a.ldy;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (k * stride + lane) * V;
-        if (c < a.C) write_y(y + c, a.C - c, t[k], w[k], rstd, scale);
-    }
+    store_row((Y*)a.y + row * a.ldy, lane, stride, a.C, t);
 }
 
-// Longer rows: a block reads a row twice (the second time from the caches).
+// Longer rows, and those of fewer values than a vector: a block reads a row twice
+// (the second time from the caches).
 // sum, which may be x or the residual, is written in the second pass, behind
 // the reads of the same values by the same thread.
 template <class X, class Y>
@@ -198,96 +203,135 @@ int next_pow2(int n) {
     return p;
 }
 
+// Waves of a row and vectors of a lane: the fewest idle vectors (2050 bf16 are 257
+// vectors: 3 x 128 rather than 2 x 256), and where that leaves a choice two vectors
+// a lane, whose loads are under way together (4096 bf16: 4 waves of 2 vectors 166
+// us at 32768 rows, 8 waves of 1 206).  nv <= 2048.
+struct RowShape {
+    int wpr, nv;
+};
+RowShape row_shape(int64_t nv, int most_nv) {
+    RowShape best{8, 4};
+    int64_t slots = 1 << 30;
+    for (int k : {2, 3, 1, 4})
+        for (int wpr = 1; wpr <= 8; wpr <<= 1) {
+            const int64_t s = (int64_t)wpr * 64 * k;
+            if (s >= nv && s < slots && (k <= most_nv || s > 1536)) {
+                slots = s;
+                best = RowShape{wpr, k};
+            }
+        }
+    return best;
+}
+
+// f.operator()<WPR, NV>() of a shape.
+template <class F>
+void with_shape(RowShape s, F&& f) {
+    auto by_nv = [&](auto wpr) {
+        constexpr int W = decltype(wpr)::value;
+        switch (s.nv) {
+            case 1: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 1>{});
+            case 2: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 2>{});
+            case 3: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 3>{});
+            default: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 4>{});
+        }
+    };
+    switch (s.wpr) {
+        case 1: return by_nv(std::integral_constant<int, 1>{});
+        case 2: return by_nv(std::integral_constant<int, 2>{});
+        case 4: return by_nv(std::integral_constant<int, 4>{});
+        default: return by_nv(std::integral_constant<int, 8>{});
+    }
+}
+
 template <class X, class Y>
 hipError_t launch_forward(const vcsr_rmsnorm_args& a, hipStream_t st) {
     constexpr int V = kVec<X>;
     const int64_t nv = ((int64_t)a.C + V - 1) / V;
-    if (nv <= 64) {
-        const int lanes = next_pow2((int)nv), rows = 256 / lanes;
-        rmsnorm_kernel<X, Y, 1, 1><<<(unsigned)((a.M + rows - 1) / rows), 256, 0, st>>>(a, lanes);
-    } else if (nv <= 256) {
-        rmsnorm_kernel<X, Y, 4, 1><<<(unsigned)a.M, 256, 0, st>>>(a, 64);
-    } else if (nv <= 512) {
-        rmsnorm_kernel<X, Y, 4, 2><<<(unsigned)a.M, 256, 0, st>>>(a, 64);
-    } else if (nv <= 1024) {
-        rmsnorm_kernel<X, Y, 4, 4><<<(unsigned)a.M, 256, 0, st>>>(a, 64);
-    } else {
+    if (nv > 2048 || a.C < V) {
         rmsnorm_long_kernel<X, Y><<<(unsigned)a.M, 1024, 0, st>>>(a);
+        return hipGetLastError();
     }
+    const int lanes = nv <= 64 ? next_pow2((int)nv) : 64;
+    with_shape(row_shape(nv, 4), [&](auto wpr, auto k) {
+        constexpr int W = decltype(wpr)::value, NV = decltype(k)::value;
+        const int rows = W > 1 ? 1 : 256 / lanes;
+        rmsnorm_kernel<X, Y, W, NV>
+            <<<(unsigned)((a.M + rows - 1) / rows), W > 1 ? 64 * W : 256, 0, st>>>(a, lanes);
+    });
     return hipGetLastError();
 }
 
 // ------------------------------------------------------------------ gradient
-// Rows of at most NV * LANES vectors (as above); each row group goes through
-// rows blockIdx, blockIdx + gridDim, ... and keeps dweight of its columns.
-template <class X, class D, int WAVES, int NV>
-__global__ __launch_bounds__(256) void rmsnorm_grad_kernel(vcsr_rmsnorm_grad_args a, float* part,
-                                                           int lanes) {
-    constexpr int V = kVec<X>;
-    __shared__ float lds[2 * WAVES];
-    __shared__ float dw_lds[WAVES > 1 ? 1 : 256 * V * NV];
+// Rows of at most NV * 64 * WPR vectors (as above); each row group goes through
+// rows blockIdx, blockIdx + gridDim, ... and keeps dweight of its columns in
+// registers.  The weight stays in LDS: with it in registers too, 2050 bf16 columns
+// leave room for three waves a SIMD instead of four.
+template <class X, class D, int WPR, int NV>
+__global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_grad_kernel(
+    vcsr_rmsnorm_grad_args a, float* part, int lanes) {
+    constexpr int V = kVec<X>, COLS = (WPR > 1 ? 64 * WPR : 64) * NV * V;
+    __shared__ float red[2][2 * WPR];
+    __shared__ __attribute__((aligned(16))) float w_lds[COLS];
     const int tid = threadIdx.x;
-    const int lane = WAVES > 1 ? tid : tid & (lanes - 1);
-    const int stride = WAVES > 1 ? 64 * WAVES : lanes;
-    const int rows = WAVES > 1 ? 1 : 256 / lanes;
-    const int sub = WAVES > 1 ? 0 : tid / lanes;
-    float w[NV][V], dw[NV][V];
+    const int lane = WPR > 1 ? tid : tid & (lanes - 1);
+    const int stride = WPR > 1 ? 64 * WPR : lanes;
+    const int threads = WPR > 1 ? 64 * WPR : 256;
+    const int rows = WPR > 1 ? 1 : 256 / lanes;
+    const int sub = WPR > 1 ? 0 : tid / lanes;
+    for (int c = tid; c < COLS; c += threads) w_lds[c] = c < a.C ? a.weight[c] : 0.f;
+    __syncthreads();
+    float dw[NV][V];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (k * stride + lane) * V;
-        load_vec(a.weight + c, c < a.C ? a.C - c : 0, w[k]);
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
-    }
     const float inv_c = 1.f / (float)a.C;
-    for (int64_t base = (int64_t)blockIdx.x * rows; base < a.M; base += (int64_t)gridDim.x * rows) {
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * rows; base < a.M;
+         base += (int64_t)gridDim.x * rows, turn ^= 1) {
         const int64_t row = base + sub;
         const bool live = row < a.M;
-        float s[NV][V], d[NV][V];
-        float rstd = 0.f, dot = 0.f, unused = 0.f;
-        if (live) rstd = a.rstd[row];
+        const int64_t at = live ? row : 0;
+        float s[NV][V], d[NV][V], o[NV][V];
+        const float rstd = a.rstd[at];
+        float dot = 0.f, unused = 0.f;
+        load_row((const X*)a.s + at * a.lds, lane, stride, a.C, s);
+        load_row((const D*)a.dy + at * a.lddy, lane, stride, a.C, d);
+        if (a.dsum) {
+            load_row((const X*)a.dsum + at * a.lddsum, lane, stride, a.C, o);
+        } else {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * stride + lane) * V;
-            const int n = live && c < a.C ? a.C - c : 0;
-            load_vec((const X*)a.s + (live ? row * a.lds : 0) + c, n, s[k]);
-            load_vec((const D*)a.dy + (live ? row * a.lddy : 0) + c, n, d[k]);
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[k][i] = 0.f;
         }
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+            const float* const w = w_lds + (k * stride + lane) * V;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 s[k][i] *= rstd;  // h
+                if (WPR == 1 && !live) s[k][i] = d[k][i] = 0.f;
                 dw[k][i] = __builtin_fmaf(d[k][i], s[k][i], dw[k][i]);
-                d[k][i] *= w[k][i];  // g
+                d[k][i] *= w[i];  // g
                 dot = __builtin_fmaf(d[k][i], s[k][i], dot);
             }
-        dot = sum_lanes(WAVES > 1 ? 64 : lanes, dot);
-        if (WAVES > 1) {
-            reduce_waves<WAVES>(lds, dot, unused);
-            __syncthreads();  // lds is written again for the next row
         }
+        dot = sum_lanes(WPR > 1 ? 64 : lanes, dot);
+        // Two sets of LDS slots in turn: the next row's sums do not meet this one's.
+        if (WPR > 1) reduce_waves<WPR>(red[turn], dot, unused);
         if (!live) continue;
         const float mean = dot * inv_c;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * stride + lane) * V;
-            if (c >= a.C) continue;
-            float o[V];
-            if (a.dsum) {
-                load_vec((const X*)a.dsum + row * a.lddsum + c, a.C - c, o);
-            } else {
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] += rstd * (d[k][i] - s[k][i] * mean);
-            store_vec((X*)a.dx + row * a.lddx + c, a.C - c, o);
-        }
+            for (int i = 0; i < V; ++i) o[k][i] += rstd * (d[k][i] - s[k][i] * mean);
+        store_row((X*)a.dx + row * a.lddx, lane, stride, a.C, o);
     }
     if (!part) return;
     float* out = part + (int64_t)blockIdx.x * a.C;
-    if (WAVES > 1) {
+    if (WPR > 1) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * stride + lane) * V;
@@ -295,20 +339,23 @@ __global__ __launch_bounds__(256) void rmsnorm_grad_kernel(vcsr_rmsnorm_grad_arg
         }
         return;
     }
-    // The block's row groups, summed in order.
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) dw_lds[(sub * NV + k) * lanes * V + lane * V + i] = dw[k][i];
+    // The block's row groups add up in LDS, one after the other.
     __syncthreads();
-    for (int c = tid; c < a.C; c += 256) {
-        float t = 0.f;
-        for (int g = 0; g < rows; ++g) t += dw_lds[g * NV * lanes * V + c];
-        out[c] = t;
+    for (int g = 0; g < rows; ++g) {
+        if (sub == g)
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float* const p = w_lds + (k * stride + lane) * V + i;
+                    *p = g ? *p + dw[k][i] : dw[k][i];
+                }
+        __syncthreads();
     }
+    for (int c = tid; c < a.C; c += 256) out[c] = w_lds[c];
 }
 
-// Longer rows: a block per row, read twice; dweight apart (column by column).
+// Longer rows, and those shorter than a vector: a block per row, read twice; dweight apart (column by column).
 template <class X, class D>
 __global__ __launch_bounds__(1024) void rmsnorm_grad_long_kernel(vcsr_rmsnorm_grad_args a) {
     constexpr int V = kVec<X>, WAVES = 16;
@@ -360,12 +407,14 @@ __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(vcsr_rmsnorm_grad_
     part[(int64_t)blockIdx.y * a.C + c] = t;
 }
 
-// Vectors of a row, and the blocks the gradient's launch has (each writes a
-// row of partial dweight): enough rows in flight for the chip, few partial
-// rows beside the data.
+// The gradient's row shape and blocks, each of which writes a row of partial
+// dweight: two waves a SIMD.  With one a SIMD 16384 x 2050 bf16 takes 97 us, with
+// two 68, with four 82 (twice the partial rows).
 struct GradShape {
     int64_t nv;
     int lanes;
+    RowShape row;
+    bool in_registers;
     int32_t blocks;
 };
 GradShape grad_shape(const vcsr_rmsnorm_grad_args& a) {
@@ -373,10 +422,13 @@ GradShape grad_shape(const vcsr_rmsnorm_grad_args& a) {
     const int v = a.x_type == VCSR_F32 ? 4 : 8;
     g.nv = ((int64_t)a.C + v - 1) / v;
     g.lanes = g.nv <= 64 ? next_pow2((int)g.nv) : 64;
-    const int64_t rows = g.nv <= 64 ? 256 / g.lanes : 1;
-    const int64_t need = (a.M + rows - 1) / rows;
-    g.blocks = (int32_t)(need < 1024 ? need : 1024);
-    if (g.nv > 1024 && g.blocks > 64) g.blocks = 64;
+    g.row = row_shape(g.nv, 3);
+    const int64_t rows = g.row.wpr > 1 ? 1 : 256 / g.lanes;
+    const int64_t waves = g.row.wpr > 1 ? g.row.wpr : 4;
+    const int64_t need = (a.M + rows - 1) / rows, most = 2048 / waves;
+    g.blocks = (int32_t)(need < most ? need : most);
+    g.in_registers = g.nv <= 2048 && a.C >= v;
+    if (!g.in_registers) g.blocks = (int32_t)(a.M < 64 ? a.M : 64);
     return g;
 }
 
@@ -384,19 +436,17 @@ template <class X, class D>
 hipError_t launch_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
     const GradShape g = grad_shape(a);
     float* part = a.dweight ? (float*)a.workspace : nullptr;
-    if (g.nv <= 64) {
-        rmsnorm_grad_kernel<X, D, 1, 1><<<g.blocks, 256, 0, st>>>(a, part, g.lanes);
-    } else if (g.nv <= 256) {
-        rmsnorm_grad_kernel<X, D, 4, 1><<<g.blocks, 256, 0, st>>>(a, part, 64);
-    } else if (g.nv <= 512) {
-        rmsnorm_grad_kernel<X, D, 4, 2><<<g.blocks, 256, 0, st>>>(a, part, 64);
-    } else if (g.nv <= 1024) {
-        rmsnorm_grad_kernel<X, D, 4, 4><<<g.blocks, 256, 0, st>>>(a, part, 64);
-    } else {
+    if (!g.in_registers) {
         rmsnorm_grad_long_kernel<X, D><<<(unsigned)a.M, 1024, 0, st>>>(a);
         if (part)
             rmsnorm_dweight_kernel<X, D>
                 <<<dim3((unsigned)((a.C + 255) / 256), g.blocks), 256, 0, st>>>(a, part);
+    } else {
+        with_shape(g.row, [&](auto wpr, auto k) {
+            constexpr int W = decltype(wpr)::value, NV = decltype(k)::value;
+            rmsnorm_grad_kernel<X, D, W, NV>
+                <<<g.blocks, W > 1 ? 64 * W : 256, 0, st>>>(a, part, g.lanes);
+        });
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !part) return e;
