@@ -371,7 +371,7 @@ int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* str
             const std::string who = "tensor " + std::to_string(i) + ": ";
             auto must = [&](bool ok, const char* what) { need(ok, (who + what).c_str()); };
             must(t.n >= 0, "negative n");
-            range(t.n < kMaxRows * vcsr::kAdamwChunk, (who + "n over 2^43").c_str());
+            range(t.n < kMaxRows * vcsr::kAdamwChunk, (who + "n over 2^42").c_str());
             must(is_wide(t.grad_type), "grad_type: VCSR_F32 or VCSR_BF16");
             must(t.state_type == VCSR_F32 || t.state_type == VCSR_FP8,
                  "state_type: VCSR_F32 or VCSR_FP8");
@@ -386,7 +386,7 @@ int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* str
                      (uintptr_t)t.copy % 2 == 0,
                  "a pointer is not aligned to its type");
             const int64_t n = (t.n + vcsr::kAdamwChunk - 1) / vcsr::kAdamwChunk;
-            range((int64_t)chunks.size() + n < kMaxRows, "tensors: over 2^31 chunks of 4096");
+            range((int64_t)chunks.size() + n < kMaxRows, "tensors: over 2^31 chunks of 2048");
             for (int64_t k = 0; k < n; ++k) chunks.push_back(make_int2(i, (int)k));
         }
         need_device();
