@@ -24,7 +24,9 @@ second GPU runtime is loaded into the process.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
+import struct
 
 import numpy as np
 
@@ -129,6 +131,19 @@ class _LinearGradArgs(C.Structure):
                 ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+def _packer(args):
+    """struct.Struct of a ctypes structure's fields: packing costs a third of
+    filling the structure, and a small call is bound by the host."""
+    codes = {C.c_int64: "q", C.c_int32: "i", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
+    st = struct.Struct("@" + "".join(codes[t] for _, t in args._fields_))
+    assert st.size == C.sizeof(args)
+    return st.pack
+
+
+_pack_rmsnorm, _pack_rmsnorm_grad = _packer(_RmsnormArgs), _packer(_RmsnormGradArgs)
+_pack_linear, _pack_linear_grad = _packer(_LinearArgs), _packer(_LinearGradArgs)
+
+
 class _AdamwTensor(C.Structure):
     _fields_ = [("n", C.c_int64), ("grad_type", C.c_int32), ("state_type", C.c_int32),
                 ("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p),
@@ -208,13 +223,13 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "vcsr_event_destroy": (C.c_int, [P]),
         "vcsr_event_record": (C.c_int, [P, P]),
         "vcsr_event_elapsed": (C.c_int, [P, P, pF]),
-        "vcsr_rmsnorm": (C.c_int, [C.POINTER(_RmsnormArgs), P, pF]),
-        "vcsr_rmsnorm_grad_workspace": (C.c_int, [C.POINTER(_RmsnormGradArgs), pS]),
-        "vcsr_rmsnorm_grad": (C.c_int, [C.POINTER(_RmsnormGradArgs), P, pF]),
-        "vcsr_linear_workspace": (C.c_int, [C.POINTER(_LinearArgs), pS]),
-        "vcsr_linear": (C.c_int, [C.POINTER(_LinearArgs), P, pF]),
-        "vcsr_linear_grad_workspace": (C.c_int, [C.POINTER(_LinearGradArgs), pS]),
-        "vcsr_linear_grad": (C.c_int, [C.POINTER(_LinearGradArgs), P, pF]),
+        "vcsr_rmsnorm": (C.c_int, [P, P, pF]),
+        "vcsr_rmsnorm_grad_workspace": (C.c_int, [P, pS]),
+        "vcsr_rmsnorm_grad": (C.c_int, [P, P, pF]),
+        "vcsr_linear_workspace": (C.c_int, [P, pS]),
+        "vcsr_linear": (C.c_int, [P, P, pF]),
+        "vcsr_linear_grad_workspace": (C.c_int, [P, pS]),
+        "vcsr_linear_grad": (C.c_int, [P, P, pF]),
         "vcsr_adamw_create": (C.c_int, [C.POINTER(_AdamwTensor), I32, P, pP]),
         "vcsr_adamw_step": (C.c_int, [P, C.POINTER(_AdamwHyper), P, pF]),
         "vcsr_adamw_free": (None, [P]),
@@ -699,26 +714,27 @@ def _type(arr, what):
 
 def _mat(arr, rows, cols, what, dtype=None):
     """(address, row stride) of a matrix argument after checking its shape,
-    type and size; (None, 0) for None."""
+    type and size; (0, 0) for None."""
     if arr is None:
-        return None, 0
+        return 0, 0
     if arr.shape != (rows, cols):
         raise VcsrError(VCSR_EINVAL, f"{what}: shape {arr.shape}, expected {(rows, cols)}")
-    if dtype is not None and arr.dtype != dtype:
-        raise VcsrError(VCSR_EINVAL, f"{what}: dtype {arr.dtype}, expected {dtype}")
+    have = arr.dtype
+    if dtype is not None and have is not dtype and have != dtype:
+        raise VcsrError(VCSR_EINVAL, f"{what}: dtype {have}, expected {dtype}")
     ld = getattr(arr, "ld", cols)
-    if rows and arr.nbytes < ((rows - 1) * ld + cols) * arr.dtype.itemsize:
+    if rows and arr.nbytes < ((rows - 1) * ld + cols) * have.itemsize:
         raise VcsrError(VCSR_EINVAL, f"{what}: {arr.nbytes} bytes are too few")
-    return arr.ptr, ld
+    return arr.ptr.value or 0, ld
 
 
 def _vec(arr, n, what):
     if arr is None:
-        return None
-    if arr.dtype != F32 or arr.nbytes < 4 * n:
+        return 0
+    if (arr.dtype is not F32 and arr.dtype != F32) or arr.nbytes < 4 * n:
         raise VcsrError(VCSR_EINVAL, f"{what}: {arr.dtype}, {arr.nbytes} bytes; "
                                      f"{n} float32 values are expected")
-    return arr.ptr
+    return arr.ptr.value or 0
 
 
 def _shape2(arr, what):
@@ -752,22 +768,50 @@ def release_workspaces():
         _workspaces.clear()
 
 
-def _with_workspace(args, query, given, stream):
+# Bytes of workspace by sizes and types alone (what the _workspace functions
+# answer), so that a call asks the library once for each.
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(M, N, K, x_type, y_type):
     need = C.c_size_t(0)
-    _check(query(C.byref(args), C.byref(need)))
-    if need.value:
-        ws = given if given is not None else workspace(need.value, stream)
-        args.workspace, args.workspace_bytes = ws.ptr, ws.nbytes
+    args = _LinearArgs(M=M, N=N, K=K, x_type=x_type, y_type=y_type)
+    _check(load_library().vcsr_linear_workspace(C.byref(args), C.byref(need)))
+    return need.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_grad_bytes(M, N, K, x_type, y_type, act, z, dx, dw, dbias):
+    need = C.c_size_t(0)
+    some = C.c_void_p(16)
+    args = _LinearGradArgs(M=M, N=N, K=K, x_type=x_type, y_type=y_type, act=act,
+                           z=some if z else None, dx=some if dx else None,
+                           dw=some if dw else None, dbias=some if dbias else None)
+    _check(load_library().vcsr_linear_grad_workspace(C.byref(args), C.byref(need)))
+    return need.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _rmsnorm_grad_bytes(M, N, x_type, y_type):
+    need = C.c_size_t(0)
+    args = _RmsnormGradArgs(M=M, C=N, x_type=x_type, y_type=y_type, dweight=16)
+    _check(load_library().vcsr_rmsnorm_grad_workspace(C.byref(args), C.byref(need)))
+    return need.value
+
+
+def _space(nbytes, given, stream):
+    if not nbytes:
+        return 0, 0
+    ws = given if given is not None else workspace(nbytes, stream)
+    return ws.ptr.value or 0, ws.nbytes
 
 
 def _call(fn, args, stream, timed):
     if not timed:
-        rc = fn(C.byref(args), _sp(stream), None)
+        rc = fn(args, stream.h if stream is not None else None, None)
         if rc:
             _check(rc)
         return None
     ms = C.c_float(0)
-    _check(fn(C.byref(args), _sp(stream), C.byref(ms)))
+    _check(fn(args, _sp(stream), C.byref(ms)))
     return ms.value
 
 
@@ -779,10 +823,10 @@ def run_rmsnorm_gpu(x, weight, y, residual=None, sum=None, y_scale=None, rstd=No
     M, N = _shape2(x, "x")
     (xp, ldx), (rp, ldr) = _mat(x, M, N, "x"), _mat(residual, M, N, "residual", x.dtype)
     (sp, lds), (yp, ldy) = _mat(sum, M, N, "sum", x.dtype), _mat(y, M, N, "y")
-    args = _RmsnormArgs(M, N, _type(x, "x"), _type(y, "y"), eps, xp, ldx, rp, ldr,
-                        _vec(weight, N, "weight"), sp, lds, yp, ldy,
-                        _vec(y_scale, M, "y_scale"), _vec(rstd, M, "rstd"))
-    return _call(load_library().vcsr_rmsnorm, args, stream, timed)
+    args = _pack_rmsnorm(M, N, _type(x, "x"), _type(y, "y"), eps, xp, ldx, rp, ldr,
+                         _vec(weight, N, "weight"), sp, lds, yp, ldy,
+                         _vec(y_scale, M, "y_scale"), _vec(rstd, M, "rstd"))
+    return _call((_lib or load_library()).vcsr_rmsnorm, args, stream, timed)
 
 
 def run_rmsnorm_grad_gpu(dy, s, weight, rstd, dx, dweight=None, dsum=None, workspace=None,
@@ -793,12 +837,12 @@ def run_rmsnorm_grad_gpu(dy, s, weight, rstd, dx, dweight=None, dsum=None, works
     M, N = _shape2(s, "s")
     (dp, lddy), (sp, lds) = _mat(dy, M, N, "dy"), _mat(s, M, N, "s")
     (up, ldu), (xp, ldx) = _mat(dsum, M, N, "dsum", s.dtype), _mat(dx, M, N, "dx", s.dtype)
-    args = _RmsnormGradArgs(M, N, _type(s, "s"), _type(dy, "dy"), dp, lddy, sp, lds,
-                            _vec(weight, N, "weight"), _vec(rstd, M, "rstd"), up, ldu, xp, ldx,
-                            _vec(dweight, N, "dweight"))
-    lib = load_library()
-    _with_workspace(args, lib.vcsr_rmsnorm_grad_workspace, workspace, stream)
-    return _call(lib.vcsr_rmsnorm_grad, args, stream, timed)
+    xt, yt = _type(s, "s"), _type(dy, "dy")
+    need = _rmsnorm_grad_bytes(M, N, xt, yt) if dweight is not None else 0
+    args = _pack_rmsnorm_grad(M, N, xt, yt, dp, lddy, sp, lds, _vec(weight, N, "weight"),
+                              _vec(rstd, M, "rstd"), up, ldu, xp, ldx,
+                              _vec(dweight, N, "dweight"), *_space(need, workspace, stream))
+    return _call((_lib or load_library()).vcsr_rmsnorm_grad, args, stream, timed)
 
 
 def _act(act):
@@ -817,12 +861,12 @@ def run_linear_gpu(x, w, y, bias=None, residual=None, act="none", z=None, x_scal
     (xp, ldx), (wp, ldw) = _mat(x, M, K, "x"), _mat(w, N, K, "w", x.dtype)
     (yp, ldy), (rp, ldr) = _mat(y, M, N, "y"), _mat(residual, M, N, "residual", y.dtype)
     zp, ldz = _mat(z, M, N, "z", y.dtype)
-    args = _LinearArgs(M, N, K, _type(x, "x"), _type(y, "y"), _act(act), xp, ldx, wp, ldw,
-                       _vec(x_scale, M, "x_scale"), _vec(w_scale, N, "w_scale"),
-                       _vec(bias, N, "bias"), rp, ldr, zp, ldz, yp, ldy)
-    lib = load_library()
-    _with_workspace(args, lib.vcsr_linear_workspace, workspace, stream)
-    return _call(lib.vcsr_linear, args, stream, timed)
+    xt, yt = _type(x, "x"), _type(y, "y")
+    args = _pack_linear(M, N, K, xt, yt, _act(act), xp, ldx, wp, ldw,
+                        _vec(x_scale, M, "x_scale"), _vec(w_scale, N, "w_scale"),
+                        _vec(bias, N, "bias"), rp, ldr, zp, ldz, yp, ldy,
+                        *_space(_linear_bytes(M, N, K, xt, yt), workspace, stream))
+    return _call((_lib or load_library()).vcsr_linear, args, stream, timed)
 
 
 def run_linear_grad_gpu(dy, x, w, z=None, act="none", dx=None, dw=None, dbias=None,
@@ -834,11 +878,13 @@ def run_linear_grad_gpu(dy, x, w, z=None, act="none", dx=None, dw=None, dbias=No
     (xp, ldx), (wp, ldw) = _mat(x, M, K, "x"), _mat(w, N, K, "w", x.dtype)
     (dp, lddy), (zp, ldz) = _mat(dy, M, N, "dy"), _mat(z, M, N, "z", dy.dtype)
     (xg, lddx), (wg, lddw) = _mat(dx, M, K, "dx", x.dtype), _mat(dw, N, K, "dw", x.dtype)
-    args = _LinearGradArgs(M, N, K, _type(x, "x"), _type(dy, "dy"), _act(act), dp, lddy, zp, ldz,
-                           xp, ldx, wp, ldw, xg, lddx, wg, lddw, _vec(dbias, N, "dbias"))
-    lib = load_library()
-    _with_workspace(args, lib.vcsr_linear_grad_workspace, workspace, stream)
-    return _call(lib.vcsr_linear_grad, args, stream, timed)
+    xt, yt, at = _type(x, "x"), _type(dy, "dy"), _act(act)
+    need = _linear_grad_bytes(M, N, K, xt, yt, at, z is not None, dx is not None, dw is not None,
+                              dbias is not None)
+    args = _pack_linear_grad(M, N, K, xt, yt, at, dp, lddy, zp, ldz, xp, ldx, wp, ldw, xg, lddx,
+                             wg, lddw, _vec(dbias, N, "dbias"),
+                             *_space(need, workspace, stream))
+    return _call((_lib or load_library()).vcsr_linear_grad, args, stream, timed)
 
 
 class AdamW:

@@ -210,14 +210,22 @@ struct Gemm {
 };
 hipError_t launch_gemm(const Gemm& g, hipStream_t st);
 size_t gemm_workspace(const Gemm& g);
-// The shapes one kernel takes (chosen by launch_gemm).
+// dx and dw of one linear layer, in one launch where that is faster.
+hipError_t launch_gemm_pair(const Gemm& dw, const Gemm& dx, hipStream_t st);
+size_t gemm_pair_workspace(const Gemm& dw, const Gemm& dx);
+// What a product's launch does: square tiles (16: the kernel for few rows), and the
+// splits of the sum, of `steps` steps of 128 bytes each; each writes partial sums.
 struct GemmPlan {
-    int tile_i, tile_j;
-    int32_t splits;  // of the sum; each writes partial sums
-    int64_t steps;   // tile steps of a split
+    int tile;
+    int32_t splits;
+    int64_t steps;
 };
 hipError_t launch_gemm_f32(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_gemm_bf16(const Gemm& g, const GemmPlan& p, hipStream_t st);
+hipError_t launch_pair_f32(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
+                           hipStream_t st);
+hipError_t launch_pair_bf16(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
+                            hipStream_t st);
 hipError_t launch_gemm_fp8(const Gemm& g, const GemmPlan& p, hipStream_t st);
 
 // --------------------------------------------------------------- adamw.hip

@@ -232,8 +232,10 @@ LinearGrad grad_of(const vcsr_linear_grad_args* args) {
     g.out = a.dw;
     g.ldo = a.lddw;
     g.part = part;
-    if (a.dx) w.part_bytes = vcsr::gemm_workspace(x);
-    if (a.dw) w.part_bytes = std::max(w.part_bytes, vcsr::gemm_workspace(g));
+    if (a.dx && a.dw)
+        w.part_bytes = vcsr::gemm_pair_workspace(g, x);
+    else if (a.dx || a.dw)
+        w.part_bytes = vcsr::gemm_workspace(a.dx ? x : g);
     return w;
 }
 
@@ -279,9 +281,9 @@ hipError_t run_grad(const LinearGrad& w, hipStream_t st) {
             e = vcsr::launch_sum_rows(bias_part, vcsr::dz_row_blocks(a.M, a.N), a.N, a.N, a.dbias,
                                       st);
     }
-    if (e == hipSuccess && a.dx) e = vcsr::launch_gemm(w.dx, st);
-    if (e == hipSuccess && a.dw) e = vcsr::launch_gemm(w.dw, st);
-    return e;
+    if (e != hipSuccess || (!a.dx && !a.dw)) return e;
+    if (a.dx && a.dw) return vcsr::launch_gemm_pair(w.dw, w.dx, st);
+    return vcsr::launch_gemm(a.dx ? w.dx : w.dw, st);
 }
 
 }  // namespace

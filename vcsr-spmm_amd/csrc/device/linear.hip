@@ -29,61 +29,140 @@ constexpr TileCost kFp8[] = {
     {128, 2, {0.95f, 1.61f}, {7.0f, 7.3f}},
     {256, 1, {2.53f}, {11.4f}}};
 
-// Of every tile and number of splits, the one with the least estimated time:
-// whole rounds of blocks, what is left, and for a split sum the join (its launch,
-// and the partial sums written and read at 4 TB/s).
-GemmPlan plan_of(const Gemm& g) {
+struct Costs {
+    const TileCost* t;
+    int n;
+};
+Costs costs_of(const Gemm& g) {
+    if (g.type == VCSR_F32) return Costs{kF32, 2};
+    return g.type == VCSR_BF16 ? Costs{kBf16, 3} : Costs{kFp8, 3};
+}
+// Steps of the whole sum.
+int64_t steps_of(const Gemm& g) {
     const int size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
-    const TileCost* costs = g.type == VCSR_F32 ? kF32 : g.type == VCSR_BF16 ? kBf16 : kFp8;
-    const int n_costs = g.type == VCSR_F32 ? 2 : 3;
-    const int64_t all = (g.R * size + tile::kStepBytes - 1) / tile::kStepBytes;
+    return (g.R * size + tile::kStepBytes - 1) / tile::kStepBytes;
+}
+int64_t tiles_of(const Gemm& g, int64_t t) {
+    return (g.I + t - 1) / t * (((int64_t)g.J + t - 1) / t);
+}
+// A block's time with b blocks on its compute unit.  Transposing reads of both
+// operands take a quarter longer in the big tile.
+float block_us(const Gemm& g, const TileCost& t, int64_t steps, int64_t b) {
+    const float slower = t.tile == 256 && g.p_cols ? 1.25f : 1.f;
+    return (float)steps * t.step[b - 1] * slower + t.rest[b - 1];
+}
+// The join of a split sum: its launch, and the partial sums written and read at 4
+// TB/s.
+float join_us(const Gemm& g, int64_t splits) {
+    return splits > 1 ? 4.f + (float)((double)splits * (double)g.I * (double)g.J * 2e-6) : 0.f;
+}
+// f(splits, steps) for every number of splits worth trying over `tiles` tiles.
+template <class F>
+void each_split(const Gemm& g, int64_t tiles, F&& f) {
+    const int64_t all = steps_of(g);
+    for (int64_t want = 1; want <= 128; want += want < 4 ? 1 : want / 2) {
+        const int64_t steps = (all + want - 1) / want, splits = (all + steps - 1) / steps;
+        if (want > 1 && (steps < 4 || tiles * splits > 8 * kCus)) break;
+        f(splits, steps);
+    }
+}
+
+// Of every tile and number of splits, the one with the least estimated time:
+// whole rounds of blocks, what is left, and the join.
+GemmPlan plan_of(const Gemm& g, float* us_out = nullptr) {
+    const int size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
     // Up to 8 rows: W is read straight into the matrix layout, 6 to 9 us up to 32 MB of
     // it against 10 of the tiles (their join is a launch of its own).  Not where
     // few blocks would read long rows alone: 512 x 8000 bf16 16 us against 10.
     if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || 16 * g.R * size <= 192 << 10))
-        return GemmPlan{16, 16, 1, all};
+        return GemmPlan{16, 1, steps_of(g)};
     GemmPlan best{};
     float best_us = 0.f;
-    for (int c = 0; c < n_costs; ++c) {
-        const TileCost& t = costs[c];
-        const int64_t tiles = (g.I + t.tile - 1) / t.tile * (((int64_t)g.J + t.tile - 1) / t.tile);
-        // Transposing reads of both operands take a quarter longer in the big tile.
-        const float slower = t.tile == 256 && g.p_cols ? 1.25f : 1.f;
-        for (int64_t want = 1; want <= 128; want += want < 4 ? 1 : want / 2) {
-            const int64_t steps = (all + want - 1) / want, splits = (all + steps - 1) / steps;
-            if (want > 1 && (steps < 4 || tiles * splits > 8 * kCus)) break;
-            const int64_t blocks = tiles * splits, round = kCus * t.room;
+    const Costs c = costs_of(g);
+    for (const TileCost* t = c.t; t < c.t + c.n; ++t) {
+        const int64_t tiles = tiles_of(g, t->tile);
+        each_split(g, tiles, [&](int64_t splits, int64_t steps) {
+            const int64_t blocks = tiles * splits, round = kCus * t->room;
             const int64_t rounds = blocks / round, left = blocks - rounds * round;
-            auto one = [&](int64_t b) {
-                return (float)steps * t.step[b - 1] * slower + t.rest[b - 1];
-            };
-            float us = (float)rounds * one(t.room);
-            if (left) us += one((left + kCus - 1) / kCus);
-            if (splits > 1)
-                us += 4.f + (float)((double)splits * (double)g.I * (double)g.J * 8e-6 / 4.0);
+            float us = (float)rounds * block_us(g, *t, steps, t->room) + join_us(g, splits);
+            if (left) us += block_us(g, *t, steps, (left + kCus - 1) / kCus);
             if (best.splits == 0 || us < best_us) {
                 best_us = us;
-                best = GemmPlan{t.tile, t.tile, (int32_t)splits, steps};
+                best = GemmPlan{t->tile, (int32_t)splits, steps};
             }
-        }
+        });
+    }
+    if (us_out) *us_out = best_us;
+    return best;
+}
+
+// Both products in one launch, if that is estimated faster than one after the
+// other: all blocks' time over the chip's room and part of a last block, or the
+// longest block, and dw's join.  (8192 x 2048 x 4096 bf16: dw has 128 tiles of 256, dx 256.)
+struct PairPlan {
+    bool together;
+    GemmPlan dw, dx;
+};
+PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
+    float us_w = 0.f, us_x = 0.f;
+    PairPlan best{false, plan_of(dw, &us_w), plan_of(dx, &us_x)};
+    float best_us = us_w + us_x + 2.f;
+    const Costs c = costs_of(dw);
+    for (const TileCost* t = c.t; t < c.t + c.n; ++t) {
+        const int64_t tiles_w = tiles_of(dw, t->tile), tiles_x = tiles_of(dx, t->tile);
+        if (tiles_x > 64 * kCus) continue;  // long by itself: nothing to gain
+        const float one_x = block_us(dx, *t, steps_of(dx), t->room);
+        each_split(dw, tiles_w, [&](int64_t splits, int64_t steps) {
+            const float one_w = block_us(dw, *t, steps, t->room);
+            float us = ((float)(tiles_w * splits) * one_w + (float)tiles_x * one_x) /
+                           (float)(kCus * t->room) + 0.25f * one_x;
+            if (us < one_w) us = one_w;
+            us += join_us(dw, splits);
+            if (us < best_us) {
+                best_us = us;
+                best = PairPlan{true, GemmPlan{t->tile, (int32_t)splits, steps},
+                                GemmPlan{t->tile, 1, steps_of(dx)}};
+            }
+        });
     }
     return best;
+}
+
+size_t part_bytes(const Gemm& g, const GemmPlan& p) {
+    return p.splits > 1 ? (size_t)p.splits * (size_t)g.I * (size_t)tile::part_ld(g.J) * 4 : 0;
 }
 
 }  // namespace
 
 size_t gemm_workspace(const Gemm& g) {
-    if (g.I <= 0 || g.J <= 0) return 0;
-    const GemmPlan p = plan_of(g);
-    return p.splits > 1 ? (size_t)p.splits * (size_t)g.I * (size_t)tile::part_ld(g.J) * 4 : 0;
+    return g.I <= 0 || g.J <= 0 ? 0 : part_bytes(g, plan_of(g));
 }
 
-hipError_t launch_gemm(const Gemm& g, hipStream_t st) {
-    if (g.I <= 0 || g.J <= 0) return hipSuccess;
-    const GemmPlan p = plan_of(g);
+size_t gemm_pair_workspace(const Gemm& dw, const Gemm& dx) {
+    const PairPlan p = plan_pair(dw, dx);
+    const size_t a = part_bytes(dw, p.dw), b = part_bytes(dx, p.dx);
+    return a > b ? a : b;
+}
+
+namespace {
+hipError_t launch(const Gemm& g, const GemmPlan& p, hipStream_t st) {
     return g.type == VCSR_F32    ? launch_gemm_f32(g, p, st)
            : g.type == VCSR_BF16 ? launch_gemm_bf16(g, p, st)
                                  : launch_gemm_fp8(g, p, st);
+}
+}  // namespace
+
+hipError_t launch_gemm(const Gemm& g, hipStream_t st) {
+    return g.I <= 0 || g.J <= 0 ? hipSuccess : launch(g, plan_of(g), st);
+}
+
+hipError_t launch_gemm_pair(const Gemm& dw, const Gemm& dx, hipStream_t st) {
+    const PairPlan p = plan_pair(dw, dx);
+    if (p.together)
+        return dw.type == VCSR_F32 ? launch_pair_f32(dw, p.dw, dx, p.dx, st)
+                                   : launch_pair_bf16(dw, p.dw, dx, p.dx, st);
+    const hipError_t e = launch(dx, p.dx, st);
+    return e != hipSuccess ? e : launch(dw, p.dw, st);
 }
 
 }  // namespace vcsr

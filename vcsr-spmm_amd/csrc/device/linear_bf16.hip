@@ -9,4 +9,9 @@ hipError_t launch_gemm_bf16(const Gemm& g, const GemmPlan& p, hipStream_t st) {
     return tile::launch_layout<bf16, false, false>(g, p, st);
 }
 
+hipError_t launch_pair_bf16(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
+                            hipStream_t st) {
+    return tile::launch_pair<bf16>(dw, p, dx, q, st);
+}
+
 }  // namespace vcsr

@@ -351,11 +351,12 @@ struct Place {
     uint32_t split;
 };
 template <int TI, int TJ>
-__device__ __forceinline__ Place place_of(const Gemm& g, uint32_t block, uint32_t splits) {
+__device__ __forceinline__ Place place_of(const Gemm& g, uint32_t block, uint32_t blocks,
+                                          uint32_t splits) {
     constexpr uint32_t kBand = 4;
     const uint32_t ti = (uint32_t)((g.I + TI - 1) / TI);
     const uint32_t tj = (uint32_t)(((int64_t)g.J + TJ - 1) / TJ);
-    const uint32_t b = xcd_remap(block, gridDim.x);
+    const uint32_t b = xcd_remap(block, blocks);
     const uint32_t split = b % splits, t = b / splits;
     const uint32_t band = t / (kBand * ti), in_band = t - band * (kBand * ti);
     const uint32_t width = tj - band * kBand < kBand ? tj - band * kBand : kBand;
@@ -477,10 +478,21 @@ __device__ __forceinline__ bool ragged_end(const Gemm& g, int64_t k_end, bool p_
                             (q_cols && g.J % EPG != 0));
 }
 
+// One of a launch's products: `blocks` blocks, each a tile and one of `splits`
+// parts of the sum, of `steps` steps.
+struct Part {
+    int splits;
+    int64_t steps;
+    uint32_t blocks;
+};
+
 // Tiles whose blocks share a compute unit: a step's loads run under the other
 // blocks' work as well as under the block's own.
+template <int TI, int TJ>
+constexpr int kSharedLds = 2 * (TI + TJ) * kStepBytes;
 template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
-__global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, int64_t steps) {
+__device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uint32_t block,
+                                            uint8_t* lds0) {
     constexpr int NT = 64 * WI * WJ;
     constexpr int FI = TI / WI / 16, FJ = TJ / WJ / 16;
     constexpr int BK = kStepBytes / (int)sizeof(T);
@@ -489,9 +501,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
     using LQ = Loader<T, TJ, NT, QCOLS, true>;
     using RP = Reader<T, TI, PCOLS, false>;
     using RQ = Reader<T, TJ, QCOLS, true>;
-    __shared__ __attribute__((aligned(128))) uint8_t lds[2][(TI + TJ) * kStepBytes];
-
-    const Place at = place_of<TI, TJ>(g, blockIdx.x, (uint32_t)splits);
+    constexpr int kStage = (TI + TJ) * kStepBytes;
+    const int splits = part.splits;
+    const int64_t steps = part.steps;
+    const Place at = place_of<TI, TJ>(g, block, part.blocks, (uint32_t)splits);
     const Operand P{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, at.i0,
                     extent<T>(g.I, g.R, g.ldp, PCOLS)};
     const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, at.j0,
@@ -527,7 +540,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
     uint32_t op[LP::GR], oq[LQ::GR];
     LP::offsets(P, op);
     LQ::offsets(Q, oq);
-    lds_byte* const to = (lds_byte*)&lds[0][0];
+    lds_byte* const to = (lds_byte*)lds0;
     int buf = 0;
     if (k_first < k_full) {
         LP::copy(P, op, k_first, to);
@@ -539,21 +552,21 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
         wait_loads<0>();
         barrier();
         if (k + BK < k_full) {
-            lds_byte* const next = to + (buf ^ 1) * (TI + TJ) * kStepBytes;
+            lds_byte* const next = to + (buf ^ 1) * kStage;
             LP::copy(P, op, k + BK, next);
             LQ::copy(Q, oq, k + BK, next + TI * kStepBytes);
         }
-        multiply(lds[buf], lds[buf] + TI * kStepBytes);
+        multiply(lds0 + buf * kStage, lds0 + buf * kStage + TI * kStepBytes);
     }
     if (ragged) {
-        LP::fetch(P, k_full, k_end, lds[buf]);
-        LQ::fetch(Q, k_full, k_end, lds[buf] + TI * kStepBytes);
+        LP::fetch(P, k_full, k_end, lds0 + buf * kStage);
+        LQ::fetch(Q, k_full, k_end, lds0 + buf * kStage + TI * kStepBytes);
         __syncthreads();
-        multiply(lds[buf], lds[buf] + TI * kStepBytes);
+        multiply(lds0 + buf * kStage, lds0 + buf * kStage + TI * kStepBytes);
     }
     __syncthreads();
-    constexpr int ROOM = (int)sizeof(lds) / (WI * WJ) / 16 * 16;
-    write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(&lds[0][0] + wave * ROOM), at.i0 + ri,
+    constexpr int ROOM = 2 * kStage / (WI * WJ) / 16 * 16;
+    write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(lds0 + wave * ROOM), at.i0 + ri,
                                     at.j0 + rj, splits, at.split);
 }
 
@@ -574,7 +587,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void gemm_kernel(Gemm g, int splits, 
 // a wave waits until all but the 8 newest have, before its half turn that ends
 // at the barrier behind which the first wave reads them.
 template <class T, bool PCOLS, bool QCOLS>
-__global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int64_t steps) {
+__device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint32_t block,
+                                           uint8_t* lds) {
     constexpr int TI = 256, TJ = 256, NT = 512, WJ = 4, FI = 8, FJ = 4, H = 4;
     constexpr int BK = kStepBytes / (int)sizeof(T);
     constexpr int kP = TI / 2 * kStepBytes, kStage = (TI + TJ) * kStepBytes;
@@ -582,9 +596,9 @@ __global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int
     using LQ = Loader<T, TJ, NT, QCOLS, true>;
     using RP = Reader<T, TI / 2, PCOLS, false>;
     using RQ = Reader<T, TJ, QCOLS, true>;
-    __shared__ __attribute__((aligned(128))) uint8_t lds[2 * kStage];
-
-    const Place at = place_of<TI, TJ>(g, blockIdx.x, (uint32_t)splits);
+    const int splits = part.splits;
+    const int64_t steps = part.steps;
+    const Place at = place_of<TI, TJ>(g, block, part.blocks, (uint32_t)splits);
     Operand P[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -609,7 +623,7 @@ __global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int
     LP::offsets(P[0], op[0]);
     LP::offsets(P[1], op[1]);
     LQ::offsets(Q, oq);
-    lds_byte* const to = (lds_byte*)&lds[0];
+    lds_byte* const to = (lds_byte*)lds;
     auto ask_front = [&](int t) {  // Q and upper P of step t
         lds_byte* const into = to + (t & 1) * kStage;
         LQ::copy(Q, oq, k_first + (int64_t)t * BK, into + 2 * kP);
@@ -679,9 +693,41 @@ __global__ __launch_bounds__(512) void gemm_turns_kernel(Gemm g, int splits, int
         }
     }
     __syncthreads();
-    constexpr int ROOM = (int)sizeof(lds) / 8;
+    constexpr int ROOM = 2 * kStage / 8;
     write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(lds + wave * ROOM), at.i0 + wi * 128,
                                     at.j0 + wj * 64, splits, at.split);
+}
+
+// A tile of TILE x TILE by the code for its size.
+template <class T, int TILE, bool PCOLS, bool QCOLS>
+__device__ __forceinline__ void gemm_block(const Gemm& g, const Part& part, uint32_t block,
+                                           uint8_t* lds) {
+    if constexpr (TILE == 256)
+        gemm_turns<T, PCOLS, QCOLS>(g, part, block, lds);
+    else
+        gemm_shared<T, TILE, TILE, 2, 2, PCOLS, QCOLS>(g, part, block, lds);
+}
+template <int TILE>
+constexpr int kThreads = TILE == 256 ? 512 : 256;
+
+template <class T, int TILE, bool PCOLS, bool QCOLS>
+__global__ __launch_bounds__(kThreads<TILE>) void gemm_kernel(Gemm g, Part part) {
+    __shared__ __attribute__((aligned(128))) uint8_t lds[kSharedLds<TILE, TILE>];
+    gemm_block<T, TILE, PCOLS, QCOLS>(g, part, blockIdx.x, lds);
+}
+
+// Both products of a gradient in one launch: dw's blocks first, whose sums over the
+// rows are long, then dx's (from a multiple of 8 on, so that both keep their XCDs).
+// Each product by itself leaves compute units idle at its end.
+template <class T, int TILE>
+__global__ __launch_bounds__(kThreads<TILE>) void gemm_pair_kernel(Gemm dw, Part dw_part, Gemm dx,
+                                                                   Part dx_part) {
+    __shared__ __attribute__((aligned(128))) uint8_t lds[kSharedLds<TILE, TILE>];
+    const uint32_t first = (dw_part.blocks + 7) & ~7u;
+    if (blockIdx.x >= first)
+        gemm_block<T, TILE, false, true>(dx, dx_part, blockIdx.x - first, lds);
+    else if (blockIdx.x < dw_part.blocks)
+        gemm_block<T, TILE, true, true>(dw, dw_part, blockIdx.x, lds);
 }
 
 // The partial sums of a split product and the epilogue, for few parts: a thread
@@ -853,39 +899,60 @@ hipError_t launch_rows(const Gemm& g, hipStream_t st) {
     return hipGetLastError();
 }
 
-template <class T, bool PCOLS, bool QCOLS>
-hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
-    if constexpr (!PCOLS && !QCOLS) {
-        if (p.tile_i == 16)
-            return g.out_type == VCSR_BF16 ? launch_rows<T, bf16>(g, st)
-                                           : launch_rows<T, float>(g, st);
-    }
-    const int64_t blocks = (g.I + p.tile_i - 1) / p.tile_i *
-                           (((int64_t)g.J + p.tile_j - 1) / p.tile_j) * (int64_t)p.splits;
-    if (blocks >= ((int64_t)1 << 31)) return hipErrorInvalidConfiguration;
-    const unsigned n = (unsigned)blocks;
-    if (p.tile_i == 64)
-        gemm_kernel<T, 64, 64, 2, 2, PCOLS, QCOLS><<<n, 256, 0, st>>>(g, p.splits, p.steps);
-    else if (p.tile_i == 128)
-        gemm_kernel<T, 128, 128, 2, 2, PCOLS, QCOLS><<<n, 256, 0, st>>>(g, p.splits, p.steps);
-    else if constexpr (sizeof(T) < 4)
-        gemm_turns_kernel<T, PCOLS, QCOLS><<<n, 512, 0, st>>>(g, p.splits, p.steps);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits <= 1) return e;
+inline Part part_of(const Gemm& g, const GemmPlan& p) {
+    const int64_t tiles = (g.I + p.tile - 1) / p.tile * (((int64_t)g.J + p.tile - 1) / p.tile);
+    return Part{p.splits, p.steps, (uint32_t)(tiles * p.splits)};
+}
+
+inline hipError_t launch_join(const Gemm& g, int splits, hipStream_t st) {
+    if (splits <= 1) return hipSuccess;
     const int64_t vectors = g.I * (part_ld(g.J) / 8);
     const unsigned few = (unsigned)((vectors + 255) / 256), many = (unsigned)((vectors + 31) / 32);
     if (g.out_type == VCSR_BF16) {
-        if (p.splits < 8)
-            gemm_join_few_kernel<bf16><<<few, 256, 0, st>>>(g, p.splits);
+        if (splits < 8)
+            gemm_join_few_kernel<bf16><<<few, 256, 0, st>>>(g, splits);
         else
-            gemm_join_kernel<bf16><<<many, 256, 0, st>>>(g, p.splits);
+            gemm_join_kernel<bf16><<<many, 256, 0, st>>>(g, splits);
     } else {
-        if (p.splits < 8)
-            gemm_join_few_kernel<float><<<few, 256, 0, st>>>(g, p.splits);
+        if (splits < 8)
+            gemm_join_few_kernel<float><<<few, 256, 0, st>>>(g, splits);
         else
-            gemm_join_kernel<float><<<many, 256, 0, st>>>(g, p.splits);
+            gemm_join_kernel<float><<<many, 256, 0, st>>>(g, splits);
     }
     return hipGetLastError();
+}
+
+template <class T, bool PCOLS, bool QCOLS>
+hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
+    if constexpr (!PCOLS && !QCOLS) {
+        if (p.tile == 16)
+            return g.out_type == VCSR_BF16 ? launch_rows<T, bf16>(g, st)
+                                           : launch_rows<T, float>(g, st);
+    }
+    const Part part = part_of(g, p);
+    if (p.tile == 64)
+        gemm_kernel<T, 64, PCOLS, QCOLS><<<part.blocks, kThreads<64>, 0, st>>>(g, part);
+    else if (p.tile == 128)
+        gemm_kernel<T, 128, PCOLS, QCOLS><<<part.blocks, kThreads<128>, 0, st>>>(g, part);
+    else if constexpr (sizeof(T) < 4)
+        gemm_kernel<T, 256, PCOLS, QCOLS><<<part.blocks, kThreads<256>, 0, st>>>(g, part);
+    hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch_join(g, p.splits, st);
+}
+
+template <class T>
+hipError_t launch_pair(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
+                       hipStream_t st) {
+    const Part a = part_of(dw, p), b = part_of(dx, q);
+    const uint32_t blocks = ((a.blocks + 7) & ~7u) + b.blocks;
+    if (p.tile == 64)
+        gemm_pair_kernel<T, 64><<<blocks, kThreads<64>, 0, st>>>(dw, a, dx, b);
+    else if (p.tile == 128)
+        gemm_pair_kernel<T, 128><<<blocks, kThreads<128>, 0, st>>>(dw, a, dx, b);
+    else if constexpr (sizeof(T) < 4)
+        gemm_pair_kernel<T, 256><<<blocks, kThreads<256>, 0, st>>>(dw, a, dx, b);
+    hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch_join(dw, p.splits, st);
 }
 
 }  // namespace tile
