@@ -701,6 +701,48 @@ class DeviceView:
         self.owner = owner
 
 
+def to_bf16(a) -> np.ndarray:
+    """float32 values as bf16 bit patterns (BF16), rounded to nearest even."""
+    a = np.ascontiguousarray(a, np.float32)
+    u = a.view(np.uint32)
+    rounded = (u + 0x7FFF + ((u >> 16) & 1)) >> 16  # no carry past 32 bits but from a NaN
+    return np.where(np.isnan(a), 0x7FC0, rounded).astype(BF16)
+
+
+def from_bf16(u) -> np.ndarray:
+    return (np.asarray(u, BF16).astype(np.uint32) << 16).view(np.float32)
+
+
+def _e4m3_values():
+    c = np.arange(128)
+    e, m = c >> 3, c & 7
+    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))
+    v[127] = np.nan
+    return np.concatenate([v, -v]).astype(np.float32)
+
+
+_E4M3 = _e4m3_values()
+
+
+def from_fp8(u) -> np.ndarray:
+    """The values of e4m3 codes (FP8)."""
+    return _E4M3[np.asarray(u, FP8)]
+
+
+def quantize_fp8(a):
+    """A matrix as e4m3 codes (FP8) and one float32 scale a row, as run_rmsnorm_gpu
+    writes them: scale = max(max |row|, 1e-30) / 448, codes a / scale rounded to
+    nearest even.  For weights that are laid out once; finite values only."""
+    a = np.ascontiguousarray(a, np.float32)
+    scale = np.maximum(np.abs(a).max(axis=1, initial=0), np.float32(1e-30)) / np.float32(448)
+    x = np.minimum(np.abs(a / scale[:, None]), np.float32(448)).astype(np.float64)
+    # The distance between neighbouring codes, from the value's exponent.
+    step = np.exp2(np.maximum(np.floor(np.log2(np.maximum(x, 2.0 ** -9))), -6) - 3)
+    v = np.round(x / step) * step  # numpy rounds halves to even
+    codes = np.searchsorted(_E4M3[:127], v).astype(FP8) | np.where(a < 0, 128, 0).astype(FP8)
+    return codes, scale
+
+
 _TYPE = {F32: 0, BF16: 1, FP8: 2}
 
 
