@@ -421,6 +421,8 @@ typedef struct {
     void* y;             int64_t ldy;
     void* workspace;     size_t workspace_bytes;
 } vcsr_linear_args;
+/* Bytes of workspace for the sizes and types of `args` (its pointers are not
+ * read, except which of them are NULL). */
 int vcsr_linear_workspace(const vcsr_linear_args* args, size_t* bytes);
 int vcsr_linear(const vcsr_linear_args* args, void* stream, float* ms);
 
@@ -443,6 +445,7 @@ typedef struct {
     float* dbias;        /* N (zeros for M = 0), or NULL                     */
     void* workspace;     size_t workspace_bytes;
 } vcsr_linear_grad_args;
+/* As vcsr_linear_workspace. */
 int vcsr_linear_grad_workspace(const vcsr_linear_grad_args* args, size_t* bytes);
 int vcsr_linear_grad(const vcsr_linear_grad_args* args, void* stream, float* ms);
 

@@ -240,7 +240,7 @@ def test_linear(gpu, shape, types):
 @pytest.mark.parametrize("types", ["f32 f32", "bf16 bf16", "fp8 bf16"])
 @pytest.mark.parametrize("shape", [(2048, 2048, 192), (4099, 1030, 96), (700, 4096, 640),
                                    (2500, 1000, 72), (513, 8200, 256),
-                                   (7956, 2048, 1024)],
+                                   (7956, 2048, 1024), (5001, 4096, 512)],
                          ids=lambda s: "x".join(map(str, s)))
 def test_linear_many_tiles(gpu, shape, types):
     """Sizes that fill the chip, whole and ragged."""

@@ -813,9 +813,10 @@ def release_workspaces():
 # Bytes of workspace by sizes and types alone (what the _workspace functions
 # answer), so that a call asks the library once for each.
 @functools.lru_cache(maxsize=4096)
-def _linear_bytes(M, N, K, x_type, y_type):
+def _linear_bytes(M, N, K, x_type, y_type, residual, z):
     need = C.c_size_t(0)
-    args = _LinearArgs(M=M, N=N, K=K, x_type=x_type, y_type=y_type)
+    args = _LinearArgs(M=M, N=N, K=K, x_type=x_type, y_type=y_type,
+                       residual=16 if residual else None, z=16 if z else None)
     _check(load_library().vcsr_linear_workspace(C.byref(args), C.byref(need)))
     return need.value
 
@@ -907,7 +908,8 @@ def run_linear_gpu(x, w, y, bias=None, residual=None, act="none", z=None, x_scal
     args = _pack_linear(M, N, K, xt, yt, _act(act), xp, ldx, wp, ldw,
                         _vec(x_scale, M, "x_scale"), _vec(w_scale, N, "w_scale"),
                         _vec(bias, N, "bias"), rp, ldr, zp, ldz, yp, ldy,
-                        *_space(_linear_bytes(M, N, K, xt, yt), workspace, stream))
+                        *_space(_linear_bytes(M, N, K, xt, yt, rp != 0, zp != 0), workspace,
+                                stream))
     return _call((_lib or load_library()).vcsr_linear, args, stream, timed)
 
 

@@ -213,12 +213,14 @@ size_t gemm_workspace(const Gemm& g);
 // dx and dw of one linear layer, in one launch where that is faster.
 hipError_t launch_gemm_pair(const Gemm& dw, const Gemm& dx, hipStream_t st);
 size_t gemm_pair_workspace(const Gemm& dw, const Gemm& dx);
-// What a product's launch does: square tiles (16: the kernel for few rows), and the
-// splits of the sum, of `steps` steps of 128 bytes each; each writes partial sums.
+// What a product's launch does: square tiles (16: the kernel for few rows), the
+// splits of the sum, of `steps` steps of 128 bytes each (each writes partial sums),
+// and how many of its rows (the rest are a product of their own).
 struct GemmPlan {
     int tile;
     int32_t splits;
     int64_t steps;
+    int64_t rows;
 };
 hipError_t launch_gemm_f32(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_gemm_bf16(const Gemm& g, const GemmPlan& p, hipStream_t st);

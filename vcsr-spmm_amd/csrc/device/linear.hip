@@ -67,15 +67,41 @@ void each_split(const Gemm& g, int64_t tiles, F&& f) {
     }
 }
 
+// z and the residual on top of out: their time at 4 TB/s, half of it hidden where
+// there is more than one round of blocks (62451 x 128 x 128 FP32 with a residual: tiles
+// of 64 in two rounds 30.5 us, of 128 in one 33.7).
+float extra_us(const Gemm& g, bool rounds) {
+    const double size = g.out_type == VCSR_F32 ? 4 : 2, count = (g.residual ? 1 : 0) + (g.z ? 1 : 0);
+    return (float)((double)g.I * (double)g.J * size * count / 4e6) * (rounds ? 0.5f : 1.f);
+}
+
+// Rows [from, g.I) of a product.
+Gemm rows_from(Gemm g, int64_t from) {
+    const int64_t size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
+    const int64_t out = g.out_type == VCSR_F32 ? 4 : 2;
+    g.I -= from;
+    if (g.p) g.p = (const char*)g.p + from * size * (g.p_cols ? 1 : g.ldp);
+    if (g.p_scale) g.p_scale += from;
+    if (g.z) g.z = (char*)g.z + from * g.ldz * out;
+    if (g.residual) g.residual = (const char*)g.residual + from * g.ldr * out;
+    if (g.out) g.out = (char*)g.out + from * g.ldo * out;
+    return g;
+}
+
 // Of every tile and number of splits, the one with the least estimated time:
-// whole rounds of blocks, what is left, and the join.
-GemmPlan plan_of(const Gemm& g, float* us_out = nullptr) {
+// whole rounds of blocks, what is left, and the join.  Where a last round would
+// leave most of the chip idle, the rows of the whole rounds go by themselves and the
+// rest as a product of its own, in smaller tiles (5001 x 4096 x 4096 bf16: 320 tiles of
+// 256 on 256 compute units).
+GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true) {
     const int size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
     // Up to 8 rows: W is read straight into the matrix layout, 6 to 9 us up to 32 MB of
     // it against 10 of the tiles (their join is a launch of its own).  Not where
     // few blocks would read long rows alone: 512 x 8000 bf16 16 us against 10.
-    if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || 16 * g.R * size <= 192 << 10))
-        return GemmPlan{16, 1, steps_of(g)};
+    if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || 16 * g.R * size <= 192 << 10)) {
+        if (us_out) *us_out = 7.f;
+        return GemmPlan{16, 1, steps_of(g), g.I};
+    }
     GemmPlan best{};
     float best_us = 0.f;
     const Costs c = costs_of(g);
@@ -84,11 +110,23 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr) {
         each_split(g, tiles, [&](int64_t splits, int64_t steps) {
             const int64_t blocks = tiles * splits, round = kCus * t->room;
             const int64_t rounds = blocks / round, left = blocks - rounds * round;
-            float us = (float)rounds * block_us(g, *t, steps, t->room) + join_us(g, splits);
+            float us = (float)rounds * block_us(g, *t, steps, t->room) + join_us(g, splits) +
+                       extra_us(g, rounds > 0);
             if (left) us += block_us(g, *t, steps, (left + kCus - 1) / kCus);
             if (best.splits == 0 || us < best_us) {
                 best_us = us;
-                best = GemmPlan{t->tile, (int32_t)splits, steps};
+                best = GemmPlan{t->tile, (int32_t)splits, steps, g.I};
+            }
+            if (!may_divide || splits > 1 || rounds < 1 || !left) return;
+            const int64_t per_row = ((int64_t)g.J + t->tile - 1) / t->tile;
+            const int64_t first = rounds * round / per_row * t->tile;
+            if (first < t->tile || first >= g.I) return;
+            float rest_us = 0.f;
+            plan_of(rows_from(g, first), &rest_us, false);
+            us = (float)rounds * block_us(g, *t, steps, t->room) + extra_us(g, true) + rest_us + 2.f;
+            if (us < best_us) {
+                best_us = us;
+                best = GemmPlan{t->tile, 1, steps, first};
             }
         });
     }
@@ -120,8 +158,8 @@ PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
             us += join_us(dw, splits);
             if (us < best_us) {
                 best_us = us;
-                best = PairPlan{true, GemmPlan{t->tile, (int32_t)splits, steps},
-                                GemmPlan{t->tile, 1, steps_of(dx)}};
+                best = PairPlan{true, GemmPlan{t->tile, (int32_t)splits, steps, dw.I},
+                                GemmPlan{t->tile, 1, steps_of(dx), dx.I}};
             }
         });
     }
@@ -129,7 +167,25 @@ PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
 }
 
 size_t part_bytes(const Gemm& g, const GemmPlan& p) {
+    if (p.rows < g.I) {
+        const Gemm rest = rows_from(g, p.rows);
+        return part_bytes(rest, plan_of(rest, nullptr, false));
+    }
     return p.splits > 1 ? (size_t)p.splits * (size_t)g.I * (size_t)tile::part_ld(g.J) * 4 : 0;
+}
+
+hipError_t launch(const Gemm& g, const GemmPlan& p, hipStream_t st) {
+    if (p.rows < g.I) {
+        Gemm first = g;
+        first.I = p.rows;
+        const hipError_t e = launch(first, p, st);
+        if (e != hipSuccess) return e;
+        const Gemm rest = rows_from(g, p.rows);
+        return launch(rest, plan_of(rest, nullptr, false), st);
+    }
+    return g.type == VCSR_F32    ? launch_gemm_f32(g, p, st)
+           : g.type == VCSR_BF16 ? launch_gemm_bf16(g, p, st)
+                                 : launch_gemm_fp8(g, p, st);
 }
 
 }  // namespace
@@ -143,14 +199,6 @@ size_t gemm_pair_workspace(const Gemm& dw, const Gemm& dx) {
     const size_t a = part_bytes(dw, p.dw), b = part_bytes(dx, p.dx);
     return a > b ? a : b;
 }
-
-namespace {
-hipError_t launch(const Gemm& g, const GemmPlan& p, hipStream_t st) {
-    return g.type == VCSR_F32    ? launch_gemm_f32(g, p, st)
-           : g.type == VCSR_BF16 ? launch_gemm_bf16(g, p, st)
-                                 : launch_gemm_fp8(g, p, st);
-}
-}  // namespace
 
 hipError_t launch_gemm(const Gemm& g, hipStream_t st) {
     return g.I <= 0 || g.J <= 0 ? hipSuccess : launch(g, plan_of(g), st);
