@@ -34,95 +34,116 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* part, int32
     }
 }
 
-// A block takes `rows` rows of 8 * TX columns: TX threads of 8 columns a row, 256
-// / TX rows at a time, two of them under way together.  Bound by memory: dy and z
-// read once, dz written once.
-template <class D, class X, int ACT>
+// A block takes `rows` rows of tx vectors of 16 bytes of dy: 256 / tx rows at a time,
+// four of them under way together without a branch between their loads (rows past
+// the block's end are its last one again and count for nothing).  Bound by memory:
+// dy and z read once, dz written once.  ENDS: how rows end: 0 in whole vectors,
+// 1 inside one, 2 before the first is whole.
+template <class D, class X, int ACT, int ENDS>
 __global__ __launch_bounds__(256) void dz_kernel(vcsr_linear_grad_args a, X* dz, int64_t lddz,
-                                                 float* part, int64_t rows, int tx_log) {
-    __shared__ float lds[256 * 8];
-    const int TX = 1 << tx_log, TY = 256 >> tx_log;
-    const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x >> tx_log;
-    const int64_t c = ((int64_t)blockIdx.x * TX + tx) * 8;
-    const int n = c >= a.N ? 0 : a.N - c < 8 ? (int)(a.N - c) : 8;
-    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                                                 float* part, int64_t rows, int tx) {
+    constexpr int U = 4, V = 16 / (int)sizeof(D);
+    __shared__ float lds[256 * V];
+    const int ty_n = 256 / tx, ty = threadIdx.x / tx;
+    const int64_t c = ((int64_t)blockIdx.x * tx + (threadIdx.x - ty * tx)) * V;
+    const int n = c >= a.N ? 0 : a.N - c < V ? (int)(a.N - c) : V;
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
     const int64_t first = (int64_t)blockIdx.y * rows;
     const int64_t last = first + rows < a.M ? first + rows : a.M;
-    if (n > 0) {
-        for (int64_t m = first + ty; m < last; m += 2 * TY) {
-            float d[2][8], z[2][8];
+    if (n > 0 && ty < ty_n) {
+        auto load = [&](const D* row, float(&v)[V]) __attribute__((always_inline)) {
+            if (ENDS == 0)
+                load_full(row + c, v);
+            else if (ENDS == 1)
+                load_tail(row, (int)c, a.N, v);
+            else
+                load_vec(row + c, n, v);
+        };
+        for (int64_t m = first + ty; m < last; m += U * ty_n) {
+            float d[U][V], z[U][V];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int64_t r = m + u * TY;
-                if (r >= last) continue;
-                load_vec((const D*)a.dy + r * a.lddy + c, n, d[u]);
-                if (ACT != VCSR_ACT_NONE) load_vec((const D*)a.z + r * a.ldz + c, n, z[u]);
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = m + u * ty_n < last ? m + u * ty_n : last - 1;
+                load((const D*)a.dy + r * a.lddy, d[u]);
+                if (ACT != VCSR_ACT_NONE) load((const D*)a.z + r * a.ldz, z[u]);
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int64_t r = m + u * TY;
-                if (r >= last) continue;
+            for (int u = 0; u < U; ++u) {
+                if (m + u * ty_n >= last) continue;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < V; ++i) {
                     if (ACT != VCSR_ACT_NONE) d[u][i] *= act_grad_f32<ACT>(z[u][i]);
-                    if (i >= n) d[u][i] = 0.f;  // act'(0) of what is not there
-                    sum[i] += d[u][i];
+                    if (ENDS == 0 || i < n) sum[i] += d[u][i];
                 }
-                if (dz) store_vec(dz + r * lddz + c, n, d[u]);
+                if (dz) store_vec(dz + (m + u * ty_n) * lddz + c, ENDS == 0 ? V : n, d[u]);
             }
         }
     }
     if (!part) return;
+    if (ty < ty_n)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lds[(ty * TX + tx) * 8 + i] = sum[i];
+        for (int i = 0; i < V; ++i) lds[threadIdx.x * V + i] = sum[i];
     __syncthreads();
-    for (int col = threadIdx.x; col < TX * 8; col += 256) {
-        const int64_t at = (int64_t)blockIdx.x * TX * 8 + col;
+    for (int col = threadIdx.x; col < tx * V; col += 256) {
+        const int64_t at = (int64_t)blockIdx.x * tx * V + col;
         if (at >= a.N) continue;
         float t = 0.f;
-        for (int g = 0; g < TY; ++g) t += lds[g * TX * 8 + col];
+        for (int g = 0; g < ty_n; ++g) t += lds[g * tx * V + col];
         part[(int64_t)blockIdx.y * a.N + at] = t;
     }
 }
 
-// Threads along a row (8, 16 or 32) and rows of a block: at least four passes of its
-// threads, and few enough blocks of rows that their partial sums stay small.
+// Vectors of a block's rows (even parts of a row's, at most 128, that leave few of
+// its threads idle) and its rows: two
+// passes of its threads at least, and few enough blocks of rows that their partial
+// sums stay small.
 struct DzShape {
-    int tx_log;
-    int64_t rows, blocks;
+    int tx;
+    int64_t columns, rows, blocks;
 };
-DzShape dz_shape(int64_t M, int32_t N) {
+DzShape dz_shape(int64_t M, int32_t N, int32_t dy_type) {
     DzShape s;
-    // As wide as leaves few threads past the row's end.
-    const int32_t vectors = (N + 7) / 8;
-    s.tx_log = 5;
-    while (s.tx_log > 3 && ((vectors + (1 << s.tx_log) - 1) >> s.tx_log << s.tx_log) >
-                               vectors + vectors / 8)
-        --s.tx_log;
-    s.rows = 4 * (256 >> s.tx_log);
+    const int64_t v = dy_type == VCSR_F32 ? 4 : 8, vectors = ((int64_t)N + v - 1) / v;
+    double best = 0.0;
+    for (int64_t k = (vectors + 127) / 128, end = k + 4; k < end; ++k) {
+        const int64_t tx = (vectors + k - 1) / k, columns = (vectors + tx - 1) / tx;
+        // Of the block's threads and of their vectors, those that are there.
+        const double used = (double)(256 / tx * tx) * (double)vectors / (double)(tx * columns);
+        if (used > best * 1.02) {
+            best = used;
+            s.tx = (int)tx;
+            s.columns = columns;
+        }
+    }
+    s.rows = 8 * (256 / s.tx);
     while ((M + s.rows - 1) / s.rows > 1024) s.rows *= 2;
     s.blocks = (M + s.rows - 1) / s.rows;
     return s;
 }
 
+template <class D, class X, int ACT>
+void launch_dz_act(const vcsr_linear_grad_args& a, X* dz, int64_t lddz, float* part,
+                   hipStream_t st) {
+    constexpr int V = 16 / (int)sizeof(D);
+    const DzShape s = dz_shape(a.M, a.N, a.y_type);
+    const dim3 grid((unsigned)s.columns, (unsigned)s.blocks);
+    if (a.N % V == 0)
+        dz_kernel<D, X, ACT, 0><<<grid, 256, 0, st>>>(a, dz, lddz, part, s.rows, s.tx);
+    else if (a.N > V)
+        dz_kernel<D, X, ACT, 1><<<grid, 256, 0, st>>>(a, dz, lddz, part, s.rows, s.tx);
+    else
+        dz_kernel<D, X, ACT, 2><<<grid, 256, 0, st>>>(a, dz, lddz, part, s.rows, s.tx);
+}
 template <class D, class X>
 hipError_t launch_dz_typed(const vcsr_linear_grad_args& a, X* dz, int64_t lddz, float* part,
                            hipStream_t st) {
-    const DzShape s = dz_shape(a.M, a.N);
-    const int cols = 8 << s.tx_log;
-    const dim3 grid((unsigned)(((int64_t)a.N + cols - 1) / cols), (unsigned)s.blocks);
     switch (a.act) {
-        case VCSR_ACT_RELU:
-            dz_kernel<D, X, VCSR_ACT_RELU><<<grid, 256, 0, st>>>(a, dz, lddz, part, s.rows, s.tx_log);
-            break;
-        case VCSR_ACT_GELU:
-            dz_kernel<D, X, VCSR_ACT_GELU><<<grid, 256, 0, st>>>(a, dz, lddz, part, s.rows, s.tx_log);
-            break;
-        case VCSR_ACT_SILU:
-            dz_kernel<D, X, VCSR_ACT_SILU><<<grid, 256, 0, st>>>(a, dz, lddz, part, s.rows, s.tx_log);
-            break;
-        default:
-            dz_kernel<D, X, VCSR_ACT_NONE><<<grid, 256, 0, st>>>(a, dz, lddz, part, s.rows, s.tx_log);
+        case VCSR_ACT_RELU: launch_dz_act<D, X, VCSR_ACT_RELU>(a, dz, lddz, part, st); break;
+        case VCSR_ACT_GELU: launch_dz_act<D, X, VCSR_ACT_GELU>(a, dz, lddz, part, st); break;
+        case VCSR_ACT_SILU: launch_dz_act<D, X, VCSR_ACT_SILU>(a, dz, lddz, part, st); break;
+        default: launch_dz_act<D, X, VCSR_ACT_NONE>(a, dz, lddz, part, st);
     }
     return hipGetLastError();
 }
@@ -141,7 +162,9 @@ hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, 
     return hipGetLastError();
 }
 
-int32_t dz_row_blocks(int64_t M, int32_t N) { return (int32_t)dz_shape(M, N).blocks; }
+int32_t dz_row_blocks(int64_t M, int32_t N, int32_t dy_type) {
+    return (int32_t)dz_shape(M, N, dy_type).blocks;
+}
 
 hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, float* part,
                      hipStream_t st) {

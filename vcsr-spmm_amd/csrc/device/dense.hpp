@@ -180,10 +180,10 @@ size_t rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args& a);
 hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, float* out,
                            hipStream_t st);
 // dz = dy * act'(z) in x_type (dz may be NULL) and, for each block of
-// dz_row_blocks(M, N), the sums of its rows of dz in `part` (ld N; may be NULL).
+// dz_row_blocks(M, N, type of dy), the sums of its rows of dz in `part` (ld N; may be NULL).
 hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, float* part,
                      hipStream_t st);
-int32_t dz_row_blocks(int64_t M, int32_t N);
+int32_t dz_row_blocks(int64_t M, int32_t N, int32_t dy_type);
 // n bytes of zeros, by a kernel.
 hipError_t launch_zero(void* p, int64_t bytes, hipStream_t st);
 

@@ -201,7 +201,7 @@ LinearGrad grad_of(const vcsr_linear_grad_args* args) {
     w.lddz = w.own_dz ? ((int64_t)a.N + 7) / 8 * 8 : a.lddy;
     if (w.own_dz) w.dz_bytes = round_up((size_t)a.M * (size_t)w.lddz * size_of(a.x_type));
     if (a.dbias)
-        w.bias_bytes = round_up((size_t)vcsr::dz_row_blocks(a.M, a.N) * (size_t)a.N * 4);
+        w.bias_bytes = round_up((size_t)vcsr::dz_row_blocks(a.M, a.N, a.y_type) * (size_t)a.N * 4);
     char* base = (char*)a.workspace;
     const void* dz = w.own_dz ? (const void*)base : a.dy;
     float* part = (float*)(base + w.dz_bytes + w.bias_bytes);
@@ -278,7 +278,7 @@ hipError_t run_grad(const LinearGrad& w, hipStream_t st) {
     if (w.own_dz || bias_part) {
         e = vcsr::launch_dz(a, w.own_dz ? base : nullptr, w.lddz, bias_part, st);
         if (e == hipSuccess && bias_part)
-            e = vcsr::launch_sum_rows(bias_part, vcsr::dz_row_blocks(a.M, a.N), a.N, a.N, a.dbias,
+            e = vcsr::launch_sum_rows(bias_part, vcsr::dz_row_blocks(a.M, a.N, a.y_type), a.N, a.N, a.dbias,
                                       st);
     }
     if (e != hipSuccess || (!a.dx && !a.dw)) return e;
