@@ -136,7 +136,7 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
 
 // Both products in one launch, if that is estimated faster than one after the
 // other: all blocks' time over the chip's room and part of a last block, or the
-// longest block, and dw's join.  (8192 x 2048 x 4096 bf16: dw has 128 tiles of 256, dx 256.)
+// longest block alone, and dw's join.  (8192 x 2048 x 4096 bf16: dw has 128 tiles of 256, dx 256.)
 struct PairPlan {
     bool together;
     GemmPlan dw, dx;
@@ -149,12 +149,14 @@ PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
     for (const TileCost* t = c.t; t < c.t + c.n; ++t) {
         const int64_t tiles_w = tiles_of(dw, t->tile), tiles_x = tiles_of(dx, t->tile);
         if (tiles_x > 64 * kCus) continue;  // long by itself: nothing to gain
-        const float one_x = block_us(dx, *t, steps_of(dx), t->room);
         each_split(dw, tiles_w, [&](int64_t splits, int64_t steps) {
-            const float one_w = block_us(dw, *t, steps, t->room);
+            const int64_t per_cu = (tiles_w * splits + tiles_x + kCus - 1) / kCus;
+            const int64_t b = per_cu < t->room ? per_cu : t->room;
+            const float one_w = block_us(dw, *t, steps, b), one_x = block_us(dx, *t, steps_of(dx), b);
             float us = ((float)(tiles_w * splits) * one_w + (float)tiles_x * one_x) /
-                           (float)(kCus * t->room) + 0.25f * one_x;
+                           (float)(kCus * b) + 0.25f * one_x;
             if (us < one_w) us = one_w;
+            if (us < one_x) us = one_x;
             us += join_us(dw, splits);
             if (us < best_us) {
                 best_us = us;

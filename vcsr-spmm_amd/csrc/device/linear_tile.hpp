@@ -313,13 +313,15 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t i, int j, float (&
     }
     store_vec((O*)g.out + i * g.ldo + j, N, v);
 }
-// The last columns of row i, fewer than 8 from j, whose sums lie in LDS.
-template <class O>
-__device__ __forceinline__ void finish_tail(const Gemm& g, int64_t i, int j, const float* sums) {
-#pragma unroll 1
-    for (int k = 0; j + k < g.J; ++k) {
-        float v[1] = {sums[k]};
-        finish<O>(g, i, j + k, v);
+// 8 columns of a row, or the first n of them (the others are its last one again),
+// with all loads under way together.
+template <class T>
+__device__ __forceinline__ void load_cols(const T* p, int n, float (&v)[8]) {
+    if (n == 8) {
+        load_full(p, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = to_f32(p[k < n ? k : n - 1]);
     }
 }
 
@@ -373,8 +375,9 @@ __device__ __forceinline__ int64_t extent(int64_t n, int64_t r, int64_t ld, bool
 // few blocks of rows at a time, so that its lanes go along rows of out: 8
 // consecutive columns a lane, the same ones in every row.  (Stores straight from
 // the matrix layout write half lines: 70 against 65 us for 8192 x 8192 at K = 128.)
-// PLAIN: out alone, as the gradients need it.
-template <class O, int ACT, bool PLAIN, bool PART, int FI, int FJ, int ROOM>
+// PLAIN: out alone, as the gradients need it.  WHOLE: all of the wave's columns
+// are there (no branch then keeps loads and stores from being under way together).
+template <class O, int ACT, bool PLAIN, bool PART, bool WHOLE, int FI, int FJ, int ROOM>
 __device__ __forceinline__ void write_rows(const Gemm& g, const f32x4 (&acc)[FI][FJ], float* mine,
                                            int64_t i_first, int64_t j_first, uint32_t split) {
     constexpr int CW = FJ * 16, LD = CW + 4;  // 4 floats on: rows start in other banks
@@ -385,11 +388,11 @@ __device__ __forceinline__ void write_rows(const Gemm& g, const f32x4 (&acc)[FI]
     const int lane = threadIdx.x & 63;
     const int col = lane % LANES * 8;
     const int64_t j = j_first + col;
-    const int n = g.J - j < 8 ? (int)(g.J - j) : 8;
+    const int n = WHOLE || g.J - j > 8 ? 8 : (int)(g.J - j);
     float bias[8], scale[8];
-    if (!PLAIN && !PART && n == 8) {
-        if (g.bias) load_vec(g.bias + j, 8, bias);
-        if (g.q_scale) load_vec(g.q_scale + j, 8, scale);
+    if (!PLAIN && !PART && n > 0) {
+        if (g.bias) load_cols(g.bias + j, n, bias);
+        if (g.q_scale) load_cols(g.q_scale + j, n, scale);
     }
 #pragma unroll
     for (int r = 0; r < FI; r += XB) {
@@ -400,13 +403,7 @@ __device__ __forceinline__ void write_rows(const Gemm& g, const f32x4 (&acc)[FI]
                 *(f32x4*)(mine + (x * 16 + (lane & 15)) * LD + (y >> 1) * 32 + (lane >> 4) * 8 +
                           (y & 1) * 4) = acc[r + x][y];
         __builtin_amdgcn_wave_barrier();
-        if (!PART && n > 0 && n < 8) {
-#pragma unroll 1
-            for (int row = lane / LANES; row < XB * 16; row += 64 / LANES) {
-                const int64_t i = i_first + r * 16 + row;
-                if (i < g.I) finish_tail<O>(g, i, (int)j, mine + row * LD + col);
-            }
-        } else if (n > 0) {
+        if (n > 0) {
 #pragma unroll
             for (int step = 0; step < XB * 16 * LANES / 64; ++step) {
                 const int row = step * (64 / LANES) + lane / LANES;
@@ -430,43 +427,47 @@ __device__ __forceinline__ void write_rows(const Gemm& g, const f32x4 (&acc)[FI]
 #pragma unroll
                         for (int k = 0; k < 8; ++k) v[k] += bias[k];
                     }
-                    if (g.z) store_vec((O*)g.z + i * g.ldz + j, 8, v);
+                    if (g.z) store_vec((O*)g.z + i * g.ldz + j, n, v);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) v[k] = act_f32<ACT>(v[k]);
                     if (g.residual) {
                         float res[8];
-                        load_vec((const O*)g.residual + i * g.ldr + j, 8, res);
+                        load_cols((const O*)g.residual + i * g.ldr + j, n, res);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) v[k] += res[k];
                     }
                 }
-                store_vec((O*)g.out + i * g.ldo + j, 8, v);
+                store_vec((O*)g.out + i * g.ldo + j, n, v);
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
-template <class O, bool PLAIN, int ROOM, int FI, int FJ>
+template <class O, bool PLAIN, bool WHOLE, int ROOM, int FI, int FJ>
 __device__ __forceinline__ void write_typed(const Gemm& g, const f32x4 (&acc)[FI][FJ], float* mine,
                                             int64_t i, int64_t j) {
     if (PLAIN || g.act == VCSR_ACT_NONE)
-        write_rows<O, VCSR_ACT_NONE, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+        write_rows<O, VCSR_ACT_NONE, PLAIN, false, WHOLE, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
     else if (g.act == VCSR_ACT_RELU)
-        write_rows<O, VCSR_ACT_RELU, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+        write_rows<O, VCSR_ACT_RELU, PLAIN, false, WHOLE, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
     else if (g.act == VCSR_ACT_GELU)
-        write_rows<O, VCSR_ACT_GELU, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+        write_rows<O, VCSR_ACT_GELU, PLAIN, false, WHOLE, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
     else
-        write_rows<O, VCSR_ACT_SILU, PLAIN, false, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
+        write_rows<O, VCSR_ACT_SILU, PLAIN, false, WHOLE, FI, FJ, ROOM>(g, acc, mine, i, j, 0);
 }
 template <bool PLAIN, int ROOM, int FI, int FJ>
 __device__ __forceinline__ void write_out(const Gemm& g, const f32x4 (&acc)[FI][FJ], float* mine,
                                           int64_t i, int64_t j, int splits, uint32_t split) {
     if (splits > 1)
-        write_rows<float, VCSR_ACT_NONE, true, true, FI, FJ, ROOM>(g, acc, mine, i, j, split);
+        write_rows<float, VCSR_ACT_NONE, true, true, false, FI, FJ, ROOM>(g, acc, mine, i, j, split);
+    else if (j + FJ * 16 <= g.J && g.out_type == VCSR_BF16)
+        write_typed<bf16, PLAIN, true, ROOM>(g, acc, mine, i, j);
+    else if (j + FJ * 16 <= g.J)
+        write_typed<float, PLAIN, true, ROOM>(g, acc, mine, i, j);
     else if (g.out_type == VCSR_BF16)
-        write_typed<bf16, PLAIN, ROOM>(g, acc, mine, i, j);
+        write_typed<bf16, PLAIN, false, ROOM>(g, acc, mine, i, j);
     else
-        write_typed<float, PLAIN, ROOM>(g, acc, mine, i, j);
+        write_typed<float, PLAIN, false, ROOM>(g, acc, mine, i, j);
 }
 
 // Whether the sum's last step goes through registers: its granules are not all
