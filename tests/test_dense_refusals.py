@@ -73,8 +73,6 @@ GRAD = {
     "8-bit dy": dict(dy=f8(4, 8)),
     "dx of another type": dict(dx=bf(4, 8)),
     "no rstd": dict(rstd=None),
-    "short workspace": dict(dweight=mat(8), workspace=f8(16)),
-    "misaligned workspace": dict(dweight=mat(8), workspace=f8(1 << 20, ptr=4104)),
 }
 
 
@@ -83,6 +81,14 @@ def test_rmsnorm_grad_refuses(vs, case):
     kw = dict(dy=mat(4, 8), s=mat(4, 8), weight=mat(8), rstd=mat(4), dx=mat(4, 8))
     kw.update(GRAD[case])
     refused(vs, vs.VCSR_EINVAL, vs.run_rmsnorm_grad_gpu, **kw)
+
+
+@pytest.mark.parametrize("ws", [f8(16), f8(1 << 20, ptr=4104)], ids=["short", "misaligned"])
+def test_rmsnorm_grad_refuses_a_workspace(vs, ws):
+    """Many rows: dweight goes through partial sums."""
+    M = 5000
+    refused(vs, vs.VCSR_EINVAL, vs.run_rmsnorm_grad_gpu, dy=mat(M, 8), s=mat(M, 8), weight=mat(8),
+            rstd=mat(M), dx=mat(M, 8), dweight=mat(8), workspace=ws)
 
 
 LINEAR = {

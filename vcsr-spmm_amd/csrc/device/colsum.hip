@@ -118,6 +118,7 @@ DzShape dz_shape(int64_t M, int32_t N, int32_t dy_type) {
         }
     }
     s.rows = 8 * (256 / s.tx);
+    if (M <= 2 * s.rows) s.rows *= 2;  // one block of rows: no partial sums to add up
     while ((M + s.rows - 1) / s.rows > 1024) s.rows *= 2;
     s.blocks = (M + s.rows - 1) / s.rows;
     return s;

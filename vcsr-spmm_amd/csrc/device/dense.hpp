@@ -210,8 +210,14 @@ struct Gemm {
 };
 hipError_t launch_gemm(const Gemm& g, hipStream_t st);
 size_t gemm_workspace(const Gemm& g);
-// dx and dw of one linear layer, in one launch where that is faster.
-hipError_t launch_gemm_pair(const Gemm& dw, const Gemm& dx, hipStream_t st);
+// Partial rows of C columns still to be added up (none for P = 0).
+struct RowSum {
+    const float* part = nullptr;
+    float* out = nullptr;
+    int32_t P = 0, C = 0;
+};
+// dx and dw of one linear layer, in one launch where that is faster, and dbias.
+hipError_t launch_gemm_pair(const Gemm& dw, const Gemm& dx, const RowSum& bias, hipStream_t st);
 size_t gemm_pair_workspace(const Gemm& dw, const Gemm& dx);
 // What a product's launch does: square tiles (16: the kernel for few rows), the
 // splits of the sum, of `steps` steps of 128 bytes each (each writes partial sums),
@@ -225,9 +231,9 @@ struct GemmPlan {
 hipError_t launch_gemm_f32(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_gemm_bf16(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_pair_f32(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
-                           hipStream_t st);
+                           const RowSum& bias, hipStream_t st);
 hipError_t launch_pair_bf16(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
-                            hipStream_t st);
+                            const RowSum& bias, hipStream_t st);
 hipError_t launch_gemm_fp8(const Gemm& g, const GemmPlan& p, hipStream_t st);
 
 // --------------------------------------------------------------- adamw.hip

@@ -274,15 +274,18 @@ hipError_t run_grad(const LinearGrad& w, hipStream_t st) {
         return e;
     }
     char* base = (char*)a.workspace;
-    float* bias_part = a.dbias ? (float*)(base + w.dz_bytes) : nullptr;
-    if (w.own_dz || bias_part) {
+    // A single block of rows writes dbias itself.
+    const int32_t row_blocks = vcsr::dz_row_blocks(a.M, a.N, a.y_type);
+    float* const bias_part =
+        !a.dbias ? nullptr : row_blocks == 1 ? a.dbias : (float*)(base + w.dz_bytes);
+    vcsr::RowSum bias;
+    if (a.dbias && row_blocks > 1) bias = vcsr::RowSum{bias_part, a.dbias, row_blocks, a.N};
+    if (w.own_dz || bias_part)
         e = vcsr::launch_dz(a, w.own_dz ? base : nullptr, w.lddz, bias_part, st);
-        if (e == hipSuccess && bias_part)
-            e = vcsr::launch_sum_rows(bias_part, vcsr::dz_row_blocks(a.M, a.N, a.y_type), a.N, a.N, a.dbias,
-                                      st);
-    }
+    if (e == hipSuccess && a.dx && a.dw) return vcsr::launch_gemm_pair(w.dw, w.dx, bias, st);
+    if (e == hipSuccess && bias.P > 0)
+        e = vcsr::launch_sum_rows(bias.part, bias.P, bias.C, bias.C, bias.out, st);
     if (e != hipSuccess || (!a.dx && !a.dw)) return e;
-    if (a.dx && a.dw) return vcsr::launch_gemm_pair(w.dw, w.dx, st);
     return vcsr::launch_gemm(a.dx ? w.dx : w.dw, st);
 }
 

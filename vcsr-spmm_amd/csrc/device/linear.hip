@@ -97,8 +97,9 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
     const int size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
     // Up to 8 rows: W is read straight into the matrix layout, 6 to 9 us up to 32 MB of
     // it against 10 of the tiles (their join is a launch of its own).  Not where
-    // few blocks would read long rows alone: 512 x 8000 bf16 16 us against 10.
-    if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || 16 * g.R * size <= 192 << 10)) {
+    // few blocks would read long rows alone, past what a wave asks for at once: 512 x
+    // 8000 bf16 16 us against 10.
+    if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || g.R * size <= 64 * 128)) {
         if (us_out) *us_out = 7.f;
         return GemmPlan{16, 1, steps_of(g), g.I};
     }
@@ -206,12 +207,14 @@ hipError_t launch_gemm(const Gemm& g, hipStream_t st) {
     return g.I <= 0 || g.J <= 0 ? hipSuccess : launch(g, plan_of(g), st);
 }
 
-hipError_t launch_gemm_pair(const Gemm& dw, const Gemm& dx, hipStream_t st) {
+hipError_t launch_gemm_pair(const Gemm& dw, const Gemm& dx, const RowSum& bias, hipStream_t st) {
     const PairPlan p = plan_pair(dw, dx);
     if (p.together)
-        return dw.type == VCSR_F32 ? launch_pair_f32(dw, p.dw, dx, p.dx, st)
-                                   : launch_pair_bf16(dw, p.dw, dx, p.dx, st);
-    const hipError_t e = launch(dx, p.dx, st);
+        return dw.type == VCSR_F32 ? launch_pair_f32(dw, p.dw, dx, p.dx, bias, st)
+                                   : launch_pair_bf16(dw, p.dw, dx, p.dx, bias, st);
+    hipError_t e = hipSuccess;
+    if (bias.P > 0) e = launch_sum_rows(bias.part, bias.P, bias.C, bias.C, bias.out, st);
+    if (e == hipSuccess) e = launch(dx, p.dx, st);
     return e != hipSuccess ? e : launch(dw, p.dw, st);
 }
 

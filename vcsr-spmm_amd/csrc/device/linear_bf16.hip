@@ -10,8 +10,8 @@ hipError_t launch_gemm_bf16(const Gemm& g, const GemmPlan& p, hipStream_t st) {
 }
 
 hipError_t launch_pair_bf16(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
-                            hipStream_t st) {
-    return tile::launch_pair<bf16>(dw, p, dx, q, st);
+                            const RowSum& bias, hipStream_t st) {
+    return tile::launch_pair<bf16>(dw, p, dx, q, bias, st);
 }
 
 }  // namespace vcsr

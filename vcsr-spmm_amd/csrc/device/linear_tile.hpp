@@ -717,15 +717,39 @@ __global__ __launch_bounds__(kThreads<TILE>) void gemm_kernel(Gemm g, Part part)
     gemm_block<T, TILE, PCOLS, QCOLS>(g, part, blockIdx.x, lds);
 }
 
+// Columns [16 * block, + 16) of the sum of partial rows, in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ void sum_columns(const RowSum& r, uint32_t block, uint8_t* lds) {
+    constexpr int G = THREADS / 16;
+    float(*const t)[17] = (float(*)[17])lds;
+    const int col = threadIdx.x & 15, grp = threadIdx.x >> 4;
+    const int64_t c = (int64_t)block * 16 + col;
+    float v = 0.f;
+    if (c < r.C) {
+#pragma unroll 8
+        for (int32_t p = grp; p < r.P; p += G) v += r.part[(int64_t)p * r.C + c];
+    }
+    t[grp][col] = v;
+    __syncthreads();
+    if (grp == 0 && c < r.C) {
+#pragma unroll
+        for (int g = 1; g < G; ++g) v += t[g][col];
+        r.out[c] = v;
+    }
+}
+
 // Both products of a gradient in one launch: dw's blocks first, whose sums over the
-// rows are long, then dx's (from a multiple of 8 on, so that both keep their XCDs).
-// Each product by itself leaves compute units idle at its end.
+// rows are long, then dx's (from a multiple of 8 on, so that both keep their XCDs),
+// then those that add up dbias' partial rows.  Each product by itself leaves
+// compute units idle at its end.
 template <class T, int TILE>
 __global__ __launch_bounds__(kThreads<TILE>) void gemm_pair_kernel(Gemm dw, Part dw_part, Gemm dx,
-                                                                   Part dx_part) {
+                                                                   Part dx_part, RowSum bias) {
     __shared__ __attribute__((aligned(128))) uint8_t lds[kSharedLds<TILE, TILE>];
     const uint32_t first = (dw_part.blocks + 7) & ~7u;
-    if (blockIdx.x >= first)
+    if (blockIdx.x >= first + dx_part.blocks)
+        sum_columns<kThreads<TILE>>(bias, blockIdx.x - first - dx_part.blocks, lds);
+    else if (blockIdx.x >= first)
         gemm_block<T, TILE, false, true>(dx, dx_part, blockIdx.x - first, lds);
     else if (blockIdx.x < dw_part.blocks)
         gemm_block<T, TILE, true, true>(dw, dw_part, blockIdx.x, lds);
@@ -943,15 +967,16 @@ hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
 
 template <class T>
 hipError_t launch_pair(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
-                       hipStream_t st) {
+                       const RowSum& bias, hipStream_t st) {
     const Part a = part_of(dw, p), b = part_of(dx, q);
-    const uint32_t blocks = ((a.blocks + 7) & ~7u) + b.blocks;
+    const uint32_t blocks = ((a.blocks + 7) & ~7u) + b.blocks +
+                            (bias.P > 0 ? (uint32_t)(((int64_t)bias.C + 15) / 16) : 0);
     if (p.tile == 64)
-        gemm_pair_kernel<T, 64><<<blocks, kThreads<64>, 0, st>>>(dw, a, dx, b);
+        gemm_pair_kernel<T, 64><<<blocks, kThreads<64>, 0, st>>>(dw, a, dx, b, bias);
     else if (p.tile == 128)
-        gemm_pair_kernel<T, 128><<<blocks, kThreads<128>, 0, st>>>(dw, a, dx, b);
+        gemm_pair_kernel<T, 128><<<blocks, kThreads<128>, 0, st>>>(dw, a, dx, b, bias);
     else if constexpr (sizeof(T) < 4)
-        gemm_pair_kernel<T, 256><<<blocks, kThreads<256>, 0, st>>>(dw, a, dx, b);
+        gemm_pair_kernel<T, 256><<<blocks, kThreads<256>, 0, st>>>(dw, a, dx, b, bias);
     hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_join(dw, p.splits, st);
 }

@@ -339,10 +339,17 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_grad_kernel(
         }
         return;
     }
-    // The block's row groups add up in LDS, one after the other.
+    // A wave's row groups add up over its lanes, then the waves in LDS, one after
+    // the other.
+    for (int m = lanes; m < 64; m <<= 1)
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) dw[k][i] += __shfl_xor(dw[k][i], m);
     __syncthreads();
-    for (int g = 0; g < rows; ++g) {
-        if (sub == g)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        if (tid >> 6 == g && (tid & 63) < lanes)
 #pragma unroll
             for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -427,6 +434,7 @@ GradShape grad_shape(const vcsr_rmsnorm_grad_args& a) {
     const int64_t waves = g.row.wpr > 1 ? g.row.wpr : 4;
     const int64_t need = (a.M + rows - 1) / rows, most = 2048 / waves;
     g.blocks = (int32_t)(need < most ? need : most);
+    if (need <= 4) g.blocks = 1;  // which then writes dweight itself
     g.in_registers = g.nv <= 2048 && a.C >= v;
     if (!g.in_registers) g.blocks = (int32_t)(a.M < 64 ? a.M : 64);
     return g;
@@ -435,7 +443,7 @@ GradShape grad_shape(const vcsr_rmsnorm_grad_args& a) {
 template <class X, class D>
 hipError_t launch_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
     const GradShape g = grad_shape(a);
-    float* part = a.dweight ? (float*)a.workspace : nullptr;
+    float* const part = !a.dweight ? nullptr : g.blocks == 1 ? a.dweight : (float*)a.workspace;
     if (!g.in_registers) {
         rmsnorm_grad_long_kernel<X, D><<<(unsigned)a.M, 1024, 0, st>>>(a);
         if (part)
@@ -449,7 +457,7 @@ hipError_t launch_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
         });
     }
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !part) return e;
+    if (e != hipSuccess || !part || g.blocks == 1) return e;
     return launch_sum_rows(part, g.blocks, a.C, a.C, a.dweight, st);
 }
 
@@ -468,7 +476,8 @@ hipError_t launch_rmsnorm(const vcsr_rmsnorm_args& a, hipStream_t st) {
 
 size_t rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args& a) {
     if (!a.dweight || a.M <= 0) return 0;
-    return (size_t)grad_shape(a).blocks * (size_t)a.C * sizeof(float);
+    const int32_t blocks = grad_shape(a).blocks;
+    return blocks > 1 ? (size_t)blocks * (size_t)a.C * sizeof(float) : 0;
 }
 
 hipError_t launch_rmsnorm_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
