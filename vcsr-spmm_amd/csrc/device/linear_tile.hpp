@@ -46,11 +46,17 @@ template <bool Q>
 __device__ __forceinline__ int key_rows(int r) {
     return Q ? key_q(r) : key_p(r);
 }
-// Key of k-row k of a tile by columns with `gran` granules a k-row.
-template <class T, int GRAN>
+// Key of k-row k of a tile by columns with GRAN granules a k-row.  bf16: 16 lanes
+// read 4 k-rows, of each two granules (P) or halves of four (Q).  FP32: four groups
+// of 16 lanes read k-rows 4 apart, of each four granules in a row (P) or every
+// second (Q), which these keys put on different banks (35% of the LDS cycles were
+// conflicts with one key for both).  For bf16's Q, keys that spread the granules
+// further made 128 x 128 tiles slower (8192 x 2048 x 4096: 179 against 156 us).
+template <class T, int GRAN, bool Q>
 __device__ __forceinline__ int key_cols(int k) {
     if (sizeof(T) == 2) return (((k & 3) | ((k >> 1) & 4)) << 1) & (GRAN - 1);
-    return ((k >> 2) & 3) << 2 & (GRAN - 1);
+    const int q = (k >> 2) & 3;
+    return Q ? (q & 1) | (q >> 1) << 3 : q << 2;
 }
 
 struct Operand {
@@ -85,7 +91,7 @@ struct Loader {
     __device__ __forceinline__ static void place(int e, int& row, int& k) {
         if (COLS) {
             k = e / KGRAN;
-            row = ((e % KGRAN) ^ key_cols<T, KGRAN>(k)) * EPG;
+            row = ((e % KGRAN) ^ key_cols<T, KGRAN, Q>(k)) * EPG;
         } else {
             row = e >> 3;
             k = ((e & 7) ^ key_rows<Q>(row)) * EPG;
@@ -201,7 +207,7 @@ struct Reader<bf16, ROWS, true, Q> {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int k = s * 32 + (lane >> 4) * 8 + h * 4 + (t >> 2);
-            const int at = k * ROWS * 2 + (((col >> 3) ^ key_cols<bf16, GRAN>(k)) << 4) +
+            const int at = k * ROWS * 2 + (((col >> 3) ^ key_cols<bf16, GRAN, Q>(k)) << 4) +
                            (col & 7) * 2;
             const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) s16x4*)(lds + at));
@@ -220,7 +226,7 @@ struct Reader<float, ROWS, true, Q> {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int k = s * 16 + (lane >> 4) * 4 + j;
-            const int at = k * ROWS * 4 + (((col >> 2) ^ key_cols<float, GRAN>(k)) << 4) +
+            const int at = k * ROWS * 4 + (((col >> 2) ^ key_cols<float, GRAN, Q>(k)) << 4) +
                            (col & 3) * 4;
             v[j] = *(const uint32_t*)(lds + at);
         }
