@@ -57,6 +57,10 @@ NORM = {
     "misaligned x": dict(x=mat(4, 8, ptr=4098)),
     "misaligned rstd": dict(rstd=mat(4, ptr=4097)),
     "y over x of another type": dict(x=mat(4, 8, ptr=8192), y=bf(4, 8, ptr=8192)),
+    "y over residual of another type": dict(residual=mat(4, 8, ptr=8192), y=bf(4, 8, ptr=8192)),
+    "sum over y": dict(sum=mat(4, 8, ptr=65536)),
+    "sum over x of another stride": dict(x=mat(4, 8, ptr=8192),
+                                         sum=mat(4, 8, ptr=8192, ld=9, nbytes=4096)),
     "no columns": dict(x=mat(4, 0), y=mat(4, 0), weight=mat(0)),
 }
 
@@ -103,6 +107,10 @@ LINEAR = {
     "unknown activation": dict(act="tanh"),
     "residual of another type": dict(residual=bf(4, 5)),
     "z over y": dict(y=mat(4, 5, ptr=8192), z=mat(4, 5, ptr=8192)),
+    "z over residual": dict(y=mat(4, 5, ptr=65536), z=mat(4, 5, ptr=8192),
+                            residual=mat(4, 5, ptr=8192)),
+    "residual over y of another stride": dict(y=mat(4, 5, ptr=8192),
+                                              residual=mat(4, 5, ptr=8192, ld=9, nbytes=4096)),
     "misaligned w": dict(w=mat(5, 8, ptr=4099)),
     "no w": dict(w=mat(5, 8, ptr=0)),
     "short workspace": dict(x=mat(4, 4096), w=mat(5, 4096), workspace=f8(16)),
@@ -125,6 +133,8 @@ def test_sizes_past_the_kernels_are_a_range_error(vs):
     a = vs._RmsnormArgs(M=1 << 31, C=4, x=4096, weight=4096, y=8192)
     assert lib.vcsr_rmsnorm(C.byref(a), None, None) == vs.VCSR_ERANGE
     assert b"M" in lib.vcsr_last_error()
+    a = vs._LinearArgs(M=(1 << 31) - 1, N=1 << 20, K=4, x=4096, w=4096, y=4096)
+    assert lib.vcsr_linear(C.byref(a), None, None) == vs.VCSR_ERANGE
 
 
 LINEAR_GRAD = {

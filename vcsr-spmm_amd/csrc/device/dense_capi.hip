@@ -24,6 +24,7 @@ void range(bool ok, const char* what) {
 // Rows are launched as a grid dimension; a product's operand tile, at most 256
 // rows, is addressed with 31-bit byte offsets.
 constexpr int64_t kMaxRows = (int64_t)1 << 31, kOperandLd = (int64_t)1 << 20;
+constexpr int64_t kMaxOut = (int64_t)1 << 42;  // values of a result: its tiles are counted in 32 bits
 
 void check_rows(int64_t M) {
     need(M >= 0, "negative M");
@@ -76,6 +77,11 @@ vcsr_rmsnorm_args checked(const vcsr_rmsnorm_args* args) {
     check_vector(a.rstd, "rstd: alignment", true);
     need(a.y != a.x || a.M == 0 || (a.y_type == a.x_type && a.ldy == a.ldx),
          "y over x: of another type or stride");
+    need(!a.residual || a.y != a.residual || (a.y_type == a.x_type && a.ldy == a.ldr),
+         "y over residual: of another type or stride");
+    need(!a.sum || a.sum != a.y, "sum: another matrix than y");
+    need(!a.sum || a.sum != a.x || a.ldsum == a.ldx, "sum over x: of another stride");
+    need(!a.sum || a.sum != a.residual || a.ldsum == a.ldr, "sum over residual: of another stride");
     return a;
 }
 
@@ -113,6 +119,8 @@ vcsr_linear_args checked_sizes(const vcsr_linear_args* args) {
     need(is_wide(a.x_type) || a.x_type == VCSR_FP8, "x_type: VCSR_F32, VCSR_BF16 or VCSR_FP8");
     need(is_wide(a.y_type), "y_type: VCSR_F32 or VCSR_BF16");
     check_act(a.act);
+    range(a.K <= kOperandLd, "K over 2^20");
+    range(a.M <= kMaxOut / a.N, "M x N over 2^42");
     if (a.ldx == 0) a.ldx = a.K;
     if (a.ldw == 0) a.ldw = a.K;
     if (a.ldy == 0) a.ldy = a.N;
@@ -156,6 +164,8 @@ vcsr_linear_args checked(const vcsr_linear_args* args) {
     check_matrix(a.z, a.ldz, a.N, a.y_type, "z: alignment or stride", true, a.M);
     check_matrix(a.y, a.ldy, a.N, a.y_type, "y: pointer, alignment or stride", false, a.M);
     need(!a.z || a.z != a.y, "z: another matrix than y");
+    need(!a.z || a.z != a.residual, "z: another matrix than the residual");
+    need(!a.residual || a.residual != a.y || a.ldr == a.ldy, "residual over y: of another stride");
     check_workspace(a.workspace, a.workspace_bytes, vcsr::gemm_workspace(gemm_of(a)));
     return a;
 }
@@ -195,6 +205,7 @@ LinearGrad grad_of(const vcsr_linear_grad_args* args) {
     stride(a.lddw, a.K);
     if (a.M == 0) return w;
     range(a.N <= kOperandLd && a.K <= kOperandLd, "N, K over 2^20");
+    range(a.M <= kMaxOut / (a.N > a.K ? a.N : a.K), "M x N or M x K over 2^42");
     const bool products = a.dx || a.dw;
     w.own_dz = products && (a.act != VCSR_ACT_NONE || a.x_type != a.y_type);
     // Rows of dz on 16-byte boundaries.
