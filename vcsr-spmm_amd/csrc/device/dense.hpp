@@ -224,6 +224,7 @@ size_t gemm_pair_workspace(const Gemm& dw, const Gemm& dx);
 // and how many of its rows (the rest are a product of their own).
 struct GemmPlan {
     int tile;
+    int stages;  // steps that have room in LDS
     int32_t splits;
     int64_t steps;
     int64_t rows;

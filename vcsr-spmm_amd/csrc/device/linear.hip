@@ -12,22 +12,26 @@ constexpr int64_t kCus = tile::kCus;
 // 128-byte step of the sum and of everything else of a tile, with 1 to `room`
 // blocks on a compute unit.  A second and third block of 64 x 64 bf16 cost next to
 // nothing (one alone waits for its loads), a fourth and fifth share the LDS
-// pipe; FP32 tiles are bound by their matrix instructions throughout.
+// pipe; with loads three steps ahead instead of one, one or two blocks take two
+// thirds of the time (1024^3 10.8 -> 8.0 us).  FP32 tiles are bound by their matrix
+// instructions throughout, e4m3 ones by widening, and gain nothing from that, nor
+// do the gradients' launches, which fill the chip with both products.
 struct TileCost {
-    int tile, room;
+    int tile, stages, room;
     float step[5], rest[5];
 };
 constexpr TileCost kF32[] = {
-    {64, 5, {0.61f, 1.07f, 1.51f, 2.0f, 2.5f}, {4.2f, 4.8f, 5.7f, 6.2f, 6.6f}},
-    {128, 2, {2.05f, 3.68f}, {8.7f, 10.4f}}};
+    {64, 2, 5, {0.61f, 1.07f, 1.51f, 2.0f, 2.5f}, {4.2f, 4.8f, 5.7f, 6.2f, 6.6f}},
+    {128, 2, 2, {2.05f, 3.68f}, {8.7f, 10.4f}}};
 constexpr TileCost kBf16[] = {
-    {64, 5, {0.454f, 0.465f, 0.533f, 0.78f, 1.04f}, {3.4f, 3.8f, 4.0f, 4.8f, 5.6f}},
-    {128, 2, {0.61f, 0.885f}, {5.7f, 7.6f}},
-    {256, 1, {1.44f}, {10.5f}}};
+    {64, 2, 5, {0.454f, 0.465f, 0.533f, 0.78f, 1.04f}, {3.4f, 3.8f, 4.0f, 4.8f, 5.6f}},
+    {128, 2, 2, {0.61f, 0.885f}, {5.7f, 7.6f}},
+    {256, 2, 1, {1.44f}, {10.5f}},
+    {64, 4, 2, {0.292f, 0.358f}, {3.3f, 4.1f}}};  // operands by rows only
 constexpr TileCost kFp8[] = {
-    {64, 5, {0.458f, 0.59f, 0.84f, 1.1f, 1.37f}, {4.0f, 4.3f, 4.7f, 5.0f, 5.3f}},
-    {128, 2, {0.95f, 1.61f}, {7.0f, 7.3f}},
-    {256, 1, {2.53f}, {11.4f}}};
+    {64, 2, 5, {0.458f, 0.59f, 0.84f, 1.1f, 1.37f}, {4.0f, 4.3f, 4.7f, 5.0f, 5.3f}},
+    {128, 2, 2, {0.95f, 1.61f}, {7.0f, 7.3f}},
+    {256, 2, 1, {2.53f}, {11.4f}}};
 
 struct Costs {
     const TileCost* t;
@@ -35,7 +39,8 @@ struct Costs {
 };
 Costs costs_of(const Gemm& g) {
     if (g.type == VCSR_F32) return Costs{kF32, 2};
-    return g.type == VCSR_BF16 ? Costs{kBf16, 3} : Costs{kFp8, 3};
+    if (g.type == VCSR_FP8) return Costs{kFp8, 3};
+    return Costs{kBf16, g.p_cols || g.q_cols ? 3 : 4};
 }
 // Steps of the whole sum.
 int64_t steps_of(const Gemm& g) {
@@ -101,7 +106,7 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
     // 8000 bf16 16 us against 10.
     if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || g.R * size <= 64 * 128)) {
         if (us_out) *us_out = 7.f;
-        return GemmPlan{16, 1, steps_of(g), g.I};
+        return GemmPlan{16, 1, 1, steps_of(g), g.I};
     }
     GemmPlan best{};
     float best_us = 0.f;
@@ -116,7 +121,7 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
             if (left) us += block_us(g, *t, steps, (left + kCus - 1) / kCus);
             if (best.splits == 0 || us < best_us) {
                 best_us = us;
-                best = GemmPlan{t->tile, (int32_t)splits, steps, g.I};
+                best = GemmPlan{t->tile, t->stages, (int32_t)splits, steps, g.I};
             }
             if (!may_divide || splits > 1 || rounds < 1 || !left) return;
             const int64_t per_row = ((int64_t)g.J + t->tile - 1) / t->tile;
@@ -127,7 +132,7 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
             us = (float)rounds * block_us(g, *t, steps, t->room) + extra_us(g, true) + rest_us + 2.f;
             if (us < best_us) {
                 best_us = us;
-                best = GemmPlan{t->tile, 1, steps, first};
+                best = GemmPlan{t->tile, t->stages, 1, steps, first};
             }
         });
     }
@@ -161,8 +166,8 @@ PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
             us += join_us(dw, splits);
             if (us < best_us) {
                 best_us = us;
-                best = PairPlan{true, GemmPlan{t->tile, (int32_t)splits, steps, dw.I},
-                                GemmPlan{t->tile, 1, steps_of(dx), dx.I}};
+                best = PairPlan{true, GemmPlan{t->tile, t->stages, (int32_t)splits, steps, dw.I},
+                                GemmPlan{t->tile, t->stages, 1, steps_of(dx), dx.I}};
             }
         });
     }

@@ -494,10 +494,12 @@ struct Part {
 };
 
 // Tiles whose blocks share a compute unit: a step's loads run under the other
-// blocks' work as well as under the block's own.
-template <int TI, int TJ>
-constexpr int kSharedLds = 2 * (TI + TJ) * kStepBytes;
-template <class T, int TI, int TJ, int WI, int WJ, bool PCOLS, bool QCOLS>
+// blocks' work as well as under the block's own.  STAGES steps have room in LDS, so
+// loads go out STAGES - 1 steps ahead: two where five blocks share a unit, four
+// where there are too few blocks to hide a trip to memory otherwise.
+template <int TILE, int STAGES>
+constexpr int kLds = STAGES * 2 * TILE * kStepBytes;
+template <class T, int TI, int TJ, int WI, int WJ, int STAGES, bool PCOLS, bool QCOLS>
 __device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uint32_t block,
                                             uint8_t* lds0) {
     constexpr int NT = 64 * WI * WJ;
@@ -548,23 +550,29 @@ __device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uin
     LP::offsets(P, op);
     LQ::offsets(Q, oq);
     lds_byte* const to = (lds_byte*)lds0;
-    int buf = 0;
-    if (k_first < k_full) {
-        LP::copy(P, op, k_first, to);
-        LQ::copy(Q, oq, k_first, to + TI * kStepBytes);
-    }
-    for (int64_t k = k_first; k < k_full; k += BK, buf ^= 1) {
-        // This step's tiles are in LDS, and all waves are done with the other
-        // buffer.
-        wait_loads<0>();
+    constexpr int AHEAD = STAGES - 1;
+    const int n = k_first < k_full ? (int)((k_full - k_first + BK - 1) / BK) : 0;
+    auto ask = [&](int t) __attribute__((always_inline)) {
+        lds_byte* const into = to + t % STAGES * kStage;
+        LP::copy(P, op, k_first + (int64_t)t * BK, into);
+        LQ::copy(Q, oq, k_first + (int64_t)t * BK, into + TI * kStepBytes);
+    };
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t)
+        if (t < n) ask(t);
+    for (int t = 0; t < n; ++t) {
+        // This step's tiles are in LDS (loads end in order; those of the steps behind
+        // it may be under way), and all waves are done with the last step's.
+        if (AHEAD > 1 && t + AHEAD - 1 < n)
+            wait_loads<(AHEAD - 1) * (LP::GR + LQ::GR)>();
+        else
+            wait_loads<0>();
         barrier();
-        if (k + BK < k_full) {
-            lds_byte* const next = to + (buf ^ 1) * kStage;
-            LP::copy(P, op, k + BK, next);
-            LQ::copy(Q, oq, k + BK, next + TI * kStepBytes);
-        }
-        multiply(lds0 + buf * kStage, lds0 + buf * kStage + TI * kStepBytes);
+        if (t + AHEAD < n) ask(t + AHEAD);
+        const uint8_t* const lp = lds0 + t % STAGES * kStage;
+        multiply(lp, lp + TI * kStepBytes);
     }
+    const int buf = n % STAGES;
     if (ragged) {
         LP::fetch(P, k_full, k_end, lds0 + buf * kStage);
         LQ::fetch(Q, k_full, k_end, lds0 + buf * kStage + TI * kStepBytes);
@@ -572,7 +580,7 @@ __device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uin
         multiply(lds0 + buf * kStage, lds0 + buf * kStage + TI * kStepBytes);
     }
     __syncthreads();
-    constexpr int ROOM = 2 * kStage / (WI * WJ) / 16 * 16;
+    constexpr int ROOM = STAGES * kStage / (WI * WJ) / 16 * 16;
     write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(lds0 + wave * ROOM), at.i0 + ri,
                                     at.j0 + rj, splits, at.split);
 }
@@ -706,21 +714,21 @@ __device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint
 }
 
 // A tile of TILE x TILE by the code for its size.
-template <class T, int TILE, bool PCOLS, bool QCOLS>
+template <class T, int TILE, int STAGES, bool PCOLS, bool QCOLS>
 __device__ __forceinline__ void gemm_block(const Gemm& g, const Part& part, uint32_t block,
                                            uint8_t* lds) {
     if constexpr (TILE == 256)
         gemm_turns<T, PCOLS, QCOLS>(g, part, block, lds);
     else
-        gemm_shared<T, TILE, TILE, 2, 2, PCOLS, QCOLS>(g, part, block, lds);
+        gemm_shared<T, TILE, TILE, 2, 2, STAGES, PCOLS, QCOLS>(g, part, block, lds);
 }
 template <int TILE>
 constexpr int kThreads = TILE == 256 ? 512 : 256;
 
-template <class T, int TILE, bool PCOLS, bool QCOLS>
+template <class T, int TILE, int STAGES, bool PCOLS, bool QCOLS>
 __global__ __launch_bounds__(kThreads<TILE>) void gemm_kernel(Gemm g, Part part) {
-    __shared__ __attribute__((aligned(128))) uint8_t lds[kSharedLds<TILE, TILE>];
-    gemm_block<T, TILE, PCOLS, QCOLS>(g, part, blockIdx.x, lds);
+    __shared__ __attribute__((aligned(128))) uint8_t lds[kLds<TILE, STAGES>];
+    gemm_block<T, TILE, STAGES, PCOLS, QCOLS>(g, part, blockIdx.x, lds);
 }
 
 // Columns [16 * block, + 16) of the sum of partial rows, in a fixed order.
@@ -748,17 +756,17 @@ __device__ __forceinline__ void sum_columns(const RowSum& r, uint32_t block, uin
 // rows are long, then dx's (from a multiple of 8 on, so that both keep their XCDs),
 // then those that add up dbias' partial rows.  Each product by itself leaves
 // compute units idle at its end.
-template <class T, int TILE>
+template <class T, int TILE, int STAGES>
 __global__ __launch_bounds__(kThreads<TILE>) void gemm_pair_kernel(Gemm dw, Part dw_part, Gemm dx,
                                                                    Part dx_part, RowSum bias) {
-    __shared__ __attribute__((aligned(128))) uint8_t lds[kSharedLds<TILE, TILE>];
+    __shared__ __attribute__((aligned(128))) uint8_t lds[kLds<TILE, STAGES>];
     const uint32_t first = (dw_part.blocks + 7) & ~7u;
     if (blockIdx.x >= first + dx_part.blocks)
         sum_columns<kThreads<TILE>>(bias, blockIdx.x - first - dx_part.blocks, lds);
     else if (blockIdx.x >= first)
-        gemm_block<T, TILE, false, true>(dx, dx_part, blockIdx.x - first, lds);
+        gemm_block<T, TILE, STAGES, false, true>(dx, dx_part, blockIdx.x - first, lds);
     else if (blockIdx.x < dw_part.blocks)
-        gemm_block<T, TILE, true, true>(dw, dw_part, blockIdx.x, lds);
+        gemm_block<T, TILE, STAGES, true, true>(dw, dw_part, blockIdx.x, lds);
 }
 
 // The partial sums of a split product and the epilogue, for few parts: a thread
@@ -961,12 +969,16 @@ hipError_t launch_layout(const Gemm& g, const GemmPlan& p, hipStream_t st) {
                                            : launch_rows<T, float>(g, st);
     }
     const Part part = part_of(g, p);
-    if (p.tile == 64)
-        gemm_kernel<T, 64, PCOLS, QCOLS><<<part.blocks, kThreads<64>, 0, st>>>(g, part);
+    constexpr bool DEEP = sizeof(T) == 2 && !PCOLS && !QCOLS;
+    if (DEEP && p.tile == 64 && p.stages == 4) {
+        if constexpr (DEEP)
+            gemm_kernel<T, 64, 4, PCOLS, QCOLS><<<part.blocks, kThreads<64>, 0, st>>>(g, part);
+    } else if (p.tile == 64)
+        gemm_kernel<T, 64, 2, PCOLS, QCOLS><<<part.blocks, kThreads<64>, 0, st>>>(g, part);
     else if (p.tile == 128)
-        gemm_kernel<T, 128, PCOLS, QCOLS><<<part.blocks, kThreads<128>, 0, st>>>(g, part);
+        gemm_kernel<T, 128, 2, PCOLS, QCOLS><<<part.blocks, kThreads<128>, 0, st>>>(g, part);
     else if constexpr (sizeof(T) < 4)
-        gemm_kernel<T, 256, PCOLS, QCOLS><<<part.blocks, kThreads<256>, 0, st>>>(g, part);
+        gemm_kernel<T, 256, 2, PCOLS, QCOLS><<<part.blocks, kThreads<256>, 0, st>>>(g, part);
     hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_join(g, p.splits, st);
 }
@@ -978,11 +990,11 @@ hipError_t launch_pair(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const 
     const uint32_t blocks = ((a.blocks + 7) & ~7u) + b.blocks +
                             (bias.P > 0 ? (uint32_t)(((int64_t)bias.C + 15) / 16) : 0);
     if (p.tile == 64)
-        gemm_pair_kernel<T, 64><<<blocks, kThreads<64>, 0, st>>>(dw, a, dx, b, bias);
+        gemm_pair_kernel<T, 64, 2><<<blocks, kThreads<64>, 0, st>>>(dw, a, dx, b, bias);
     else if (p.tile == 128)
-        gemm_pair_kernel<T, 128><<<blocks, kThreads<128>, 0, st>>>(dw, a, dx, b, bias);
+        gemm_pair_kernel<T, 128, 2><<<blocks, kThreads<128>, 0, st>>>(dw, a, dx, b, bias);
     else if constexpr (sizeof(T) < 4)
-        gemm_pair_kernel<T, 256><<<blocks, kThreads<256>, 0, st>>>(dw, a, dx, b, bias);
+        gemm_pair_kernel<T, 256, 2><<<blocks, kThreads<256>, 0, st>>>(dw, a, dx, b, bias);
     hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_join(dw, p.splits, st);
 }
