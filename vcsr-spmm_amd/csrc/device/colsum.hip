@@ -37,7 +37,8 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* part, int32
 // A block takes `rows` rows of tx vectors of 16 bytes of dy: 256 / tx rows at a time,
 // four of them under way together without a branch between their loads (rows past
 // the block's end are its last one again and count for nothing).  Bound by memory:
-// dy and z read once, dz written once.  ENDS: how rows end: 0 in whole vectors,
+// dy and z read once, dz written once (8192 x 4096 bf16 with gelu 38 us, 5.3 TB/s; 30011
+// x 257 FP32, whose rows begin anywhere in a line, 28 us, 3.3 TB/s).  ENDS: how rows end: 0 in whole vectors,
 // 1 inside one, 2 before the first is whole.
 template <class D, class X, int ACT, int ENDS>
 __global__ __launch_bounds__(256) void dz_kernel(vcsr_linear_grad_args a, X* dz, int64_t lddz,

@@ -151,21 +151,13 @@ __device__ __forceinline__ float act_grad_f32(float z) {
     }
     return 1.f;
 }
-// The same by a runtime (wave-uniform) choice.
+// act by a runtime (wave-uniform) choice.
 __device__ __forceinline__ float act_f32(int act, float z) {
     switch (act) {
         case VCSR_ACT_RELU: return act_f32<VCSR_ACT_RELU>(z);
         case VCSR_ACT_GELU: return act_f32<VCSR_ACT_GELU>(z);
         case VCSR_ACT_SILU: return act_f32<VCSR_ACT_SILU>(z);
         default: return z;
-    }
-}
-__device__ __forceinline__ float act_grad_f32(int act, float z) {
-    switch (act) {
-        case VCSR_ACT_RELU: return act_grad_f32<VCSR_ACT_RELU>(z);
-        case VCSR_ACT_GELU: return act_grad_f32<VCSR_ACT_GELU>(z);
-        case VCSR_ACT_SILU: return act_grad_f32<VCSR_ACT_SILU>(z);
-        default: return 1.f;
     }
 }
 

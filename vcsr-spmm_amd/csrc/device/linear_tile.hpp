@@ -3,9 +3,14 @@
 //
 // out[i][j] = epilogue(sum_k P(i, k) Q(j, k)).  A block computes a TI x TJ tile
 // of out; its WI x WJ waves take equal parts.  The sum goes in steps of 128
-// bytes of k: both operands' tiles are brought to LDS (two buffers: the next
-// step's tiles arrive while this one's are multiplied), and a wave multiplies
-// 16 x 16 blocks with v_mfma_f32_16x16x4_f32 or _16x16x32_bf16.
+// bytes of k: both operands' tiles go straight from memory to LDS, one to three
+// steps ahead of the one that is multiplied, and a wave multiplies 16 x 16 blocks
+// with v_mfma_f32_16x16x4_f32 or _16x16x32_bf16.
+//
+// What bounds it: big bf16 products the chip's power (8192 x 4096 x 8192 with gelu
+// 429 to 458 us, 1.2 to 1.28 PFLOP/s, the matrix units busy 56% at 2.0 to 2.15 GHz),
+// FP32 ones the matrix units (92% of their rate in full tiles), e4m3 ones widening
+// (4096 x 8192 x 4096 173 us, 1.59 PFLOP/s), few rows the weight's read.
 //
 // LDS tiles are TI (or TJ) x 128 bytes in 16-byte granules:
 //   by rows     row r at r * 128, granule g of its k at slot g ^ key(r);
@@ -29,7 +34,6 @@ namespace tile {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 
 constexpr int kStepBytes = 128;
@@ -349,7 +353,7 @@ __device__ __forceinline__ void wait_loads() {
     else
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-constexpr int kAhead = 8;  // loads a wave of gemm_turns_kernel has under way at a wait
+constexpr int kAhead = 8;  // loads a wave of gemm_turns has under way at a wait
 
 // Where block b of a launch works: tile and part of the sum.  Blocks of one XCD
 // take neighbouring tiles, `band` columns of tiles at a time, so that those that
@@ -611,6 +615,7 @@ __device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint
     using LQ = Loader<T, TJ, NT, QCOLS, true>;
     using RP = Reader<T, TI / 2, PCOLS, false>;
     using RQ = Reader<T, TJ, QCOLS, true>;
+    static_assert(LQ::GR + 2 * LP::GR == kAhead, "loads of a step");
     const int splits = part.splits;
     const int64_t steps = part.steps;
     const Place at = place_of<TI, TJ>(g, block, part.blocks, (uint32_t)splits);
