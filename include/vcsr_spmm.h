@@ -488,6 +488,8 @@ void vcsr_adamw_free(vcsr_adamw* plan);
 /* --------------------------------------------------- device plumbing */
 /* Minimal HIP helpers so hosts (ctypes, the CLI) need no other GPU runtime. */
 int vcsr_device_count(int32_t* n);
+/* The calling thread's device. */
+int vcsr_device_current(int32_t* device);
 int vcsr_device_name(char* buf, int32_t len);
 int vcsr_dev_malloc(void** ptr, size_t bytes);
 int vcsr_dev_free(void* ptr);

@@ -27,6 +27,7 @@ import ctypes as C
 import functools
 import os
 import struct
+import threading
 
 import numpy as np
 
@@ -51,8 +52,8 @@ EXPORTS = (
     "vcsr_fmt_set_tile_rows vcsr_fmt_set_tile_windows vcsr_fmt_tile_info vcsr_fmt_free spmm_csr_naive spmm_csr_wave spmm_vcsr "
     "spmm_vcsr_ex spmm_vcsr_noalloc spmm_vcsr_mfma vcsr_mfma_work vcsr_launch_info_get vcsr_tile_mfma_work spmm_csr_cpu "
     "vcsr_vendor_plan_create vcsr_vendor_spmm vcsr_vendor_plan_free spmm_csr_vendor "
-    "vcsr_device_count vcsr_device_name vcsr_dev_malloc vcsr_dev_free vcsr_memcpy_h2d "
-    "vcsr_memcpy_d2h vcsr_memcpy_d2d vcsr_memset_d vcsr_stream_create vcsr_stream_destroy "
+    "vcsr_device_count vcsr_device_current vcsr_device_name vcsr_dev_malloc vcsr_dev_free "
+    "vcsr_memcpy_h2d vcsr_memcpy_d2h vcsr_memcpy_d2d vcsr_memset_d vcsr_stream_create vcsr_stream_destroy "
     "vcsr_stream_sync vcsr_device_sync vcsr_event_create vcsr_event_destroy "
     "vcsr_event_record vcsr_event_elapsed "
     "vcsr_rmsnorm vcsr_rmsnorm_grad_workspace vcsr_rmsnorm_grad vcsr_linear_workspace vcsr_linear "
@@ -131,17 +132,22 @@ class _LinearGradArgs(C.Structure):
                 ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
-def _packer(args):
+def _packer(fields, size):
     """struct.Struct of a ctypes structure's fields: packing costs a third of
     filling the structure, and a small call is bound by the host."""
     codes = {C.c_int64: "q", C.c_int32: "i", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
-    st = struct.Struct("@" + "".join(codes[t] for _, t in args._fields_))
-    assert st.size == C.sizeof(args)
+    st = struct.Struct("@" + "".join(codes[t] for _, t in fields))
+    assert st.size == size
     return st.pack
 
 
-_pack_rmsnorm, _pack_rmsnorm_grad = _packer(_RmsnormArgs), _packer(_RmsnormGradArgs)
-_pack_linear, _pack_linear_grad = _packer(_LinearArgs), _packer(_LinearGradArgs)
+# The workspace's pointer and size end the structures that have them, and are packed
+# by themselves.
+_pack_rmsnorm = _packer(_RmsnormArgs._fields_, C.sizeof(_RmsnormArgs))
+_pack_space = _packer(_LinearArgs._fields_[-2:], 16)
+_pack_rmsnorm_grad, _pack_linear, _pack_linear_grad = (
+    _packer(args._fields_[:-2], C.sizeof(args) - 16)
+    for args in (_RmsnormGradArgs, _LinearArgs, _LinearGradArgs))
 
 
 class _AdamwTensor(C.Structure):
@@ -208,6 +214,7 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "vcsr_vendor_plan_free": (None, [P]),
         "spmm_csr_vendor": (C.c_int, [I32, I32, I32, P, P, P, P, I32, P, P, pF]),
         "vcsr_device_count": (C.c_int, [pI]),
+        "vcsr_device_current": (C.c_int, [pI]),
         "vcsr_device_name": (C.c_int, [C.c_char_p, I32]),
         "vcsr_dev_malloc": (C.c_int, [pP, C.c_size_t]),
         "vcsr_dev_free": (C.c_int, [P]),
@@ -450,6 +457,12 @@ def device_count() -> int:
     return n.value
 
 
+def current_device() -> int:
+    d = C.c_int32(0)
+    _check(load_library().vcsr_device_current(C.byref(d)))
+    return d.value
+
+
 def device_name() -> str:
     buf = C.create_string_buffer(128)
     _check(load_library().vcsr_device_name(buf, 128))
@@ -466,6 +479,9 @@ class Stream:
 
     def __del__(self):
         if getattr(self, "h", None) and _lib is not None and self.h.value:
+            # The next stream may get this one's handle, and its workspace with it.
+            if _workspaces and any(key[1] == self.h.value for key in list(_workspaces)):
+                _lib.vcsr_stream_sync(self.h)
             _lib.vcsr_stream_destroy(self.h)
             self.h = C.c_void_p()
 
@@ -785,29 +801,57 @@ def _shape2(arr, what):
     return arr.shape
 
 
-_workspaces = {}  # stream handle -> DeviceArray
+# (device, stream handle) -> DeviceArray; the buffers that these replaced, by device.
+_workspaces, _outgrown = {}, {}
+# Held from the choice of a workspace until the call that uses it has enqueued its
+# kernels: between those of two host threads on one stream nothing else may write it.
+_workspace_lock = threading.RLock()
+_one_device = None  # whether the process sees a single device
+
+
+def _device():
+    global _one_device
+    if _one_device is None:
+        _one_device = device_count() <= 1
+    return 0 if _one_device else current_device()
 
 
 def workspace(nbytes, stream=None):
-    """The binding's workspace of a stream, at least nbytes large: grown (after
-    the stream's work is done) when a call needs more, kept until
-    release_workspaces().  Calls on one stream run one after the other, so they
-    share it; for a call that is captured into a graph pass a DeviceArray of
-    its own, or make the same call once before the capture."""
-    key = stream.h.value if stream is not None else None
-    have = _workspaces.get(key)
-    if have is None or have.nbytes < nbytes:
-        if have is not None:
-            _check(load_library().vcsr_stream_sync(_sp(stream)))
-        have = _workspaces[key] = DeviceArray((max(int(nbytes), 1 << 20),), np.uint8)
-    return have
+    """The binding's workspace of a stream on the current device, at least nbytes
+    large.  Calls on one stream run one after the other, so they share it.  A call
+    that needs more gets a larger one; the one before stays allocated, since work
+    under way or a captured graph may use it, until release_workspaces().  A call
+    that is captured into a graph takes the workspace that is there: make the same
+    call once before the capture, and replay the graph on the stream it was captured
+    on; for replays elsewhere, beside other calls, pass a DeviceArray of its own."""
+    key = (_device(), stream.h.value if stream is not None else None)
+    with _workspace_lock:
+        have = _workspaces.get(key)
+        if have is None or have.nbytes < nbytes:
+            size = max(int(nbytes), 1 << 20)
+            if have is None:
+                new = DeviceArray((size,), np.uint8)
+            else:
+                try:  # twice as large, so that all that were outgrown take less than the last
+                    new = DeviceArray((max(size, 2 * have.nbytes),), np.uint8)
+                except VcsrError:
+                    new = DeviceArray((size,), np.uint8)
+                _outgrown.setdefault(key[0], []).append(have)
+            have = _workspaces[key] = new
+        return have
 
 
 def release_workspaces():
-    """Frees the workspaces of all streams once the device is idle."""
-    if _workspaces:
-        _check(load_library().vcsr_device_sync())
-        _workspaces.clear()
+    """Frees the current device's workspaces, those of all its streams, once the
+    device is idle; no graph captured with them may be replayed any more."""
+    device = _device()
+    with _workspace_lock:
+        mine = [key for key in _workspaces if key[0] == device]
+        if mine:
+            _check(load_library().vcsr_device_sync())
+            for key in mine:
+                del _workspaces[key]
+            _outgrown.pop(device, None)
 
 
 # Bytes of workspace by sizes and types alone (what the _workspace functions
@@ -840,13 +884,6 @@ def _rmsnorm_grad_bytes(M, N, x_type, y_type):
     return need.value
 
 
-def _space(nbytes, given, stream):
-    if not nbytes:
-        return 0, 0
-    ws = given if given is not None else workspace(nbytes, stream)
-    return ws.ptr.value or 0, ws.nbytes
-
-
 def _call(fn, args, stream, timed):
     if not timed:
         rc = fn(args, stream.h if stream is not None else None, None)
@@ -856,6 +893,18 @@ def _call(fn, args, stream, timed):
     ms = C.c_float(0)
     _check(fn(args, _sp(stream), C.byref(ms)))
     return ms.value
+
+
+def _call_with_space(fn, args, need, given, stream, timed):
+    """_call with `need` bytes of workspace, whose two fields end the structure:
+    `given`, or the binding's own."""
+    if not need:
+        return _call(fn, args + _pack_space(0, 0), stream, timed)
+    if given is not None:
+        return _call(fn, args + _pack_space(given.ptr.value or 0, given.nbytes), stream, timed)
+    with _workspace_lock:
+        own = workspace(need, stream)
+        return _call(fn, args + _pack_space(own.ptr.value, own.nbytes), stream, timed)
 
 
 def run_rmsnorm_gpu(x, weight, y, residual=None, sum=None, y_scale=None, rstd=None, eps=1e-6,
@@ -884,8 +933,9 @@ def run_rmsnorm_grad_gpu(dy, s, weight, rstd, dx, dweight=None, dsum=None, works
     need = _rmsnorm_grad_bytes(M, N, xt, yt) if dweight is not None else 0
     args = _pack_rmsnorm_grad(M, N, xt, yt, dp, lddy, sp, lds, _vec(weight, N, "weight"),
                               _vec(rstd, M, "rstd"), up, ldu, xp, ldx,
-                              _vec(dweight, N, "dweight"), *_space(need, workspace, stream))
-    return _call((_lib or load_library()).vcsr_rmsnorm_grad, args, stream, timed)
+                              _vec(dweight, N, "dweight"))
+    return _call_with_space((_lib or load_library()).vcsr_rmsnorm_grad, args, need, workspace,
+                            stream, timed)
 
 
 def _act(act):
@@ -907,10 +957,10 @@ def run_linear_gpu(x, w, y, bias=None, residual=None, act="none", z=None, x_scal
     xt, yt = _type(x, "x"), _type(y, "y")
     args = _pack_linear(M, N, K, xt, yt, _act(act), xp, ldx, wp, ldw,
                         _vec(x_scale, M, "x_scale"), _vec(w_scale, N, "w_scale"),
-                        _vec(bias, N, "bias"), rp, ldr, zp, ldz, yp, ldy,
-                        *_space(_linear_bytes(M, N, K, xt, yt, rp != 0, zp != 0), workspace,
-                                stream))
-    return _call((_lib or load_library()).vcsr_linear, args, stream, timed)
+                        _vec(bias, N, "bias"), rp, ldr, zp, ldz, yp, ldy)
+    return _call_with_space((_lib or load_library()).vcsr_linear, args,
+                            _linear_bytes(M, N, K, xt, yt, rp != 0, zp != 0), workspace, stream,
+                            timed)
 
 
 def run_linear_grad_gpu(dy, x, w, z=None, act="none", dx=None, dw=None, dbias=None,
@@ -926,9 +976,9 @@ def run_linear_grad_gpu(dy, x, w, z=None, act="none", dx=None, dw=None, dbias=No
     need = _linear_grad_bytes(M, N, K, xt, yt, at, z is not None, dx is not None, dw is not None,
                               dbias is not None)
     args = _pack_linear_grad(M, N, K, xt, yt, at, dp, lddy, zp, ldz, xp, ldx, wp, ldw, xg, lddx,
-                             wg, lddw, _vec(dbias, N, "dbias"),
-                             *_space(need, workspace, stream))
-    return _call((_lib or load_library()).vcsr_linear_grad, args, stream, timed)
+                             wg, lddw, _vec(dbias, N, "dbias"))
+    return _call_with_space((_lib or load_library()).vcsr_linear_grad, args, need, workspace,
+                            stream, timed)
 
 
 class AdamW:

@@ -525,6 +525,16 @@ int vcsr_device_count(int32_t* n) {
     });
 }
 
+int vcsr_device_current(int32_t* device) {
+    return guarded([&] {
+        need(device != nullptr, "null output");
+        need_device();
+        int d = 0;
+        hip_check(hipGetDevice(&d), "hipGetDevice");
+        *device = d;
+    });
+}
+
 int vcsr_device_name(char* buf, int32_t len) {
     return guarded([&] {
         need(buf && len > 0, "bad buffer");
