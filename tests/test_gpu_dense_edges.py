@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 
 from conftest import capture, hip_runtime
-from dense_ref import Mat, pack
+from dense_ref import EPS, Mat, close, pack, rms_norm, rms_norm_grad, vector
+from test_gpu_dense import check_norm, rounding, values
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,86 @@ def test_a_graph_outlives_the_workspace_it_was_captured_with(gpu):
             hip.hipGraphExecDestroy(gexec)
         hip.hipGraphDestroy(graph)
     vs.release_workspaces()
+
+
+def put(vs, st, array, at, values_):
+    """values_ to element `at` of a device array."""
+    v = np.ascontiguousarray(values_, array.dtype)
+    vs._check(vs.load_library().vcsr_memcpy_h2d(array.ptr.value + at * v.itemsize, v.ctypes.data,
+                                                v.nbytes, st.h))
+
+
+def take(vs, st, array, at, n):
+    out = np.empty(n, array.dtype)
+    vs._check(vs.load_library().vcsr_memcpy_d2h(out.ctypes.data,
+                                                array.ptr.value + at * out.itemsize, out.nbytes,
+                                                st.h))
+    return out
+
+
+@pytest.mark.parametrize("kinds, C", [("f32 f32", 3), ("f32 fp8", 1), ("bf16 bf16", 7),
+                                      ("bf16 fp8", 2), ("bf16 f32", 5)])
+def test_rmsnorm_of_millions_of_narrow_rows(gpu, kinds, C):
+    """Rows shorter than a vector, more of them than 2^32 threads would be at 1024 a row."""
+    xk, yk = kinds.split()
+    rng = np.random.default_rng(C)
+    M = (1 << 22) + 3
+    print(f"narrow rows {kinds} {M}x{C}", flush=True)
+    x, r = values(rng, (M, C), xk), values(rng, (M, C), xk)
+    w = (1 + 0.2 * rng.standard_normal(C)).astype(np.float32).astype(np.float64)
+    check_norm(gpu, gpu.Stream(), x, r, w, xk, yk, 1e-6, f"{kinds} {M}x{C}", pad=C % 2, off=1)
+
+
+@pytest.mark.parametrize("kinds, C", [("f32 f32", 3), ("bf16 bf16", 7), ("f32 bf16", 2)])
+@pytest.mark.parametrize("M", [1, 255, 257, 5000, (1 << 22) + 3])
+def test_rmsnorm_grad_of_narrow_rows(gpu, kinds, C, M):
+    xk, yk = kinds.split()
+    vs, st = gpu, gpu.Stream()
+    rng = np.random.default_rng(M % 1000 + C)
+    print(f"narrow rows grad {kinds} {M}x{C}", flush=True)
+    s, dy = values(rng, (M, C), xk, 1.5), values(rng, (M, C), yk)
+    ds = values(rng, (M, C), xk)
+    w = (1 + 0.2 * rng.standard_normal(C)).astype(np.float32).astype(np.float64)
+    rstd = (1 / np.sqrt(np.mean(s * s, axis=1) + 1e-6)).astype(np.float32)
+    DX = Mat(vs, st, None, xk, 1, 1, (M, C))
+    dweight = vector(vs, st, np.full(C, np.nan))
+    vs.run_rmsnorm_grad_gpu(Mat(vs, st, dy, yk, 2, 1).view, Mat(vs, st, s, xk, 0, 1).view,
+                            vector(vs, st, w), vector(vs, st, rstd), DX.view, dweight,
+                            dsum=Mat(vs, st, ds, xk).view, stream=st)
+    st.sync()
+    rd = rstd.astype(np.float64)[:, None]
+    want, want_w = rms_norm_grad(dy, s, w, rd, ds)
+    h, g = np.abs(s * rd), np.abs(dy * w)
+    dot = np.sum(g * h, axis=1, keepdims=True) / C
+    tol = 8 * EPS * (rd * (g + h * dot) + np.abs(want)) + rd * h * dot * (C + 4) * EPS
+    close(DX.values(), want, tol + rounding(want, xk), "dx")
+    # A thread's chain of at most 17 rows, 6 steps over lanes, 3 over waves, and the
+    # partial rows: 16 a thread, then 14; 3 roundings in each product.
+    close(dweight.numpy(st), want_w, 64 * EPS * np.sum(np.abs(dy) * h, axis=0) + 1e-30, "dweight")
+
+
+def test_rmsnorm_of_rows_for_two_launches(gpu):
+    """64 threads a row and 2^26 rows: in place, 35 GB."""
+    vs, st = gpu, gpu.Stream()
+    rng = np.random.default_rng(80)
+    M, C = (1 << 26) + 5, 132
+    big = vs.DeviceArray((M, C), np.float32)
+    big.zero(st)
+    rstd = vs.DeviceArray((M,), np.float32)
+    rstd.zero(st)
+    rows = [0, 1, (1 << 26) - 257, (1 << 26) - 256, (1 << 26) - 1, 1 << 26, M - 1]
+    x = rng.standard_normal((len(rows), C)).astype(np.float32)
+    w = (1 + 0.2 * rng.standard_normal(C)).astype(np.float32)
+    for r, v in zip(rows, x):
+        put(vs, st, big, r * C, v)
+    print("rows for two launches", flush=True)
+    vs.run_rmsnorm_gpu(big, vector(vs, st, w), big, rstd=rstd, eps=1e-6, stream=st)
+    st.sync()
+    u = (C / 8 + 16) * EPS
+    for r, v in zip(rows, x.astype(np.float64)):
+        _, want_r, want = rms_norm(v[None], None, w.astype(np.float64), 1e-6)
+        close(take(vs, st, big, r * C, C), want[0], np.abs(want[0]) * (u + 5 * EPS), f"row {r}")
+        close(take(vs, st, rstd, r, 1), want_r[0], want_r[0] * u, f"rstd {r}")
+    zero = take(vs, st, rstd, (1 << 26) - 255, 3)
+    close(zero, np.full(3, 1e3), np.full(3, 1e3) * u, "rstd of zeros")
+    assert not take(vs, st, big, 12345678 * C, C).any()

@@ -152,10 +152,9 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_kernel(vcsr_
     store_row((Y*)a.y + row * a.ldy, lane, stride, a.C, t);
 }
 
-// Longer rows, and those of fewer values than a vector: a block reads a row twice
-// (the second time from the caches).
-// sum, which may be x or the residual, is written in the second pass, behind
-// the reads of the same values by the same thread.
+// Longer rows: a block reads a row twice (the second time from the caches).  sum,
+// which may be x or the residual, is written in the second pass, behind the reads
+// of the same values by the same thread.
 template <class X, class Y>
 __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(vcsr_rmsnorm_args a) {
     constexpr int V = kVec<X>, WAVES = 16;
@@ -197,6 +196,53 @@ __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(vcsr_rmsnorm_args a)
         if (a.sum) store_vec((X*)a.sum + row * a.ldsum + c, n, t);
         write_y((Y*)a.y + row * a.ldy + c, n, t, w, rstd, scale);
     }
+}
+
+// Rows of fewer values than a vector: a thread takes a row.
+template <class X, class Y>
+__global__ __launch_bounds__(256) void rmsnorm_narrow_kernel(vcsr_rmsnorm_args a) {
+    constexpr int V = kVec<X>;
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row >= a.M) return;
+    float t[V], w[V], sum = 0.f, top = 0.f;
+    load_vec((const X*)a.x + row * a.ldx, a.C, t);
+    load_vec(a.weight, a.C, w);
+    if (a.residual) {
+        float v[V];
+        load_vec((const X*)a.residual + row * a.ldr, a.C, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] += v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        sum = __builtin_fmaf(t[i], t[i], sum);
+        if (sizeof(Y) == 1) top = max_nan(top, __builtin_fabsf(t[i] * w[i]));
+    }
+    const float rstd = 1.f / __builtin_sqrtf(sum / (float)a.C + a.eps);
+    if (a.rstd) a.rstd[row] = rstd;
+    const float scale = row_factor<Y>(rstd, top, a.y_scale, row, true);
+    if (a.sum) store_vec((X*)a.sum + row * a.ldsum, a.C, t);
+    write_y((Y*)a.y + row * a.ldy, a.C, t, w, rstd, scale);
+}
+
+// A launch has fewer than 2^32 threads: more rows than that, at `threads` each, go
+// in several.  launch(first, count) takes whole blocks of at most 256 rows.
+template <class F>
+void by_rows(int64_t M, int64_t threads, F&& launch) {
+    const int64_t most = ((((int64_t)1 << 32) - 1) / threads) & ~(int64_t)255;
+    for (int64_t first = 0; first < M; first += most)
+        launch(first, M - first < most ? M - first : most);
+}
+template <class X, class Y>
+vcsr_rmsnorm_args rows_of(vcsr_rmsnorm_args a, int64_t first, int64_t count) {
+    a.M = count;
+    a.x = (const X*)a.x + first * a.ldx;
+    if (a.residual) a.residual = (const X*)a.residual + first * a.ldr;
+    if (a.sum) a.sum = (X*)a.sum + first * a.ldsum;
+    a.y = (Y*)a.y + first * a.ldy;
+    if (a.y_scale) a.y_scale += first;
+    if (a.rstd) a.rstd += first;
+    return a;
 }
 
 int next_pow2(int n) {
@@ -250,16 +296,26 @@ template <class X, class Y>
 hipError_t launch_forward(const vcsr_rmsnorm_args& a, hipStream_t st) {
     constexpr int V = kVec<X>;
     const int64_t nv = ((int64_t)a.C + V - 1) / V;
-    if (nv > 2048 || a.C < V) {
-        rmsnorm_long_kernel<X, Y><<<(unsigned)a.M, 1024, 0, st>>>(a);
+    if (a.C < V) {
+        rmsnorm_narrow_kernel<X, Y><<<(unsigned)((a.M + 255) / 256), 256, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    if (nv > 2048) {
+        by_rows(a.M, 1024, [&](int64_t first, int64_t count) {
+            rmsnorm_long_kernel<X, Y>
+                <<<(unsigned)count, 1024, 0, st>>>(rows_of<X, Y>(a, first, count));
+        });
         return hipGetLastError();
     }
     const int lanes = nv <= 64 ? next_pow2((int)nv) : 64;
     with_shape(row_shape(nv, 4), [&](auto wpr, auto k) {
         constexpr int W = decltype(wpr)::value, NV = decltype(k)::value;
         const int rows = W > 1 ? 1 : 256 / lanes;
-        rmsnorm_kernel<X, Y, W, NV>
-            <<<(unsigned)((a.M + rows - 1) / rows), W > 1 ? 64 * W : 256, 0, st>>>(a, lanes);
+        by_rows(a.M, W > 1 ? 64 * W : lanes, [&](int64_t first, int64_t count) {
+            rmsnorm_kernel<X, Y, W, NV>
+                <<<(unsigned)((count + rows - 1) / rows), W > 1 ? 64 * W : 256, 0, st>>>(
+                    rows_of<X, Y>(a, first, count), lanes);
+        });
     });
     return hipGetLastError();
 }
@@ -364,7 +420,7 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_grad_kernel(
     for (int c = tid; c < a.C; c += 256) out[c] = w_lds[c];
 }
 
-// Longer rows, and those shorter than a vector: a block per row, read twice; dweight apart (column by column).
+// Longer rows: a block per row, read twice; dweight apart (column by column).
 template <class X, class D>
 __global__ __launch_bounds__(1024) void rmsnorm_grad_long_kernel(vcsr_rmsnorm_grad_args a) {
     constexpr int V = kVec<X>, WAVES = 16;
@@ -416,6 +472,54 @@ __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(vcsr_rmsnorm_grad_
     part[(int64_t)blockIdx.y * a.C + c] = t;
 }
 
+// Rows of fewer values than a vector: a thread takes rows blocks apart and keeps
+// dweight in registers; lanes, then waves, add theirs up.
+template <class X, class D>
+__global__ __launch_bounds__(256) void rmsnorm_grad_narrow_kernel(vcsr_rmsnorm_grad_args a,
+                                                                  float* part) {
+    constexpr int V = kVec<X>;
+    __shared__ float lds[4][V];
+    float w[V], dw[V];
+    load_vec(a.weight, a.C, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[i] = 0.f;
+    const float inv_c = 1.f / (float)a.C;
+    for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.M;
+         row += (int64_t)gridDim.x * 256) {
+        float h[V], g[V], o[V], dot = 0.f;
+        const float rstd = a.rstd[row];
+        load_vec((const X*)a.s + row * a.lds, a.C, h);
+        load_vec((const D*)a.dy + row * a.lddy, a.C, g);
+        if (a.dsum) {
+            load_vec((const X*)a.dsum + row * a.lddsum, a.C, o);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            h[i] *= rstd;
+            if (i < a.C) dw[i] = __builtin_fmaf(g[i], h[i], dw[i]);  // a factor may be infinite
+            g[i] *= w[i];
+            if (i < a.C) dot = __builtin_fmaf(g[i], h[i], dot);
+        }
+        const float mean = dot * inv_c;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] += rstd * (g[i] - h[i] * mean);
+        store_vec((X*)a.dx + row * a.lddx, a.C, o);
+    }
+    if (!part) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        dw[i] = sum_lanes(64, dw[i]);
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6][i] = dw[i];
+    }
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < a.C)
+        part[(int64_t)blockIdx.x * a.C + c] = ((lds[0][c] + lds[1][c]) + lds[2][c]) + lds[3][c];
+}
+
 // The gradient's row shape and blocks, each of which writes a row of partial
 // dweight: two waves a SIMD.  With one a SIMD 16384 x 2050 bf16 takes 97 us, with
 // two 68, with four 82 (twice the partial rows).
@@ -423,7 +527,7 @@ struct GradShape {
     int64_t nv;
     int lanes;
     RowShape row;
-    bool in_registers;
+    bool narrow, in_registers;
     int32_t blocks;
 };
 GradShape grad_shape(const vcsr_rmsnorm_grad_args& a) {
@@ -437,8 +541,10 @@ GradShape grad_shape(const vcsr_rmsnorm_grad_args& a) {
     const int64_t need = (a.M + rows - 1) / rows, most = 2048 / waves;
     g.blocks = (int32_t)(need < most ? need : most);
     if (need <= 4) g.blocks = 1;  // which then writes dweight itself
-    g.in_registers = g.nv <= 2048 && a.C >= v;
-    if (!g.in_registers) g.blocks = (int32_t)(a.M < 64 ? a.M : 64);
+    g.narrow = a.C < v;
+    g.in_registers = g.nv <= 2048 && !g.narrow;
+    if (g.narrow) g.blocks = (int32_t)(a.M < 256 * 1024 ? (a.M + 255) / 256 : 1024);
+    else if (!g.in_registers) g.blocks = (int32_t)(a.M < 64 ? a.M : 64);
     return g;
 }
 
@@ -446,8 +552,19 @@ template <class X, class D>
 hipError_t launch_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
     const GradShape g = grad_shape(a);
     float* const part = !a.dweight ? nullptr : g.blocks == 1 ? a.dweight : (float*)a.workspace;
-    if (!g.in_registers) {
-        rmsnorm_grad_long_kernel<X, D><<<(unsigned)a.M, 1024, 0, st>>>(a);
+    if (g.narrow) {
+        rmsnorm_grad_narrow_kernel<X, D><<<(unsigned)g.blocks, 256, 0, st>>>(a, part);
+    } else if (!g.in_registers) {
+        by_rows(a.M, 1024, [&](int64_t first, int64_t count) {
+            vcsr_rmsnorm_grad_args b = a;
+            b.M = count;
+            b.dy = (const D*)a.dy + first * a.lddy;
+            b.s = (const X*)a.s + first * a.lds;
+            b.rstd = a.rstd + first;
+            if (a.dsum) b.dsum = (const X*)a.dsum + first * a.lddsum;
+            b.dx = (X*)a.dx + first * a.lddx;
+            rmsnorm_grad_long_kernel<X, D><<<(unsigned)count, 1024, 0, st>>>(b);
+        });
         if (part)
             rmsnorm_dweight_kernel<X, D>
                 <<<dim3((unsigned)((a.C + 255) / 256), g.blocks), 256, 0, st>>>(a, part);
