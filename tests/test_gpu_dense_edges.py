@@ -157,3 +157,32 @@ def test_rmsnorm_of_rows_for_two_launches(gpu):
     zero = take(vs, st, rstd, (1 << 26) - 255, 3)
     close(zero, np.full(3, 1e3), np.full(3, 1e3) * u, "rstd of zeros")
     assert not take(vs, st, big, 12345678 * C, C).any()
+
+
+def test_rmsnorm_grad_of_columns_for_two_launches(gpu):
+    """64 threads add up a column of dweight's partial rows: 2^26 columns."""
+    vs, st = gpu, gpu.Stream()
+    rng = np.random.default_rng(81)
+    M, C = 2, (1 << 26) + 5
+    s, dy, dx = (vs.DeviceArray((M, C), np.float32) for _ in range(3))
+    w, dweight = vs.DeviceArray((C,), np.float32), vs.DeviceArray((C,), np.float32)
+    for a in (s, dy, w):
+        a.zero(st)
+    rstd = np.float32([0.5, 2.0])
+    cols = [0, 31, (1 << 25) - 1, 1 << 25, (1 << 26) - 1, 1 << 26, C - 1]
+    sv, dv = rng.standard_normal((M, len(cols))), rng.standard_normal((M, len(cols)))
+    for m in range(M):
+        for i, c in enumerate(cols):
+            put(vs, st, s, m * C + c, np.float32([sv[m, i]]))
+            put(vs, st, dy, m * C + c, np.float32([dv[m, i]]))
+    put(vs, st, dweight, 0, np.full(C, 7, np.float32))
+    print("columns for two launches", flush=True)
+    vs.run_rmsnorm_grad_gpu(dy, s, w, vector(vs, st, rstd), dx, dweight, stream=st)
+    st.sync()
+    got = dweight.numpy(st)
+    sv, dv = sv.astype(np.float32).astype(np.float64), dv.astype(np.float32).astype(np.float64)
+    terms = dv * sv * rstd[:, None]
+    close(got[cols], terms.sum(0), 4 * EPS * np.abs(terms).sum(0), "dweight")
+    got[cols] = 0
+    assert not got.any()
+    vs.release_workspaces()

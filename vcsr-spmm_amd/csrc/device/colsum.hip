@@ -160,7 +160,12 @@ __global__ __launch_bounds__(256) void zero_kernel(uint8_t* p, int64_t bytes) {
 
 hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, float* out,
                            hipStream_t st) {
-    sum_rows_kernel<<<(unsigned)(((int64_t)C + 15) / 16), 1024, 0, st>>>(part, P, C, ld, out);
+    // 64 threads a column, and fewer than 2^32 threads a launch.
+    constexpr int32_t kMost = 1 << 25;
+    for (int64_t c = 0; c < C; c += kMost) {
+        const int32_t n = C - c < kMost ? (int32_t)(C - c) : kMost;
+        sum_rows_kernel<<<(unsigned)((n + 15) / 16), 1024, 0, st>>>(part + c, P, n, ld, out + c);
+    }
     return hipGetLastError();
 }
 
