@@ -186,3 +186,26 @@ def test_rmsnorm_grad_of_columns_for_two_launches(gpu):
     got[cols] = 0
     assert not got.any()
     vs.release_workspaces()
+
+
+def test_no_rows_and_a_large_weight_gradient(gpu):
+    """Zeros in 17 GB of dw, and in a million rows with a gap between them, by a kernel each."""
+    vs, st = gpu, gpu.Stream()
+    N, K = 1 << 17, (1 << 15) + 8
+    big = vs.DeviceArray((N, K), np.float32)
+    vs._check(vs.load_library().vcsr_memset_d(big.ptr, 0x5B, big.nbytes, st.h))
+    x, dy = vs.DeviceView(0, (0, K), vs.F32), vs.DeviceView(0, (0, N), vs.F32)
+    w = vs.DeviceView(big.ptr, (N, K), vs.F32)
+    print("17 GB of zeros", flush=True)
+    vs.run_linear_grad_gpu(dy, x, w, dw=big, stream=st)
+    st.sync()
+    for at in (0, 1 << 30, (1 << 32) - 4, 1 << 32, N * K - 64):
+        assert not take(vs, st, big, at, 64).any(), at
+    N = 1 << 20  # the most outputs of a gradient
+    DW = Mat(vs, st, np.ones((N, 1)), "bf16", pad=2, off=1)
+    db = vector(vs, st, np.ones(N))
+    print("rows with gaps", flush=True)
+    vs.run_linear_grad_gpu(vs.DeviceView(0, (0, N), vs.F32), vs.DeviceView(0, (0, 1), vs.BF16),
+                           DW.view, dw=DW.view, dbias=db, stream=st)
+    st.sync()
+    assert not DW.codes().any() and not db.numpy(st).any()

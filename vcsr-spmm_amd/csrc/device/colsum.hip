@@ -150,10 +150,12 @@ hipError_t launch_dz_typed(const vcsr_linear_grad_args& a, X* dz, int64_t lddz, 
     return hipGetLastError();
 }
 
-__global__ __launch_bounds__(256) void zero_kernel(uint8_t* p, int64_t bytes) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    for (int k = 0; k < 4; ++k)
-        if (i + k < bytes) p[i + k] = 0;
+// Rows of `n` 16-bit values, `ld` apart.
+__global__ __launch_bounds__(256) void zero_kernel(uint16_t* p, int64_t ld, int64_t rows,
+                                                   int64_t n) {
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256)
+            p[r * ld + i] = 0;
 }
 
 }  // namespace
@@ -183,9 +185,16 @@ hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, flo
                                 : launch_dz_typed<bf16, bf16>(a, (bf16*)dz, lddz, part, st);
 }
 
-hipError_t launch_zero(void* p, int64_t bytes, hipStream_t st) {
-    if (bytes <= 0) return hipSuccess;
-    zero_kernel<<<(unsigned)((bytes + 1023) / 1024), 256, 0, st>>>((uint8_t*)p, bytes);
+hipError_t launch_zero(void* p, int64_t ld, int64_t rows, int64_t bytes, hipStream_t st) {
+    if (rows <= 0 || bytes <= 0) return hipSuccess;
+    if (ld == bytes) {  // one row
+        bytes *= rows;
+        rows = 1;
+    }
+    const int64_t n = bytes / 2, columns = (n + 255) / 256, most = rows == 1 ? 4096 : 16;
+    const dim3 grid((unsigned)(columns < most ? columns : most),
+                    (unsigned)(rows < 4096 ? rows : 4096));
+    zero_kernel<<<grid, 256, 0, st>>>((uint16_t*)p, ld / 2, rows, n);
     return hipGetLastError();
 }
 

@@ -176,8 +176,9 @@ hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, 
 hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, float* part,
                      hipStream_t st);
 int32_t dz_row_blocks(int64_t M, int32_t N, int32_t dy_type);
-// n bytes of zeros, by a kernel.
-hipError_t launch_zero(void* p, int64_t bytes, hipStream_t st);
+// Zeros in `rows` rows of `bytes` bytes, `ld` bytes apart (all even, as FP32 and bf16
+// matrices have them), by a kernel.
+hipError_t launch_zero(void* p, int64_t ld, int64_t rows, int64_t bytes, hipStream_t st);
 
 // ------------------------------------------------------------ linear*.hip
 // out[i][j] = epilogue(sum_k P(i, k) Q(j, k)).  An operand lies by rows (k

@@ -265,23 +265,16 @@ LinearGrad checked(const vcsr_linear_grad_args* args) {
     return w;
 }
 
-hipError_t zero_matrix(void* p, int64_t ld, int64_t rows, int64_t row_bytes, int64_t size,
-                       hipStream_t st) {
-    if (ld * size == row_bytes) return vcsr::launch_zero(p, rows * row_bytes, st);
-    for (int64_t r = 0; r < rows; ++r) {
-        hipError_t e = vcsr::launch_zero((char*)p + r * ld * size, row_bytes, st);
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
-}
-
 hipError_t run_grad(const LinearGrad& w, hipStream_t st) {
     const vcsr_linear_grad_args& a = w.a;
     hipError_t e = hipSuccess;
     if (a.M == 0) {
         const int64_t size = (int64_t)size_of(a.x_type);
-        if (a.dw) e = zero_matrix(a.dw, a.lddw, a.N, a.K * size, size, st);
-        if (e == hipSuccess && a.dbias) e = vcsr::launch_zero(a.dbias, (int64_t)a.N * 4, st);
+        if (a.dw) e = vcsr::launch_zero(a.dw, a.lddw * size, a.N, a.K * size, st);
+        if (e == hipSuccess && a.dbias) {
+            const int64_t bytes = (int64_t)a.N * 4;
+            e = vcsr::launch_zero(a.dbias, bytes, 1, bytes, st);
+        }
         return e;
     }
     char* base = (char*)a.workspace;

@@ -600,8 +600,10 @@ size_t rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args& a) {
 }
 
 hipError_t launch_rmsnorm_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
-    if (a.M <= 0)
-        return a.dweight ? launch_zero(a.dweight, (int64_t)a.C * 4, st) : hipSuccess;
+    if (a.M <= 0) {
+        const int64_t bytes = (int64_t)a.C * 4;
+        return a.dweight ? launch_zero(a.dweight, bytes, 1, bytes, st) : hipSuccess;
+    }
     if (a.x_type == VCSR_F32)
         return a.y_type == VCSR_F32 ? launch_grad<float, float>(a, st)
                                     : launch_grad<float, bf16>(a, st);
