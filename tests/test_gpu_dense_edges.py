@@ -209,3 +209,22 @@ def test_no_rows_and_a_large_weight_gradient(gpu):
                            DW.view, dw=DW.view, dbias=db, stream=st)
     st.sync()
     assert not DW.codes().any() and not db.numpy(st).any()
+
+
+def test_linear_of_more_rows_than_small_tiles_have_blocks(gpu):
+    """2^30 + 3 rows: 64 x 64 tiles of 256 threads would need 2^32 threads."""
+    vs, st = gpu, gpu.Stream()
+    M = (1 << 30) + 3
+    x, y = vs.DeviceArray((M, 1), np.float32), vs.DeviceArray((M, 1), np.float32)
+    x.zero(st)
+    vs._check(vs.load_library().vcsr_memset_d(y.ptr, 0x5B, y.nbytes, st.h))
+    rows = [0, 63, (1 << 29) + 1, (1 << 30) - 1, 1 << 30, M - 1]
+    for r in rows:
+        put(vs, st, x, r, np.float32([r % 1000 + 0.5]))
+    print("2^30 rows", flush=True)
+    vs.run_linear_gpu(x, vector(vs, st, [[3.0]]), y, bias=vector(vs, st, [-1.0]), stream=st)
+    st.sync()
+    for r in rows:
+        assert take(vs, st, y, r, 1)[0] == 3 * (r % 1000 + 0.5) - 1, r
+    assert (take(vs, st, y, 1 << 28, 1000) == -1).all()
+    assert (take(vs, st, y, M - 100, 96) == -1).all()

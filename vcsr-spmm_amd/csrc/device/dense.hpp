@@ -202,6 +202,7 @@ struct Gemm {
     float* part = nullptr;  // partial sums of a split product (gemm_workspace bytes)
 };
 hipError_t launch_gemm(const Gemm& g, hipStream_t st);
+// Throws VCSR_ERANGE for more tiles than a launch has blocks, as the pair's does.
 size_t gemm_workspace(const Gemm& g);
 // Partial rows of C columns still to be added up (none for P = 0).
 struct RowSum {

@@ -50,6 +50,10 @@ int64_t steps_of(const Gemm& g) {
 int64_t tiles_of(const Gemm& g, int64_t t) {
     return (g.I + t - 1) / t * (((int64_t)g.J + t - 1) / t);
 }
+// Whether a launch of these blocks can be made: HIP has none of 2^32 threads or more.
+bool launches(int64_t blocks, int tile) {
+    return blocks * (tile == 256 ? 512 : 256) < (int64_t)1 << 32;
+}
 // A block's time with b blocks on its compute unit.  Transposing reads of both
 // operands take a quarter longer in the big tile.
 float block_us(const Gemm& g, const TileCost& t, int64_t steps, int64_t b) {
@@ -97,14 +101,15 @@ Gemm rows_from(Gemm g, int64_t from) {
 // whole rounds of blocks, what is left, and the join.  Where a last round would
 // leave most of the chip idle, the rows of the whole rounds go by themselves and the
 // rest as a product of its own, in smaller tiles (5001 x 4096 x 4096 bf16: 320 tiles of
-// 256 on 256 compute units).
+// 256 on 256 compute units).  splits = 0: no launch has that many blocks.
 GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true) {
     const int size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
     // Up to 8 rows: W is read straight into the matrix layout, 6 to 9 us up to 32 MB of
     // it against 10 of the tiles (their join is a launch of its own).  Not where
     // few blocks would read long rows alone, past what a wave asks for at once: 512 x
     // 8000 bf16 16 us against 10.
-    if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || g.R * size <= 64 * 128)) {
+    if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || g.R * size <= 64 * 128) &&
+        g.J < 1 << 27) {  // 32 threads a column, and fewer than 2^32 a launch
         if (us_out) *us_out = 7.f;
         return GemmPlan{16, 1, 1, steps_of(g), g.I};
     }
@@ -115,20 +120,21 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
         const int64_t tiles = tiles_of(g, t->tile);
         each_split(g, tiles, [&](int64_t splits, int64_t steps) {
             const int64_t blocks = tiles * splits, round = kCus * t->room;
+            const bool whole = launches(blocks, t->tile);
             const int64_t rounds = blocks / round, left = blocks - rounds * round;
             float us = (float)rounds * block_us(g, *t, steps, t->room) + join_us(g, splits) +
                        extra_us(g, rounds > 0);
             if (left) us += block_us(g, *t, steps, (left + kCus - 1) / kCus);
-            if (best.splits == 0 || us < best_us) {
+            if (whole && (best.splits == 0 || us < best_us)) {
                 best_us = us;
                 best = GemmPlan{t->tile, t->stages, (int32_t)splits, steps, g.I};
             }
-            if (!may_divide || splits > 1 || rounds < 1 || !left) return;
+            if (!may_divide || !whole || splits > 1 || rounds < 1 || !left) return;
             const int64_t per_row = ((int64_t)g.J + t->tile - 1) / t->tile;
             const int64_t first = rounds * round / per_row * t->tile;
             if (first < t->tile || first >= g.I) return;
             float rest_us = 0.f;
-            plan_of(rows_from(g, first), &rest_us, false);
+            if (plan_of(rows_from(g, first), &rest_us, false).splits == 0) return;
             us = (float)rounds * block_us(g, *t, steps, t->room) + extra_us(g, true) + rest_us + 2.f;
             if (us < best_us) {
                 best_us = us;
@@ -150,6 +156,7 @@ struct PairPlan {
 PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
     float us_w = 0.f, us_x = 0.f;
     PairPlan best{false, plan_of(dw, &us_w), plan_of(dx, &us_x)};
+    if (best.dw.splits == 0 || best.dx.splits == 0) return best;
     float best_us = us_w + us_x + 2.f;
     const Costs c = costs_of(dw);
     for (const TileCost* t = c.t; t < c.t + c.n; ++t) {
@@ -164,7 +171,8 @@ PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
             if (us < one_w) us = one_w;
             if (us < one_x) us = one_x;
             us += join_us(dw, splits);
-            if (us < best_us) {
+            const int64_t blocks = (tiles_w * splits + 7) / 8 * 8 + tiles_x + (dw.I + 15) / 16;
+            if (us < best_us && launches(blocks, t->tile)) {
                 best_us = us;
                 best = PairPlan{true, GemmPlan{t->tile, t->stages, (int32_t)splits, steps, dw.I},
                                 GemmPlan{t->tile, t->stages, 1, steps_of(dx), dx.I}};
@@ -172,6 +180,11 @@ PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
         });
     }
     return best;
+}
+
+const GemmPlan& launchable(const GemmPlan& p) {
+    if (p.splits == 0) throw Error(VCSR_ERANGE, "M, N: more tiles than a launch has blocks");
+    return p;
 }
 
 size_t part_bytes(const Gemm& g, const GemmPlan& p) {
@@ -199,12 +212,12 @@ hipError_t launch(const Gemm& g, const GemmPlan& p, hipStream_t st) {
 }  // namespace
 
 size_t gemm_workspace(const Gemm& g) {
-    return g.I <= 0 || g.J <= 0 ? 0 : part_bytes(g, plan_of(g));
+    return g.I <= 0 || g.J <= 0 ? 0 : part_bytes(g, launchable(plan_of(g)));
 }
 
 size_t gemm_pair_workspace(const Gemm& dw, const Gemm& dx) {
     const PairPlan p = plan_pair(dw, dx);
-    const size_t a = part_bytes(dw, p.dw), b = part_bytes(dx, p.dx);
+    const size_t a = part_bytes(dw, launchable(p.dw)), b = part_bytes(dx, launchable(p.dx));
     return a > b ? a : b;
 }
 
