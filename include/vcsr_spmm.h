@@ -478,7 +478,8 @@ typedef struct {
 } vcsr_adamw_hyper;
 typedef struct vcsr_adamw vcsr_adamw;
 /* Binds the tensors' addresses (they stay the caller's) to a plan on the
- * current device; tensors must not overlap.  A step only enqueues its kernel. */
+ * current device; tensors must not overlap.  A step only enqueues its kernel.
+ * All tensors together have fewer than 2^24 chunks of up to 2048 values. */
 int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* stream,
                       vcsr_adamw** out);
 int vcsr_adamw_step(const vcsr_adamw* plan, const vcsr_adamw_hyper* hyper, void* stream,

@@ -26,3 +26,14 @@ def test_products_of_just_fewer_pass_the_checks(vs):
         a = vs._LinearArgs(M=M, N=N, K=4, x=4096, w=4096, y=8192)
         assert lib.vcsr_linear_workspace(C.byref(a), C.byref(need)) == vs.VCSR_OK, (M, N)
         assert need.value == 0
+
+
+def test_adamw_of_more_chunks_than_a_launch_has_blocks(vs):
+    """2^24 chunks of 2,048 values, 256 threads each: in one tensor, and in two."""
+    lib = vs.load_library()
+    for sizes in ([1 << 35], [1 << 34, (1 << 34) - 2047]):
+        t = (vs._AdamwTensor * len(sizes))(*[
+            vs._AdamwTensor(n, 0, 0, 4096, 4096, 4096, 4096, None, None, None, 0.0) for n in sizes])
+        out = C.c_void_p()
+        assert lib.vcsr_adamw_create(t, len(sizes), None, C.byref(out)) == vs.VCSR_ERANGE, sizes
+        assert not out.value

@@ -26,6 +26,8 @@ void range(bool ok, const char* what) {
 constexpr int64_t kMaxRows = (int64_t)1 << 31, kOperandLd = (int64_t)1 << 20;
 constexpr int64_t kMaxOut = (int64_t)1 << 42;  // values of a result: its tiles are counted in 32 bits
 
+constexpr int64_t kMaxChunks = (int64_t)1 << 24;  // AdamW: 256 threads each, fewer than 2^32 in all
+
 void check_rows(int64_t M) {
     need(M >= 0, "negative M");
     range(M < kMaxRows, "M over 2^31 - 1");
@@ -380,7 +382,7 @@ int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* str
             const std::string who = "tensor " + std::to_string(i) + ": ";
             auto must = [&](bool ok, const char* what) { need(ok, (who + what).c_str()); };
             must(t.n >= 0, "negative n");
-            range(t.n < kMaxRows * vcsr::kAdamwChunk, (who + "n over 2^42").c_str());
+            range(t.n < kMaxChunks * vcsr::kAdamwChunk, (who + "n of 2^35 or more").c_str());
             must(is_wide(t.grad_type), "grad_type: VCSR_F32 or VCSR_BF16");
             must(t.state_type == VCSR_F32 || t.state_type == VCSR_FP8,
                  "state_type: VCSR_F32 or VCSR_FP8");
@@ -395,7 +397,7 @@ int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* str
                      (uintptr_t)t.copy % 2 == 0,
                  "a pointer is not aligned to its type");
             const int64_t n = (t.n + vcsr::kAdamwChunk - 1) / vcsr::kAdamwChunk;
-            range((int64_t)chunks.size() + n < kMaxRows, "tensors: over 2^31 chunks of 2048");
+            range((int64_t)chunks.size() + n < kMaxChunks, "tensors: 2^24 or more chunks of 2048");
             for (int64_t k = 0; k < n; ++k) chunks.push_back(make_int2(i, (int)k));
         }
         need_device();
