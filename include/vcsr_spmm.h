@@ -392,7 +392,7 @@ typedef struct {
     const float* weight; /* C                                                */
     const float* rstd;   /* M                                                */
     const void* dsum;    int64_t lddsum; /* NULL, or what flows into `sum`   */
-    void* dx;            int64_t lddx;   /* may be dsum itself               */
+    void* dx;            int64_t lddx;   /* may be dsum, s or dy itself      */
     float* dweight;      /* C (zeros for M = 0), or NULL                     */
     void* workspace;     size_t workspace_bytes;
 } vcsr_rmsnorm_grad_args;

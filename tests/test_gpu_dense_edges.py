@@ -228,3 +228,27 @@ def test_linear_of_more_rows_than_small_tiles_have_blocks(gpu):
         assert take(vs, st, y, r, 1)[0] == 3 * (r % 1000 + 0.5) - 1, r
     assert (take(vs, st, y, 1 << 28, 1000) == -1).all()
     assert (take(vs, st, y, M - 100, 96) == -1).all()
+
+
+@pytest.mark.parametrize("C", [3, 100, 2000, 20000])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rmsnorm_grad_in_place(gpu, kind, C):
+    """dx over dsum, s and dy: the bits of dx and dweight apart."""
+    vs, st = gpu, gpu.Stream()
+    rng = np.random.default_rng(C)
+    M = 70
+    host = {k: values(rng, (M, C), kind) for k in ("dy", "s", "dsum")}
+    w = vector(vs, st, 1 + 0.1 * rng.standard_normal(C))
+    rstd = vector(vs, st, 0.5 + rng.random(M))
+    want = None
+    for over in (None, "dsum", "s", "dy"):
+        mats = {k: Mat(vs, st, v, kind, pad=8) for k, v in host.items()}
+        dx = mats[over] if over else Mat(vs, st, None, kind, pad=8, shape=(M, C))
+        dweight = vector(vs, st, np.full(C, np.nan))
+        print(f"norm gradient in place {kind} C={C} over {over}", flush=True)
+        vs.run_rmsnorm_grad_gpu(mats["dy"].view, mats["s"].view, w, rstd, dx.view, dweight,
+                                dsum=mats["dsum"].view, stream=st)
+        st.sync()
+        got = (dx.codes().tobytes(), dweight.numpy(st).tobytes())
+        want = want or got
+        assert got == want, over

@@ -105,6 +105,12 @@ vcsr_rmsnorm_grad_args checked(const vcsr_rmsnorm_grad_args* args) {
     check_matrix(a.dsum, a.lddsum, a.C, a.x_type, "dsum: alignment or stride", true, a.M);
     check_matrix(a.dx, a.lddx, a.C, a.x_type, "dx: pointer, alignment or stride", false, a.M);
     check_vector(a.dweight, "dweight: alignment", true);
+    if (a.M > 0) {
+        need(a.dx != a.dsum || a.lddx == a.lddsum, "dx over dsum: of another stride");
+        need(a.dx != a.s || a.lddx == a.lds, "dx over s: of another stride");
+        need(a.dx != a.dy || (a.x_type == a.y_type && a.lddx == a.lddy),
+             "dx over dy: of another type or stride");
+    }
     check_workspace(a.workspace, a.workspace_bytes, vcsr::rmsnorm_grad_workspace(a));
     return a;
 }

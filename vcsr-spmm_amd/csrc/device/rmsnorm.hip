@@ -555,6 +555,9 @@ hipError_t launch_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
     if (g.narrow) {
         rmsnorm_grad_narrow_kernel<X, D><<<(unsigned)g.blocks, 256, 0, st>>>(a, part);
     } else if (!g.in_registers) {
+        if (part)  // before dx, which may be s or dy itself
+            rmsnorm_dweight_kernel<X, D>
+                <<<dim3((unsigned)((a.C + 255) / 256), g.blocks), 256, 0, st>>>(a, part);
         by_rows(a.M, 1024, [&](int64_t first, int64_t count) {
             vcsr_rmsnorm_grad_args b = a;
             b.M = count;
@@ -565,9 +568,6 @@ hipError_t launch_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st) {
             b.dx = (X*)a.dx + first * a.lddx;
             rmsnorm_grad_long_kernel<X, D><<<(unsigned)count, 1024, 0, st>>>(b);
         });
-        if (part)
-            rmsnorm_dweight_kernel<X, D>
-                <<<dim3((unsigned)((a.C + 255) / 256), g.blocks), 256, 0, st>>>(a, part);
     } else {
         with_shape(g.row, [&](auto wpr, auto k) {
             constexpr int W = decltype(wpr)::value, NV = decltype(k)::value;
