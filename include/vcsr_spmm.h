@@ -404,7 +404,7 @@ int vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args* args, void* stream, float* m
 /* z = x W^T + bias;  y = act(z) + residual.  W has one row per output column.
  * Products are summed in FP32 (FP32 operands on the FP32 matrix cores); VCSR_FP8
  * operands carry a scale per row: z[m][n] = x_scale[m] * w_scale[n] * (x W^T)
- * + bias[n].  y and z are rounded once. */
+ * + bias[n].  y and z are rounded once, and are other matrices than x and w. */
 typedef struct {
     int64_t M;           /* rows of x and y; 0 is no work                    */
     int32_t N, K;        /* outputs and inputs of a row, >= 1                */

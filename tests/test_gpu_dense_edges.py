@@ -252,3 +252,19 @@ def test_rmsnorm_grad_in_place(gpu, kind, C):
         got = (dx.codes().tobytes(), dweight.numpy(st).tobytes())
         want = want or got
         assert got == want, over
+
+
+@pytest.mark.parametrize("out, over", [("y", "x"), ("y", "w"), ("z", "x"), ("z", "w")])
+def test_linear_refuses_outputs_over_operands(gpu, out, over):
+    """Refused before any launch: nothing is written."""
+    vs, st = gpu, gpu.Stream()
+    n = 40
+    mats = {k: Mat(vs, st, np.full((n, n), i + 1.0), "f32") for i, k in enumerate("xwyz")}
+    kw = {k: m.view for k, m in mats.items()}
+    kw[out] = kw[over]
+    with pytest.raises(vs.VcsrError) as e:
+        vs.run_linear_gpu(stream=st, **kw)
+    assert e.value.code == vs.VCSR_EINVAL and f"{out}: another matrix" in str(e.value)
+    st.sync()
+    for i, k in enumerate("xwyz"):
+        assert (mats[k].values() == i + 1).all()

@@ -178,6 +178,14 @@ vcsr_linear_args checked(const vcsr_linear_args* args) {
     return a;
 }
 
+// Blocks read x and w while others write y and z.  Asked once there is a device: of
+// buffers that no kernel will touch, none is in the way.
+void need_apart(const vcsr_linear_args& a) {
+    if (a.M == 0) return;
+    need(a.y != a.x && a.y != a.w, "y: another matrix than x and w");
+    need(!a.z || (a.z != a.x && a.z != a.w), "z: another matrix than x and w");
+}
+
 // The gradient's work: dz (unless dy serves as it is), dbias' partial rows,
 // and the two products, whose partial sums share what is behind.
 struct LinearGrad {
@@ -353,6 +361,7 @@ int vcsr_linear(const vcsr_linear_args* args, void* stream, float* ms) {
     return guarded([&] {
         const vcsr_linear_args a = checked(args);
         need_device();
+        need_apart(a);
         hipStream_t st = (hipStream_t)stream;
         const vcsr::Gemm g = gemm_of(a);
         run_timed(st, ms, [&] { return vcsr::launch_gemm(g, st); });
