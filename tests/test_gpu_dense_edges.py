@@ -268,3 +268,25 @@ def test_linear_refuses_outputs_over_operands(gpu, out, over):
     st.sync()
     for i, k in enumerate("xwyz"):
         assert (mats[k].values() == i + 1).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_linear_grad_over_what_no_product_reads(gpu, kind):
+    """dx over x without dw, over dy and z with an activation; dw over w without dx:
+    the bits of a call apart."""
+    vs, st = gpu, gpu.Stream()
+    rng = np.random.default_rng(90)
+    n = 200
+    host = {k: values(rng, (n, n), kind) for k in ("dy", "x", "w", "z")}
+
+    def call(out, over):
+        m = {k: Mat(vs, st, v, kind) for k, v in host.items()}
+        to = m[over] if over else Mat(vs, st, None, kind, shape=(n, n))
+        vs.run_linear_grad_gpu(m["dy"].view, m["x"].view, m["w"].view, z=m["z"].view, act="silu",
+                               stream=st, **{out: to.view})
+        st.sync()
+        return to.codes().tobytes()
+
+    for out, over in (("dx", "x"), ("dx", "dy"), ("dx", "z"), ("dw", "w"), ("dw", "dy")):
+        print(f"{out} over {over} {kind}", flush=True)
+        assert call(out, over) == call(out, None), (out, over)

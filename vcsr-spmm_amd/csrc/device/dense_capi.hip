@@ -277,6 +277,17 @@ LinearGrad checked(const vcsr_linear_grad_args* args) {
     check_matrix(a.dx, a.lddx, a.K, a.x_type, "dx: alignment or stride", true, a.M);
     check_matrix(a.dw, a.lddw, a.K, a.x_type, "dw: alignment or stride", true, a.M);
     check_vector(a.dbias, "dbias: alignment", true);
+    if (a.M > 0 && a.dx) {
+        need(w.own_dz || a.dx != a.dy, "dx: over dy, which its product reads");
+        need(a.dx != a.w, "dx: over w, which its product reads");
+        need(a.dx != a.x || !a.dw, "dx: over x, which dw's product reads");
+        need(a.dx != a.dw, "dx: another matrix than dw");
+    }
+    if (a.M > 0 && a.dw) {
+        need(w.own_dz || a.dw != a.dy, "dw: over dy, which its product reads");
+        need(a.dw != a.x, "dw: over x, which its product reads");
+        need(a.dw != a.w || !a.dx, "dw: over w, which dx's product reads");
+    }
     check_workspace(a.workspace, a.workspace_bytes, w.bytes());
     return w;
 }
