@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 
 from conftest import capture, hip_runtime
-from dense_ref import EPS, Mat, close, pack, rms_norm, rms_norm_grad, vector
+from dense_ref import (EPS, Mat, act_grad, close, from_bf16, pack, rms_norm, rms_norm_grad, unpack,
+                       vector)
 from test_gpu_dense import check_norm, rounding, values
 
 pytestmark = pytest.mark.gpu
@@ -290,3 +291,43 @@ def test_linear_grad_over_what_no_product_reads(gpu, kind):
     for out, over in (("dx", "x"), ("dx", "dy"), ("dx", "z"), ("dw", "w"), ("dw", "dy")):
         print(f"{out} over {over} {kind}", flush=True)
         assert call(out, over) == call(out, None), (out, over)
+
+
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_activation_gradients_of_every_magnitude(gpu, kind, act):
+    """act'(z) over the whole range of z, a column each (dbias of one row of ones):
+    a finite z has a finite gradient, also where z^2 or z^3 is past FP32's range."""
+    vs, st = gpu, gpu.Stream()
+    if kind == "bf16":
+        z = from_bf16(np.arange(1 << 16, dtype=np.uint16))
+        z = z[np.isfinite(z)].astype(np.float64)
+    else:
+        z = np.concatenate([np.linspace(-30, 30, 4001), 2.0 ** np.linspace(-126, 127.9, 3000),
+                            -2.0 ** np.linspace(-126, 127.9, 3000)])
+    z = unpack(pack(z[None, :], kind), kind)
+    n = z.shape[1]
+    one = np.ones((1, n))
+    db = vector(vs, st, np.full(n, np.nan))
+    print(f"act' {act} {kind}", flush=True)
+    vs.run_linear_grad_gpu(Mat(vs, st, one, kind).view, Mat(vs, st, np.ones((1, 1)), kind).view,
+                           Mat(vs, st, one.T, kind).view, z=Mat(vs, st, z, kind).view, act=act,
+                           dbias=db, stream=st)
+    st.sync()
+    z = z[0]
+    # act' = p + b p (1 - p) for p = 1 / (1 + e^-u).  The sum and the reciprocal round p
+    # (4 u of it), the exponential's argument u and itself move it by p (1 - p) (|u| + 2)
+    # 4 u; where e^-u is under 2^-26, p is one and what it lacks is lost.  1e-30: p
+    # past FP32's range.
+    with np.errstate(all="ignore"):
+        k = 2 * np.sqrt(2 / np.pi)
+        arg, b = (k * (z + 0.044715 * z ** 3), np.abs(z) * k * (1 + 0.134145 * z * z)) \
+            if act == "gelu" else (z, np.abs(z))
+        p, q = 1 / (1 + np.exp(-arg)), 1 / (1 + np.exp(arg))
+        # Not through tanh, whose 1 + t and 1 - t^2 lose what is small.
+        want = act_grad(z, act) if act == "relu" else p + np.sign(z) * b * p * q
+        dp = np.where(np.exp(-arg) < 2.0 ** -26, q, 4 * EPS * p + 4 * EPS * p * q * (np.abs(arg) + 2))
+        tol = dp + np.where(dp > 0, dp * b, 0) + np.where(q > 0, 8 * EPS * p * q * b, 0)
+    tol = np.zeros(n) if act == "relu" else np.nan_to_num(tol) + 4 * EPS * np.abs(want) + 1e-30
+    assert np.isfinite(want).all() and tol.max() < 2.0 ** -16
+    close(db.numpy(st), want, tol, f"{act} {kind}")

@@ -143,7 +143,10 @@ __device__ __forceinline__ float act_grad_f32(float z) {
     if (ACT == VCSR_ACT_RELU) return z > 0.f ? 1.f : 0.f;
     if (ACT == VCSR_ACT_GELU) {
         const float p = sigmoid_f32(kGelu2 * (z + 0.044715f * z * z * z));
-        return p + z * p * (1.f - p) * kGelu2 * (1.f + 0.134145f * z * z);
+        // Where z^2 passes FP32's range, p (1 - p) is zero and stays the product: z^2 is
+        // held at 2^80 there (fmin would take that for a NaN too, but p then is one).
+        const float z2 = __builtin_fminf(z * z, 0x1p80f);
+        return p + z * p * (1.f - p) * kGelu2 * (1.f + 0.134145f * z2);
     }
     if (ACT == VCSR_ACT_SILU) {
         const float p = sigmoid_f32(z);
