@@ -360,7 +360,9 @@ enum {
 /* t = x + residual;  y = t / sqrt(mean(t^2) + eps) * weight, row by row, in
  * FP32.  For y of VCSR_FP8, y_scale[m] = max(max_c |y|, 1e-30) / 448 and the
  * codes are y / y_scale[m] rounded to e4m3.  A row with a NaN or an infinity
- * gives NaN for all of y or for what it multiplies, and no other row does. */
+ * gives NaN for all of y or for what it multiplies, and no other row does.  The
+ * sum of a row's squares is FP32's too: past 3.4e38 (all |t| from 1.8e19 on) its
+ * rstd and finite y are zero. */
 typedef struct {
     int64_t M;           /* rows; 0 is no work                               */
     int32_t C;           /* columns, >= 1                                    */

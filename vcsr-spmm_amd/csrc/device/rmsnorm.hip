@@ -54,15 +54,25 @@ __device__ __forceinline__ void reduce_waves(float* lds, float& sum, float& top)
     }
 }
 
+// Whether max |t * w| stands for max |y| / rstd: it does not where that product is
+// past FP32's range (or loses bits below it), which y = t * rstd * w need not be (1e-18
+// * 1e-27, or 1e18 * 1e22).  y's own maximum is taken there.
+__device__ __forceinline__ bool top_lost(float top) { return top < 0x1p-100f || top > 0x1p126f; }
+// Scale of a row whose largest |y| is `top`.
 template <class Y>
-__device__ __forceinline__ float row_factor(float rstd, float top, float* y_scale, int64_t row,
-                                            bool writes) {
+__device__ __forceinline__ float row_factor(float top, float* y_scale, int64_t row, bool writes) {
     if (sizeof(Y) != 1) return 1.f;
-    float a = top * rstd;
-    a = a < 1e-30f ? 1e-30f : a;  // a NaN stays one
+    const float a = top < 1e-30f ? 1e-30f : top;  // a NaN stays one
     const float scale = a / 448.f;
     if (writes) y_scale[row] = scale;
     return scale;
+}
+template <int V>
+__device__ __forceinline__ float y_top(const float (&t)[V], const float (&w)[V], float rstd,
+                                       float top) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = max_nan(top, __builtin_fabsf(t[i] * rstd * w[i]));
+    return top;
 }
 
 // y's values of one vector.
@@ -106,7 +116,7 @@ template <class X, class Y, int WPR, int NV>
 __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_kernel(vcsr_rmsnorm_args a,
                                                                            int lanes) {
     constexpr int V = kVec<X>;
-    __shared__ float lds[2 * WPR];
+    __shared__ float lds[4 * WPR];
     const int tid = threadIdx.x;
     const int lane = WPR > 1 ? tid : tid & (lanes - 1);
     const int stride = WPR > 1 ? 64 * WPR : lanes;
@@ -138,7 +148,17 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_kernel(vcsr_
     if (!live) return;
     const float rstd = 1.f / __builtin_sqrtf(sum / (float)a.C + a.eps);
     if (a.rstd && lane == 0) a.rstd[row] = rstd;
-    const float scale = row_factor<Y>(rstd, top, a.y_scale, row, lane == 0);
+    if (sizeof(Y) == 1 && top_lost(top)) {  // for all lanes of the row
+        float unused = 0.f;
+        top = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) top = y_top(t[k], w[k], rstd, top);
+        reduce_lanes(WPR > 1 ? 64 : lanes, unused, top);
+        if (WPR > 1) reduce_waves<WPR>(lds + 2 * WPR, unused, top);
+    } else {
+        top *= rstd;
+    }
+    const float scale = row_factor<Y>(top, a.y_scale, row, lane == 0);
     if (a.sum) store_row((X*)a.sum + row * a.ldsum, lane, stride, a.C, t);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -158,7 +178,7 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void rmsnorm_kernel(vcsr_
 template <class X, class Y>
 __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(vcsr_rmsnorm_args a) {
     constexpr int V = kVec<X>, WAVES = 16;
-    __shared__ float lds[2 * WAVES];
+    __shared__ float lds[4 * WAVES];
     const int64_t row = blockIdx.x;
     const X* x = (const X*)a.x + row * a.ldx;
     const X* r = a.residual ? (const X*)a.residual + row * a.ldr : nullptr;
@@ -188,7 +208,21 @@ __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(vcsr_rmsnorm_args a)
     reduce_waves<WAVES>(lds, sum, top);
     const float rstd = 1.f / __builtin_sqrtf(sum / (float)a.C + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
-    const float scale = row_factor<Y>(rstd, top, a.y_scale, row, threadIdx.x == 0);
+    if (sizeof(Y) == 1 && top_lost(top)) {
+        float unused = 0.f;
+        top = 0.f;
+        for (int64_t c = (int64_t)threadIdx.x * V; c < a.C; c += 1024 * V) {
+            float t[V], w[V];
+            const int n = load_t(c, t);
+            load_vec(a.weight + c, n, w);
+            top = y_top(t, w, rstd, top);
+        }
+        reduce_lanes(64, unused, top);
+        reduce_waves<WAVES>(lds + 2 * WAVES, unused, top);
+    } else {
+        top *= rstd;
+    }
+    const float scale = row_factor<Y>(top, a.y_scale, row, threadIdx.x == 0);
     for (int64_t c = (int64_t)threadIdx.x * V; c < a.C; c += 1024 * V) {
         float t[V], w[V];
         const int n = load_t(c, t);
@@ -214,13 +248,16 @@ __global__ __launch_bounds__(256) void rmsnorm_narrow_kernel(vcsr_rmsnorm_args a
         for (int i = 0; i < V; ++i) t[i] += v[i];
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        sum = __builtin_fmaf(t[i], t[i], sum);
-        if (sizeof(Y) == 1) top = max_nan(top, __builtin_fabsf(t[i] * w[i]));
-    }
+    for (int i = 0; i < V; ++i) sum = __builtin_fmaf(t[i], t[i], sum);
     const float rstd = 1.f / __builtin_sqrtf(sum / (float)a.C + a.eps);
     if (a.rstd) a.rstd[row] = rstd;
-    const float scale = row_factor<Y>(rstd, top, a.y_scale, row, true);
+    if (sizeof(Y) == 1) {
+        top = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < a.C) top = max_nan(top, __builtin_fabsf(t[i] * rstd * w[i]));
+    }
+    const float scale = row_factor<Y>(top, a.y_scale, row, true);
     if (a.sum) store_vec((X*)a.sum + row * a.ldsum, a.C, t);
     write_y((Y*)a.y + row * a.ldy, a.C, t, w, rstd, scale);
 }
