@@ -226,6 +226,18 @@ struct GemmPlan {
     int64_t steps;
     int64_t rows;
 };
+// dw's and dx's; `together`: in one launch.
+struct PairPlan {
+    bool together;
+    GemmPlan dw, dx;
+};
+GemmPlan gemm_plan(const Gemm& g);
+PairPlan gemm_pair_plan(const Gemm& dw, const Gemm& dx);
+// For tests: the calling thread's products take this tile, splits and (where `rows`
+// is less than a product's) division of rows, as far as a product has them, and pairs
+// go together or not; tile 0 ends it.
+void force_plan(const GemmPlan& p, bool together);
+
 hipError_t launch_gemm_f32(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_gemm_bf16(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_pair_f32(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,

@@ -2,6 +2,7 @@
 // checks, workspaces and launches.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <memory>
 #include <string>
@@ -471,5 +472,30 @@ int vcsr_adamw_step(const vcsr_adamw* plan, const vcsr_adamw_hyper* hyper, void*
 }
 
 void vcsr_adamw_free(vcsr_adamw* plan) { delete plan; }
+
+// Not part of the interface (no header declares them): the tests run every kernel of
+// the products at small sizes through the first, and hold sizes to the kernels that
+// they are there for with the others.
+void vcsr_test_force_plan(int32_t tile, int32_t stages, int32_t splits, int64_t rows,
+                          int32_t together) {
+    vcsr::force_plan(vcsr::GemmPlan{tile, stages, splits, 0, rows}, together != 0);
+}
+// {tile, stages, splits, rows}
+int vcsr_test_linear_plan(const vcsr_linear_args* args, int64_t* out) {
+    return guarded([&] {
+        const vcsr::GemmPlan p = vcsr::gemm_plan(gemm_of(checked_sizes(args)));
+        const int64_t v[4] = {p.tile, p.stages, p.splits, p.rows};
+        std::copy(v, v + 4, out);
+    });
+}
+// {together, dw's tile and splits, dx's}
+int vcsr_test_linear_grad_plan(const vcsr_linear_grad_args* args, int64_t* out) {
+    return guarded([&] {
+        const LinearGrad w = grad_of(args);
+        const vcsr::PairPlan p = vcsr::gemm_pair_plan(w.dw, w.dx);
+        const int64_t v[5] = {p.together, p.dw.tile, p.dw.splits, p.dx.tile, p.dx.splits};
+        std::copy(v, v + 5, out);
+    });
+}
 
 }  // extern "C"

@@ -84,6 +84,28 @@ float extra_us(const Gemm& g, bool rounds) {
     return (float)((double)g.I * (double)g.J * size * count / 4e6) * (rounds ? 0.5f : 1.f);
 }
 
+// Of force_plan().
+struct Forced {
+    GemmPlan plan{};
+    bool together = false;
+};
+thread_local Forced forced;
+bool forced_takes(const Gemm& g) {
+    if (forced.plan.tile == 16) return g.I <= 16 && !g.p_cols && !g.q_cols;
+    const Costs c = costs_of(g);
+    for (const TileCost* t = c.t; t < c.t + c.n; ++t)
+        if (t->tile == forced.plan.tile && t->stages == forced.plan.stages) return true;
+    return false;
+}
+GemmPlan forced_plan(const Gemm& g) {
+    GemmPlan p = forced.plan;
+    const int64_t all = steps_of(g), want = p.splits < all ? p.splits : all;
+    p.steps = p.tile == 16 ? all : (all + want - 1) / want;
+    p.splits = (int32_t)((all + p.steps - 1) / p.steps);
+    if (p.rows <= 0 || p.rows >= g.I || p.splits > 1) p.rows = g.I;
+    return p;
+}
+
 // Rows [from, g.I) of a product.
 Gemm rows_from(Gemm g, int64_t from) {
     const int64_t size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
@@ -104,6 +126,7 @@ Gemm rows_from(Gemm g, int64_t from) {
 // 256 on 256 compute units).  splits = 0: no launch has that many blocks.
 GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true) {
     const int size = g.type == VCSR_F32 ? 4 : g.type == VCSR_BF16 ? 2 : 1;
+    if (forced.plan.tile && forced_takes(g)) return forced_plan(g);
     // Up to 8 rows: W is read straight into the matrix layout, 6 to 9 us up to 32 MB of
     // it against 10 of the tiles (their join is a launch of its own).  Not where
     // few blocks would read long rows alone, past what a wave asks for at once: 512 x
@@ -149,14 +172,20 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
 // Both products in one launch, if that is estimated faster than one after the
 // other: all blocks' time over the chip's room and part of a last block, or the
 // longest block alone, and dw's join.  (8192 x 2048 x 4096 bf16: dw has 128 tiles of 256, dx 256.)
-struct PairPlan {
-    bool together;
-    GemmPlan dw, dx;
-};
 PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
     float us_w = 0.f, us_x = 0.f;
     PairPlan best{false, plan_of(dw, &us_w), plan_of(dx, &us_x)};
     if (best.dw.splits == 0 || best.dx.splits == 0) return best;
+    if (forced.plan.tile && forced_takes(dw)) {
+        if (forced.together) {
+            best.together = true;
+            best.dx.splits = 1;
+            best.dx.steps = steps_of(dx);
+            best.dw.rows = dw.I;
+            best.dx.rows = dx.I;
+        }
+        return best;
+    }
     float best_us = us_w + us_x + 2.f;
     const Costs c = costs_of(dw);
     for (const TileCost* t = c.t; t < c.t + c.n; ++t) {
@@ -210,6 +239,10 @@ hipError_t launch(const Gemm& g, const GemmPlan& p, hipStream_t st) {
 }
 
 }  // namespace
+
+GemmPlan gemm_plan(const Gemm& g) { return plan_of(g); }
+PairPlan gemm_pair_plan(const Gemm& dw, const Gemm& dx) { return plan_pair(dw, dx); }
+void force_plan(const GemmPlan& p, bool together) { forced = Forced{p, together}; }
 
 size_t gemm_workspace(const Gemm& g) {
     return g.I <= 0 || g.J <= 0 ? 0 : part_bytes(g, launchable(plan_of(g)));
