@@ -1,12 +1,13 @@
-"""Every kernel of the dense products at small odd sizes, and the sizes that choose
-the large ones by themselves."""
+"""Every kernel of the dense products at small odd sizes, the sizes that choose the
+large ones by themselves, and every row shape of the norm."""
 from __future__ import annotations
 
 import numpy as np
 import pytest
 
 from dense_plans import STEP, TILES, forced, grad_plan, linear_plan
-from test_gpu_dense import grad_once, linear_once
+from dense_ref import EPS, Mat, close, rms_norm_grad, vector
+from test_gpu_dense import check_norm, grad_once, linear_once, rounding, values
 
 pytestmark = pytest.mark.gpu
 
@@ -143,3 +144,55 @@ def test_gradient_sizes_choose_their_kernels(gpu, size):
     assert all(w is None or g == w for g, w in zip(got, want)), got
     print(f"gradient {M}x{N}x{K} {kind}", flush=True)
     grad_once(gpu, gpu.Stream(), np.random.default_rng(8), M, N, K, kind, kind, "gelu")
+
+
+# ---------------------------------------------------------------- the norm's rows
+# Vectors of 16 bytes a row: one for each choice of waves and vectors a lane, at its
+# ends, and the first length that is read twice.
+VECTORS = [1, 2, 3, 64, 65, 128, 129, 192, 193, 256, 257, 384, 385, 512, 513, 768, 769, 1024, 1025,
+           1536, 1537, 2048, 2049]
+
+
+@pytest.mark.parametrize("vectors", VECTORS)
+@pytest.mark.parametrize("kinds", ["f32 bf16", "bf16 fp8"])
+def test_norm_rows_of_every_shape(gpu, kinds, vectors):
+    xk, yk = kinds.split()
+    V = 4 if xk == "f32" else 8
+    rng, st = np.random.default_rng(vectors), gpu.Stream()
+    for C in {vectors * V, vectors * V - V + 1, vectors * V - 1}:
+        if C < V:
+            continue
+        for M, pad, off in ((3, 0, 0), (9, 5, 1)):
+            print(f"norm {kinds} {M}x{C}", flush=True)
+            x, r = values(rng, (M, C), xk), values(rng, (M, C), xk)
+            w = (1 + 0.2 * rng.standard_normal(C)).astype(np.float32).astype(np.float64)
+            check_norm(gpu, st, x, r, w, xk, yk, 1e-6, f"{kinds} {M}x{C}", pad=pad, off=off)
+
+
+@pytest.mark.parametrize("vectors", VECTORS)
+@pytest.mark.parametrize("kinds", ["f32 bf16", "bf16 f32"])
+def test_norm_gradient_rows_of_every_shape(gpu, kinds, vectors):
+    xk, yk = kinds.split()
+    V = 4 if xk == "f32" else 8
+    rng, st = np.random.default_rng(vectors), gpu.Stream()
+    for C, M in ((vectors * V, 5), (vectors * V - V + 1, 300)):
+        if C < V:
+            continue
+        print(f"norm gradient {kinds} {M}x{C}", flush=True)
+        s, dy, ds = values(rng, (M, C), xk, 1.5), values(rng, (M, C), yk), values(rng, (M, C), xk)
+        w = (1 + 0.2 * rng.standard_normal(C)).astype(np.float32).astype(np.float64)
+        rstd = (1 / np.sqrt(np.mean(s * s, axis=1) + 1e-6)).astype(np.float32)
+        DX = Mat(gpu, st, None, xk, 3, 1, (M, C))
+        dweight = vector(gpu, st, np.full(C, np.nan))
+        gpu.run_rmsnorm_grad_gpu(Mat(gpu, st, dy, yk, 1, 1).view, Mat(gpu, st, s, xk, 2, 0).view,
+                                 vector(gpu, st, w), vector(gpu, st, rstd), DX.view, dweight,
+                                 dsum=Mat(gpu, st, ds, xk).view, stream=st)
+        st.sync()
+        rd = rstd.astype(np.float64)[:, None]
+        want, want_w = rms_norm_grad(dy, s, w, rd, ds)
+        h, g = np.abs(s * rd), np.abs(dy * w)
+        dot = np.sum(g * h, axis=1, keepdims=True) / C
+        tol = 8 * EPS * (rd * (g + h * dot) + np.abs(want)) + rd * h * dot * (C + 4) * EPS
+        close(DX.values(), want, tol + rounding(want, xk), f"dx {kinds} {M}x{C}")
+        close(dweight.numpy(st), want_w, (M + 6) * EPS * np.sum(np.abs(dy) * h, axis=0) + 1e-30,
+              "dweight")
