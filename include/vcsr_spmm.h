@@ -374,7 +374,8 @@ typedef struct {
     const float* weight; /* C                                                */
     void* sum;           int64_t ldsum; /* NULL, or t rounded to x_type; may
                                            be x or residual itself           */
-    void* y;             int64_t ldy;
+    void* y;             int64_t ldy;   /* may be x or residual itself, if of
+                                           one type                          */
     float* y_scale;      /* M, for VCSR_FP8 (NULL otherwise)                 */
     float* rstd;         /* NULL, or M: 1 / sqrt(mean(t^2) + eps)            */
 } vcsr_rmsnorm_args;
@@ -431,7 +432,8 @@ int vcsr_linear(const vcsr_linear_args* args, void* stream, float* ms);
 /* Gradients of vcsr_linear on VCSR_F32 or VCSR_BF16 operands: dz = dy *
  * act'(z), dx = dz W, dw = dz^T x, dbias = sum over rows of dz (the residual's
  * gradient is dy).  For VCSR_BF16 operands dz is rounded to bf16 before the two
- * products (the matrix cores' operand type); dbias sums the unrounded dz.
+ * products (the matrix cores' operand type), an FP32 dy too; dbias sums the
+ * unrounded dz.
  * dx and dw are other matrices than those their products read: w for dx, x for dw,
  * for both dy where it is dz as it lies (no activation, x_type = y_type), and
  * each other's operands where both are asked for. */

@@ -6,9 +6,8 @@
 // reduction over the wave and each state byte moves as part of a 4-byte word; the
 // loads of both blocks go out together, without branches between them where the
 // blocks are whole.  Everything is read and written once; bound by memory: 201M
-// values with 8-bit states, bf16 gradients and copies 606 to 628 us (5.2 TB/s), 1.05M
-// with FP32 states 7.1 us.  The
-// arithmetic is FP32 with each operation rounded on its own (no fused
+// values with 8-bit states, bf16 gradients and copies 611 to 637 us (5.1 to 5.3 TB/s),
+// 1.05M with FP32 states 7.2 us.  The arithmetic is FP32 with each operation rounded on its own (no fused
 // multiply-adds), in the order of the header's formula, so a step does not depend
 // on how the compiler contracts it.
 #include "dense.hpp"

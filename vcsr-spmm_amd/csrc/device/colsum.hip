@@ -37,9 +37,16 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* part, int32
 // A block takes `rows` rows of tx vectors of 16 bytes of dy: 256 / tx rows at a time,
 // four of them under way together without a branch between their loads (rows past
 // the block's end are its last one again and count for nothing).  Bound by memory:
-// dy and z read once, dz written once (8192 x 4096 bf16 with gelu 38 us, 5.3 TB/s; 30011
-// x 257 FP32, whose rows begin anywhere in a line, 28 us, 3.3 TB/s).  ENDS: how rows end: 0 in whole vectors,
-// 1 inside one, 2 before the first is whole.
+// dy and z read once, dz written once (8192 x 4096 bf16 with gelu 37 to 40 us, 5.0 to
+// 5.4 TB/s; 30011 x 257 FP32, whose rows begin anywhere in a line, 28 us, 3.3 TB/s).
+// ENDS: how rows end: 0 in whole vectors, 1 inside one, 2 before the first is whole.
+//
+// For bf16 operands dz is rounded to bf16, also where dy and z are FP32: the products'
+// matrix instruction takes no more.  Each dz moves by 2^-8 of itself at most, so a
+// product's error stays small against its own terms; the gradients of 8192 x 2048 x 4096
+// are 0.0023 from 64 bits, and 0.0017 with dz unrounded, which is their own last
+// rounding.  Two bf16 parts of dz would keep its bits for twice the matrix work (some
+// 280 of the call's 318 us again).
 template <class D, class X, int ACT, int ENDS>
 __global__ __launch_bounds__(256) void dz_kernel(vcsr_linear_grad_args a, X* dz, int64_t lddz,
                                                  float* part, int64_t rows, int tx) {

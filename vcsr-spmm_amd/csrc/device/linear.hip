@@ -16,6 +16,10 @@ constexpr int64_t kCus = tile::kCus;
 // thirds of the time (1024^3 10.8 -> 8.0 us).  FP32 tiles are bound by their matrix
 // instructions throughout, e4m3 ones by widening, and gain nothing from that, nor
 // do the gradients' launches, which fill the chip with both products.
+//
+// The times are of operands by rows.  Gradients, whose operands lie by columns, are
+// estimated with the same ones, which is too little for them (8192 x 2048 x 4096 bf16: dx
+// 103 us by the table, 124 to 131 measured; dw in 128 tiles 121, 158 to 178).
 struct TileCost {
     int tile, stages, room;
     float step[5], rest[5];
@@ -77,8 +81,8 @@ void each_split(const Gemm& g, int64_t tiles, F&& f) {
 }
 
 // z and the residual on top of out: their time at 4 TB/s, half of it hidden where
-// there is more than one round of blocks (62451 x 128 x 128 FP32 with a residual: tiles
-// of 64 in two rounds 30.5 us, of 128 in one 33.7).
+// there is more than one round of blocks.  Both numbers stand on one size: 62451 x 128 x
+// 128 FP32 with a residual, tiles of 64 in two rounds 30.3 us, of 128 in one 33.7.
 float extra_us(const Gemm& g, bool rounds) {
     const double size = g.out_type == VCSR_F32 ? 4 : 2, count = (g.residual ? 1 : 0) + (g.z ? 1 : 0);
     return (float)((double)g.I * (double)g.J * size * count / 4e6) * (rounds ? 0.5f : 1.f);

@@ -8,9 +8,10 @@
 // with v_mfma_f32_16x16x4_f32 or _16x16x32_bf16.
 //
 // What bounds it: big bf16 products the chip's power (8192 x 4096 x 8192 with gelu
-// 429 to 458 us, 1.2 to 1.28 PFLOP/s, the matrix units busy 56% at 2.0 to 2.15 GHz),
-// FP32 ones the matrix units (92% of their rate in full tiles), e4m3 ones widening
-// (4096 x 8192 x 4096 173 us, 1.59 PFLOP/s), few rows the weight's read.
+// 444 to 473 us, 1.16 to 1.24 PFLOP/s, the matrix units busy 57% at 1.8 to 2.15 GHz),
+// FP32 ones the matrix units (4096^3 130 TFLOP/s, a large library product 127 to 155),
+// e4m3 ones widening (4096 x 8192 x 4096 176 us, 1.56 PFLOP/s), few rows the weight's
+// read.
 //
 // LDS tiles are TI (or TJ) x 128 bytes in 16-byte granules:
 //   by rows     row r at r * 128, granule g of its k at slot g ^ key(r);
@@ -256,8 +257,9 @@ __device__ __forceinline__ f32x4 mma<float>(const u32x4& q, const u32x4& p, f32x
 }
 // e4m3: the values become bf16 exactly and go through the bf16 instruction,
 // whose sums are FP32.  The e4m3 instructions (16x16x32 and 16x16x128) align
-// their products to the largest and drop bits: up to 2^-12 of the largest product
-// was measured over 128 random terms, far more than FP32's rounding.
+// their products to the largest and drop bits: up to 2^-11.6 of the largest product
+// was measured over 128 random terms.  That is far more than FP32's rounding, and of
+// the largest product, not of each: a sum of many small ones beside it loses them.
 __device__ __forceinline__ void widen(const u32x4& v, bf16x8 (&o)[2]) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll

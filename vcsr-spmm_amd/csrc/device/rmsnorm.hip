@@ -9,7 +9,7 @@
 // over the rows a block takes in registers, then over the blocks (colsum.hip),
 // in a fixed order.  All of it is bound by memory: 32768 x 4096 bf16 with a residual
 // to e4m3 163 us (5.8 TB/s), 62451 x 128 FP32 28 us (4.6 TB/s), the gradient of
-// 16384 x 2050 bf16 69 us (3.9 TB/s), of 32768 x 4096 210 us (5.1 TB/s).
+// 16384 x 2050 bf16 68 us (3.9 TB/s), of 32768 x 4096 217 us (4.9 TB/s).
 #include <type_traits>
 
 #include "dense.hpp"
@@ -232,7 +232,9 @@ __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(vcsr_rmsnorm_args a)
     }
 }
 
-// Rows of fewer values than a vector: a thread takes a row.
+// Rows of fewer values than a vector: a thread takes a row.  Neighbouring threads'
+// rows share lines, so memory bounds it: 4.2M x 3 FP32 with a residual 52 us (3.9
+// TB/s), its gradient 50; with a block a row, as long ones have it, 19.5 and 32.7 ms.
 template <class X, class Y>
 __global__ __launch_bounds__(256) void rmsnorm_narrow_kernel(vcsr_rmsnorm_args a) {
     constexpr int V = kVec<X>;
