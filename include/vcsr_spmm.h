@@ -404,6 +404,55 @@ typedef struct {
 int vcsr_rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args* args, size_t* bytes);
 int vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args* args, void* stream, float* ms);
 
+/* t = x + residual;  y = (t - mean(t)) / sqrt(mean((t - mean(t))^2) + eps) * weight +
+ * bias, row by row, in FP32; the variance is that of the centred values.  y of
+ * VCSR_FP8 as vcsr_rmsnorm has it.  A row with a NaN or an infinity gives NaN for all of
+ * y, and no other row does.  The row's sums are FP32's too: where that of t passes
+ * 3.4e38 y is NaN, where that of the squares does rstd is zero and y the bias. */
+typedef struct {
+    int64_t M;           /* rows; 0 is no work                               */
+    int32_t C;           /* columns, >= 1                                    */
+    int32_t x_type;      /* x, residual, sum: VCSR_F32 or VCSR_BF16          */
+    int32_t y_type;      /* VCSR_F32, VCSR_BF16 or VCSR_FP8                  */
+    float eps;           /* >= 0                                             */
+    const void* x;       int64_t ldx;
+    const void* residual; int64_t ldr;  /* NULL: t = x                       */
+    const float* weight; /* C                                                */
+    const float* bias;   /* C, or NULL                                       */
+    void* sum;           int64_t ldsum; /* NULL, or t rounded to x_type; may
+                                           be x or residual itself           */
+    void* y;             int64_t ldy;   /* may be x or residual itself, if of
+                                           one type                          */
+    float* y_scale;      /* M, for VCSR_FP8 (NULL otherwise)                 */
+    float* mean;         /* NULL, or M: mean(t)                              */
+    float* rstd;         /* NULL, or M: 1 / sqrt(variance + eps)             */
+} vcsr_layernorm_args;
+int vcsr_layernorm(const vcsr_layernorm_args* args, void* stream, float* ms);
+
+/* Gradients of vcsr_layernorm: with s the saved sum (or x), h = (s - mean) * rstd and
+ * g = dy * weight:  dx = dsum + rstd * (g - mean(g) - h * mean(g * h)),
+ * dweight = sum over rows of dy * h, dbias = sum over rows of dy.  dx is the gradient
+ * of x and of the residual alike. */
+typedef struct {
+    int64_t M;
+    int32_t C;
+    int32_t x_type;      /* s, dsum, dx: VCSR_F32 or VCSR_BF16               */
+    int32_t y_type;      /* dy: VCSR_F32 or VCSR_BF16                        */
+    const void* dy;      int64_t lddy;
+    const void* s;       int64_t lds;
+    const float* weight; /* C                                                */
+    const float* mean;   /* M                                                */
+    const float* rstd;   /* M                                                */
+    const void* dsum;    int64_t lddsum; /* NULL, or what flows into `sum`   */
+    void* dx;            int64_t lddx;   /* may be dsum, s or dy itself      */
+    float* dweight;      /* C (zeros for M = 0), or NULL                     */
+    float* dbias;        /* C (zeros for M = 0), or NULL                     */
+    void* workspace;     size_t workspace_bytes;
+} vcsr_layernorm_grad_args;
+/* As vcsr_rmsnorm_grad_workspace. */
+int vcsr_layernorm_grad_workspace(const vcsr_layernorm_grad_args* args, size_t* bytes);
+int vcsr_layernorm_grad(const vcsr_layernorm_grad_args* args, void* stream, float* ms);
+
 /* z = x W^T + bias;  y = act(z) + residual.  W has one row per output column.
  * Products are summed in FP32 (FP32 operands on the FP32 matrix cores); VCSR_FP8
  * operands carry a scale per row: z[m][n] = x_scale[m] * w_scale[n] * (x W^T)

@@ -56,7 +56,9 @@ EXPORTS = (
     "vcsr_memcpy_h2d vcsr_memcpy_d2h vcsr_memcpy_d2d vcsr_memset_d vcsr_stream_create vcsr_stream_destroy "
     "vcsr_stream_sync vcsr_device_sync vcsr_event_create vcsr_event_destroy "
     "vcsr_event_record vcsr_event_elapsed "
-    "vcsr_rmsnorm vcsr_rmsnorm_grad_workspace vcsr_rmsnorm_grad vcsr_linear_workspace vcsr_linear "
+    "vcsr_rmsnorm vcsr_rmsnorm_grad_workspace vcsr_rmsnorm_grad "
+    "vcsr_layernorm vcsr_layernorm_grad_workspace vcsr_layernorm_grad "
+    "vcsr_linear_workspace vcsr_linear "
     "vcsr_linear_grad_workspace vcsr_linear_grad vcsr_adamw_create vcsr_adamw_step vcsr_adamw_free"
 ).split()
 
@@ -114,6 +116,24 @@ class _RmsnormGradArgs(C.Structure):
                 ("workspace_bytes", C.c_size_t)]
 
 
+class _LayernormArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("C", C.c_int32), ("x_type", C.c_int32), ("y_type", C.c_int32),
+                ("eps", C.c_float), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("weight", C.c_void_p),
+                ("bias", C.c_void_p), ("sum", C.c_void_p), ("ldsum", C.c_int64),
+                ("y", C.c_void_p), ("ldy", C.c_int64), ("y_scale", C.c_void_p),
+                ("mean", C.c_void_p), ("rstd", C.c_void_p)]
+
+
+class _LayernormGradArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("C", C.c_int32), ("x_type", C.c_int32), ("y_type", C.c_int32),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("s", C.c_void_p), ("lds", C.c_int64),
+                ("weight", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+                ("dsum", C.c_void_p), ("lddsum", C.c_int64), ("dx", C.c_void_p),
+                ("lddx", C.c_int64), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class _LinearArgs(C.Structure):
     _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("x_type", C.c_int32),
                 ("y_type", C.c_int32), ("act", C.c_int32), ("x", C.c_void_p), ("ldx", C.c_int64),
@@ -145,9 +165,10 @@ def _packer(fields, size):
 # by themselves.
 _pack_rmsnorm = _packer(_RmsnormArgs._fields_, C.sizeof(_RmsnormArgs))
 _pack_space = _packer(_LinearArgs._fields_[-2:], 16)
-_pack_rmsnorm_grad, _pack_linear, _pack_linear_grad = (
+_pack_layernorm = _packer(_LayernormArgs._fields_, C.sizeof(_LayernormArgs))
+_pack_rmsnorm_grad, _pack_layernorm_grad, _pack_linear, _pack_linear_grad = (
     _packer(args._fields_[:-2], C.sizeof(args) - 16)
-    for args in (_RmsnormGradArgs, _LinearArgs, _LinearGradArgs))
+    for args in (_RmsnormGradArgs, _LayernormGradArgs, _LinearArgs, _LinearGradArgs))
 
 
 class _AdamwTensor(C.Structure):
@@ -233,6 +254,9 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "vcsr_rmsnorm": (C.c_int, [P, P, pF]),
         "vcsr_rmsnorm_grad_workspace": (C.c_int, [P, pS]),
         "vcsr_rmsnorm_grad": (C.c_int, [P, P, pF]),
+        "vcsr_layernorm": (C.c_int, [P, P, pF]),
+        "vcsr_layernorm_grad_workspace": (C.c_int, [P, pS]),
+        "vcsr_layernorm_grad": (C.c_int, [P, P, pF]),
         "vcsr_linear_workspace": (C.c_int, [P, pS]),
         "vcsr_linear": (C.c_int, [P, P, pF]),
         "vcsr_linear_grad_workspace": (C.c_int, [P, pS]),
@@ -884,6 +908,15 @@ def _rmsnorm_grad_bytes(M, N, x_type, y_type):
     return need.value
 
 
+@functools.lru_cache(maxsize=4096)
+def _layernorm_grad_bytes(M, N, x_type, y_type, dweight, dbias):
+    need = C.c_size_t(0)
+    args = _LayernormGradArgs(M=M, C=N, x_type=x_type, y_type=y_type,
+                              dweight=16 if dweight else None, dbias=32 if dbias else None)
+    _check(load_library().vcsr_layernorm_grad_workspace(C.byref(args), C.byref(need)))
+    return need.value
+
+
 def _call(fn, args, stream, timed):
     if not timed:
         rc = fn(args, stream.h if stream is not None else None, None)
@@ -935,6 +968,38 @@ def run_rmsnorm_grad_gpu(dy, s, weight, rstd, dx, dweight=None, dsum=None, works
                               _vec(rstd, M, "rstd"), up, ldu, xp, ldx,
                               _vec(dweight, N, "dweight"))
     return _call_with_space((_lib or load_library()).vcsr_rmsnorm_grad, args, need, workspace,
+                            stream, timed)
+
+
+def run_layernorm_gpu(x, weight, y, bias=None, residual=None, sum=None, y_scale=None, mean=None,
+                      rstd=None, eps=1e-5, stream=None, timed=False):
+    """y = (t - mean(t)) / sqrt(var(t) + eps) * weight + bias for t = x + residual,
+    row by row (vcsr_layernorm).  Types as run_rmsnorm_gpu's; sum receives t, mean and
+    rstd each row's mean and factor."""
+    M, N = _shape2(x, "x")
+    (xp, ldx), (rp, ldr) = _mat(x, M, N, "x"), _mat(residual, M, N, "residual", x.dtype)
+    (sp, lds), (yp, ldy) = _mat(sum, M, N, "sum", x.dtype), _mat(y, M, N, "y")
+    args = _pack_layernorm(M, N, _type(x, "x"), _type(y, "y"), eps, xp, ldx, rp, ldr,
+                           _vec(weight, N, "weight"), _vec(bias, N, "bias"), sp, lds, yp, ldy,
+                           _vec(y_scale, M, "y_scale"), _vec(mean, M, "mean"),
+                           _vec(rstd, M, "rstd"))
+    return _call((_lib or load_library()).vcsr_layernorm, args, stream, timed)
+
+
+def run_layernorm_grad_gpu(dy, s, weight, mean, rstd, dx, dweight=None, dbias=None, dsum=None,
+                           workspace=None, stream=None, timed=False):
+    """Gradients of run_layernorm_gpu (vcsr_layernorm_grad): s is the saved sum (x
+    without a residual), dsum what flows into it from elsewhere; dx is the gradient of
+    x and of the residual."""
+    M, N = _shape2(s, "s")
+    (dp, lddy), (sp, lds) = _mat(dy, M, N, "dy"), _mat(s, M, N, "s")
+    (up, ldu), (xp, ldx) = _mat(dsum, M, N, "dsum", s.dtype), _mat(dx, M, N, "dx", s.dtype)
+    xt, yt = _type(s, "s"), _type(dy, "dy")
+    need = _layernorm_grad_bytes(M, N, xt, yt, dweight is not None, dbias is not None)
+    args = _pack_layernorm_grad(M, N, xt, yt, dp, lddy, sp, lds, _vec(weight, N, "weight"),
+                                _vec(mean, M, "mean"), _vec(rstd, M, "rstd"), up, ldu, xp, ldx,
+                                _vec(dweight, N, "dweight"), _vec(dbias, N, "dbias"))
+    return _call_with_space((_lib or load_library()).vcsr_layernorm_grad, args, need, workspace,
                             stream, timed)
 
 

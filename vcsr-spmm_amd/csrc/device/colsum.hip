@@ -7,9 +7,15 @@ namespace {
 
 // 16 columns a block, 64 threads a column: each adds every 64th partial row, then
 // LDS adds the threads in order.
+// blockIdx.y: of two sums, whose partial rows lie `next` apart, `out` or `out2`.
 __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* part, int32_t P, int32_t C,
-                                                        int64_t ld, float* out) {
+                                                        int64_t ld, float* out, float* out2,
+                                                        int64_t next) {
     __shared__ float lds[64][17];
+    if (blockIdx.y) {
+        part += next;
+        out = out2;
+    }
     const int col = threadIdx.x & 15, grp = threadIdx.x >> 4;
     const int64_t c = (int64_t)blockIdx.x * 16 + col;
     float t = 0.f;
@@ -167,15 +173,20 @@ __global__ __launch_bounds__(256) void zero_kernel(uint16_t* p, int64_t ld, int6
 
 }  // namespace
 
-hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, float* out,
-                           hipStream_t st) {
+hipError_t launch_sum_row_pairs(const float* part, int32_t P, int32_t C, int64_t ld, float* a,
+                                float* b, hipStream_t st) {
     // 64 threads a column, and fewer than 2^32 threads a launch.
-    constexpr int32_t kMost = 1 << 25;
-    for (int64_t c = 0; c < C; c += kMost) {
-        const int32_t n = C - c < kMost ? (int32_t)(C - c) : kMost;
-        sum_rows_kernel<<<(unsigned)((n + 15) / 16), 1024, 0, st>>>(part + c, P, n, ld, out + c);
+    const int32_t most = b ? 1 << 24 : 1 << 25;
+    for (int64_t c = 0; c < C; c += most) {
+        const int32_t n = C - c < most ? (int32_t)(C - c) : most;
+        sum_rows_kernel<<<dim3((unsigned)((n + 15) / 16), b ? 2 : 1), 1024, 0, st>>>(
+            part + c, P, n, ld, a + c, b ? b + c : nullptr, C);
     }
     return hipGetLastError();
+}
+hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, float* out,
+                           hipStream_t st) {
+    return launch_sum_row_pairs(part, P, C, ld, out, nullptr, st);
 }
 
 int32_t dz_row_blocks(int64_t M, int32_t N, int32_t dy_type) {

@@ -170,10 +170,19 @@ hipError_t launch_rmsnorm(const vcsr_rmsnorm_args& a, hipStream_t st);
 hipError_t launch_rmsnorm_grad(const vcsr_rmsnorm_grad_args& a, hipStream_t st);
 size_t rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args& a);
 
+// ----------------------------------------------------------- layernorm.hip
+// As rmsnorm.hip's.
+hipError_t launch_layernorm(const vcsr_layernorm_args& a, hipStream_t st);
+hipError_t launch_layernorm_grad(const vcsr_layernorm_grad_args& a, hipStream_t st);
+size_t layernorm_grad_workspace(const vcsr_layernorm_grad_args& a);
+
 // -------------------------------------------------------------- colsum.hip
 // out[c] = sum over p < P of part[p * ld + c] for c < C, in a fixed order.
 hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, float* out,
                            hipStream_t st);
+// The same of part into `a` and, where given, of part + C into `b`, in one launch.
+hipError_t launch_sum_row_pairs(const float* part, int32_t P, int32_t C, int64_t ld, float* a,
+                                float* b, hipStream_t st);
 // dz = dy * act'(z) in x_type (dz may be NULL) and, for each block of
 // dz_row_blocks(M, N, type of dy), the sums of its rows of dz in `part` (ld N; may be NULL).
 hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, float* part,

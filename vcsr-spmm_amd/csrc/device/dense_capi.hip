@@ -61,9 +61,9 @@ void check_workspace(const void* p, size_t have, size_t want) {
     need((uintptr_t)p % 16 == 0, "workspace: not 16-byte aligned");
 }
 
-vcsr_rmsnorm_args checked(const vcsr_rmsnorm_args* args) {
-    need(args, "null argument");
-    vcsr_rmsnorm_args a = *args;
+// What the two norms check alike.
+template <class Args>
+void check_norm(Args& a) {
     check_rows(a.M);
     need(a.C >= 1, "C: at least 1");
     need(is_wide(a.x_type), "x_type: VCSR_F32 or VCSR_BF16");
@@ -85,20 +85,35 @@ vcsr_rmsnorm_args checked(const vcsr_rmsnorm_args* args) {
     need(!a.sum || a.sum != a.y, "sum: another matrix than y");
     need(!a.sum || a.sum != a.x || a.ldsum == a.ldx, "sum over x: of another stride");
     need(!a.sum || a.sum != a.residual || a.ldsum == a.ldr, "sum over residual: of another stride");
+}
+vcsr_rmsnorm_args checked(const vcsr_rmsnorm_args* args) {
+    need(args, "null argument");
+    vcsr_rmsnorm_args a = *args;
+    check_norm(a);
+    return a;
+}
+vcsr_layernorm_args checked(const vcsr_layernorm_args* args) {
+    need(args, "null argument");
+    vcsr_layernorm_args a = *args;
+    check_norm(a);
+    check_vector(a.bias, "bias: alignment", true);
+    check_vector(a.mean, "mean: alignment", true);
     return a;
 }
 
-vcsr_rmsnorm_grad_args checked_sizes(const vcsr_rmsnorm_grad_args* args) {
+template <class Args>
+Args checked_norm_sizes(const Args* args) {
     need(args, "null argument");
-    vcsr_rmsnorm_grad_args a = *args;
+    Args a = *args;
     check_rows(a.M);
     need(a.C >= 1, "C: at least 1");
     need(is_wide(a.x_type), "x_type: VCSR_F32 or VCSR_BF16");
     need(is_wide(a.y_type), "y_type: VCSR_F32 or VCSR_BF16");
     return a;
 }
-vcsr_rmsnorm_grad_args checked(const vcsr_rmsnorm_grad_args* args) {
-    vcsr_rmsnorm_grad_args a = checked_sizes(args);
+template <class Args>
+Args checked_norm_grad(const Args* args) {
+    Args a = checked_norm_sizes(args);
     check_matrix(a.dy, a.lddy, a.C, a.y_type, "dy: pointer, alignment or stride", false, a.M);
     check_matrix(a.s, a.lds, a.C, a.x_type, "s: pointer, alignment or stride", false, a.M);
     check_vector(a.weight, "weight: pointer or alignment");
@@ -112,7 +127,19 @@ vcsr_rmsnorm_grad_args checked(const vcsr_rmsnorm_grad_args* args) {
         need(a.dx != a.dy || (a.x_type == a.y_type && a.lddx == a.lddy),
              "dx over dy: of another type or stride");
     }
+    return a;
+}
+vcsr_rmsnorm_grad_args checked(const vcsr_rmsnorm_grad_args* args) {
+    const vcsr_rmsnorm_grad_args a = checked_norm_grad(args);
     check_workspace(a.workspace, a.workspace_bytes, vcsr::rmsnorm_grad_workspace(a));
+    return a;
+}
+vcsr_layernorm_grad_args checked(const vcsr_layernorm_grad_args* args) {
+    const vcsr_layernorm_grad_args a = checked_norm_grad(args);
+    check_vector(a.mean, "mean: pointer or alignment", a.M == 0);
+    check_vector(a.dbias, "dbias: alignment", true);
+    need(!a.dbias || a.dbias != a.dweight, "dbias: another vector than dweight");
+    check_workspace(a.workspace, a.workspace_bytes, vcsr::layernorm_grad_workspace(a));
     return a;
 }
 
@@ -348,7 +375,7 @@ int vcsr_rmsnorm(const vcsr_rmsnorm_args* args, void* stream, float* ms) {
 int vcsr_rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args* args, size_t* bytes) {
     return guarded([&] {
         need(bytes, "null argument");
-        *bytes = vcsr::rmsnorm_grad_workspace(checked_sizes(args));
+        *bytes = vcsr::rmsnorm_grad_workspace(checked_norm_sizes(args));
     });
 }
 
@@ -358,6 +385,31 @@ int vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args* args, void* stream, float* m
         need_device();
         hipStream_t st = (hipStream_t)stream;
         run_timed(st, ms, [&] { return vcsr::launch_rmsnorm_grad(a, st); });
+    });
+}
+
+int vcsr_layernorm(const vcsr_layernorm_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_layernorm_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return vcsr::launch_layernorm(a, st); });
+    });
+}
+
+int vcsr_layernorm_grad_workspace(const vcsr_layernorm_grad_args* args, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = vcsr::layernorm_grad_workspace(checked_norm_sizes(args));
+    });
+}
+
+int vcsr_layernorm_grad(const vcsr_layernorm_grad_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_layernorm_grad_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return vcsr::launch_layernorm_grad(a, st); });
     });
 }
 

@@ -10,63 +10,18 @@
 // in a fixed order.  All of it is bound by memory: 32768 x 4096 bf16 with a residual
 // to e4m3 163 us (5.8 TB/s), 62451 x 128 FP32 28 us (4.6 TB/s), the gradient of
 // 16384 x 2050 bf16 68 us (3.9 TB/s), of 32768 x 4096 217 us (4.9 TB/s).
-#include <type_traits>
-
 #include "dense.hpp"
-#include "launch.hpp"
+#include "norm_rows.hpp"
 
 namespace vcsr {
 namespace {
 
-// Values of one lane's vector: 16 bytes of x.
-template <class X>
-constexpr int kVec = 16 / (int)sizeof(X);
-
-// Sum and maximum over groups of `lanes` (a power of two <= 64) lanes.  The
-// maximum keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) { return a > b || a != a ? a : b; }
-__device__ __forceinline__ void reduce_lanes(int lanes, float& sum, float& top) {
-    for (int m = 1; m < lanes; m <<= 1) {
-        sum += __shfl_xor(sum, m);
-        top = max_nan(top, __shfl_xor(top, m));
-    }
-}
-__device__ __forceinline__ float sum_lanes(int lanes, float x) {
-    for (int m = 1; m < lanes; m <<= 1) x += __shfl_xor(x, m);
-    return x;
-}
-// The same over the block's waves; every wave calls it, in the same order of
-// addition.
-template <int WAVES>
-__device__ __forceinline__ void reduce_waves(float* lds, float& sum, float& top) {
-    const int w = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-        lds[w] = sum;
-        lds[WAVES + w] = top;
-    }
-    __syncthreads();
-    sum = lds[0];
-    top = lds[WAVES];
-#pragma unroll
-    for (int i = 1; i < WAVES; ++i) {
-        sum += lds[i];
-        top = max_nan(top, lds[WAVES + i]);
-    }
-}
+using namespace norm;
 
 // Whether max |t * w| stands for max |y| / rstd: it does not where that product is
 // past FP32's range (or loses bits below it), which y = t * rstd * w need not be (1e-18
 // * 1e-27, or 1e18 * 1e22).  y's own maximum is taken there.
 __device__ __forceinline__ bool top_lost(float top) { return top < 0x1p-100f || top > 0x1p126f; }
-// Scale of a row whose largest |y| is `top`.
-template <class Y>
-__device__ __forceinline__ float row_factor(float top, float* y_scale, int64_t row, bool writes) {
-    if (sizeof(Y) != 1) return 1.f;
-    const float a = top < 1e-30f ? 1e-30f : top;  // a NaN stays one
-    const float scale = a / 448.f;
-    if (writes) y_scale[row] = scale;
-    return scale;
-}
 template <int V>
 __device__ __forceinline__ float y_top(const float (&t)[V], const float (&w)[V], float rstd,
                                        float top) {
@@ -86,27 +41,6 @@ __device__ __forceinline__ void write_y(Y* p, int n, const float (&t)[V], const 
         if (sizeof(Y) == 1) y[i] = y[i] / scale;
     }
     store_vec(p, n, y);
-}
-
-// A lane's NV vectors of a row of C >= V values: all but the last are whole.
-template <class T, int NV, int V>
-__device__ __forceinline__ void load_row(const T* row, int lane, int stride, int C,
-                                         float (&v)[NV][V]) {
-#pragma unroll
-    for (int k = 0; k + 1 < NV; ++k) load_full(row + (k * stride + lane) * V, v[k]);
-    load_tail(row, ((NV - 1) * stride + lane) * V, C, v[NV - 1]);
-}
-template <class T, int NV, int V>
-__device__ __forceinline__ void store_row(T* row, int lane, int stride, int C,
-                                          const float (&v)[NV][V]) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = (k * stride + lane) * V;
-        if (k + 1 < NV)
-            store_vec(row + c, V, v[k]);
-        else if (c < C)
-            store_vec(row + c, C - c, v[k]);
-    }
 }
 
 // Rows of at most NV * 64 * WPR vectors, held in registers.  WPR = 1: groups of
@@ -264,14 +198,6 @@ __global__ __launch_bounds__(256) void rmsnorm_narrow_kernel(vcsr_rmsnorm_args a
     write_y((Y*)a.y + row * a.ldy, a.C, t, w, rstd, scale);
 }
 
-// A launch has fewer than 2^32 threads: more rows than that, at `threads` each, go
-// in several.  launch(first, count) takes whole blocks of at most 256 rows.
-template <class F>
-void by_rows(int64_t M, int64_t threads, F&& launch) {
-    const int64_t most = ((((int64_t)1 << 32) - 1) / threads) & ~(int64_t)255;
-    for (int64_t first = 0; first < M; first += most)
-        launch(first, M - first < most ? M - first : most);
-}
 template <class X, class Y>
 vcsr_rmsnorm_args rows_of(vcsr_rmsnorm_args a, int64_t first, int64_t count) {
     a.M = count;
@@ -282,53 +208,6 @@ vcsr_rmsnorm_args rows_of(vcsr_rmsnorm_args a, int64_t first, int64_t count) {
     if (a.y_scale) a.y_scale += first;
     if (a.rstd) a.rstd += first;
     return a;
-}
-
-int next_pow2(int n) {
-    int p = 1;
-    while (p < n) p <<= 1;
-    return p;
-}
-
-// Waves of a row and vectors of a lane: the fewest idle vectors (2050 bf16 are 257
-// vectors: 3 x 128 rather than 2 x 256), and where that leaves a choice two vectors
-// a lane, whose loads are under way together (4096 bf16: 4 waves of 2 vectors 166
-// us at 32768 rows, 8 waves of 1 206).  nv <= 2048.
-struct RowShape {
-    int wpr, nv;
-};
-RowShape row_shape(int64_t nv, int most_nv) {
-    RowShape best{8, 4};
-    int64_t slots = 1 << 30;
-    for (int k : {2, 3, 1, 4})
-        for (int wpr = 1; wpr <= 8; wpr <<= 1) {
-            const int64_t s = (int64_t)wpr * 64 * k;
-            if (s >= nv && s < slots && (k <= most_nv || s > 1536)) {
-                slots = s;
-                best = RowShape{wpr, k};
-            }
-        }
-    return best;
-}
-
-// f.operator()<WPR, NV>() of a shape.
-template <class F>
-void with_shape(RowShape s, F&& f) {
-    auto by_nv = [&](auto wpr) {
-        constexpr int W = decltype(wpr)::value;
-        switch (s.nv) {
-            case 1: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 1>{});
-            case 2: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 2>{});
-            case 3: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 3>{});
-            default: return f(std::integral_constant<int, W>{}, std::integral_constant<int, 4>{});
-        }
-    };
-    switch (s.wpr) {
-        case 1: return by_nv(std::integral_constant<int, 1>{});
-        case 2: return by_nv(std::integral_constant<int, 2>{});
-        case 4: return by_nv(std::integral_constant<int, 4>{});
-        default: return by_nv(std::integral_constant<int, 8>{});
-    }
 }
 
 template <class X, class Y>
