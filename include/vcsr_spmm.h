@@ -453,6 +453,42 @@ typedef struct {
 int vcsr_layernorm_grad_workspace(const vcsr_layernorm_grad_args* args, size_t* bytes);
 int vcsr_layernorm_grad(const vcsr_layernorm_grad_args* args, void* stream, float* ms);
 
+/* y[m] = scale * table[ids[m]], row by row; a table of VCSR_FP8 carries a scale per row,
+ * y[m] = scale * table_scale[ids[m]] * table[ids[m]].  The product is FP32's, y rounded
+ * once.  An id outside [0, V), such as -1 for padding, gives a row of zeros. */
+typedef struct {
+    int64_t M;           /* tokens, rows of y; 0 is no work                  */
+    int32_t V, C;        /* rows and columns of the table, >= 1; C <= 2^20   */
+    int32_t table_type;  /* VCSR_F32, VCSR_BF16 or VCSR_FP8                  */
+    int32_t y_type;      /* VCSR_F32 or VCSR_BF16                            */
+    float scale;         /* finite                                           */
+    const void* table;   int64_t ldt;
+    const float* table_scale; /* V, for VCSR_FP8 (NULL otherwise)            */
+    const int32_t* ids;  /* M                                                */
+    void* y;             int64_t ldy;   /* another matrix than the table     */
+} vcsr_embed_args;
+int vcsr_embed(const vcsr_embed_args* args, void* stream, float* ms);
+
+/* Gradient of vcsr_embed: dtable[v] = scale * sum of dy[m] over ids[m] = v, in FP32 and
+ * in an order that the ids alone decide, rounded once; zeros in rows without a token.
+ * With `accumulate` that is added to what dtable holds, and rows without a token are
+ * neither read nor written. */
+typedef struct {
+    int64_t M;
+    int32_t V, C;
+    int32_t table_type;  /* dtable: VCSR_F32 or VCSR_BF16                    */
+    int32_t y_type;      /* dy: VCSR_F32 or VCSR_BF16                        */
+    int32_t accumulate;  /* 0 or 1                                           */
+    float scale;
+    const void* dy;      int64_t lddy;
+    const int32_t* ids;  /* M                                                */
+    void* dtable;        int64_t lddt;  /* V x C, another matrix than dy     */
+    void* workspace;     size_t workspace_bytes;
+} vcsr_embed_grad_args;
+/* As vcsr_rmsnorm_grad_workspace. */
+int vcsr_embed_grad_workspace(const vcsr_embed_grad_args* args, size_t* bytes);
+int vcsr_embed_grad(const vcsr_embed_grad_args* args, void* stream, float* ms);
+
 /* z = x W^T + bias;  y = act(z) + residual.  W has one row per output column.
  * Products are summed in FP32 (FP32 operands on the FP32 matrix cores); VCSR_FP8
  * operands carry a scale per row: z[m][n] = x_scale[m] * w_scale[n] * (x W^T)

@@ -58,7 +58,7 @@ EXPORTS = (
     "vcsr_event_record vcsr_event_elapsed "
     "vcsr_rmsnorm vcsr_rmsnorm_grad_workspace vcsr_rmsnorm_grad "
     "vcsr_layernorm vcsr_layernorm_grad_workspace vcsr_layernorm_grad "
-    "vcsr_linear_workspace vcsr_linear "
+    "vcsr_embed vcsr_embed_grad_workspace vcsr_embed_grad vcsr_linear_workspace vcsr_linear "
     "vcsr_linear_grad_workspace vcsr_linear_grad vcsr_adamw_create vcsr_adamw_step vcsr_adamw_free"
 ).split()
 
@@ -134,6 +134,21 @@ class _LayernormGradArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class _EmbedArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("V", C.c_int32), ("C", C.c_int32), ("table_type", C.c_int32),
+                ("y_type", C.c_int32), ("scale", C.c_float), ("table", C.c_void_p),
+                ("ldt", C.c_int64), ("table_scale", C.c_void_p), ("ids", C.c_void_p),
+                ("y", C.c_void_p), ("ldy", C.c_int64)]
+
+
+class _EmbedGradArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("V", C.c_int32), ("C", C.c_int32), ("table_type", C.c_int32),
+                ("y_type", C.c_int32), ("accumulate", C.c_int32), ("scale", C.c_float),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("ids", C.c_void_p),
+                ("dtable", C.c_void_p), ("lddt", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 class _LinearArgs(C.Structure):
     _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("x_type", C.c_int32),
                 ("y_type", C.c_int32), ("act", C.c_int32), ("x", C.c_void_p), ("ldx", C.c_int64),
@@ -166,9 +181,11 @@ def _packer(fields, size):
 _pack_rmsnorm = _packer(_RmsnormArgs._fields_, C.sizeof(_RmsnormArgs))
 _pack_space = _packer(_LinearArgs._fields_[-2:], 16)
 _pack_layernorm = _packer(_LayernormArgs._fields_, C.sizeof(_LayernormArgs))
-_pack_rmsnorm_grad, _pack_layernorm_grad, _pack_linear, _pack_linear_grad = (
+_pack_embed = _packer(_EmbedArgs._fields_, C.sizeof(_EmbedArgs))
+_pack_rmsnorm_grad, _pack_layernorm_grad, _pack_embed_grad, _pack_linear, _pack_linear_grad = (
     _packer(args._fields_[:-2], C.sizeof(args) - 16)
-    for args in (_RmsnormGradArgs, _LayernormGradArgs, _LinearArgs, _LinearGradArgs))
+    for args in (_RmsnormGradArgs, _LayernormGradArgs, _EmbedGradArgs, _LinearArgs,
+                 _LinearGradArgs))
 
 
 class _AdamwTensor(C.Structure):
@@ -257,6 +274,9 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "vcsr_layernorm": (C.c_int, [P, P, pF]),
         "vcsr_layernorm_grad_workspace": (C.c_int, [P, pS]),
         "vcsr_layernorm_grad": (C.c_int, [P, P, pF]),
+        "vcsr_embed": (C.c_int, [P, P, pF]),
+        "vcsr_embed_grad_workspace": (C.c_int, [P, pS]),
+        "vcsr_embed_grad": (C.c_int, [P, P, pF]),
         "vcsr_linear_workspace": (C.c_int, [P, pS]),
         "vcsr_linear": (C.c_int, [P, P, pF]),
         "vcsr_linear_grad_workspace": (C.c_int, [P, pS]),
@@ -819,6 +839,14 @@ def _vec(arr, n, what):
     return arr.ptr.value or 0
 
 
+def _ids(arr, what):
+    """(address, count) of int32 indices, back to back."""
+    if arr.dtype != np.int32 or len(arr.shape) != 1 or arr.nbytes < 4 * arr.shape[0]:
+        raise VcsrError(VCSR_EINVAL, f"{what}: {arr.dtype} {arr.shape}, {arr.nbytes} bytes; a "
+                                     "vector of int32 is expected")
+    return arr.ptr.value or 0, arr.shape[0]
+
+
 def _shape2(arr, what):
     if len(arr.shape) != 2:
         raise VcsrError(VCSR_EINVAL, f"{what}: shape {arr.shape}, a matrix is expected")
@@ -917,6 +945,14 @@ def _layernorm_grad_bytes(M, N, x_type, y_type, dweight, dbias):
     return need.value
 
 
+@functools.lru_cache(maxsize=4096)
+def _embed_grad_bytes(M, V, N, table_type, y_type):
+    need = C.c_size_t(0)
+    args = _EmbedGradArgs(M=M, V=V, C=N, table_type=table_type, y_type=y_type)
+    _check(load_library().vcsr_embed_grad_workspace(C.byref(args), C.byref(need)))
+    return need.value
+
+
 def _call(fn, args, stream, timed):
     if not timed:
         rc = fn(args, stream.h if stream is not None else None, None)
@@ -1001,6 +1037,31 @@ def run_layernorm_grad_gpu(dy, s, weight, mean, rstd, dx, dweight=None, dbias=No
                                 _vec(dweight, N, "dweight"), _vec(dbias, N, "dbias"))
     return _call_with_space((_lib or load_library()).vcsr_layernorm_grad, args, need, workspace,
                             stream, timed)
+
+
+def run_embed_gpu(table, ids, y, scale=1.0, table_scale=None, stream=None, timed=False):
+    """y[m] = scale * table[ids[m]] (vcsr_embed).  table: float32, BF16, or FP8 with
+    table_scale, one scale a row; ids: int32, those outside the table (padding) give rows
+    of zeros; y: float32 or BF16."""
+    (V, N), (ip, M) = _shape2(table, "table"), _ids(ids, "ids")
+    (tp, ldt), (yp, ldy) = _mat(table, V, N, "table"), _mat(y, M, N, "y")
+    args = _pack_embed(M, V, N, _type(table, "table"), _type(y, "y"), scale, tp, ldt,
+                       _vec(table_scale, V, "table_scale"), ip, yp, ldy)
+    return _call((_lib or load_library()).vcsr_embed, args, stream, timed)
+
+
+def run_embed_grad_gpu(dy, ids, dtable, scale=1.0, accumulate=False, workspace=None, stream=None,
+                       timed=False):
+    """Gradient of run_embed_gpu (vcsr_embed_grad): dtable[v] = scale * the sum of dy's
+    rows whose id is v, or that added to dtable's rows with accumulate.  dy, dtable:
+    float32 or BF16."""
+    (V, N), (ip, M) = _shape2(dtable, "dtable"), _ids(ids, "ids")
+    (dp, lddy), (tp, lddt) = _mat(dy, M, N, "dy"), _mat(dtable, V, N, "dtable")
+    tt, yt = _type(dtable, "dtable"), _type(dy, "dy")
+    need = _embed_grad_bytes(M, V, N, tt, yt)
+    args = _pack_embed_grad(M, V, N, tt, yt, 1 if accumulate else 0, scale, dp, lddy, ip, tp, lddt)
+    return _call_with_space((_lib or load_library()).vcsr_embed_grad, args, need, workspace, stream,
+                            timed)
 
 
 def _act(act):

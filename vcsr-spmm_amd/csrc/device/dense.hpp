@@ -87,6 +87,15 @@ __device__ __forceinline__ void load_full(const T* p, float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = to_f32(m.v[i]);
 }
+// v moved down by `bytes` (0 to 15), zeros behind.
+__device__ __forceinline__ u32x4 shift_down(u32x4 v, int bytes) {
+    if (bytes & 8) v = u32x4{v.z, v.w, 0, 0};
+    if (bytes & 4) v = u32x4{v.y, v.z, v.w, 0};
+    const uint32_t b = bytes & 3;
+    return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, b), __builtin_amdgcn_alignbyte(v.z, v.y, b),
+                 __builtin_amdgcn_alignbyte(v.w, v.z, b), __builtin_amdgcn_alignbyte(0, v.w, b)};
+}
+
 // The first n <= N values of v to p, rounded to nearest even.
 template <class T, int N>
 __device__ __forceinline__ void store_vec(T* p, int n, const float (&v)[N]) {
@@ -175,6 +184,12 @@ size_t rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args& a);
 hipError_t launch_layernorm(const vcsr_layernorm_args& a, hipStream_t st);
 hipError_t launch_layernorm_grad(const vcsr_layernorm_grad_args& a, hipStream_t st);
 size_t layernorm_grad_workspace(const vcsr_layernorm_grad_args& a);
+
+// --------------------------------------------------------------- embed.hip
+// The arguments are checked, and strides of 0 resolved, by the caller.
+hipError_t launch_embed(const vcsr_embed_args& a, hipStream_t st);
+hipError_t launch_embed_grad(const vcsr_embed_grad_args& a, hipStream_t st);
+size_t embed_grad_workspace(const vcsr_embed_grad_args& a);
 
 // -------------------------------------------------------------- colsum.hip
 // out[c] = sum over p < P of part[p * ld + c] for c < C, in a fixed order.

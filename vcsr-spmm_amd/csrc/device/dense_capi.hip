@@ -143,6 +143,51 @@ vcsr_layernorm_grad_args checked(const vcsr_layernorm_grad_args* args) {
     return a;
 }
 
+// Columns of a table, which are a grid dimension of its kernels.
+constexpr int32_t kMostColumns = 1 << 20;
+void check_embed_sizes(int64_t M, int32_t V, int32_t C, int32_t y_type) {
+    check_rows(M);
+    need(V >= 1 && C >= 1, "V, C: at least 1");
+    range(C <= kMostColumns, "C over 2^20");
+    need(is_wide(y_type), "y_type: VCSR_F32 or VCSR_BF16");
+}
+vcsr_embed_args checked(const vcsr_embed_args* args) {
+    need(args, "null argument");
+    vcsr_embed_args a = *args;
+    check_embed_sizes(a.M, a.V, a.C, a.y_type);
+    need(is_wide(a.table_type) || a.table_type == VCSR_FP8,
+         "table_type: VCSR_F32, VCSR_BF16 or VCSR_FP8");
+    need(std::isfinite(a.scale), "scale: not finite");
+    check_matrix(a.table, a.ldt, a.C, a.table_type, "table: pointer, alignment or stride", false,
+                 a.M);
+    check_vector(a.ids, "ids: pointer or alignment", a.M == 0);
+    check_matrix(a.y, a.ldy, a.C, a.y_type, "y: pointer, alignment or stride", false, a.M);
+    need((a.table_scale != nullptr) == (a.table_type == VCSR_FP8) || a.M == 0,
+         "table_scale: given for VCSR_FP8 and only then");
+    check_vector(a.table_scale, "table_scale: alignment", true);
+    need(a.y != a.table || a.M == 0, "y: another matrix than the table");
+    return a;
+}
+vcsr_embed_grad_args checked_sizes(const vcsr_embed_grad_args* args) {
+    need(args, "null argument");
+    vcsr_embed_grad_args a = *args;
+    check_embed_sizes(a.M, a.V, a.C, a.y_type);
+    need(is_wide(a.table_type), "table_type: VCSR_F32 or VCSR_BF16");
+    return a;
+}
+vcsr_embed_grad_args checked(const vcsr_embed_grad_args* args) {
+    vcsr_embed_grad_args a = checked_sizes(args);
+    need(std::isfinite(a.scale), "scale: not finite");
+    need(a.accumulate == 0 || a.accumulate == 1, "accumulate: 0 or 1");
+    check_matrix(a.dy, a.lddy, a.C, a.y_type, "dy: pointer, alignment or stride", false, a.M);
+    check_vector(a.ids, "ids: pointer or alignment", a.M == 0);
+    check_matrix(a.dtable, a.lddt, a.C, a.table_type, "dtable: pointer, alignment or stride", false,
+                 a.V);
+    need(a.dtable != a.dy || a.M == 0, "dtable: another matrix than dy");
+    check_workspace(a.workspace, a.workspace_bytes, vcsr::embed_grad_workspace(a));
+    return a;
+}
+
 void check_act(int32_t act) {
     need(act >= VCSR_ACT_NONE && act <= VCSR_ACT_SILU, "act: one of VCSR_ACT_*");
 }
@@ -410,6 +455,31 @@ int vcsr_layernorm_grad(const vcsr_layernorm_grad_args* args, void* stream, floa
         need_device();
         hipStream_t st = (hipStream_t)stream;
         run_timed(st, ms, [&] { return vcsr::launch_layernorm_grad(a, st); });
+    });
+}
+
+int vcsr_embed(const vcsr_embed_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_embed_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return vcsr::launch_embed(a, st); });
+    });
+}
+
+int vcsr_embed_grad_workspace(const vcsr_embed_grad_args* args, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = vcsr::embed_grad_workspace(checked_sizes(args));
+    });
+}
+
+int vcsr_embed_grad(const vcsr_embed_grad_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_embed_grad_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return vcsr::launch_embed_grad(a, st); });
     });
 }
 

@@ -1,0 +1,598 @@
+// embed.hip - rows of a table by token (embedding) and the table's gradient.
+//
+// Forward: y[m] = scale * table[ids[m]], a copy that memory bounds.
+// Gradient: dtable[v] = scale * sum of dy[m] over ids[m] = v.  Tokens are sorted by id,
+// equal ones in the order they came, so that a row of the table is the sum of a run of
+// sorted tokens and results repeat bit for bit (no atomics on values).  The sorted
+// tokens are cut into chunks of E, a wave's work for 64 vectors of columns: it adds
+// the rows of dy of each run in order and writes the run's row.  Runs of up to E tokens
+// are the work of the chunk they start in, also past its end; longer ones (a few
+// tokens make up much of a text) are added chunk by chunk, and their partial rows by
+// another launch, in order.
+#include "common.hpp"
+#include "dense.hpp"
+#include "launch.hpp"
+#include "vecops.hpp"
+
+namespace vcsr {
+namespace {
+
+// The FP32 values of 16 bytes.
+__device__ __forceinline__ void widen(const u32x4& r, float (&v)[4], float) {
+    const f32x4 f = __builtin_bit_cast(f32x4, r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f[i];
+}
+__device__ __forceinline__ void widen(const u32x4& r, float (&v)[8], bf16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __builtin_bit_cast(float, r[i] << 16);
+        v[2 * i + 1] = __builtin_bit_cast(float, r[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void widen(const u32x4& r, float (&v)[16], fp8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[4 * i] = fp8_to_f32<0>(r[i]);
+        v[4 * i + 1] = fp8_to_f32<1>(r[i]);
+        v[4 * i + 2] = fp8_to_f32<2>(r[i]);
+        v[4 * i + 3] = fp8_to_f32<3>(r[i]);
+    }
+}
+
+// How rows end: in whole vectors of 16 bytes, inside one, or before the first is whole.
+enum { kWhole = 0, kRagged = 1, kShort = 2 };
+template <class T>
+int ends_of(int32_t C) {
+    constexpr int V = 16 / (int)sizeof(T);
+    return C % V == 0 ? kWhole : C > V ? kRagged : kShort;
+}
+
+// Values [c, c + V) of a row of C, for c a multiple of V: anything past the row's
+// end.  No branch but for rows that are shorter than a vector.
+template <class T, int ENDS>
+__device__ __forceinline__ u32x4 load16(const T* row, int64_t c, int64_t C) {
+    constexpr int V = 16 / (int)sizeof(T);
+    u32x4 r;
+    if (ENDS == kShort) {
+        T t[V];
+        __builtin_memset(t, 0, 16);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (c + i < C) t[i] = row[c + i];
+        __builtin_memcpy(&r, t, 16);
+        return r;
+    }
+    // A vector that reaches past the end is read ending with the row, and shifted.
+    const int64_t back = c + V > C ? c + V - C : 0;
+    const Mem<uint8_t, 16> m = *(const Mem<uint8_t, 16>*)(row + (back < V ? c - back : 0));
+    __builtin_memcpy(&r, &m, 16);
+    return ENDS == kWhole ? r : shift_down(r, (int)(back & (V - 1)) * (int)sizeof(T));
+}
+
+// ------------------------------------------------------------------- forward
+// Groups of `lanes` (a power of two <= 64) lanes take U rows each, of them NV vectors
+// a lane from blockIdx.y's slab on; all loads go out together.
+template <class X, class Y, int ENDS, int NV, int U>
+__global__ __launch_bounds__(256) void embed_kernel(vcsr_embed_args a, int lanes) {
+    constexpr int V = 16 / (int)sizeof(X);
+    const int lane = threadIdx.x & (lanes - 1);
+    const int64_t first = ((int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes) * U;
+    int32_t id[U];
+    float f[U];
+    u32x4 r[U][NV];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        id[u] = first + u < a.M ? a.ids[first + u] : -1;
+        if ((uint32_t)id[u] >= (uint32_t)a.V) id[u] = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t at = id[u] < 0 ? 0 : id[u];
+        const X* const row = (const X*)a.table + at * a.ldt;
+        f[u] = sizeof(X) == 1 ? a.scale * a.table_scale[at] : a.scale;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            r[u][k] = load16<X, ENDS>(
+                row, (((int64_t)blockIdx.y * NV + k) * lanes + lane) * V, a.C);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (first + u >= a.M) continue;
+        Y* const to = (Y*)a.y + (first + u) * a.ldy;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int64_t c = (((int64_t)blockIdx.y * NV + k) * lanes + lane) * V;
+            if (c >= a.C) continue;
+            float v[V];
+            widen(r[u][k], v, X());
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = id[u] < 0 ? 0.f : v[i] * f[u];
+            store_vec(to + c, ENDS == kWhole || a.C - c > V ? V : (int)(a.C - c), v);
+        }
+    }
+}
+
+template <class X, class Y, int ENDS>
+void launch_ends(const vcsr_embed_args& a, hipStream_t st) {
+    constexpr int V = 16 / (int)sizeof(X);
+    const int64_t nv = ((int64_t)a.C + V - 1) / V;
+    int lanes = 1;
+    while (lanes < 64 && lanes < nv) lanes *= 2;
+    auto go = [&](auto nvec, auto rows) {
+        constexpr int NV = decltype(nvec)::value, U = decltype(rows)::value;
+        const int64_t per = 256 / lanes * U, slab = (int64_t)lanes * NV;
+        const unsigned slabs = (unsigned)((nv + slab - 1) / slab);
+        // A launch has fewer than 2^32 threads: more rows go in several.
+        const int64_t most = per << 23;
+        for (int64_t m = 0; m < a.M; m += most) {
+            vcsr_embed_args b = a;
+            b.M = a.M - m < most ? a.M - m : most;
+            b.ids += m;
+            b.y = (Y*)a.y + m * a.ldy;
+            embed_kernel<X, Y, ENDS, NV, U>
+                <<<dim3((unsigned)((b.M + per - 1) / per), slabs), 256, 0, st>>>(b, lanes);
+        }
+    };
+    if (nv > 128)
+        go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+    else if (nv > 64)
+        go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+    else
+        go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+}
+template <class X, class Y>
+hipError_t launch_forward(const vcsr_embed_args& a, hipStream_t st) {
+    switch (ends_of<X>(a.C)) {
+        case kWhole: launch_ends<X, Y, kWhole>(a, st); break;
+        case kRagged: launch_ends<X, Y, kRagged>(a, st); break;
+        default: launch_ends<X, Y, kShort>(a, st);
+    }
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------- sort
+// Key of a token: its id, or V (behind all others) for one outside the table.
+__device__ __forceinline__ int32_t key_of(int32_t id, int32_t V) {
+    return (uint32_t)id < (uint32_t)V ? id : V;
+}
+
+// Few tokens: each one's place is the number of tokens before it.  A block takes 64
+// tokens, each of its 16 waves a part of all keys; a token's own block is the only one
+// where the order of equal keys has to be told apart.
+__global__ __launch_bounds__(1024) void rank_kernel(const int32_t* ids, int32_t n, int32_t V,
+                                                    int32_t* keys, int32_t* pos) {
+    __shared__ int32_t count[16][64];
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    const int32_t i0 = (int32_t)blockIdx.x * 64, i = i0 + lane;
+    const int32_t key = i < n ? key_of(ids[i], V) : V;
+    const int32_t part = ((n + 63) / 64 + 15) / 16 * 64;
+    const int32_t j0 = wave * part, j1 = j0 + part < n ? j0 + part : n;
+    int32_t before = 0;
+    auto run = [&](int32_t from, int32_t to, uint32_t limit) {  // limit: up to 2^31
+        for (int32_t b = from; b < to; b += 64) {
+            const int32_t mine = b + lane < to ? key_of(ids[b + lane], V) : -1;
+#pragma unroll
+            for (int l = 0; l < 64; ++l)
+                before += (uint32_t)__builtin_amdgcn_readlane(mine, l) < limit ? 1 : 0;
+        }
+    };
+    if (j0 < i0) run(j0, j1 < i0 ? j1 : i0, (uint32_t)key + 1);
+    if (j0 <= i0 && i0 < j1) {  // the block's own tokens
+#pragma unroll
+        for (int l = 0; l < 64; ++l) {
+            const int32_t k = __builtin_amdgcn_readlane(key, l);
+            before += i0 + l < n && (k < key || (k == key && l < lane)) ? 1 : 0;
+        }
+    }
+    if (j1 > i0 + 64) run(j0 > i0 + 64 ? j0 : i0 + 64, j1, key);
+    count[wave][lane] = before;
+    __syncthreads();
+    if (wave || i >= n) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) before += count[w][lane];
+    keys[before] = key;
+    pos[before] = i;
+}
+
+// More: by digits of up to 9 bits, the lowest first, two launches each.  A block takes a
+// tile of `tile` keys in a row, each of its 4 waves a quarter; `pos` is null for the
+// first digit, whose keys are the ids themselves.
+constexpr int kDigits = 512;
+struct Radix {
+    const int32_t *keys, *pos;
+    int32_t n, V, tile, shift, digits;
+};
+__device__ __forceinline__ int32_t radix_key(const Radix& r, int64_t i) {
+    const int32_t k = r.keys[i];
+    return r.pos ? k : key_of(k, r.V);
+}
+__global__ __launch_bounds__(256) void digit_count_kernel(Radix r, int32_t* counts) {
+    __shared__ int32_t lds[kDigits];
+    for (int d = threadIdx.x; d < r.digits; d += 256) lds[d] = 0;
+    __syncthreads();
+    const int64_t first = (int64_t)blockIdx.x * r.tile;
+    const int64_t last = first + r.tile < r.n ? first + r.tile : r.n;
+    for (int64_t i = first + threadIdx.x; i < last; i += 256)
+        atomicAdd(&lds[(radix_key(r, i) >> r.shift) & (r.digits - 1)], 1);
+    __syncthreads();
+    for (int d = threadIdx.x; d < r.digits; d += 256)
+        counts[(int64_t)blockIdx.x * r.digits + d] = lds[d];
+}
+__global__ __launch_bounds__(256) void digit_place_kernel(Radix r, const int32_t* counts,
+                                                          int32_t* keys, int32_t* pos) {
+    __shared__ int32_t next[4][kDigits], base[kDigits], sums[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    for (int d = tid; d < r.digits; d += 256)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) next[w][d] = 0;
+    // Digits [2 tid, 2 tid + 2): how many keys of them there are, and in blocks before.
+    int32_t all[2] = {0, 0}, before[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int d = 2 * tid + h;
+        if (d >= r.digits) continue;
+#pragma unroll 8
+        for (int32_t b = 0; b < (int32_t)gridDim.x; ++b) {
+            const int32_t c = counts[(int64_t)b * r.digits + d];
+            all[h] += c;
+            before[h] += b < (int32_t)blockIdx.x ? c : 0;
+        }
+    }
+    const int32_t two = all[0] + all[1], scan = wave_inclusive_scan(two, lane);
+    if (lane == 63) sums[wave] = scan;
+    __syncthreads();
+    int32_t start = scan - two;
+    for (int w = 0; w < wave; ++w) start += sums[w];
+    if (2 * tid < r.digits) base[2 * tid] = start + before[0];
+    if (2 * tid + 1 < r.digits) base[2 * tid + 1] = start + all[0] + before[1];
+    // The wave's quarter: how many of each digit.
+    const int64_t first = (int64_t)blockIdx.x * r.tile + (int64_t)wave * (r.tile / 4);
+    int64_t last = first + r.tile / 4;
+    if (last > r.n) last = r.n;
+    for (int64_t i = first + lane; i < last; i += 64)
+        atomicAdd(&next[wave][(radix_key(r, i) >> r.shift) & (r.digits - 1)], 1);
+    __syncthreads();
+    for (int d = tid; d < r.digits; d += 256) {
+        int32_t at = base[d];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int32_t c = next[w][d];
+            next[w][d] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    // 64 keys at a time, in order: lanes with one digit go behind one another.
+    for (int64_t b = first; b < last; b += 64) {
+        const bool in = b + lane < last;
+        const int32_t key = in ? radix_key(r, b + lane) : 0;
+        const int32_t from = in ? (r.pos ? r.pos[b + lane] : (int32_t)(b + lane)) : 0;
+        const int d = (key >> r.shift) & (r.digits - 1);
+        uint64_t same = __ballot(in);
+        for (int bit = 1; bit < r.digits; bit <<= 1) {
+            const uint64_t set = __ballot(d & bit);
+            same &= d & bit ? set : ~set;
+        }
+        const int rank = __popcll(same & (((uint64_t)1 << lane) - 1));
+        int32_t at = 0;
+        if (in) at = next[wave][d] + rank;
+        wave_sync();
+        if (in && rank == 0) next[wave][d] = at + __popcll(same);
+        wave_sync();
+        if (in) {
+            keys[at] = key;
+            pos[at] = from;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ gradient
+// A chunk of E sorted tokens from `first` on, as a wave's lanes hold them: its keys and
+// those of the chunks before and behind it (-1 and V where there is none).
+struct Chunk {
+    int32_t before, key, behind;
+    // Which of the chunk's tokens, and how many behind it, the wave adds; tokens under
+    // `lead` belong to a long run from before, those from `tail` on to one that goes on.
+    int from, to, lead, tail;
+};
+__device__ __forceinline__ int count_equal(int32_t k, int32_t x, uint64_t mask) {
+    return __popcll(__ballot(k == x) & mask);
+}
+__device__ __forceinline__ void find_runs(Chunk& c, bool first, int E, int32_t V) {
+    const uint64_t mask = ~(uint64_t)0 >> (64 - E);
+    const int32_t k0 = __builtin_amdgcn_readlane(c.key, 0);
+    const int32_t kl = __builtin_amdgcn_readlane(c.key, E - 1);
+    const bool joins = !first && __builtin_amdgcn_readlane(c.before, E - 1) == k0;
+    const int valid = __popcll(__ballot(c.key < V) & mask);
+    c.from = c.lead = 0;
+    c.to = valid;
+    c.tail = 2 * E;
+    if (joins) {
+        const int len = count_equal(c.key, k0, mask);
+        if (count_equal(c.before, k0, mask) + len > E)
+            c.lead = len;
+        else
+            c.from = len;
+    }
+    if (valid < E) return;
+    const int more = count_equal(c.behind, kl, mask), own = count_equal(c.key, kl, mask);
+    if (more == 0 || (own == E && joins)) return;
+    if (own + more > E)
+        c.tail = E - own;
+    else
+        c.to = E + more;
+}
+__device__ __forceinline__ Chunk load_chunk(const int32_t* keys, int64_t first, int64_t n, int E,
+                                            int32_t V, int lane) {
+    Chunk c;
+    c.before = first > 0 && lane < E ? keys[first - E + lane] : -1;
+    c.key = lane < E && first + lane < n ? keys[first + lane] : V;
+    c.behind = lane < E && first + E + lane < n ? keys[first + E + lane] : V;
+    return c;
+}
+
+struct Runs {
+    const int32_t *keys, *pos;
+    float* part;     // two partial rows a chunk: of a long run from before, and of one that goes on
+    int64_t ldp;
+    int64_t chunks;
+    int E, slabs, width;  // tokens a chunk; slabs of `width` vectors of columns
+    int64_t first;        // chunk (and slab) that the launch begins with
+};
+// Blocks of a launch, which has fewer than 2^32 threads.
+constexpr int64_t kMostBlocks = (int64_t)1 << 23;
+
+// SORTS: all tokens are one chunk, which each wave sorts by itself.
+template <class D, class X, int ENDS, bool SORTS>
+__global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, Runs r) {
+    constexpr int V = 16 / (int)sizeof(D), U = 8;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = r.first + (int64_t)blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6));
+    const int64_t chunk = item / r.slabs;
+    if (chunk >= r.chunks) return;
+    const int E = r.E;
+    Chunk k;
+    int32_t pos, pos_behind = 0;
+    if (SORTS) {
+        const int32_t mine = lane < a.M ? key_of(a.ids[lane], a.V) : a.V;
+        int rank = 0;
+#pragma unroll
+        for (int l = 0; l < 64; ++l) {
+            const int32_t o = __builtin_amdgcn_readlane(mine, l);
+            rank += o < mine || (o == mine && l < lane) ? 1 : 0;
+        }
+        k.before = -1;
+        k.behind = a.V;
+        k.key = __builtin_amdgcn_ds_permute(rank * 4, mine);
+        pos = __builtin_amdgcn_ds_permute(rank * 4, lane);
+    } else {
+        k = load_chunk(r.keys, chunk * E, a.M, E, a.V, lane);
+        pos = lane < E && chunk * E + lane < a.M ? r.pos[chunk * E + lane] : 0;
+        pos_behind = lane < E && (chunk + 1) * E + lane < a.M ? r.pos[(chunk + 1) * E + lane] : 0;
+    }
+    find_runs(k, chunk == 0, E, a.V);
+    const int64_t vec = (item - chunk * r.slabs) * r.width + lane;
+    const bool live = lane < r.width && vec * V < a.C;
+    const int64_t c = live ? vec * V : a.C;
+    const int n = a.C - c < V ? (int)(a.C - c) : V;
+    auto key_at = [&](int e) {
+        return e < E ? __builtin_amdgcn_readlane(k.key, e)
+                     : __builtin_amdgcn_readlane(k.behind, e - E);
+    };
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    int32_t key = k.from < k.to ? key_at(k.from) : 0;
+    for (int e = k.from; e < k.to; e += U) {
+        u32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = e + u < k.to ? e + u : k.to - 1;
+            const int64_t m = at < E ? __builtin_amdgcn_readlane(pos, at)
+                                     : __builtin_amdgcn_readlane(pos_behind, at - E);
+            v[u] = load16<D, ENDS>((const D*)a.dy + m * a.lddy, c, a.C);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (e + u >= k.to) break;
+            float d[V];
+            widen(v[u], d, D());
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] += d[i];
+            const int32_t next = e + u + 1 < k.to ? key_at(e + u + 1) : -1;
+            if (next == key) continue;
+            if (live) {
+                if (e + u < k.lead || e + u >= k.tail) {
+                    float* const to =
+                        r.part + (2 * chunk + (e + u < k.lead ? 0 : 1)) * r.ldp + c;
+                    store_vec(to, V, acc);
+                } else {
+                    X* const to = (X*)a.dtable + (int64_t)key * a.lddt + c;
+                    float o[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] = 0.f;
+                    if (a.accumulate) load_vec(to, n, o);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(a.scale, acc[i], o[i]);
+                    store_vec(to, n, o);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[i] = 0.f;
+            key = next;
+        }
+    }
+}
+
+// The partial rows of the long run that begins in chunk blockIdx.x, 256 columns a
+// block: each wave adds every fourth one, then LDS adds the waves, in order.
+template <class X>
+__global__ __launch_bounds__(256) void embed_join_kernel(vcsr_embed_grad_args a, Runs r) {
+    __shared__ float lds[4][64][5];
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    const int64_t chunk = r.first + blockIdx.x, first = chunk * r.E;
+    Chunk k = load_chunk(r.keys, first, a.M, r.E, a.V, lane);
+    find_runs(k, chunk == 0, r.E, a.V);
+    if (k.tail > r.E) return;
+    const int32_t key = __builtin_amdgcn_readlane(k.key, r.E - 1);
+    // The chunks behind it that begin with the run, one after the other.
+    int64_t parts = 1;
+    for (;;) {
+        const int64_t at = (chunk + parts + lane) * r.E;
+        const int more = __popcll(__ballot(at < a.M && r.keys[at < a.M ? at : 0] == key));
+        parts += more;
+        if (more < 64) break;
+    }
+    const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * 4;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < a.C) {
+#pragma unroll 4
+        for (int64_t p = wave; p < parts; p += 4) {
+            float v[4];
+            load_full(r.part + (2 * (chunk + p) + (p == 0 ? 1 : 0)) * r.ldp + c, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] += v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[wave][lane][i] = t[i];
+    __syncthreads();
+    if (wave || c >= a.C) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] += lds[w][lane][i];
+    X* const to = (X*)a.dtable + (int64_t)key * a.lddt + c;
+    const int n = a.C - c < 4 ? (int)(a.C - c) : 4;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    if (a.accumulate) load_vec(to, n, o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(a.scale, t[i], o[i]);
+    store_vec(to, n, o);
+}
+
+// How the gradient's tokens are sorted and cut.
+constexpr int64_t kMostRanked = 8192;
+struct Shape {
+    Runs runs{};
+    int32_t passes = 0, tile = 0, bits = 0;  // of the sort by digits
+    int64_t tiles = 0;
+    size_t array = 0, counts = 0, parts = 0;  // bytes; an array of n numbers
+    int arrays = 0;
+    size_t bytes() const { return arrays * array + counts + parts; }
+};
+size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
+Shape shape_of(const vcsr_embed_grad_args& a) {
+    Shape s;
+    const int64_t v = a.y_type == VCSR_F32 ? 4 : 8, nv = ((int64_t)a.C + v - 1) / v;
+    const int64_t slabs = (nv + 63) / 64;
+    s.runs.slabs = (int)slabs;
+    s.runs.width = (int)((nv + slabs - 1) / slabs);
+    s.runs.E = 64;
+    s.runs.ldp = nv * v;
+    if (a.M > 64)  // enough waves to have the chip's loads under way
+        while (s.runs.E > 8 && a.M / s.runs.E * slabs < 2048) s.runs.E /= 2;
+    s.runs.chunks = (a.M + s.runs.E - 1) / s.runs.E;
+    if (a.M <= 64) return s;
+    s.array = round_up((size_t)a.M * 4);
+    s.arrays = 2;
+    s.parts = round_up((size_t)s.runs.chunks * 2 * (size_t)s.runs.ldp * 4);
+    if (a.M <= kMostRanked) return s;
+    int bits = 1;
+    while (bits < 31 && a.V >> bits) ++bits;
+    s.passes = (bits + 8) / 9;
+    s.bits = (bits + s.passes - 1) / s.passes;
+    if (s.passes > 1) s.arrays = 4;
+    s.tile = 1024;
+    while ((a.M + s.tile - 1) / s.tile > 128) s.tile *= 2;
+    s.tiles = (a.M + s.tile - 1) / s.tile;
+    s.counts = round_up((size_t)s.tiles << s.bits << 2);
+    return s;
+}
+
+template <class D, class X, int ENDS>
+hipError_t launch_sums(const vcsr_embed_grad_args& a, const Shape& s, hipStream_t st) {
+    Runs r = s.runs;
+    const int64_t blocks = (r.chunks * r.slabs + 3) / 4;
+    if (a.M <= 64) {
+        embed_sum_kernel<D, X, ENDS, true><<<(unsigned)blocks, 256, 0, st>>>(a, r);
+        return hipGetLastError();
+    }
+    for (int64_t b = 0; b < blocks; b += kMostBlocks) {
+        const int64_t count = blocks - b < kMostBlocks ? blocks - b : kMostBlocks;
+        r.first = 4 * b;
+        embed_sum_kernel<D, X, ENDS, false><<<(unsigned)count, 256, 0, st>>>(a, r);
+    }
+    for (int64_t c = 0; c < r.chunks; c += kMostBlocks) {
+        const int64_t count = r.chunks - c < kMostBlocks ? r.chunks - c : kMostBlocks;
+        r.first = c;
+        embed_join_kernel<X><<<dim3((unsigned)count, (unsigned)((a.C + 255) / 256)), 256, 0, st>>>(
+            a, r);
+    }
+    return hipGetLastError();
+}
+template <class D, class X>
+hipError_t launch_grad(const vcsr_embed_grad_args& a, const Shape& s, hipStream_t st) {
+    switch (ends_of<D>(a.C)) {
+        case kWhole: return launch_sums<D, X, kWhole>(a, s, st);
+        case kRagged: return launch_sums<D, X, kRagged>(a, s, st);
+        default: return launch_sums<D, X, kShort>(a, s, st);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_embed(const vcsr_embed_args& a, hipStream_t st) {
+    if (a.M <= 0) return hipSuccess;
+    if (a.table_type == VCSR_F32)
+        return a.y_type == VCSR_F32 ? launch_forward<float, float>(a, st)
+                                    : launch_forward<float, bf16>(a, st);
+    if (a.table_type == VCSR_BF16)
+        return a.y_type == VCSR_F32 ? launch_forward<bf16, float>(a, st)
+                                    : launch_forward<bf16, bf16>(a, st);
+    return a.y_type == VCSR_F32 ? launch_forward<fp8, float>(a, st)
+                                : launch_forward<fp8, bf16>(a, st);
+}
+
+size_t embed_grad_workspace(const vcsr_embed_grad_args& a) {
+    return a.M > 0 ? shape_of(a).bytes() : 0;
+}
+
+hipError_t launch_embed_grad(const vcsr_embed_grad_args& a, hipStream_t st) {
+    const int64_t size = a.table_type == VCSR_F32 ? 4 : 2;
+    hipError_t e = hipSuccess;
+    if (!a.accumulate) e = launch_zero(a.dtable, a.lddt * size, a.V, a.C * size, st);
+    if (e != hipSuccess || a.M <= 0) return e;
+    Shape s = shape_of(a);
+    char* const base = (char*)a.workspace;
+    auto array = [&](int i) { return (int32_t*)(base + i * s.array); };
+    if (a.M > 64) {
+        s.runs.keys = array(0);
+        s.runs.pos = array(1);
+        s.runs.part = (float*)(base + s.arrays * s.array + s.counts);
+    }
+    if (a.M > 64 && a.M <= kMostRanked) {
+        rank_kernel<<<(unsigned)((a.M + 63) / 64), 1024, 0, st>>>(a.ids, (int32_t)a.M, a.V,
+                                                                 array(0), array(1));
+    } else if (a.M > 64) {
+        int32_t* const counts = (int32_t*)(base + s.arrays * s.array);
+        for (int p = 0; p < s.passes; ++p) {
+            const int to = (s.passes - 1 - p) % 2 * 2;  // the last digit's go to 0 and 1
+            const Radix r{p ? array(2 - to) : a.ids, p ? array(3 - to) : nullptr, (int32_t)a.M,
+                          a.V,  s.tile, p * s.bits, 1 << s.bits};
+            digit_count_kernel<<<(unsigned)s.tiles, 256, 0, st>>>(r, counts);
+            digit_place_kernel<<<(unsigned)s.tiles, 256, 0, st>>>(r, counts, array(to),
+                                                                  array(to + 1));
+        }
+    }
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.y_type == VCSR_F32)
+        return a.table_type == VCSR_F32 ? launch_grad<float, float>(a, s, st)
+                                        : launch_grad<float, bf16>(a, s, st);
+    return a.table_type == VCSR_F32 ? launch_grad<bf16, float>(a, s, st)
+                                    : launch_grad<bf16, bf16>(a, s, st);
+}
+
+}  // namespace vcsr

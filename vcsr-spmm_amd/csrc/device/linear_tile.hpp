@@ -72,15 +72,6 @@ struct Operand {
     int64_t bytes;  // from p to the end of its last row
 };
 
-// v moved down by `bytes` (0 to 15), zeros behind.
-__device__ __forceinline__ u32x4 shift_down(u32x4 v, int bytes) {
-    if (bytes & 8) v = u32x4{v.z, v.w, 0, 0};
-    if (bytes & 4) v = u32x4{v.y, v.z, v.w, 0};
-    const uint32_t b = bytes & 3;
-    return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, b), __builtin_amdgcn_alignbyte(v.z, v.y, b),
-                 __builtin_amdgcn_alignbyte(v.w, v.z, b), __builtin_amdgcn_alignbyte(0, v.w, b)};
-}
-
 // One operand's tile loader: NT threads bring ROWS x 128 bytes.  `GR` granules a
 // thread; granule e = it * NT + tid of the tile lies at e * 16 in LDS.  SEG > 0:
 // the tile's rows are runs of SEG rows, 2 * SEG apart.
