@@ -541,6 +541,63 @@ typedef struct {
 int vcsr_linear_grad_workspace(const vcsr_linear_grad_args* args, size_t* bytes);
 int vcsr_linear_grad(const vcsr_linear_grad_args* args, void* stream, float* ms);
 
+/* A gated projection: z_gate = x Wg^T + gate_bias, z_up = x Wu^T + up_bias,
+ * y = act(z_gate) * z_up, in one pass over x (the first half of a gated feed-forward
+ * block; vcsr_linear is the second).  Types, scales and sums as vcsr_linear has them; y
+ * is formed from the unrounded z.  The outputs are other matrices than x and the
+ * weights, and than each other. */
+typedef struct {
+    int64_t M;           /* rows of x and y; 0 is no work                    */
+    int32_t N, K;        /* outputs and inputs of a row, >= 1; N <= 2^29     */
+    int32_t x_type;      /* x and weights: VCSR_F32, VCSR_BF16 or VCSR_FP8   */
+    int32_t y_type;      /* y, z_gate, z_up: VCSR_F32 or VCSR_BF16           */
+    int32_t act;         /* VCSR_ACT_*                                       */
+    const void* x;       int64_t ldx;
+    const void* w_gate;  int64_t ldwg;  /* N x K                             */
+    const void* w_up;    int64_t ldwu;  /* N x K                             */
+    const float* x_scale;    /* M, for VCSR_FP8 (NULL otherwise)             */
+    const float* gate_scale; /* N, for VCSR_FP8 (NULL otherwise)             */
+    const float* up_scale;   /* N, for VCSR_FP8 (NULL otherwise)             */
+    const float* gate_bias;  /* N or NULL                                    */
+    const float* up_bias;    /* N or NULL                                    */
+    void* z_gate;            /* NULL both, or z for the gradient, of one     */
+    void* z_up;          int64_t ldz;   /* stride                            */
+    void* y;             int64_t ldy;
+    void* workspace;     size_t workspace_bytes;
+} vcsr_gated_args;
+/* As vcsr_linear_workspace. */
+int vcsr_gated_workspace(const vcsr_gated_args* args, size_t* bytes);
+int vcsr_gated(const vcsr_gated_args* args, void* stream, float* ms);
+
+/* Gradients of vcsr_gated on VCSR_F32 or VCSR_BF16 operands: dz_gate = dy * z_up *
+ * act'(z_gate), dz_up = dy * act(z_gate), dx = dz_gate Wg + dz_up Wu, dw_gate =
+ * dz_gate^T x, dw_up = dz_up^T x, each bias' the sum over rows of its dz.  For VCSR_BF16
+ * operands both dz are rounded to bf16 before the products, as vcsr_linear_grad has it.
+ * dx and the dw are other matrices than those their products read (the weights for dx,
+ * x for the dw, and each other's operands where both are asked for). */
+typedef struct {
+    int64_t M;
+    int32_t N, K;
+    int32_t x_type;      /* x, weights, dx, dw: VCSR_F32 or VCSR_BF16        */
+    int32_t y_type;      /* dy, z_gate, z_up: VCSR_F32 or VCSR_BF16          */
+    int32_t act;
+    const void* dy;      int64_t lddy;
+    const void* z_gate;
+    const void* z_up;    int64_t ldz;   /* of both                           */
+    const void* x;       int64_t ldx;   /* needed for dw                     */
+    const void* w_gate;  int64_t ldwg;  /* needed for dx                     */
+    const void* w_up;    int64_t ldwu;  /* needed for dx                     */
+    void* dx;            int64_t lddx;  /* M x K, or NULL                    */
+    void* dw_gate;       int64_t lddwg; /* N x K both (zeros for M = 0),     */
+    void* dw_up;         int64_t lddwu; /* or NULL both                      */
+    float* dgate_bias;   /* N (zeros for M = 0), or NULL                     */
+    float* dup_bias;     /* N (zeros for M = 0), or NULL                     */
+    void* workspace;     size_t workspace_bytes;
+} vcsr_gated_grad_args;
+/* As vcsr_linear_workspace. */
+int vcsr_gated_grad_workspace(const vcsr_gated_grad_args* args, size_t* bytes);
+int vcsr_gated_grad(const vcsr_gated_grad_args* args, void* stream, float* ms);
+
 /* AdamW over all tensors of a model in one launch.  With g = grad_scale *
  * grad:  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  * param = param (1 - lr weight_decay)

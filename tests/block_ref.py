@@ -59,3 +59,38 @@ def layer_norm_grad(dy, s, w, mean, rstd, dsum):
     tw = (M + 8) * EPS * np.sum(np.abs(dy) * ah, axis=0) + 1e-30
     tb = (M + 4) * EPS * np.sum(np.abs(dy), axis=0) + 1e-30
     return (dx, np.sum(dy * h, axis=0), np.sum(dy, axis=0)), (tol, tw, tb)
+
+
+# ------------------------------------------------------------ gated projection
+def gated(x, wg, wu, bg, bu, kind):
+    """(z_gate, z_up, y) and their errors in FP32: sums of K products and a bias in any
+    order; each act's slope is at most 1.13, and its own arithmetic good to 16 u."""
+    K = x.shape[1]
+    out, tol = [], []
+    for w, b in ((wg, bg), (wu, bu)):
+        out.append(x @ w.T + (0 if b is None else b))
+        tol.append((K + 4) * EPS * (np.abs(x) @ np.abs(w).T + (0 if b is None else np.abs(b))))
+    a = act(out[0], kind)
+    ta = 1.13 * tol[0] + 16 * EPS * np.abs(out[0])
+    y = a * out[1]
+    ty = (np.abs(a) + ta) * tol[1] + np.abs(out[1]) * ta + 2 * EPS * np.abs(y)
+    return (*out, y), (*tol, ty)
+
+
+def gated_grad(dy, x, wg, wu, zg, zu, kind, operand):
+    """dx, dw_gate, dw_up, dgate_bias, dup_bias and their errors: act' is at most 1.13
+    and good to 32 u there, act to 16 u |z|, two products each; both dz round to the
+    operands' type; sums of 2 N and of M products in any order."""
+    M, N = dy.shape
+    dg, du = dy * zu * act_grad(zg, kind), dy * act(zg, kind)
+    eg, eu = 44 * EPS * 1.13 * np.abs(dy * zu), 20 * EPS * np.abs(dy * zg)
+    bias = (dg.sum(0), du.sum(0))
+    tb = (eg.sum(0) + (M + 4) * EPS * np.abs(dg).sum(0), eu.sum(0) + (M + 4) * EPS * np.abs(du).sum(0))
+    if operand == "bf16":
+        eg, eu = eg + rounding(dg, "bf16") * 1.01, eu + rounding(du, "bf16") * 1.01
+    ag, au = np.abs(dg), np.abs(du)
+    dx = dg @ wg + du @ wu
+    tx = eg @ np.abs(wg) + eu @ np.abs(wu) + (2 * N + 6) * EPS * (ag @ np.abs(wg) + au @ np.abs(wu))
+    tg = eg.T @ np.abs(x) + (M + 4) * EPS * (ag.T @ np.abs(x))
+    tu = eu.T @ np.abs(x) + (M + 4) * EPS * (au.T @ np.abs(x))
+    return (dx, dg.T @ x, du.T @ x, *bias), (tx, tg, tu, *tb)

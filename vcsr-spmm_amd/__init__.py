@@ -59,7 +59,8 @@ EXPORTS = (
     "vcsr_rmsnorm vcsr_rmsnorm_grad_workspace vcsr_rmsnorm_grad "
     "vcsr_layernorm vcsr_layernorm_grad_workspace vcsr_layernorm_grad "
     "vcsr_embed vcsr_embed_grad_workspace vcsr_embed_grad vcsr_linear_workspace vcsr_linear "
-    "vcsr_linear_grad_workspace vcsr_linear_grad vcsr_adamw_create vcsr_adamw_step vcsr_adamw_free"
+    "vcsr_linear_grad_workspace vcsr_linear_grad vcsr_gated_workspace vcsr_gated "
+    "vcsr_gated_grad_workspace vcsr_gated_grad vcsr_adamw_create vcsr_adamw_step vcsr_adamw_free"
 ).split()
 
 
@@ -167,6 +168,29 @@ class _LinearGradArgs(C.Structure):
                 ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class _GatedArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("x_type", C.c_int32),
+                ("y_type", C.c_int32), ("act", C.c_int32), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("w_gate", C.c_void_p), ("ldwg", C.c_int64), ("w_up", C.c_void_p),
+                ("ldwu", C.c_int64), ("x_scale", C.c_void_p), ("gate_scale", C.c_void_p),
+                ("up_scale", C.c_void_p), ("gate_bias", C.c_void_p), ("up_bias", C.c_void_p),
+                ("z_gate", C.c_void_p), ("z_up", C.c_void_p), ("ldz", C.c_int64),
+                ("y", C.c_void_p), ("ldy", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class _GatedGradArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int32), ("K", C.c_int32), ("x_type", C.c_int32),
+                ("y_type", C.c_int32), ("act", C.c_int32), ("dy", C.c_void_p),
+                ("lddy", C.c_int64), ("z_gate", C.c_void_p), ("z_up", C.c_void_p),
+                ("ldz", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("w_gate", C.c_void_p), ("ldwg", C.c_int64), ("w_up", C.c_void_p),
+                ("ldwu", C.c_int64), ("dx", C.c_void_p), ("lddx", C.c_int64),
+                ("dw_gate", C.c_void_p), ("lddwg", C.c_int64), ("dw_up", C.c_void_p),
+                ("lddwu", C.c_int64), ("dgate_bias", C.c_void_p), ("dup_bias", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 def _packer(fields, size):
     """struct.Struct of a ctypes structure's fields: packing costs a third of
     filling the structure, and a small call is bound by the host."""
@@ -182,10 +206,11 @@ _pack_rmsnorm = _packer(_RmsnormArgs._fields_, C.sizeof(_RmsnormArgs))
 _pack_space = _packer(_LinearArgs._fields_[-2:], 16)
 _pack_layernorm = _packer(_LayernormArgs._fields_, C.sizeof(_LayernormArgs))
 _pack_embed = _packer(_EmbedArgs._fields_, C.sizeof(_EmbedArgs))
-_pack_rmsnorm_grad, _pack_layernorm_grad, _pack_embed_grad, _pack_linear, _pack_linear_grad = (
+(_pack_rmsnorm_grad, _pack_layernorm_grad, _pack_embed_grad, _pack_linear, _pack_linear_grad,
+ _pack_gated, _pack_gated_grad) = (
     _packer(args._fields_[:-2], C.sizeof(args) - 16)
     for args in (_RmsnormGradArgs, _LayernormGradArgs, _EmbedGradArgs, _LinearArgs,
-                 _LinearGradArgs))
+                 _LinearGradArgs, _GatedArgs, _GatedGradArgs))
 
 
 class _AdamwTensor(C.Structure):
@@ -281,6 +306,10 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
         "vcsr_linear": (C.c_int, [P, P, pF]),
         "vcsr_linear_grad_workspace": (C.c_int, [P, pS]),
         "vcsr_linear_grad": (C.c_int, [P, P, pF]),
+        "vcsr_gated_workspace": (C.c_int, [P, pS]),
+        "vcsr_gated": (C.c_int, [P, P, pF]),
+        "vcsr_gated_grad_workspace": (C.c_int, [P, pS]),
+        "vcsr_gated_grad": (C.c_int, [P, P, pF]),
         "vcsr_adamw_create": (C.c_int, [C.POINTER(_AdamwTensor), I32, P, pP]),
         "vcsr_adamw_step": (C.c_int, [P, C.POINTER(_AdamwHyper), P, pF]),
         "vcsr_adamw_free": (None, [P]),
@@ -953,6 +982,26 @@ def _embed_grad_bytes(M, V, N, table_type, y_type):
     return need.value
 
 
+@functools.lru_cache(maxsize=4096)
+def _gated_bytes(M, N, K, x_type, y_type, z):
+    need = C.c_size_t(0)
+    args = _GatedArgs(M=M, N=N, K=K, x_type=x_type, y_type=y_type, z_gate=16 if z else None,
+                      z_up=32 if z else None)
+    _check(load_library().vcsr_gated_workspace(C.byref(args), C.byref(need)))
+    return need.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _gated_grad_bytes(M, N, K, x_type, y_type, dx, dw, dgate_bias, dup_bias):
+    need = C.c_size_t(0)
+    args = _GatedGradArgs(M=M, N=N, K=K, x_type=x_type, y_type=y_type, dx=16 if dx else None,
+                          dw_gate=32 if dw else None, dw_up=48 if dw else None,
+                          dgate_bias=64 if dgate_bias else None,
+                          dup_bias=80 if dup_bias else None)
+    _check(load_library().vcsr_gated_grad_workspace(C.byref(args), C.byref(need)))
+    return need.value
+
+
 def _call(fn, args, stream, timed):
     if not timed:
         rc = fn(args, stream.h if stream is not None else None, None)
@@ -1105,6 +1154,55 @@ def run_linear_grad_gpu(dy, x, w, z=None, act="none", dx=None, dw=None, dbias=No
                              wg, lddw, _vec(dbias, N, "dbias"))
     return _call_with_space((_lib or load_library()).vcsr_linear_grad, args, need, workspace,
                             stream, timed)
+
+
+def _one_stride(a, b, what):
+    if a is not None and b is not None and getattr(a, "ld", 0) != getattr(b, "ld", 0) and \
+            getattr(a, "ld", a.shape[-1]) != getattr(b, "ld", b.shape[-1]):
+        raise VcsrError(VCSR_EINVAL, f"{what}: row strides differ")
+
+
+def run_gated_gpu(x, w_gate, w_up, y, gate_bias=None, up_bias=None, act="silu", z_gate=None,
+                  z_up=None, x_scale=None, gate_scale=None, up_scale=None, workspace=None,
+                  stream=None, timed=False):
+    """y = act(x Wg^T + gate_bias) * (x Wu^T + up_bias) (vcsr_gated); the weights have one
+    row per output column.  x, weights: float32, BF16, or FP8 with x_scale, gate_scale
+    and up_scale, one scale a row; y, z_gate, z_up: float32 or BF16.  z_gate and z_up
+    (both or neither, of one row stride) receive the two products."""
+    (M, K), N = _shape2(x, "x"), _shape2(w_gate, "w_gate")[0]
+    (xp, ldx), (gp, ldg) = _mat(x, M, K, "x"), _mat(w_gate, N, K, "w_gate", x.dtype)
+    (up, ldu), (yp, ldy) = _mat(w_up, N, K, "w_up", x.dtype), _mat(y, M, N, "y")
+    (zg, ldz), (zu, _) = _mat(z_gate, M, N, "z_gate", y.dtype), _mat(z_up, M, N, "z_up", y.dtype)
+    _one_stride(z_gate, z_up, "z_gate, z_up")
+    xt, yt = _type(x, "x"), _type(y, "y")
+    args = _pack_gated(M, N, K, xt, yt, _act(act), xp, ldx, gp, ldg, up, ldu,
+                       _vec(x_scale, M, "x_scale"), _vec(gate_scale, N, "gate_scale"),
+                       _vec(up_scale, N, "up_scale"), _vec(gate_bias, N, "gate_bias"),
+                       _vec(up_bias, N, "up_bias"), zg, zu, ldz, yp, ldy)
+    return _call_with_space((_lib or load_library()).vcsr_gated, args,
+                            _gated_bytes(M, N, K, xt, yt, zg != 0), workspace, stream, timed)
+
+
+def run_gated_grad_gpu(dy, x, w_gate, w_up, z_gate, z_up, act="silu", dx=None, dw_gate=None,
+                       dw_up=None, dgate_bias=None, dup_bias=None, workspace=None, stream=None,
+                       timed=False):
+    """Gradients of run_gated_gpu (vcsr_gated_grad) from dy and the saved z_gate and z_up:
+    those of dx, dw_gate with dw_up, dgate_bias and dup_bias that are given."""
+    (M, K), N = _shape2(x, "x"), _shape2(w_gate, "w_gate")[0]
+    (xp, ldx), (gp, ldg) = _mat(x, M, K, "x"), _mat(w_gate, N, K, "w_gate", x.dtype)
+    (up, ldu), (dp, lddy) = _mat(w_up, N, K, "w_up", x.dtype), _mat(dy, M, N, "dy")
+    (zg, ldz), (zu, _) = _mat(z_gate, M, N, "z_gate", dy.dtype), _mat(z_up, M, N, "z_up", dy.dtype)
+    _one_stride(z_gate, z_up, "z_gate, z_up")
+    (xg, lddx), (gg, lddg) = _mat(dx, M, K, "dx", x.dtype), _mat(dw_gate, N, K, "dw_gate", x.dtype)
+    ug, lddu = _mat(dw_up, N, K, "dw_up", x.dtype)
+    xt, yt = _type(x, "x"), _type(dy, "dy")
+    need = _gated_grad_bytes(M, N, K, xt, yt, dx is not None, dw_gate is not None,
+                             dgate_bias is not None, dup_bias is not None)
+    args = _pack_gated_grad(M, N, K, xt, yt, _act(act), dp, lddy, zg, zu, ldz, xp, ldx, gp, ldg, up,
+                            ldu, xg, lddx, gg, lddg, ug, lddu,
+                            _vec(dgate_bias, N, "dgate_bias"), _vec(dup_bias, N, "dup_bias"))
+    return _call_with_space((_lib or load_library()).vcsr_gated_grad, args, need, workspace, stream,
+                            timed)
 
 
 class AdamW:

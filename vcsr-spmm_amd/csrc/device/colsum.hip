@@ -163,6 +163,108 @@ hipError_t launch_dz_typed(const vcsr_linear_grad_args& a, X* dz, int64_t lddz, 
     return hipGetLastError();
 }
 
+// The gated projection's, as dz_kernel: dy, z_gate and z_up read once, dz_gate and dz_up
+// written once and rounded to the products' type.
+template <class D, class X, int ACT, int ENDS>
+__global__ __launch_bounds__(256) void gated_dz_kernel(vcsr_gated_grad_args a, X* dz, int64_t lddz,
+                                                       float* part_gate, float* part_up,
+                                                       int64_t rows, int tx) {
+    constexpr int U = 2, V = 16 / (int)sizeof(D);
+    __shared__ float lds[2][256 * V];
+    const int ty_n = 256 / tx, ty = threadIdx.x / tx;
+    const int64_t c = ((int64_t)blockIdx.x * tx + (threadIdx.x - ty * tx)) * V;
+    const int n = c >= a.N ? 0 : a.N - c < V ? (int)(a.N - c) : V;
+    float sum[2][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[0][i] = sum[1][i] = 0.f;
+    const int64_t first = (int64_t)blockIdx.y * rows;
+    const int64_t last = first + rows < a.M ? first + rows : a.M;
+    if (n > 0 && ty < ty_n) {
+        auto load = [&](const D* row, float(&v)[V]) __attribute__((always_inline)) {
+            if (ENDS == 0)
+                load_full(row + c, v);
+            else if (ENDS == 1)
+                load_tail(row, (int)c, a.N, v);
+            else
+                load_vec(row + c, n, v);
+        };
+        for (int64_t m = first + ty; m < last; m += U * ty_n) {
+            float d[U][V], g[U][V], w[U][V];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = m + u * ty_n < last ? m + u * ty_n : last - 1;
+                load((const D*)a.dy + r * a.lddy, d[u]);
+                load((const D*)a.z_gate + r * a.ldz, g[u]);
+                load((const D*)a.z_up + r * a.ldz, w[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (m + u * ty_n >= last) continue;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float z = g[u][i];
+                    g[u][i] = d[u][i] * w[u][i] * act_grad_f32<ACT>(z);
+                    w[u][i] = d[u][i] * act_f32<ACT>(z);
+                    if (ENDS == 0 || i < n) {
+                        sum[0][i] += g[u][i];
+                        sum[1][i] += w[u][i];
+                    }
+                }
+                if (dz) {
+                    X* const to = dz + (m + u * ty_n) * lddz + c;
+                    store_vec(to, ENDS == 0 ? V : n, g[u]);
+                    store_vec(to + a.M * lddz, ENDS == 0 ? V : n, w[u]);
+                }
+            }
+        }
+    }
+    if (!part_gate && !part_up) return;
+    if (ty < ty_n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < V; ++i) lds[h][threadIdx.x * V + i] = sum[h][i];
+    __syncthreads();
+    for (int col = threadIdx.x; col < tx * V; col += 256) {
+        const int64_t at = (int64_t)blockIdx.x * tx * V + col;
+        if (at >= a.N) continue;
+        float t[2] = {0.f, 0.f};
+        for (int k = 0; k < ty_n; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) t[h] += lds[h][k * tx * V + col];
+        if (part_gate) part_gate[(int64_t)blockIdx.y * a.N + at] = t[0];
+        if (part_up) part_up[(int64_t)blockIdx.y * a.N + at] = t[1];
+    }
+}
+
+template <class D, class X, int ACT>
+void launch_gated_act(const vcsr_gated_grad_args& a, X* dz, int64_t lddz, float* part_gate,
+                      float* part_up, hipStream_t st) {
+    constexpr int V = 16 / (int)sizeof(D);
+    const DzShape s = dz_shape(a.M, a.N, a.y_type);
+    const dim3 grid((unsigned)s.columns, (unsigned)s.blocks);
+    if (a.N % V == 0)
+        gated_dz_kernel<D, X, ACT, 0>
+            <<<grid, 256, 0, st>>>(a, dz, lddz, part_gate, part_up, s.rows, s.tx);
+    else if (a.N > V)
+        gated_dz_kernel<D, X, ACT, 1>
+            <<<grid, 256, 0, st>>>(a, dz, lddz, part_gate, part_up, s.rows, s.tx);
+    else
+        gated_dz_kernel<D, X, ACT, 2>
+            <<<grid, 256, 0, st>>>(a, dz, lddz, part_gate, part_up, s.rows, s.tx);
+}
+template <class D, class X>
+hipError_t launch_gated_typed(const vcsr_gated_grad_args& a, X* dz, int64_t lddz, float* g,
+                              float* u, hipStream_t st) {
+    switch (a.act) {
+        case VCSR_ACT_RELU: launch_gated_act<D, X, VCSR_ACT_RELU>(a, dz, lddz, g, u, st); break;
+        case VCSR_ACT_GELU: launch_gated_act<D, X, VCSR_ACT_GELU>(a, dz, lddz, g, u, st); break;
+        case VCSR_ACT_SILU: launch_gated_act<D, X, VCSR_ACT_SILU>(a, dz, lddz, g, u, st); break;
+        default: launch_gated_act<D, X, VCSR_ACT_NONE>(a, dz, lddz, g, u, st);
+    }
+    return hipGetLastError();
+}
+
 // Rows of `n` 16-bit values, `ld` apart.
 __global__ __launch_bounds__(256) void zero_kernel(uint16_t* p, int64_t ld, int64_t rows,
                                                    int64_t n) {
@@ -173,20 +275,20 @@ __global__ __launch_bounds__(256) void zero_kernel(uint16_t* p, int64_t ld, int6
 
 }  // namespace
 
-hipError_t launch_sum_row_pairs(const float* part, int32_t P, int32_t C, int64_t ld, float* a,
-                                float* b, hipStream_t st) {
+hipError_t launch_sum_row_pairs(const float* part, int32_t P, int32_t C, int64_t ld, int64_t next,
+                                float* a, float* b, hipStream_t st) {
     // 64 threads a column, and fewer than 2^32 threads a launch.
     const int32_t most = b ? 1 << 24 : 1 << 25;
     for (int64_t c = 0; c < C; c += most) {
         const int32_t n = C - c < most ? (int32_t)(C - c) : most;
         sum_rows_kernel<<<dim3((unsigned)((n + 15) / 16), b ? 2 : 1), 1024, 0, st>>>(
-            part + c, P, n, ld, a + c, b ? b + c : nullptr, C);
+            part + c, P, n, ld, a + c, b ? b + c : nullptr, next);
     }
     return hipGetLastError();
 }
 hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, float* out,
                            hipStream_t st) {
-    return launch_sum_row_pairs(part, P, C, ld, out, nullptr, st);
+    return launch_sum_row_pairs(part, P, C, ld, 0, out, nullptr, st);
 }
 
 int32_t dz_row_blocks(int64_t M, int32_t N, int32_t dy_type) {
@@ -201,6 +303,16 @@ hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, flo
                    : launch_dz_typed<float, bf16>(a, (bf16*)dz, lddz, part, st);
     return a.x_type == VCSR_F32 ? launch_dz_typed<bf16, float>(a, (float*)dz, lddz, part, st)
                                 : launch_dz_typed<bf16, bf16>(a, (bf16*)dz, lddz, part, st);
+}
+
+hipError_t launch_gated_dz(const vcsr_gated_grad_args& a, void* dz, int64_t lddz, float* g,
+                           float* u, hipStream_t st) {
+    if (a.y_type == VCSR_F32)
+        return a.x_type == VCSR_F32
+                   ? launch_gated_typed<float, float>(a, (float*)dz, lddz, g, u, st)
+                   : launch_gated_typed<float, bf16>(a, (bf16*)dz, lddz, g, u, st);
+    return a.x_type == VCSR_F32 ? launch_gated_typed<bf16, float>(a, (float*)dz, lddz, g, u, st)
+                                : launch_gated_typed<bf16, bf16>(a, (bf16*)dz, lddz, g, u, st);
 }
 
 hipError_t launch_zero(void* p, int64_t ld, int64_t rows, int64_t bytes, hipStream_t st) {

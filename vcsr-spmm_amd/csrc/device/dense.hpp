@@ -195,14 +195,19 @@ size_t embed_grad_workspace(const vcsr_embed_grad_args& a);
 // out[c] = sum over p < P of part[p * ld + c] for c < C, in a fixed order.
 hipError_t launch_sum_rows(const float* part, int32_t P, int32_t C, int64_t ld, float* out,
                            hipStream_t st);
-// The same of part into `a` and, where given, of part + C into `b`, in one launch.
-hipError_t launch_sum_row_pairs(const float* part, int32_t P, int32_t C, int64_t ld, float* a,
-                                float* b, hipStream_t st);
+// The same of part into `a` and, where given, of part + next into `b`, in one launch.
+hipError_t launch_sum_row_pairs(const float* part, int32_t P, int32_t C, int64_t ld, int64_t next,
+                                float* a, float* b, hipStream_t st);
 // dz = dy * act'(z) in x_type (dz may be NULL) and, for each block of
 // dz_row_blocks(M, N, type of dy), the sums of its rows of dz in `part` (ld N; may be NULL).
 hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, float* part,
                      hipStream_t st);
 int32_t dz_row_blocks(int64_t M, int32_t N, int32_t dy_type);
+// The same of a gated projection: dz_gate = dy * z_up * act'(z_gate) and dz_up = dy *
+// act(z_gate), M rows `lddz` apart one behind the other in dz (may be NULL), and their
+// sums of rows in part_gate and part_up (either may be NULL).
+hipError_t launch_gated_dz(const vcsr_gated_grad_args& a, void* dz, int64_t lddz, float* part_gate,
+                           float* part_up, hipStream_t st);
 // Zeros in `rows` rows of `bytes` bytes, `ld` bytes apart (all even, as FP32 and bf16
 // matrices have them), by a kernel.
 hipError_t launch_zero(void* p, int64_t ld, int64_t rows, int64_t bytes, hipStream_t st);
@@ -227,6 +232,26 @@ struct Gemm {
     void* out = nullptr;
     int64_t ldo = 0;
     float* part = nullptr;  // partial sums of a split product (gemm_workspace bytes)
+};
+// A gated projection: out[i][j] = act(sum_k P(i, k) Q(j, k)) * sum_k P(i, k) Q2(j, k) for
+// J / 2 columns j, both sums with scales and bias of their own and, where z is given,
+// written to z and z2 (`ldz` both).  J counts the columns of both, as the tiles do.
+struct GatedGemm : Gemm {
+    const void* q2 = nullptr;
+    int64_t ldq2 = 0;
+    const float *q2_scale = nullptr, *bias2 = nullptr;
+    void* z2 = nullptr;
+};
+// Its dx: the sum of two products, P Q and P2 Q2, both of length R; p2 has p's stride.
+struct TwiceGemm : Gemm {
+    const void *p2 = nullptr, *q2 = nullptr;
+    int64_t ldq2 = 0;
+};
+// Its dw: two products of one size, P Q into out and P2 Q into out2.
+struct TwinGemm : Gemm {
+    const void* p2 = nullptr;
+    void* out2 = nullptr;
+    int64_t ldo2 = 0;
 };
 hipError_t launch_gemm(const Gemm& g, hipStream_t st);
 // Throws VCSR_ERANGE for more tiles than a launch has blocks, as the pair's does.
@@ -262,6 +287,17 @@ PairPlan gemm_pair_plan(const Gemm& dw, const Gemm& dx);
 // go together or not; tile 0 ends it.
 void force_plan(const GemmPlan& p, bool together);
 
+// The gated projection and its gradients, from their workspace (GatedGemm::part,
+// TwinGemm::part, which both products of a gradient share).
+hipError_t launch_gated(const GatedGemm& g, hipStream_t st);
+size_t gated_workspace(const GatedGemm& g);
+GemmPlan gated_plan(const GatedGemm& g);
+// Of dw and dx those whose `out` is not null, and the sums of dbias' partial rows.
+hipError_t launch_gated_grad(const TwinGemm& dw, const TwiceGemm& dx, const RowSum (&bias)[2],
+                             hipStream_t st);
+size_t gated_grad_workspace(const TwinGemm& dw, const TwiceGemm& dx);
+PairPlan gated_grad_plan(const TwinGemm& dw, const TwiceGemm& dx);
+
 hipError_t launch_gemm_f32(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_gemm_bf16(const Gemm& g, const GemmPlan& p, hipStream_t st);
 hipError_t launch_pair_f32(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
@@ -269,6 +305,14 @@ hipError_t launch_pair_f32(const Gemm& dw, const GemmPlan& p, const Gemm& dx, co
 hipError_t launch_pair_bf16(const Gemm& dw, const GemmPlan& p, const Gemm& dx, const GemmPlan& q,
                             const RowSum& bias, hipStream_t st);
 hipError_t launch_gemm_fp8(const Gemm& g, const GemmPlan& p, hipStream_t st);
+hipError_t launch_gated_f32(const GatedGemm& g, const GemmPlan& p, hipStream_t st);
+hipError_t launch_gated_bf16(const GatedGemm& g, const GemmPlan& p, hipStream_t st);
+hipError_t launch_gated_fp8(const GatedGemm& g, const GemmPlan& p, hipStream_t st);
+// dw (p.splits > 0) and dx (q.splits > 0), in one launch where both are.
+hipError_t launch_gated_grad_f32(const TwinGemm& dw, const GemmPlan& p, const TwiceGemm& dx,
+                                 const GemmPlan& q, const RowSum (&bias)[2], hipStream_t st);
+hipError_t launch_gated_grad_bf16(const TwinGemm& dw, const GemmPlan& p, const TwiceGemm& dx,
+                                  const GemmPlan& q, const RowSum (&bias)[2], hipStream_t st);
 
 // --------------------------------------------------------------- adamw.hip
 // One chunk of a tensor is kAdamwChunk values, a block's work.

@@ -259,6 +259,76 @@ void need_apart(const vcsr_linear_args& a) {
     need(!a.z || (a.z != a.x && a.z != a.w), "z: another matrix than x and w");
 }
 
+vcsr_gated_args checked_sizes(const vcsr_gated_args* args) {
+    need(args, "null argument");
+    vcsr_gated_args a = *args;
+    check_rows(a.M);
+    need(a.N >= 1 && a.K >= 1, "N, K: at least 1");
+    need(is_wide(a.x_type) || a.x_type == VCSR_FP8, "x_type: VCSR_F32, VCSR_BF16 or VCSR_FP8");
+    need(is_wide(a.y_type), "y_type: VCSR_F32 or VCSR_BF16");
+    check_act(a.act);
+    range(a.K <= kOperandLd, "K over 2^20");
+    range(a.N <= 1 << 29, "N over 2^29");  // the columns of both products are counted in 31 bits
+    range(a.M <= kMaxOut / 2 / a.N, "M x N over 2^41");
+    return a;
+}
+vcsr::GatedGemm gemm_of(const vcsr_gated_args& a) {
+    vcsr::GatedGemm g;
+    g.I = a.M;
+    g.J = 2 * a.N;
+    g.R = a.K;
+    g.type = a.x_type;
+    g.out_type = a.y_type;
+    g.act = a.act;
+    g.p = a.x;
+    g.ldp = a.ldx;
+    g.p_scale = a.x_scale;
+    g.q = a.w_gate;
+    g.ldq = a.ldwg;
+    g.q_scale = a.gate_scale;
+    g.bias = a.gate_bias;
+    g.z = a.z_gate;
+    g.ldz = a.ldz;
+    g.q2 = a.w_up;
+    g.ldq2 = a.ldwu;
+    g.q2_scale = a.up_scale;
+    g.bias2 = a.up_bias;
+    g.z2 = a.z_up;
+    g.out = a.y;
+    g.ldo = a.ldy;
+    g.part = (float*)a.workspace;
+    return g;
+}
+vcsr_gated_args checked(const vcsr_gated_args* args) {
+    vcsr_gated_args a = checked_sizes(args);
+    check_operand(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", false, a.M);
+    check_operand(a.w_gate, a.ldwg, a.K, a.x_type, "w_gate: pointer, alignment or stride", false,
+                  a.M);
+    check_operand(a.w_up, a.ldwu, a.K, a.x_type, "w_up: pointer, alignment or stride", false, a.M);
+    const bool scaled = a.x_type == VCSR_FP8;
+    need(a.M == 0 || ((a.x_scale != nullptr) == scaled && (a.gate_scale != nullptr) == scaled &&
+                      (a.up_scale != nullptr) == scaled),
+         "x_scale, gate_scale, up_scale: given for VCSR_FP8 and only then");
+    check_vector(a.x_scale, "x_scale: alignment", true);
+    check_vector(a.gate_scale, "gate_scale: alignment", true);
+    check_vector(a.up_scale, "up_scale: alignment", true);
+    check_vector(a.gate_bias, "gate_bias: alignment", true);
+    check_vector(a.up_bias, "up_bias: alignment", true);
+    need(!a.z_gate == !a.z_up, "z_gate, z_up: both or neither");
+    int64_t ldz = a.ldz;
+    check_matrix(a.z_gate, a.ldz, a.N, a.y_type, "z_gate: alignment or stride", true, a.M);
+    check_matrix(a.z_up, ldz, a.N, a.y_type, "z_up: alignment or stride", true, a.M);
+    check_matrix(a.y, a.ldy, a.N, a.y_type, "y: pointer, alignment or stride", false, a.M);
+    need(!a.z_gate || (a.z_gate != a.z_up && a.z_gate != a.y && a.z_up != a.y),
+         "y, z_gate, z_up: three matrices");
+    if (a.M > 0)
+        for (const void* out : {(const void*)a.y, (const void*)a.z_gate, (const void*)a.z_up})
+            need(!out || (out != a.x && out != a.w_gate && out != a.w_up),
+                 "y, z_gate, z_up: other matrices than x, w_gate and w_up");
+    check_workspace(a.workspace, a.workspace_bytes, vcsr::gated_workspace(gemm_of(a)));
+    return a;
+}
+
 // The gradient's work: dz (unless dy serves as it is), dbias' partial rows,
 // and the two products, whose partial sums share what is behind.
 struct LinearGrad {
@@ -363,6 +433,162 @@ LinearGrad checked(const vcsr_linear_grad_args* args) {
     }
     check_workspace(a.workspace, a.workspace_bytes, w.bytes());
     return w;
+}
+
+// The gated projection's gradient: both dz in the workspace, the biases' partial rows,
+// and the products.
+struct GatedGrad {
+    vcsr_gated_grad_args a;
+    int64_t lddz = 0;
+    int32_t row_blocks = 0;
+    size_t dz_bytes = 0, bias_bytes = 0, part_bytes = 0;  // bias_bytes: one bias' partial rows
+    vcsr::TwinGemm dw;
+    vcsr::TwiceGemm dx;
+    size_t bytes() const {
+        return dz_bytes + ((a.dgate_bias ? 1 : 0) + (a.dup_bias ? 1 : 0)) * bias_bytes + part_bytes;
+    }
+    float* bias_part(int which) const {
+        char* const at = (char*)a.workspace + dz_bytes;
+        return (float*)(at + (which && a.dgate_bias ? bias_bytes : 0));
+    }
+};
+
+GatedGrad grad_of(const vcsr_gated_grad_args* args) {
+    need(args, "null argument");
+    GatedGrad w;
+    vcsr_gated_grad_args& a = w.a;
+    a = *args;
+    check_rows(a.M);
+    need(a.N >= 1 && a.K >= 1, "N, K: at least 1");
+    need(is_wide(a.x_type), "x_type: VCSR_F32 or VCSR_BF16");
+    need(is_wide(a.y_type), "y_type: VCSR_F32 or VCSR_BF16");
+    check_act(a.act);
+    need(!a.dw_gate == !a.dw_up, "dw_gate, dw_up: both or neither");
+    auto stride = [](int64_t& ld, int64_t cols) {
+        if (ld == 0) ld = cols;
+    };
+    stride(a.lddy, a.N);
+    stride(a.ldz, a.N);
+    stride(a.ldx, a.K);
+    stride(a.ldwg, a.K);
+    stride(a.ldwu, a.K);
+    stride(a.lddx, a.K);
+    stride(a.lddwg, a.K);
+    stride(a.lddwu, a.K);
+    if (a.M == 0) return w;
+    range(a.N <= kOperandLd && a.K <= kOperandLd, "N, K over 2^20");
+    range(a.M <= kMaxOut / 2 / (a.N > a.K ? a.N : a.K), "M x N or M x K over 2^41");
+    const bool products = a.dx || a.dw_gate;
+    w.lddz = ((int64_t)a.N + 7) / 8 * 8;  // rows of dz on 16-byte boundaries
+    if (products) w.dz_bytes = round_up(2 * (size_t)a.M * (size_t)w.lddz * size_of(a.x_type));
+    w.row_blocks = vcsr::dz_row_blocks(a.M, a.N, a.y_type);
+    // A single block of rows writes dbias itself.
+    if (w.row_blocks > 1) w.bias_bytes = round_up((size_t)w.row_blocks * (size_t)a.N * 4);
+    char* const base = (char*)a.workspace;
+    const void* const dz[2] = {base, base + (size_t)a.M * (size_t)w.lddz * size_of(a.x_type)};
+    float* const part = (float*)(base + w.bytes());  // part_bytes is zero so far
+    vcsr::TwiceGemm& x = w.dx;
+    x.type = x.out_type = a.x_type;
+    x.I = a.M;
+    x.J = a.K;
+    x.R = a.N;
+    x.p = dz[0];
+    x.p2 = dz[1];
+    x.ldp = w.lddz;
+    x.q = a.w_gate;
+    x.ldq = a.ldwg;
+    x.q2 = a.w_up;
+    x.ldq2 = a.ldwu;
+    x.q_cols = true;
+    x.out = a.dx;
+    x.ldo = a.lddx;
+    x.part = part;
+    vcsr::TwinGemm& g = w.dw;
+    g.type = g.out_type = a.x_type;
+    g.I = a.N;
+    g.J = a.K;
+    g.R = a.M;
+    g.p = dz[0];
+    g.p2 = dz[1];
+    g.ldp = w.lddz;
+    g.p_cols = true;
+    g.q = a.x;
+    g.ldq = a.ldx;
+    g.q_cols = true;
+    g.out = a.dw_gate;
+    g.ldo = a.lddwg;
+    g.out2 = a.dw_up;
+    g.ldo2 = a.lddwu;
+    g.part = part;
+    if (products) w.part_bytes = vcsr::gated_grad_workspace(g, x);
+    return w;
+}
+
+GatedGrad checked(const vcsr_gated_grad_args* args) {
+    GatedGrad w = grad_of(args);
+    vcsr_gated_grad_args& a = w.a;
+    int64_t ldz = a.ldz;
+    check_matrix(a.dy, a.lddy, a.N, a.y_type, "dy: pointer, alignment or stride", false, a.M);
+    check_matrix(a.z_gate, a.ldz, a.N, a.y_type, "z_gate: pointer, alignment or stride", false, a.M);
+    check_matrix(a.z_up, ldz, a.N, a.y_type, "z_up: pointer, alignment or stride", false, a.M);
+    check_operand(a.x, a.ldx, a.K, a.x_type, "x: pointer, alignment or stride", !a.dw_gate, a.M);
+    check_operand(a.w_gate, a.ldwg, a.K, a.x_type, "w_gate: pointer, alignment or stride", !a.dx,
+                  a.M);
+    check_operand(a.w_up, a.ldwu, a.K, a.x_type, "w_up: pointer, alignment or stride", !a.dx, a.M);
+    check_matrix(a.dx, a.lddx, a.K, a.x_type, "dx: alignment or stride", true, a.M);
+    check_matrix(a.dw_gate, a.lddwg, a.K, a.x_type, "dw_gate: alignment or stride", true, a.M);
+    check_matrix(a.dw_up, a.lddwu, a.K, a.x_type, "dw_up: alignment or stride", true, a.M);
+    check_vector(a.dgate_bias, "dgate_bias: alignment", true);
+    check_vector(a.dup_bias, "dup_bias: alignment", true);
+    need(!a.dgate_bias || a.dgate_bias != a.dup_bias, "dgate_bias: another vector than dup_bias");
+    need(!a.dw_gate || a.dw_gate != a.dw_up, "dw_gate: another matrix than dw_up");
+    if (a.M > 0 && a.dx) {
+        need(a.dx != a.w_gate && a.dx != a.w_up, "dx: over a weight, which its product reads");
+        need(a.dx != a.x || !a.dw_gate, "dx: over x, which dw's products read");
+        need(a.dx != a.dw_gate && a.dx != a.dw_up, "dx: another matrix than dw_gate and dw_up");
+    }
+    if (a.M > 0 && a.dw_gate)
+        for (const void* dw : {(const void*)a.dw_gate, (const void*)a.dw_up}) {
+            need(dw != a.x, "dw_gate, dw_up: over x, which their products read");
+            need((dw != a.w_gate && dw != a.w_up) || !a.dx,
+                 "dw_gate, dw_up: over a weight, which dx's product reads");
+        }
+    check_workspace(a.workspace, a.workspace_bytes, w.bytes());
+    return w;
+}
+
+hipError_t run_grad(const GatedGrad& w, hipStream_t st) {
+    const vcsr_gated_grad_args& a = w.a;
+    hipError_t e = hipSuccess;
+    if (a.M == 0) {
+        const int64_t size = (int64_t)size_of(a.x_type), bytes = (int64_t)a.N * 4;
+        auto zero = [&](void* p, int64_t ld, int64_t rows, int64_t row_bytes) {
+            if (p && e == hipSuccess) e = vcsr::launch_zero(p, ld, rows, row_bytes, st);
+        };
+        zero(a.dw_gate, a.lddwg * size, a.N, a.K * size);
+        zero(a.dw_up, a.lddwu * size, a.N, a.K * size);
+        zero(a.dgate_bias, bytes, 1, bytes);
+        zero(a.dup_bias, bytes, 1, bytes);
+        return e;
+    }
+    const bool products = a.dx || a.dw_gate;
+    float* const out[2] = {a.dgate_bias, a.dup_bias};
+    float* part[2] = {out[0], out[1]};
+    vcsr::RowSum sums[2];
+    if (w.row_blocks > 1)
+        for (int h = 0; h < 2; ++h)
+            if (out[h]) {
+                part[h] = w.bias_part(h);
+                sums[h] = vcsr::RowSum{part[h], out[h], w.row_blocks, a.N};
+            }
+    if (products || out[0] || out[1])
+        e = vcsr::launch_gated_dz(a, products ? a.workspace : nullptr, w.lddz, part[0], part[1], st);
+    if (e != hipSuccess) return e;
+    if (products) return vcsr::launch_gated_grad(w.dw, w.dx, sums, st);
+    for (const vcsr::RowSum& s : sums)
+        if (e == hipSuccess && s.P > 0)
+            e = vcsr::launch_sum_rows(s.part, s.P, s.C, s.C, s.out, st);
+    return e;
 }
 
 hipError_t run_grad(const LinearGrad& w, hipStream_t st) {
@@ -518,6 +744,40 @@ int vcsr_linear_grad(const vcsr_linear_grad_args* args, void* stream, float* ms)
     });
 }
 
+int vcsr_gated_workspace(const vcsr_gated_args* args, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        const vcsr_gated_args a = checked_sizes(args);
+        *bytes = a.M > 0 ? vcsr::gated_workspace(gemm_of(a)) : 0;
+    });
+}
+
+int vcsr_gated(const vcsr_gated_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const vcsr_gated_args a = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        const vcsr::GatedGemm g = gemm_of(a);
+        run_timed(st, ms, [&] { return vcsr::launch_gated(g, st); });
+    });
+}
+
+int vcsr_gated_grad_workspace(const vcsr_gated_grad_args* args, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = grad_of(args).bytes();
+    });
+}
+
+int vcsr_gated_grad(const vcsr_gated_grad_args* args, void* stream, float* ms) {
+    return guarded([&] {
+        const GatedGrad w = checked(args);
+        need_device();
+        hipStream_t st = (hipStream_t)stream;
+        run_timed(st, ms, [&] { return run_grad(w, st); });
+    });
+}
+
 int vcsr_adamw_create(const vcsr_adamw_tensor* tensors, int32_t count, void* stream,
                       vcsr_adamw** out) {
     return guarded([&] {
@@ -608,6 +868,21 @@ int vcsr_test_linear_plan(const vcsr_linear_args* args, int64_t* out) {
         const vcsr::GemmPlan p = vcsr::gemm_plan(gemm_of(checked_sizes(args)));
         const int64_t v[4] = {p.tile, p.stages, p.splits, p.rows};
         std::copy(v, v + 4, out);
+    });
+}
+int vcsr_test_gated_plan(const vcsr_gated_args* args, int64_t* out) {
+    return guarded([&] {
+        const vcsr::GemmPlan p = vcsr::gated_plan(gemm_of(checked_sizes(args)));
+        const int64_t v[4] = {p.tile, p.stages, p.splits, p.rows};
+        std::copy(v, v + 4, out);
+    });
+}
+int vcsr_test_gated_grad_plan(const vcsr_gated_grad_args* args, int64_t* out) {
+    return guarded([&] {
+        const GatedGrad w = grad_of(args);
+        const vcsr::PairPlan p = vcsr::gated_grad_plan(w.dw, w.dx);
+        const int64_t v[5] = {p.together, p.dw.tile, p.dw.splits, p.dx.tile, p.dx.splits};
+        std::copy(v, v + 5, out);
     });
 }
 // {together, dw's tile and splits, dx's}

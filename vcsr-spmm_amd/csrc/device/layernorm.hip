@@ -538,7 +538,7 @@ hipError_t launch_grad(const vcsr_layernorm_grad_args& a, hipStream_t st) {
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !sums || g.blocks == 1) return e;
-    return launch_sum_row_pairs(part, g.blocks, a.C, out.ld, a.dweight ? a.dweight : a.dbias,
+    return launch_sum_row_pairs(part, g.blocks, a.C, out.ld, a.C, a.dweight ? a.dweight : a.dbias,
                                 a.dweight ? a.dbias : nullptr, st);
 }
 

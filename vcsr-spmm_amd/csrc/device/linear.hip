@@ -122,6 +122,12 @@ Gemm rows_from(Gemm g, int64_t from) {
     if (g.out) g.out = (char*)g.out + from * g.ldo * out;
     return g;
 }
+GatedGemm rows_from(GatedGemm g, int64_t from) {
+    const int64_t out = g.out_type == VCSR_F32 ? 4 : 2;
+    static_cast<Gemm&>(g) = rows_from(static_cast<const Gemm&>(g), from);
+    if (g.z2) g.z2 = (char*)g.z2 + from * g.ldz * out;
+    return g;
+}
 
 // Of every tile and number of splits, the one with the least estimated time:
 // whole rounds of blocks, what is left, and the join.  Where a last round would
@@ -176,9 +182,9 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
 // Both products in one launch, if that is estimated faster than one after the
 // other: all blocks' time over the chip's room and part of a last block, or the
 // longest block alone, and dw's join.  (8192 x 2048 x 4096 bf16: dw has 128 tiles of 256, dx 256.)
-PairPlan plan_pair(const Gemm& dw, const Gemm& dx) {
+PairPlan plan_pair(const Gemm& dw, const Gemm& dx, bool may_divide = true) {
     float us_w = 0.f, us_x = 0.f;
-    PairPlan best{false, plan_of(dw, &us_w), plan_of(dx, &us_x)};
+    PairPlan best{false, plan_of(dw, &us_w, may_divide), plan_of(dx, &us_x, may_divide)};
     if (best.dw.splits == 0 || best.dx.splits == 0) return best;
     if (forced.plan.tile && forced_takes(dw)) {
         if (forced.together) {
@@ -243,6 +249,86 @@ hipError_t launch(const Gemm& g, const GemmPlan& p, hipStream_t st) {
 }
 
 }  // namespace
+
+// ----------------------------------------------------------- gated projection
+namespace {
+
+size_t part_bytes(const GatedGemm& g, const GemmPlan& p) {
+    if (p.rows < g.I) {
+        const GatedGemm rest = rows_from(g, p.rows);
+        return part_bytes(rest, plan_of(rest, nullptr, false));
+    }
+    return p.splits > 1 ? (size_t)p.splits * (size_t)g.I * 8 * (size_t)tile::part_ld(g.J / 2) : 0;
+}
+
+hipError_t launch(const GatedGemm& g, const GemmPlan& p, hipStream_t st) {
+    if (p.rows < g.I) {
+        GatedGemm first = g;
+        first.I = p.rows;
+        const hipError_t e = launch(first, p, st);
+        if (e != hipSuccess) return e;
+        const GatedGemm rest = rows_from(g, p.rows);
+        return launch(rest, plan_of(rest, nullptr, false), st);
+    }
+    return g.type == VCSR_F32    ? launch_gated_f32(g, p, st)
+           : g.type == VCSR_BF16 ? launch_gated_bf16(g, p, st)
+                                 : launch_gated_fp8(g, p, st);
+}
+
+// Planned as products of the same blocks: dw with the rows of both, dx with a sum as
+// long as both.  Neither is divided into rows.
+PairPlan plan_grad(const TwinGemm& dw, const TwiceGemm& dx) {
+    Gemm w = dw, x = dx;
+    w.I = 2 * dw.I;
+    const int64_t step = tile::kStepBytes / (dx.type == VCSR_F32 ? 4 : 2);
+    x.R = 2 * ((dx.R + step - 1) / step) * step;
+    PairPlan p{};
+    if (dw.out && dx.out)
+        p = plan_pair(w, x, false);
+    else if (dw.out)
+        p.dw = plan_of(w, nullptr, false);
+    else
+        p.dx = plan_of(x, nullptr, false);
+    p.dw.rows = dw.I;
+    p.dx.rows = dx.I;
+    return p;
+}
+size_t dw_bytes(const TwinGemm& g, const GemmPlan& p) {
+    return p.splits > 1 ? (size_t)p.splits * 2 * (size_t)g.I * (size_t)tile::part_ld(g.J) * 4 : 0;
+}
+
+}  // namespace
+
+GemmPlan gated_plan(const GatedGemm& g) { return plan_of(g); }
+size_t gated_workspace(const GatedGemm& g) {
+    return g.I <= 0 ? 0 : part_bytes(g, launchable(plan_of(g)));
+}
+hipError_t launch_gated(const GatedGemm& g, hipStream_t st) {
+    return g.I <= 0 ? hipSuccess : launch(g, plan_of(g), st);
+}
+
+PairPlan gated_grad_plan(const TwinGemm& dw, const TwiceGemm& dx) { return plan_grad(dw, dx); }
+size_t gated_grad_workspace(const TwinGemm& dw, const TwiceGemm& dx) {
+    const PairPlan p = plan_grad(dw, dx);
+    const size_t a = dw.out ? dw_bytes(dw, launchable(p.dw)) : 0;
+    const size_t b = dx.out ? part_bytes(dx, launchable(p.dx)) : 0;
+    return a > b ? a : b;
+}
+hipError_t launch_gated_grad(const TwinGemm& dw, const TwiceGemm& dx, const RowSum (&bias)[2],
+                             hipStream_t st) {
+    PairPlan p = plan_grad(dw, dx);
+    const RowSum none[2] = {};
+    auto go = [&](bool w, bool x, const RowSum(&sums)[2]) {
+        GemmPlan a = p.dw, b = p.dx;
+        if (!w) a.splits = 0;
+        if (!x) b.splits = 0;
+        return dw.type == VCSR_F32 ? launch_gated_grad_f32(dw, a, dx, b, sums, st)
+                                   : launch_gated_grad_bf16(dw, a, dx, b, sums, st);
+    };
+    if (!dw.out || !dx.out || p.together) return go(dw.out, dx.out, bias);
+    const hipError_t e = go(false, true, bias);
+    return e != hipSuccess ? e : go(true, false, none);
+}
 
 GemmPlan gemm_plan(const Gemm& g) { return plan_of(g); }
 PairPlan gemm_pair_plan(const Gemm& dw, const Gemm& dx) { return plan_pair(dw, dx); }

@@ -27,6 +27,8 @@
 // consecutive j, a 16-byte store of bf16.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "dense.hpp"
 
@@ -168,6 +170,89 @@ struct Loader {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 rsrc, (__attribute__((address_space(3))) void*)(lds + (it * NT + wave * 64) * 16),
                 16, off[it], 0, 0, 0);
+    }
+};
+
+// The same of a gated projection's two weights, by rows: of each 64 rows of the tile
+// the first 32 are rows of the one and the others the same rows of the other.  A
+// wave's load takes 8 rows of the tile, so it goes to one of them.
+template <class T, int ROWS, int NT>
+struct PairLoader {
+    using One = Loader<T, ROWS, NT, false, true>;
+    static constexpr int GR = One::GR;
+    static_assert(NT == 512 || NT == 256, "8 or 4 waves");
+
+    // Whether the wave's granules `it` are the second weight's.
+    __device__ __forceinline__ static bool second(int it, int wave) {
+        return NT == 512 ? wave >= 4 : it & 1;
+    }
+    __device__ __forceinline__ static int row_of(int row) { return (row >> 6) * 32 + (row & 31); }
+    __device__ __forceinline__ static Operand pick(const Operand (&o)[2], bool second) {
+        return Operand{second ? o[1].p : o[0].p, second ? o[1].ld : o[0].ld, o[0].n, o[0].first,
+                       second ? o[1].bytes : o[0].bytes};
+    }
+    __device__ __forceinline__ static void fetch(const Operand (&o)[2], int64_t k0, int64_t k_end,
+                                                 uint8_t* lds) {
+        constexpr int EPG = One::EPG;
+        const int wave = uniform((int)(threadIdx.x >> 6));
+        u32x4 v[GR];
+#pragma unroll
+        for (int it = 0; it < GR; ++it) {
+            const Operand w = pick(o, second(it, wave));
+            int row, k;
+            One::place(it * NT + (int)threadIdx.x, row, k);
+            const int64_t kk = k0 + k, r = w.first + row_of(row);
+            v[it] = u32x4{0, 0, 0, 0};
+            if (r < w.n && kk < k_end && k_end >= EPG) {
+                const int back = k_end - kk < EPG ? (int)(EPG - (k_end - kk)) : 0;
+                const Mem<T, EPG> m =
+                    *(const Mem<T, EPG>*)((const T*)(w.p + r * w.ld) + (kk - back));
+                __builtin_memcpy(&v[it], &m, 16);
+                v[it] = shift_down(v[it], back * (int)sizeof(T));
+            }
+        }
+#pragma unroll
+        for (int it = 0; it < GR; ++it)
+            *(u32x4*)(lds + (it * NT + (int)threadIdx.x) * 16) = v[it];
+        if (k_end >= EPG) return;
+#pragma unroll 1
+        for (int it = 0; it < GR; ++it) {
+            const Operand w = pick(o, second(it, wave));
+            int row, k;
+            One::place(it * NT + (int)threadIdx.x, row, k);
+            const int64_t kk = k0 + k, r = w.first + row_of(row);
+            if (r >= w.n) continue;
+#pragma unroll 1
+            for (int i = 0; kk + i < k_end; ++i)
+                ((T*)(lds + (it * NT + (int)threadIdx.x) * 16))[i] =
+                    ((const T*)(w.p + r * w.ld))[kk + i];
+        }
+    }
+    __device__ __forceinline__ static void offsets(const Operand (&o)[2], uint32_t (&off)[GR]) {
+        const int wave = uniform((int)(threadIdx.x >> 6));
+#pragma unroll
+        for (int it = 0; it < GR; ++it) {
+            int row, k;
+            One::place(it * NT + (int)threadIdx.x, row, k);
+            const int64_t last = o[0].n - 1 - o[0].first, r = row_of(row);
+            off[it] = (uint32_t)((r < last ? r : last) * pick(o, second(it, wave)).ld) +
+                      k * (int)sizeof(T);
+        }
+    }
+    __device__ __forceinline__ static void copy(const Operand (&o)[2], const uint32_t (&off)[GR],
+                                                int64_t k0, lds_byte* lds) {
+        const int wave = uniform((int)(threadIdx.x >> 6));
+#pragma unroll
+        for (int it = 0; it < GR; ++it) {
+            const Operand w = pick(o, second(it, wave));
+            const int64_t at = w.first * w.ld + k0 * (int64_t)sizeof(T), left = w.bytes - at;
+            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)(w.p + at), 0, left < 0 ? 0 : left < kRange ? (int)left : kRange,
+                0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                rsrc, (__attribute__((address_space(3))) void*)(lds + (it * NT + wave * 64) * 16),
+                16, off[it], 0, 0, 0);
+        }
     }
 };
 
@@ -314,6 +399,41 @@ __device__ __forceinline__ void finish(const Gemm& g, int64_t i, int j, float (&
 #pragma unroll
         for (int k = 0; k < N; ++k) v[k] += r[k];
     }
+    store_vec((O*)g.out + i * g.ldo + j, N, v);
+}
+// The gated projection's: `v` are the sums of the first weight, `u` of the second.
+template <class O, int N>
+__device__ __forceinline__ void finish(const GatedGemm& g, int64_t i, int j, float (&v)[N],
+                                       float (&u)[N]) {
+    if (g.p_scale) {
+        const float ps = g.p_scale[i];
+        float a[N], b[N];
+        load_vec(g.q_scale + j, N, a);
+        load_vec(g.q2_scale + j, N, b);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            v[k] *= ps * a[k];
+            u[k] *= ps * b[k];
+        }
+    }
+    if (g.bias) {
+        float b[N];
+        load_vec(g.bias + j, N, b);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += b[k];
+    }
+    if (g.bias2) {
+        float b[N];
+        load_vec(g.bias2 + j, N, b);
+#pragma unroll
+        for (int k = 0; k < N; ++k) u[k] += b[k];
+    }
+    if (g.z) {
+        store_vec((O*)g.z + i * g.ldz + j, N, v);
+        store_vec((O*)g.z2 + i * g.ldz + j, N, u);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = act_f32(g.act, v[k]) * u[k];
     store_vec((O*)g.out + i * g.ldo + j, N, v);
 }
 // 8 columns of a row, or the first n of them (the others are its last one again),
@@ -473,6 +593,113 @@ __device__ __forceinline__ void write_out(const Gemm& g, const f32x4 (&acc)[FI][
         write_typed<float, PLAIN, false, ROOM>(g, acc, mine, i, j);
 }
 
+// The gated projection's: a wave's 64 columns are 32 of the one weight and the same 32
+// of the other.  i and j are out's.
+template <class O, int ACT, bool PART, bool WHOLE, int FI, int ROOM>
+__device__ __forceinline__ void write_gated_rows(const GatedGemm& g, const f32x4 (&acc)[FI][4],
+                                                 float* mine, int64_t i_first, int64_t j_first,
+                                                 uint32_t split) {
+    constexpr int LD = 64 + 4, BLOCKS = ROOM / (16 * LD * 4);
+    constexpr int XB = BLOCKS >= FI ? FI : BLOCKS >= FI / 2 ? FI / 2 : BLOCKS >= FI / 4 ? FI / 4 : 1;
+    static_assert(BLOCKS >= 1 && FI % XB == 0, "rounds of whole blocks");
+    const int32_t J = g.J / 2;
+    const int lane = threadIdx.x & 63, col = (lane & 3) * 8;
+    const int64_t j = j_first + col;
+    const int n = WHOLE || J - j > 8 ? 8 : (int)(J - j);
+    float bias[2][8], scale[2][8];
+    if (!PART && n > 0) {
+        if (g.bias) load_cols(g.bias + j, n, bias[0]);
+        if (g.bias2) load_cols(g.bias2 + j, n, bias[1]);
+        if (g.q_scale) {
+            load_cols(g.q_scale + j, n, scale[0]);
+            load_cols(g.q2_scale + j, n, scale[1]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < FI; r += XB) {
+#pragma unroll
+        for (int x = 0; x < XB; ++x)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                *(f32x4*)(mine + (x * 16 + (lane & 15)) * LD + (y >> 1) * 32 + (lane >> 4) * 8 +
+                          (y & 1) * 4) = acc[r + x][y];
+        __builtin_amdgcn_wave_barrier();
+        if (n > 0) {
+#pragma unroll
+            for (int step = 0; step < XB; ++step) {
+                const int row = step * 16 + (lane >> 2);
+                const int64_t i = i_first + r * 16 + row;
+                if (i >= g.I) continue;
+                const float* sums = mine + row * LD + col;
+                float v[8], u[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    v[k] = sums[k];
+                    u[k] = sums[32 + k];
+                }
+                if (PART) {
+                    float* const to = g.part + ((int64_t)split * g.I + i) * 2 * part_ld(J) + j;
+                    store_vec(to, 8, v);
+                    store_vec(to + part_ld(J), 8, u);
+                    continue;
+                }
+                if (g.p_scale) {
+                    const float ps = g.p_scale[i];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        v[k] *= ps * scale[0][k];
+                        u[k] *= ps * scale[1][k];
+                    }
+                }
+                if (g.bias) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] += bias[0][k];
+                }
+                if (g.bias2) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) u[k] += bias[1][k];
+                }
+                if (g.z) {
+                    store_vec((O*)g.z + i * g.ldz + j, n, v);
+                    store_vec((O*)g.z2 + i * g.ldz + j, n, u);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = act_f32<ACT>(v[k]) * u[k];
+                store_vec((O*)g.out + i * g.ldo + j, n, v);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+template <class O, bool WHOLE, int ROOM, int FI>
+__device__ __forceinline__ void write_gated_typed(const GatedGemm& g, const f32x4 (&acc)[FI][4],
+                                                  float* mine, int64_t i, int64_t j) {
+    if (g.act == VCSR_ACT_NONE)
+        write_gated_rows<O, VCSR_ACT_NONE, false, WHOLE, FI, ROOM>(g, acc, mine, i, j, 0);
+    else if (g.act == VCSR_ACT_RELU)
+        write_gated_rows<O, VCSR_ACT_RELU, false, WHOLE, FI, ROOM>(g, acc, mine, i, j, 0);
+    else if (g.act == VCSR_ACT_GELU)
+        write_gated_rows<O, VCSR_ACT_GELU, false, WHOLE, FI, ROOM>(g, acc, mine, i, j, 0);
+    else
+        write_gated_rows<O, VCSR_ACT_SILU, false, WHOLE, FI, ROOM>(g, acc, mine, i, j, 0);
+}
+template <bool PLAIN, int ROOM, int FI>
+__device__ __forceinline__ void write_out(const GatedGemm& g, const f32x4 (&acc)[FI][4],
+                                          float* mine, int64_t i, int64_t j2, int splits,
+                                          uint32_t split) {
+    const int64_t j = j2 / 2;
+    if (splits > 1)
+        write_gated_rows<float, VCSR_ACT_NONE, true, false, FI, ROOM>(g, acc, mine, i, j, split);
+    else if (j + 32 <= g.J / 2 && g.out_type == VCSR_BF16)
+        write_gated_typed<bf16, true, ROOM>(g, acc, mine, i, j);
+    else if (j + 32 <= g.J / 2)
+        write_gated_typed<float, true, ROOM>(g, acc, mine, i, j);
+    else if (g.out_type == VCSR_BF16)
+        write_gated_typed<bf16, false, ROOM>(g, acc, mine, i, j);
+    else
+        write_gated_typed<float, false, ROOM>(g, acc, mine, i, j);
+}
+
 // Whether the sum's last step goes through registers: its granules are not all
 // whole.
 template <class T>
@@ -481,6 +708,74 @@ __device__ __forceinline__ bool ragged_end(const Gemm& g, int64_t k_end, bool p_
     return k_end == g.R && ((g.R % BK) != 0 || (p_cols && g.I % EPG != 0) ||
                             (q_cols && g.J % EPG != 0));
 }
+
+// The operands of a block's tile: the two weights of a gated projection, or both
+// summands' of a TwiceGemm.
+template <class T, class G, bool PCOLS, bool QCOLS>
+struct Sides {
+    static constexpr bool GATED = std::is_same<G, GatedGemm>::value;
+    static constexpr bool TWICE = std::is_same<G, TwiceGemm>::value;
+    Operand p[TWICE ? 2 : 1], q[GATED || TWICE ? 2 : 1];
+
+    __device__ __forceinline__ Sides(const G& g, const Place& at) {
+        constexpr int64_t size = sizeof(T);
+        const int64_t J = GATED ? g.J / 2 : g.J, j0 = GATED ? at.j0 / 2 : at.j0;
+        p[0] = Operand{(const uint8_t*)g.p, g.ldp * size, g.I, at.i0,
+                       extent<T>(g.I, g.R, g.ldp, PCOLS)};
+        q[0] = Operand{(const uint8_t*)g.q, g.ldq * size, J, j0, extent<T>(J, g.R, g.ldq, QCOLS)};
+        if constexpr (TWICE) {
+            p[1] = p[0];
+            p[1].p = (const uint8_t*)g.p2;
+        }
+        if constexpr (GATED || TWICE)
+            q[1] = Operand{(const uint8_t*)g.q2, g.ldq2 * size, J, j0,
+                           extent<T>(J, g.R, g.ldq2, QCOLS)};
+    }
+};
+
+// A block's steps of the sum: n whole ones, whose k and summand step t gives, then those
+// that go through registers (`ends` of them, one a summand at most).  A TwiceGemm's two
+// summands have their steps one behind the other.
+template <class T, class G>
+struct Steps {
+    static constexpr bool TWICE = std::is_same<G, TwiceGemm>::value;
+    static constexpr int BK = kStepBytes / (int)sizeof(T);
+    int64_t first, second;  // k of the first whole step of each summand
+    int n0, n;              // whole steps of the first summand, and of both
+    int64_t end_k, k_end;   // of the steps through registers
+    bool end0, end1;
+
+    __device__ __forceinline__ Steps(const G& g, int64_t steps, uint32_t split, bool p_cols,
+                                     bool q_cols) {
+        if (!TWICE) {
+            first = (int64_t)split * steps * BK;
+            k_end = first + steps * BK < g.R ? first + steps * BK : g.R;
+            end0 = ragged_end<T>(g, k_end, p_cols, q_cols);
+            end1 = false;
+            end_k = end0 ? first + (k_end - first - 1) / BK * BK : k_end;
+            second = 0;
+            n0 = n = first < end_k ? (int)((end_k - first + BK - 1) / BK) : 0;
+            return;
+        }
+        const int64_t all = (g.R + BK - 1) / BK;
+        const bool ragged = ragged_end<T>(g, g.R, p_cols, q_cols);
+        const int64_t whole = ragged ? all - 1 : all;
+        const int64_t b = (int64_t)split * steps, e = b + steps < 2 * all ? b + steps : 2 * all;
+        auto clamp = [&](int64_t t) { return t < 0 ? 0 : t < whole ? t : whole; };
+        first = clamp(b) * BK;
+        second = clamp(b - all) * BK;
+        n0 = (int)(clamp(e) - clamp(b));
+        n = n0 + (int)(clamp(e - all) - clamp(b - all));
+        end_k = whole * BK;
+        k_end = g.R;
+        end0 = ragged && b < all && e >= all;
+        end1 = ragged && e == 2 * all;
+    }
+    __device__ __forceinline__ bool in_second(int t) const { return TWICE && t >= n0; }
+    __device__ __forceinline__ int64_t k(int t) const {
+        return TWICE && t >= n0 ? second + (int64_t)(t - n0) * BK : first + (int64_t)t * BK;
+    }
+};
 
 // One of a launch's products: `blocks` blocks, each a tile and one of `splits`
 // parts of the sum, of `steps` steps.
@@ -496,27 +791,24 @@ struct Part {
 // where there are too few blocks to hide a trip to memory otherwise.
 template <int TILE, int STAGES>
 constexpr int kLds = STAGES * 2 * TILE * kStepBytes;
-template <class T, int TI, int TJ, int WI, int WJ, int STAGES, bool PCOLS, bool QCOLS>
-__device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uint32_t block,
+template <class T, int TI, int TJ, int WI, int WJ, int STAGES, bool PCOLS, bool QCOLS, class G>
+__device__ __forceinline__ void gemm_shared(const G& g, const Part& part, uint32_t block,
                                             uint8_t* lds0) {
+    constexpr bool GATED = std::is_same<G, GatedGemm>::value;
+    constexpr bool TWICE = std::is_same<G, TwiceGemm>::value;
     constexpr int NT = 64 * WI * WJ;
     constexpr int FI = TI / WI / 16, FJ = TJ / WJ / 16;
-    constexpr int BK = kStepBytes / (int)sizeof(T);
     static_assert(FJ % 2 == 0, "column blocks go in pairs");
     using LP = Loader<T, TI, NT, PCOLS, false>;
-    using LQ = Loader<T, TJ, NT, QCOLS, true>;
+    using LQ = typename std::conditional<GATED, PairLoader<T, TJ, NT>,
+                                         Loader<T, TJ, NT, QCOLS, true>>::type;
     using RP = Reader<T, TI, PCOLS, false>;
     using RQ = Reader<T, TJ, QCOLS, true>;
     constexpr int kStage = (TI + TJ) * kStepBytes;
     const int splits = part.splits;
-    const int64_t steps = part.steps;
     const Place at = place_of<TI, TJ>(g, block, part.blocks, (uint32_t)splits);
-    const Operand P{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, at.i0,
-                    extent<T>(g.I, g.R, g.ldp, PCOLS)};
-    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, at.j0,
-                    extent<T>(g.J, g.R, g.ldq, QCOLS)};
-    const int64_t k_first = (int64_t)at.split * steps * BK;
-    const int64_t k_end = k_first + steps * BK < g.R ? k_first + steps * BK : g.R;
+    const Sides<T, G, PCOLS, QCOLS> o(g, at);
+    const Steps<T, G> steps(g, part.steps, at.split, PCOLS, QCOLS);
 
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int ri = (wave / WJ) * (TI / WI), rj = (wave % WJ) * (TJ / WJ);
@@ -541,18 +833,35 @@ __device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uin
             }
         }
     };
-    const bool ragged = ragged_end<T>(g, k_end, PCOLS, QCOLS);
-    const int64_t k_full = ragged ? k_first + (k_end - k_first - 1) / BK * BK : k_end;
-    uint32_t op[LP::GR], oq[LQ::GR];
-    LP::offsets(P, op);
-    LQ::offsets(Q, oq);
+    uint32_t op[LP::GR], oq[TWICE ? 2 : 1][LQ::GR];
+    LP::offsets(o.p[0], op);
+    if constexpr (GATED) {
+        LQ::offsets(o.q, oq[0]);
+    } else {
+        LQ::offsets(o.q[0], oq[0]);
+        if constexpr (TWICE) LQ::offsets(o.q[1], oq[1]);
+    }
     lds_byte* const to = (lds_byte*)lds0;
     constexpr int AHEAD = STAGES - 1;
-    const int n = k_first < k_full ? (int)((k_full - k_first + BK - 1) / BK) : 0;
+    const int n = steps.n;
     auto ask = [&](int t) __attribute__((always_inline)) {
         lds_byte* const into = to + t % STAGES * kStage;
-        LP::copy(P, op, k_first + (int64_t)t * BK, into);
-        LQ::copy(Q, oq, k_first + (int64_t)t * BK, into + TI * kStepBytes);
+        const int64_t k = steps.k(t);
+        if constexpr (GATED) {
+            LP::copy(o.p[0], op, k, into);
+            LQ::copy(o.q, oq[0], k, into + TI * kStepBytes);
+        } else if constexpr (TWICE) {
+            if (steps.in_second(t)) {
+                LP::copy(o.p[1], op, k, into);
+                LQ::copy(o.q[1], oq[1], k, into + TI * kStepBytes);
+            } else {
+                LP::copy(o.p[0], op, k, into);
+                LQ::copy(o.q[0], oq[0], k, into + TI * kStepBytes);
+            }
+        } else {
+            LP::copy(o.p[0], op, k, into);
+            LQ::copy(o.q[0], oq[0], k, into + TI * kStepBytes);
+        }
     };
 #pragma unroll
     for (int t = 0; t < AHEAD; ++t)
@@ -569,13 +878,26 @@ __device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uin
         const uint8_t* const lp = lds0 + t % STAGES * kStage;
         multiply(lp, lp + TI * kStepBytes);
     }
-    const int buf = n % STAGES;
-    if (ragged) {
-        LP::fetch(P, k_full, k_end, lds0 + buf * kStage);
-        LQ::fetch(Q, k_full, k_end, lds0 + buf * kStage + TI * kStepBytes);
+    // A step's room is free once all waves are done with the step before the last.
+    int buf = n % STAGES;
+    auto end = [&](const Operand& p, auto&& fetch_q) __attribute__((always_inline)) {
+        uint8_t* const lp = lds0 + buf * kStage;
+        LP::fetch(p, steps.end_k, steps.k_end, lp);
+        fetch_q(lp + TI * kStepBytes);
         __syncthreads();
-        multiply(lds0 + buf * kStage, lds0 + buf * kStage + TI * kStepBytes);
-    }
+        multiply(lp, lp + TI * kStepBytes);
+        buf = (buf + 1) % STAGES;
+    };
+    if (steps.end0)
+        end(o.p[0], [&](uint8_t* lq) __attribute__((always_inline)) {
+            if constexpr (GATED) LQ::fetch(o.q, steps.end_k, steps.k_end, lq);
+            else LQ::fetch(o.q[0], steps.end_k, steps.k_end, lq);
+        });
+    if constexpr (TWICE)
+        if (steps.end1)
+            end(o.p[1], [&](uint8_t* lq) __attribute__((always_inline)) {
+                LQ::fetch(o.q[1], steps.end_k, steps.k_end, lq);
+            });
     __syncthreads();
     constexpr int ROOM = STAGES * kStage / (WI * WJ) / 16 * 16;
     write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(lds0 + wave * ROOM), at.i0 + ri,
@@ -598,31 +920,28 @@ __device__ __forceinline__ void gemm_shared(const Gemm& g, const Part& part, uin
 // all of it left 58 of 468 us waiting at 8192 x 8192 x 4096.  Loads end in order:
 // a wave waits until all but the 8 newest have, before its half turn that ends
 // at the barrier behind which the first wave reads them.
-template <class T, bool PCOLS, bool QCOLS>
-__device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint32_t block,
+template <class T, bool PCOLS, bool QCOLS, class G>
+__device__ __forceinline__ void gemm_turns(const G& g, const Part& part, uint32_t block,
                                            uint8_t* lds) {
+    constexpr bool GATED = std::is_same<G, GatedGemm>::value;
+    constexpr bool TWICE = std::is_same<G, TwiceGemm>::value;
     constexpr int TI = 256, TJ = 256, NT = 512, WJ = 4, FI = 8, FJ = 4, H = 4;
-    constexpr int BK = kStepBytes / (int)sizeof(T);
     constexpr int kP = TI / 2 * kStepBytes, kStage = (TI + TJ) * kStepBytes;
     using LP = Loader<T, TI / 2, NT, PCOLS, false, 64>;
-    using LQ = Loader<T, TJ, NT, QCOLS, true>;
+    using LQ = typename std::conditional<GATED, PairLoader<T, TJ, NT>,
+                                         Loader<T, TJ, NT, QCOLS, true>>::type;
     using RP = Reader<T, TI / 2, PCOLS, false>;
     using RQ = Reader<T, TJ, QCOLS, true>;
     static_assert(LQ::GR + 2 * LP::GR == kAhead, "loads of a step");
     const int splits = part.splits;
-    const int64_t steps = part.steps;
     const Place at = place_of<TI, TJ>(g, block, part.blocks, (uint32_t)splits);
-    Operand P[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        P[h] = Operand{(const uint8_t*)g.p, g.ldp * (int64_t)sizeof(T), g.I, at.i0 + h * 64,
-                       extent<T>(g.I, g.R, g.ldp, PCOLS)};
-    const Operand Q{(const uint8_t*)g.q, g.ldq * (int64_t)sizeof(T), g.J, at.j0,
-                    extent<T>(g.J, g.R, g.ldq, QCOLS)};
-    const int64_t k_first = (int64_t)at.split * steps * BK;
-    const int64_t k_end = k_first + steps * BK < g.R ? k_first + steps * BK : g.R;
-    const bool ragged = ragged_end<T>(g, k_end, PCOLS, QCOLS);
-    const int n = (int)((k_end - k_first - (ragged ? 1 : 0)) / BK);  // whole steps
+    const Sides<T, G, PCOLS, QCOLS> o(g, at);
+    const Steps<T, G> steps(g, part.steps, at.split, PCOLS, QCOLS);
+    const int n = steps.n;
+    auto lower = [&](Operand p) __attribute__((always_inline)) {
+        p.first += 64;
+        return p;
+    };
 
     const int wave = uniform((int)(threadIdx.x >> 6));
     const int wi = wave / WJ, wj = wave % WJ;
@@ -632,18 +951,41 @@ __device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint
 #pragma unroll
         for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    uint32_t op[2][LP::GR], oq[LQ::GR];
-    LP::offsets(P[0], op[0]);
-    LP::offsets(P[1], op[1]);
-    LQ::offsets(Q, oq);
+    uint32_t op[2][LP::GR], oq[TWICE ? 2 : 1][LQ::GR];
+    LP::offsets(o.p[0], op[0]);
+    LP::offsets(lower(o.p[0]), op[1]);
+    if constexpr (GATED) {
+        LQ::offsets(o.q, oq[0]);
+    } else {
+        LQ::offsets(o.q[0], oq[0]);
+        if constexpr (TWICE) LQ::offsets(o.q[1], oq[1]);
+    }
     lds_byte* const to = (lds_byte*)lds;
-    auto ask_front = [&](int t) {  // Q and upper P of step t
+    auto ask_front = [&](int t) __attribute__((always_inline)) {  // Q and upper P of step t
         lds_byte* const into = to + (t & 1) * kStage;
-        LQ::copy(Q, oq, k_first + (int64_t)t * BK, into + 2 * kP);
-        LP::copy(P[0], op[0], k_first + (int64_t)t * BK, into);
+        const int64_t k = steps.k(t);
+        if constexpr (GATED) {
+            LQ::copy(o.q, oq[0], k, into + 2 * kP);
+            LP::copy(o.p[0], op[0], k, into);
+        } else if constexpr (TWICE) {
+            if (steps.in_second(t)) {
+                LQ::copy(o.q[1], oq[1], k, into + 2 * kP);
+                LP::copy(o.p[1], op[0], k, into);
+            } else {
+                LQ::copy(o.q[0], oq[0], k, into + 2 * kP);
+                LP::copy(o.p[0], op[0], k, into);
+            }
+        } else {
+            LQ::copy(o.q[0], oq[0], k, into + 2 * kP);
+            LP::copy(o.p[0], op[0], k, into);
+        }
     };
-    auto ask_back = [&](int t) {  // lower P
-        LP::copy(P[1], op[1], k_first + (int64_t)t * BK, to + (t & 1) * kStage + kP);
+    auto ask_back = [&](int t) __attribute__((always_inline)) {  // lower P
+        lds_byte* const into = to + (t & 1) * kStage + kP;
+        if constexpr (TWICE)
+            LP::copy(lower(steps.in_second(t) ? o.p[1] : o.p[0]), op[1], steps.k(t), into);
+        else
+            LP::copy(lower(o.p[0]), op[1], steps.k(t), into);
     };
     if (n > 0) ask_front(0), ask_back(0);
     if (n > 1) ask_front(1);
@@ -684,12 +1026,12 @@ __device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint
         }
     }
     if (!wi) barrier();
-    if (ragged) {
-        uint8_t* const stage = lds + (n & 1) * kStage;
-        const int64_t k = k_first + (int64_t)n * BK;
-        LP::fetch(P[0], k, k_end, stage);
-        LP::fetch(P[1], k, k_end, stage + kP);
-        LQ::fetch(Q, k, k_end, stage + 2 * kP);
+    int last = n & 1;
+    auto end = [&](const Operand& p, auto&& fetch_q) __attribute__((always_inline)) {
+        uint8_t* const stage = lds + last * kStage;
+        LP::fetch(p, steps.end_k, steps.k_end, stage);
+        LP::fetch(lower(p), steps.end_k, steps.k_end, stage + kP);
+        fetch_q(stage + 2 * kP);
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -704,7 +1046,18 @@ __device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint
                 for (int y = 0; y < FJ; ++y) acc[x][y] = mma<T>(q[y], p, acc[x][y]);
             }
         }
-    }
+        last ^= 1;
+    };
+    if (steps.end0)
+        end(o.p[0], [&](uint8_t* lq) __attribute__((always_inline)) {
+            if constexpr (GATED) LQ::fetch(o.q, steps.end_k, steps.k_end, lq);
+            else LQ::fetch(o.q[0], steps.end_k, steps.k_end, lq);
+        });
+    if constexpr (TWICE)
+        if (steps.end1)
+            end(o.p[1], [&](uint8_t* lq) __attribute__((always_inline)) {
+                LQ::fetch(o.q[1], steps.end_k, steps.k_end, lq);
+            });
     __syncthreads();
     constexpr int ROOM = 2 * kStage / 8;
     write_out<PCOLS || QCOLS, ROOM>(g, acc, (float*)(lds + wave * ROOM), at.i0 + wi * 128,
@@ -712,11 +1065,14 @@ __device__ __forceinline__ void gemm_turns(const Gemm& g, const Part& part, uint
 }
 
 // A tile of TILE x TILE by the code for its size.
-template <class T, int TILE, int STAGES, bool PCOLS, bool QCOLS>
-__device__ __forceinline__ void gemm_block(const Gemm& g, const Part& part, uint32_t block,
+template <class T, int TILE, int STAGES, bool PCOLS, bool QCOLS, class G>
+__device__ __forceinline__ void gemm_block(const G& g, const Part& part, uint32_t block,
                                            uint8_t* lds) {
     if constexpr (TILE == 256)
         gemm_turns<T, PCOLS, QCOLS>(g, part, block, lds);
+    else if constexpr (TILE == 64 && std::is_same<G, GatedGemm>::value)
+        // A wave has 32 columns of each weight.
+        gemm_shared<T, TILE, TILE, 4, 1, STAGES, PCOLS, QCOLS>(g, part, block, lds);
     else
         gemm_shared<T, TILE, TILE, 2, 2, STAGES, PCOLS, QCOLS>(g, part, block, lds);
 }
@@ -860,15 +1216,13 @@ __device__ __forceinline__ u32x4 load_granule(const T* run, int64_t pos, int64_t
 // row asked for at once and straight from memory into the matrix layout (all of a
 // 4096-wide bf16 row, so that the chip has the whole W under way).  The waves'
 // sums meet in LDS and are added in order: one launch, no partial sums in memory.
-template <class T, class O, int UN>
-__global__ __launch_bounds__(512) void gemm_rows_kernel(Gemm g) {
+//
+// A wave's sums; w is the row of W that the lane reads.
+template <class T, int UN>
+__device__ __forceinline__ f32x4 rows_sum(const Gemm& g, const T* w) {
     constexpr int EPG = 16 / (int)sizeof(T), WAVES = 8;
-    __shared__ __attribute__((aligned(16))) float lds[WAVES][16][20];
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
-    const int64_t j0 = (int64_t)blockIdx.x * 16;
-    const int64_t jr = j0 + (lane & 15) < g.J ? j0 + (lane & 15) : g.J - 1;
     const int64_t i = lane & 15;
-    const T* const w = (const T*)g.q + jr * g.ldq;
     const T* const x = (const T*)g.p + (i < g.I ? i : 0) * g.ldp;
     f32x4 acc{0.f, 0.f, 0.f, 0.f};
     const int64_t lines = (g.R + EPG * 8 - 1) / (EPG * 8);
@@ -913,6 +1267,16 @@ __global__ __launch_bounds__(512) void gemm_rows_kernel(Gemm g) {
                 acc = mma<T>(a, b, acc);
             }
     }
+    return acc;
+}
+template <class T, class O, int UN>
+__global__ __launch_bounds__(512) void gemm_rows_kernel(Gemm g) {
+    constexpr int WAVES = 8;
+    __shared__ __attribute__((aligned(16))) float lds[WAVES][16][20];
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    const int64_t j0 = (int64_t)blockIdx.x * 16;
+    const int64_t jr = j0 + (lane & 15) < g.J ? j0 + (lane & 15) : g.J - 1;
+    const f32x4 acc = rows_sum<T, UN>(g, (const T*)g.q + jr * g.ldq);
     *(f32x4*)&lds[wave][lane & 15][(lane >> 4) * 4] = acc;
     __syncthreads();
     const int row = threadIdx.x >> 4, col = threadIdx.x & 15;
