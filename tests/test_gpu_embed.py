@@ -12,7 +12,7 @@ import scipy.sparse
 
 from block_ref import rounding, values
 from conftest import capture, hip_runtime
-from dense_ref import EPS, Mat, close, vector
+from dense_ref import EPS, NP, Mat, close, vector
 
 pytestmark = pytest.mark.gpu
 
@@ -297,3 +297,59 @@ def test_embed_replayed_from_a_graph(gpu, M):
         if gexec.value:
             hip.hipGraphExecDestroy(gexec)
         hip.hipGraphDestroy(graph)
+
+
+@pytest.mark.parametrize("kinds", ["f32 f32", "bf16 f32", "f32 bf16", "bf16 bf16", "fp8 f32",
+                                   "fp8 bf16"])
+def test_embed_of_large_results(gpu, kinds):
+    """y of 128 MB and more, written past the caches: every value."""
+    xk, yk = kinds.split()
+    vs, st = gpu, gpu.Stream()
+    rng = np.random.default_rng(21)
+    M, V, C = (1 << 17) + 3, 500, 512
+    table, ids = values(rng, (V, C), xk), tokens(rng, M, V, "uniform")
+    ts = (0.5 + rng.random(V)).astype(np.float32) if xk == "fp8" else None
+    out = vs.DeviceArray((M, C), NP[yk])
+    print(f"embed large {kinds}", flush=True)
+    vs.run_embed_gpu(Mat(vs, st, table, xk).view, ints(vs, st, ids), out,
+                     table_scale=vector(vs, st, ts) if ts is not None else None, stream=st)
+    st.sync()
+    # Each row of the table once, and that all of y's rows are theirs bit for bit.
+    rows = vs.DeviceArray((V + 1, C), NP[yk])
+    vs.run_embed_gpu(Mat(vs, st, table, xk).view, ints(vs, st, np.arange(V + 1)), rows,
+                     table_scale=vector(vs, st, ts) if ts is not None else None, stream=st)
+    st.sync()
+    inside = (ids >= 0) & (ids < V)
+    same = np.array_equal(out.numpy(st), rows.numpy(st)[np.where(inside, ids, V)])
+    assert same
+
+
+def test_embed_grad_of_a_large_table(gpu):
+    """Zeros of 128 MB and more, past the caches, beside the rows of few and of many
+    tokens."""
+    vs, st = gpu, gpu.Stream()
+    rng = np.random.default_rng(22)
+    V, C = 70000, 512
+    for M in (20, 700, 20000):
+        ids = tokens(rng, M, V, "frequent")
+        dy = values(rng, (M, C), "bf16")
+        out = vs.DeviceArray((V, C), np.float32)
+        vs._check(vs.load_library().vcsr_memset_d(out.ptr, 0x5B, out.nbytes, st.h))
+        print(f"embed grad large M={M}", flush=True)
+        vs.run_embed_grad_gpu(Mat(vs, st, dy, "bf16").view, ints(vs, st, ids), out, stream=st)
+        st.sync()
+        got = out.numpy(st)
+        met = np.unique(ids[(ids >= 0) & (ids < V)])
+        one = vs.DeviceArray((V, C), np.float32)
+        one.zero(st)
+        vs.run_embed_grad_gpu(Mat(vs, st, dy, "bf16").view, ints(vs, st, ids), one,
+                              accumulate=True, stream=st)
+        st.sync()
+        same = np.array_equal(got, one.numpy(st))
+        assert same
+        want = np.stack([dy[ids == v].sum(0) for v in met[:200]])
+        size = np.stack([np.abs(dy[ids == v]).sum(0) for v in met[:200]])
+        n = np.array([(ids == v).sum() for v in met[:200]])[:, None]
+        close(got[met[:200]], want, (n + 2) * EPS * size, "rows with tokens")
+        got[met] = 0
+        assert not got.any()

@@ -975,9 +975,10 @@ def _layernorm_grad_bytes(M, N, x_type, y_type, dweight, dbias):
 
 
 @functools.lru_cache(maxsize=4096)
-def _embed_grad_bytes(M, V, N, table_type, y_type):
+def _embed_grad_bytes(M, V, N, table_type, y_type, accumulate):
     need = C.c_size_t(0)
-    args = _EmbedGradArgs(M=M, V=V, C=N, table_type=table_type, y_type=y_type)
+    args = _EmbedGradArgs(M=M, V=V, C=N, table_type=table_type, y_type=y_type,
+                          accumulate=accumulate)
     _check(load_library().vcsr_embed_grad_workspace(C.byref(args), C.byref(need)))
     return need.value
 
@@ -1107,8 +1108,9 @@ def run_embed_grad_gpu(dy, ids, dtable, scale=1.0, accumulate=False, workspace=N
     (V, N), (ip, M) = _shape2(dtable, "dtable"), _ids(ids, "ids")
     (dp, lddy), (tp, lddt) = _mat(dy, M, N, "dy"), _mat(dtable, V, N, "dtable")
     tt, yt = _type(dtable, "dtable"), _type(dy, "dy")
-    need = _embed_grad_bytes(M, V, N, tt, yt)
-    args = _pack_embed_grad(M, V, N, tt, yt, 1 if accumulate else 0, scale, dp, lddy, ip, tp, lddt)
+    add = 1 if accumulate else 0
+    need = _embed_grad_bytes(M, V, N, tt, yt, add)
+    args = _pack_embed_grad(M, V, N, tt, yt, add, scale, dp, lddy, ip, tp, lddt)
     return _call_with_space((_lib or load_library()).vcsr_embed_grad, args, need, workspace, stream,
                             timed)
 

@@ -40,6 +40,13 @@ __device__ __forceinline__ void widen(const u32x4& r, float (&v)[16], fp8) {
     }
 }
 
+// 16 bytes anywhere.
+typedef u32x4 Any16 __attribute__((aligned(1)));
+
+// What a call writes past the caches: as many bytes leave nothing there for whoever reads
+// them next, half of the 256 MB that the last cache has.
+constexpr int64_t kLarge = (int64_t)128 << 20;
+
 // How rows end: in whole vectors of 16 bytes, inside one, or before the first is whole.
 enum { kWhole = 0, kRagged = 1, kShort = 2 };
 template <class T>
@@ -50,7 +57,8 @@ int ends_of(int32_t C) {
 
 // Values [c, c + V) of a row of C, for c a multiple of V: anything past the row's
 // end.  No branch but for rows that are shorter than a vector.
-template <class T, int ENDS>
+// ONCE: of values that are read once.
+template <class T, int ENDS, bool ONCE = false>
 __device__ __forceinline__ u32x4 load16(const T* row, int64_t c, int64_t C) {
     constexpr int V = 16 / (int)sizeof(T);
     u32x4 r;
@@ -65,15 +73,42 @@ __device__ __forceinline__ u32x4 load16(const T* row, int64_t c, int64_t C) {
     }
     // A vector that reaches past the end is read ending with the row, and shifted.
     const int64_t back = c + V > C ? c + V - C : 0;
-    const Mem<uint8_t, 16> m = *(const Mem<uint8_t, 16>*)(row + (back < V ? c - back : 0));
-    __builtin_memcpy(&r, &m, 16);
+    const Any16* const from = (const Any16*)(row + (back < V ? c - back : 0));
+    r = ONCE ? __builtin_nontemporal_load(from) : *from;
     return ENDS == kWhole ? r : shift_down(r, (int)(back & (V - 1)) * (int)sizeof(T));
 }
 
 // ------------------------------------------------------------------- forward
+// Stores past the caches, of whole 16 bytes.
+template <int V>
+__device__ __forceinline__ void store_large(float* p, const float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4)
+        __builtin_nontemporal_store(
+            __builtin_bit_cast(u32x4, f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]}), (Any16*)(p + i));
+}
+template <int V>
+__device__ __forceinline__ void store_large(bf16* p, const float (&v)[V]) {
+    if constexpr (V < 8) {
+        store_vec(p, V, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 8) {
+            Mem<bf16, 8> m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) m.v[k] = (bf16)v[i + k];
+            u32x4 q;
+            __builtin_memcpy(&q, &m, 16);
+            __builtin_nontemporal_store(q, (Any16*)(p + i));
+        }
+    }
+}
+
 // Groups of `lanes` (a power of two <= 64) lanes take U rows each, of them NV vectors
-// a lane from blockIdx.y's slab on; all loads go out together.
-template <class X, class Y, int ENDS, int NV, int U>
+// a lane from blockIdx.y's slab on; all loads go out together.  The table's rows stay
+// in the caches, since tokens repeat; y, where it is large (whole rows alone), goes past
+// them: 65536 tokens of 2048 bf16 60 us, 75 through them.
+template <class X, class Y, int ENDS, int NV, int U, bool LARGE>
 __global__ __launch_bounds__(256) void embed_kernel(vcsr_embed_args a, int lanes) {
     constexpr int V = 16 / (int)sizeof(X);
     const int lane = threadIdx.x & (lanes - 1);
@@ -108,7 +143,10 @@ __global__ __launch_bounds__(256) void embed_kernel(vcsr_embed_args a, int lanes
             widen(r[u][k], v, X());
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] = id[u] < 0 ? 0.f : v[i] * f[u];
-            store_vec(to + c, ENDS == kWhole || a.C - c > V ? V : (int)(a.C - c), v);
+            if (LARGE)
+                store_large(to + c, v);
+            else
+                store_vec(to + c, ENDS == kWhole || a.C - c > V ? V : (int)(a.C - c), v);
         }
     }
 }
@@ -130,8 +168,11 @@ void launch_ends(const vcsr_embed_args& a, hipStream_t st) {
             b.M = a.M - m < most ? a.M - m : most;
             b.ids += m;
             b.y = (Y*)a.y + m * a.ldy;
-            embed_kernel<X, Y, ENDS, NV, U>
-                <<<dim3((unsigned)((b.M + per - 1) / per), slabs), 256, 0, st>>>(b, lanes);
+            const dim3 grid((unsigned)((b.M + per - 1) / per), slabs);
+            if (ENDS == kWhole && a.M * a.C * (int64_t)sizeof(Y) >= kLarge)
+                embed_kernel<X, Y, ENDS, NV, U, ENDS == kWhole><<<grid, 256, 0, st>>>(b, lanes);
+            else
+                embed_kernel<X, Y, ENDS, NV, U, false><<<grid, 256, 0, st>>>(b, lanes);
         }
     };
     if (nv > 128)
@@ -157,42 +198,104 @@ __device__ __forceinline__ int32_t key_of(int32_t id, int32_t V) {
     return (uint32_t)id < (uint32_t)V ? id : V;
 }
 
-// Few tokens: each one's place is the number of tokens before it.  A block takes 64
-// tokens, each of its 16 waves a part of all keys; a token's own block is the only one
-// where the order of equal keys has to be told apart.
-__global__ __launch_bounds__(1024) void rank_kernel(const int32_t* ids, int32_t n, int32_t V,
-                                                    int32_t* keys, int32_t* pos) {
-    __shared__ int32_t count[16][64];
-    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
-    const int32_t i0 = (int32_t)blockIdx.x * 64, i = i0 + lane;
-    const int32_t key = i < n ? key_of(ids[i], V) : V;
-    const int32_t part = ((n + 63) / 64 + 15) / 16 * 64;
-    const int32_t j0 = wave * part, j1 = j0 + part < n ? j0 + part : n;
-    int32_t before = 0;
-    auto run = [&](int32_t from, int32_t to, uint32_t limit) {  // limit: up to 2^31
-        for (int32_t b = from; b < to; b += 64) {
-            const int32_t mine = b + lane < to ? key_of(ids[b + lane], V) : -1;
-#pragma unroll
-            for (int l = 0; l < 64; ++l)
-                before += (uint32_t)__builtin_amdgcn_readlane(mine, l) < limit ? 1 : 0;
-        }
-    };
-    if (j0 < i0) run(j0, j1 < i0 ? j1 : i0, (uint32_t)key + 1);
-    if (j0 <= i0 && i0 < j1) {  // the block's own tokens
-#pragma unroll
-        for (int l = 0; l < 64; ++l) {
-            const int32_t k = __builtin_amdgcn_readlane(key, l);
-            before += i0 + l < n && (k < key || (k == key && l < lane)) ? 1 : 0;
-        }
+// A piece of 16 bytes of a span of zeros, the last one moved back to end with it.
+template <bool LARGE>
+__device__ __forceinline__ void zero_piece(uint8_t* p, int64_t bytes, int64_t i) {
+    if (bytes >= 16) {
+        Any16* const to = (Any16*)(p + (16 * i + 16 <= bytes ? 16 * i : bytes - 16));
+        const u32x4 zero{0, 0, 0, 0};
+        if (LARGE) __builtin_nontemporal_store(zero, to);
+        else *to = zero;
+    } else {
+        for (int64_t b = 0; b < bytes; b += 2) *(uint16_t*)(p + b) = 0;
     }
-    if (j1 > i0 + 64) run(j0 > i0 + 64 ? j0 : i0 + 64, j1, key);
-    count[wave][lane] = before;
-    __syncthreads();
-    if (wave || i >= n) return;
+}
+// The rows of dtable, of which those without a token are to be cleared.  `owner` tells
+// which: the first launch writes to owner[v] some token of id v, so that a row has one if
+// its owner is a token of its id; what else lies there does not matter, and nothing has
+// to be cleared first.  They are cleared beside the sums, past the caches where they are
+// many (`large`): 32768 tokens and 32768 x 2048 FP32 take 107 us, 120 through the caches
+// (with dy's loads past them too 123); clearing every row beside the sort and writing
+// some again 131.
+struct Zeros {
+    uint8_t* p;
+    int64_t ld, bytes;  // of a row
+    int64_t rows;
+    const int32_t *owner, *ids;
+    int32_t M;
+    bool large;
+};
+// Waves take groups of up to 64 rows, a lane a row to see which have a token (`met`).
+template <bool LARGE, class F>
+__device__ __forceinline__ void zero_rows(const Zeros& z, int64_t wave, int64_t waves, F&& met) {
+    const int lane = threadIdx.x & 63;
+    int64_t most = 16384 / z.bytes;
+    most = most < 1 ? 1 : most < 64 ? most : 64;
+    for (int64_t r0 = wave * most; r0 < z.rows; r0 += waves * most) {
+        const int rows = z.rows - r0 < most ? (int)(z.rows - r0) : (int)most;
+        const uint64_t kept = __ballot(lane < rows && met(lane < rows ? r0 + lane : r0));
+        if (!kept && z.ld == z.bytes) {
+            for (int64_t i = lane; 16 * i < rows * z.bytes; i += 64)
+                zero_piece<LARGE>(z.p + r0 * z.ld, rows * z.bytes, i);
+            continue;
+        }
+        for (int k = 0; k < rows; ++k)
+            if (!(kept >> k & 1))
+                for (int64_t i = lane; 16 * i < z.bytes; i += 64)
+                    zero_piece<LARGE>(z.p + (r0 + k) * z.ld, z.bytes, i);
+    }
+}
+// Few tokens: each one's place is the number of tokens before it.  All keys go to LDS; a
+// block takes 16 tokens, a lane one of them and a thirty-second of the keys, and LDS adds
+// the parts.
+constexpr int kMostRanked = 12288;
+__global__ __launch_bounds__(512) void rank_kernel(const int32_t* __restrict__ ids, int32_t n,
+                                                   int32_t V, int32_t* __restrict__ keys,
+                                                   int32_t* __restrict__ pos,
+                                                   int32_t* __restrict__ owner) {
+    __shared__ __attribute__((aligned(16))) int32_t all[kMostRanked];
+    __shared__ int32_t count[32][17];
+    const int t = threadIdx.x & 15, run = threadIdx.x >> 4;
+    const int32_t i = (int32_t)blockIdx.x * 16 + t;
+    const int32_t groups = (n + 3) / 4;
+#pragma unroll 4
+    for (int32_t g = threadIdx.x; g < groups; g += 512) {
+        int32_t k[4];
+        if (4 * g + 4 <= n) {
+            const Mem<int32_t, 4> m = *(const Mem<int32_t, 4>*)(ids + 4 * g);
 #pragma unroll
-    for (int w = 1; w < 16; ++w) before += count[w][lane];
+            for (int q = 0; q < 4; ++q) k[q] = key_of(m.v[q], V);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) k[q] = 4 * g + q < n ? key_of(ids[4 * g + q], V) : -1;
+        }
+        *(int4*)(all + 4 * g) = make_int4(k[0], k[1], k[2], k[3]);
+    }
+    __syncthreads();
+    const int32_t key = i < n ? all[i] : V, own = i >> 2;
+    const int32_t len = (groups + 31) / 32, g0 = run * len;
+    const int32_t g1 = g0 + len < groups ? g0 + len : groups;
+    // As unsigned numbers: what fills the last group (-1) is behind all keys, and a key
+    // and one is at most 2^31.  Of equal keys those of lower tokens come first.
+    int32_t before = 0;
+#pragma unroll 4
+    for (int32_t g = g0; g < g1; ++g) {
+        const int4 k = *(const int4*)(all + 4 * g);
+        const uint32_t limit = (uint32_t)key + (g < own ? 1 : 0);
+        before += (uint32_t)k.x < limit ? 1 : 0;
+        before += (uint32_t)k.y < limit ? 1 : 0;
+        before += (uint32_t)k.z < limit ? 1 : 0;
+        before += (uint32_t)k.w < limit ? 1 : 0;
+    }
+    count[run][t] = before;
+    __syncthreads();
+    if (run || i >= n) return;
+#pragma unroll
+    for (int w = 1; w < 32; ++w) before += count[w][t];
+    for (int32_t j = 4 * own; j < i; ++j) before += all[j] == key ? 1 : 0;
     keys[before] = key;
     pos[before] = i;
+    if (owner && key < V) owner[key] = i;
 }
 
 // More: by digits of up to 9 bits, the lowest first, two launches each.  A block takes a
@@ -202,6 +305,7 @@ constexpr int kDigits = 512;
 struct Radix {
     const int32_t *keys, *pos;
     int32_t n, V, tile, shift, digits;
+    int32_t* owner;  // of the first digit's counts, or null
 };
 __device__ __forceinline__ int32_t radix_key(const Radix& r, int64_t i) {
     const int32_t k = r.keys[i];
@@ -213,8 +317,12 @@ __global__ __launch_bounds__(256) void digit_count_kernel(Radix r, int32_t* coun
     __syncthreads();
     const int64_t first = (int64_t)blockIdx.x * r.tile;
     const int64_t last = first + r.tile < r.n ? first + r.tile : r.n;
-    for (int64_t i = first + threadIdx.x; i < last; i += 256)
-        atomicAdd(&lds[(radix_key(r, i) >> r.shift) & (r.digits - 1)], 1);
+#pragma unroll 4
+    for (int64_t i = first + threadIdx.x; i < last; i += 256) {
+        const int32_t k = radix_key(r, i);
+        atomicAdd(&lds[(k >> r.shift) & (r.digits - 1)], 1);
+        if (r.owner && k < r.V) r.owner[k] = (int32_t)i;
+    }
     __syncthreads();
     for (int d = threadIdx.x; d < r.digits; d += 256)
         counts[(int64_t)blockIdx.x * r.digits + d] = lds[d];
@@ -228,15 +336,14 @@ __global__ __launch_bounds__(256) void digit_place_kernel(Radix r, const int32_t
         for (int w = 0; w < 4; ++w) next[w][d] = 0;
     // Digits [2 tid, 2 tid + 2): how many keys of them there are, and in blocks before.
     int32_t all[2] = {0, 0}, before[2] = {0, 0};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int d = 2 * tid + h;
-        if (d >= r.digits) continue;
-#pragma unroll 8
+    if (2 * tid < r.digits) {
+#pragma unroll 16
         for (int32_t b = 0; b < (int32_t)gridDim.x; ++b) {
-            const int32_t c = counts[(int64_t)b * r.digits + d];
-            all[h] += c;
-            before[h] += b < (int32_t)blockIdx.x ? c : 0;
+            const int2 c = *(const int2*)(counts + (int64_t)b * r.digits + 2 * tid);
+            all[0] += c.x;
+            all[1] += c.y;
+            before[0] += b < (int32_t)blockIdx.x ? c.x : 0;
+            before[1] += b < (int32_t)blockIdx.x ? c.y : 0;
         }
     }
     const int32_t two = all[0] + all[1], scan = wave_inclusive_scan(two, lane);
@@ -250,6 +357,7 @@ __global__ __launch_bounds__(256) void digit_place_kernel(Radix r, const int32_t
     const int64_t first = (int64_t)blockIdx.x * r.tile + (int64_t)wave * (r.tile / 4);
     int64_t last = first + r.tile / 4;
     if (last > r.n) last = r.n;
+#pragma unroll 4
     for (int64_t i = first + lane; i < last; i += 64)
         atomicAdd(&next[wave][(radix_key(r, i) >> r.shift) & (r.digits - 1)], 1);
     __syncthreads();
@@ -343,15 +451,37 @@ struct Runs {
 // Blocks of a launch, which has fewer than 2^32 threads.
 constexpr int64_t kMostBlocks = (int64_t)1 << 23;
 
-// SORTS: all tokens are one chunk, which each wave sorts by itself.
+// SORTS: up to 64 tokens, which each wave sorts by itself; it adds the runs that begin
+// among its E.  Blocks behind `sums` clear the rows of no token.
 template <class D, class X, int ENDS, bool SORTS>
-__global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, Runs r) {
+__global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, Runs r, Zeros z,
+                                                        int32_t sums) {
     constexpr int V = 16 / (int)sizeof(D), U = 8;
-    const int lane = threadIdx.x & 63;
-    const int64_t item = r.first + (int64_t)blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6));
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    if ((int32_t)blockIdx.x >= sums) {
+        const int32_t key = SORTS && lane < a.M ? key_of(a.ids[lane], a.V) : a.V;
+        auto met = [&](int64_t row) {
+            if (!SORTS) {
+                const uint32_t m = (uint32_t)z.owner[row];
+                return m < (uint32_t)z.M && z.ids[m] == row;
+            }
+            bool any = false;
+#pragma unroll
+            for (int l = 0; l < 64; ++l) any |= __builtin_amdgcn_readlane(key, l) == row;
+            return any;
+        };
+        const int64_t first = ((int64_t)blockIdx.x - sums) * 4 + wave;
+        const int64_t waves = ((int64_t)gridDim.x - sums) * 4;
+        if (z.large)
+            zero_rows<true>(z, first, waves, met);
+        else
+            zero_rows<false>(z, first, waves, met);
+        return;
+    }
+    const int64_t item = r.first + (int64_t)blockIdx.x * 4 + wave;
     const int64_t chunk = item / r.slabs;
     if (chunk >= r.chunks) return;
-    const int E = r.E;
+    const int E = SORTS ? 64 : r.E;
     Chunk k;
     int32_t pos, pos_behind = 0;
     if (SORTS) {
@@ -362,16 +492,26 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, 
             const int32_t o = __builtin_amdgcn_readlane(mine, l);
             rank += o < mine || (o == mine && l < lane) ? 1 : 0;
         }
-        k.before = -1;
-        k.behind = a.V;
         k.key = __builtin_amdgcn_ds_permute(rank * 4, mine);
         pos = __builtin_amdgcn_ds_permute(rank * 4, lane);
+        const int valid = __popcll(__ballot(k.key < a.V)), first = (int)chunk * r.E;
+        const uint64_t starts = __ballot(lane < valid && (lane == 0 || __shfl_up(k.key, 1) != k.key));
+        // The first run that begins in a token from `at` on.
+        auto start_from = [&](int at) {
+            const uint64_t later = at < 64 ? starts >> at << at : 0;
+            return later ? __builtin_ctzll(later) : valid;
+        };
+        k.from = start_from(first);
+        k.to = start_from(first + r.E);
+        k.lead = 0;
+        k.tail = 64;
+        k.behind = a.V;
     } else {
         k = load_chunk(r.keys, chunk * E, a.M, E, a.V, lane);
         pos = lane < E && chunk * E + lane < a.M ? r.pos[chunk * E + lane] : 0;
         pos_behind = lane < E && (chunk + 1) * E + lane < a.M ? r.pos[(chunk + 1) * E + lane] : 0;
+        find_runs(k, chunk == 0, E, a.V);
     }
-    find_runs(k, chunk == 0, E, a.V);
     const int64_t vec = (item - chunk * r.slabs) * r.width + lane;
     const bool live = lane < r.width && vec * V < a.C;
     const int64_t c = live ? vec * V : a.C;
@@ -383,21 +523,25 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, 
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    int32_t key = k.from < k.to ? key_at(k.from) : 0;
-    for (int e = k.from; e < k.to; e += U) {
-        u32x4 v[U];
+    if (k.from >= k.to) return;
+    int32_t key = key_at(k.from);
+    // Two sets of U rows of dy: one is under way while the other is added.
+    u32x4 v[2][U];
+    auto load = [&](u32x4(&to)[U], int e) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int at = e + u < k.to ? e + u : k.to - 1;
             const int64_t m = at < E ? __builtin_amdgcn_readlane(pos, at)
                                      : __builtin_amdgcn_readlane(pos_behind, at - E);
-            v[u] = load16<D, ENDS>((const D*)a.dy + m * a.lddy, c, a.C);
+            to[u] = load16<D, ENDS, true>((const D*)a.dy + m * a.lddy, c, a.C);
         }
+    };
+    auto add = [&](const u32x4(&from)[U], int e) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (e + u >= k.to) break;
             float d[V];
-            widen(v[u], d, D());
+            widen(from[u], d, D());
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[i] += d[i];
             const int32_t next = e + u + 1 < k.to ? key_at(e + u + 1) : -1;
@@ -422,6 +566,13 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, 
             for (int i = 0; i < V; ++i) acc[i] = 0.f;
             key = next;
         }
+    };
+    load(v[0], k.from);
+    for (int e = k.from; e < k.to; e += 2 * U) {
+        if (e + U < k.to) load(v[1], e + U);
+        add(v[0], e);
+        if (e + 2 * U < k.to) load(v[0], e + 2 * U);
+        if (e + U < k.to) add(v[1], e + U);
     }
 }
 
@@ -473,14 +624,13 @@ __global__ __launch_bounds__(256) void embed_join_kernel(vcsr_embed_grad_args a,
 }
 
 // How the gradient's tokens are sorted and cut.
-constexpr int64_t kMostRanked = 8192;
 struct Shape {
     Runs runs{};
     int32_t passes = 0, tile = 0, bits = 0;  // of the sort by digits
     int64_t tiles = 0;
-    size_t array = 0, counts = 0, parts = 0;  // bytes; an array of n numbers
+    size_t array = 0, counts = 0, owners = 0, parts = 0;  // bytes; an array of n numbers
     int arrays = 0;
-    size_t bytes() const { return arrays * array + counts + parts; }
+    size_t bytes() const { return arrays * array + counts + owners + parts; }
 };
 size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 Shape shape_of(const vcsr_embed_grad_args& a) {
@@ -491,12 +641,13 @@ Shape shape_of(const vcsr_embed_grad_args& a) {
     s.runs.width = (int)((nv + slabs - 1) / slabs);
     s.runs.E = 64;
     s.runs.ldp = nv * v;
-    if (a.M > 64)  // enough waves to have the chip's loads under way
-        while (s.runs.E > 8 && a.M / s.runs.E * slabs < 2048) s.runs.E /= 2;
+    // Enough waves to have the chip's loads under way.
+    while (s.runs.E > 8 && a.M / s.runs.E * slabs < 2048) s.runs.E /= 2;
     s.runs.chunks = (a.M + s.runs.E - 1) / s.runs.E;
     if (a.M <= 64) return s;
     s.array = round_up((size_t)a.M * 4);
     s.arrays = 2;
+    if (!a.accumulate) s.owners = round_up((size_t)a.V * 4);
     s.parts = round_up((size_t)s.runs.chunks * 2 * (size_t)s.runs.ldp * 4);
     if (a.M <= kMostRanked) return s;
     int bits = 1;
@@ -511,18 +662,28 @@ Shape shape_of(const vcsr_embed_grad_args& a) {
     return s;
 }
 
+// Blocks of 256 threads that clear these rows, 16 KB a wave and more.
+int32_t zero_blocks(const Zeros& z) {
+    const int64_t need = (z.rows * z.bytes + 65535) / 65536;
+    return (int32_t)(need < 4096 ? need : 4096);
+}
+
 template <class D, class X, int ENDS>
-hipError_t launch_sums(const vcsr_embed_grad_args& a, const Shape& s, hipStream_t st) {
+hipError_t launch_sums(const vcsr_embed_grad_args& a, const Shape& s, const Zeros& z,
+                       hipStream_t st) {
     Runs r = s.runs;
     const int64_t blocks = (r.chunks * r.slabs + 3) / 4;
     if (a.M <= 64) {
-        embed_sum_kernel<D, X, ENDS, true><<<(unsigned)blocks, 256, 0, st>>>(a, r);
+        embed_sum_kernel<D, X, ENDS, true>
+            <<<(unsigned)blocks + (unsigned)zero_blocks(z), 256, 0, st>>>(a, r, z, (int32_t)blocks);
         return hipGetLastError();
     }
     for (int64_t b = 0; b < blocks; b += kMostBlocks) {
         const int64_t count = blocks - b < kMostBlocks ? blocks - b : kMostBlocks;
         r.first = 4 * b;
-        embed_sum_kernel<D, X, ENDS, false><<<(unsigned)count, 256, 0, st>>>(a, r);
+        const unsigned zeros = b == 0 ? (unsigned)zero_blocks(z) : 0;
+        embed_sum_kernel<D, X, ENDS, false>
+            <<<(unsigned)count + zeros, 256, 0, st>>>(a, r, z, (int32_t)count);
     }
     for (int64_t c = 0; c < r.chunks; c += kMostBlocks) {
         const int64_t count = r.chunks - c < kMostBlocks ? r.chunks - c : kMostBlocks;
@@ -533,11 +694,12 @@ hipError_t launch_sums(const vcsr_embed_grad_args& a, const Shape& s, hipStream_
     return hipGetLastError();
 }
 template <class D, class X>
-hipError_t launch_grad(const vcsr_embed_grad_args& a, const Shape& s, hipStream_t st) {
+hipError_t launch_grad(const vcsr_embed_grad_args& a, const Shape& s, const Zeros& z,
+                       hipStream_t st) {
     switch (ends_of<D>(a.C)) {
-        case kWhole: return launch_sums<D, X, kWhole>(a, s, st);
-        case kRagged: return launch_sums<D, X, kRagged>(a, s, st);
-        default: return launch_sums<D, X, kShort>(a, s, st);
+        case kWhole: return launch_sums<D, X, kWhole>(a, s, z, st);
+        case kRagged: return launch_sums<D, X, kRagged>(a, s, z, st);
+        default: return launch_sums<D, X, kShort>(a, s, z, st);
     }
 }
 
@@ -561,38 +723,41 @@ size_t embed_grad_workspace(const vcsr_embed_grad_args& a) {
 
 hipError_t launch_embed_grad(const vcsr_embed_grad_args& a, hipStream_t st) {
     const int64_t size = a.table_type == VCSR_F32 ? 4 : 2;
-    hipError_t e = hipSuccess;
-    if (!a.accumulate) e = launch_zero(a.dtable, a.lddt * size, a.V, a.C * size, st);
-    if (e != hipSuccess || a.M <= 0) return e;
+    if (a.M <= 0)
+        return a.accumulate ? hipSuccess
+                            : launch_zero(a.dtable, a.lddt * size, a.V, a.C * size, st);
     Shape s = shape_of(a);
     char* const base = (char*)a.workspace;
     auto array = [&](int i) { return (int32_t*)(base + i * s.array); };
+    int32_t* const counts = (int32_t*)(base + s.arrays * s.array);
+    int32_t* const owner = s.owners ? (int32_t*)((char*)counts + s.counts) : nullptr;
+    const Zeros zeros{(uint8_t*)a.dtable, a.lddt * size, a.C * size, a.accumulate ? 0 : a.V,
+                      owner, a.ids, (int32_t)a.M, (int64_t)a.V * a.C * size >= kLarge};
     if (a.M > 64) {
         s.runs.keys = array(0);
         s.runs.pos = array(1);
-        s.runs.part = (float*)(base + s.arrays * s.array + s.counts);
+        s.runs.part = (float*)((char*)counts + s.counts + s.owners);
     }
     if (a.M > 64 && a.M <= kMostRanked) {
-        rank_kernel<<<(unsigned)((a.M + 63) / 64), 1024, 0, st>>>(a.ids, (int32_t)a.M, a.V,
-                                                                 array(0), array(1));
+        rank_kernel<<<(unsigned)((a.M + 15) / 16), 512, 0, st>>>(a.ids, (int32_t)a.M, a.V, array(0),
+                                                                array(1), owner);
     } else if (a.M > 64) {
-        int32_t* const counts = (int32_t*)(base + s.arrays * s.array);
         for (int p = 0; p < s.passes; ++p) {
             const int to = (s.passes - 1 - p) % 2 * 2;  // the last digit's go to 0 and 1
-            const Radix r{p ? array(2 - to) : a.ids, p ? array(3 - to) : nullptr, (int32_t)a.M,
-                          a.V,  s.tile, p * s.bits, 1 << s.bits};
+            const Radix r{p ? array(2 - to) : a.ids, p ? array(3 - to) : nullptr, (int32_t)a.M, a.V,
+                          s.tile, p * s.bits, 1 << s.bits, p ? nullptr : owner};
             digit_count_kernel<<<(unsigned)s.tiles, 256, 0, st>>>(r, counts);
             digit_place_kernel<<<(unsigned)s.tiles, 256, 0, st>>>(r, counts, array(to),
                                                                   array(to + 1));
         }
     }
-    e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (a.y_type == VCSR_F32)
-        return a.table_type == VCSR_F32 ? launch_grad<float, float>(a, s, st)
-                                        : launch_grad<float, bf16>(a, s, st);
-    return a.table_type == VCSR_F32 ? launch_grad<bf16, float>(a, s, st)
-                                    : launch_grad<bf16, bf16>(a, s, st);
+        return a.table_type == VCSR_F32 ? launch_grad<float, float>(a, s, zeros, st)
+                                        : launch_grad<float, bf16>(a, s, zeros, st);
+    return a.table_type == VCSR_F32 ? launch_grad<bf16, float>(a, s, zeros, st)
+                                    : launch_grad<bf16, bf16>(a, s, zeros, st);
 }
 
 }  // namespace vcsr
