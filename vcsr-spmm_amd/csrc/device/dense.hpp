@@ -204,8 +204,10 @@ hipError_t launch_dz(const vcsr_linear_grad_args& a, void* dz, int64_t lddz, flo
                      hipStream_t st);
 int32_t dz_row_blocks(int64_t M, int32_t N, int32_t dy_type);
 // The same of a gated projection: dz_gate = dy * z_up * act'(z_gate) and dz_up = dy *
-// act(z_gate), M rows `lddz` apart one behind the other in dz (may be NULL), and their
-// sums of rows in part_gate and part_up (either may be NULL).
+// act(z_gate), M rows of `lddz` values (a multiple of 8, zeros behind N) one behind the
+// other in dz (may be NULL), and their sums of rows in part_gate and part_up (either may
+// be NULL), for blocks of gated_row_blocks(M, lddz, type of dy) rows.
+int32_t gated_row_blocks(int64_t M, int64_t lddz, int32_t dy_type);
 hipError_t launch_gated_dz(const vcsr_gated_grad_args& a, void* dz, int64_t lddz, float* part_gate,
                            float* part_up, hipStream_t st);
 // Zeros in `rows` rows of `bytes` bytes, `ld` bytes apart (all even, as FP32 and bf16
@@ -243,9 +245,11 @@ struct GatedGemm : Gemm {
     void* z2 = nullptr;
 };
 // Its dx: the sum of two products, P Q and P2 Q2, both of length R; p2 has p's stride.
+// `whole`: P's rows hold zeros behind R, up to whole steps of the sum.
 struct TwiceGemm : Gemm {
     const void *p2 = nullptr, *q2 = nullptr;
     int64_t ldq2 = 0;
+    bool whole = false;
 };
 // Its dw: two products of one size, P Q into out and P2 Q into out2.
 struct TwinGemm : Gemm {

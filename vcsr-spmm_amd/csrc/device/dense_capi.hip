@@ -479,9 +479,12 @@ GatedGrad grad_of(const vcsr_gated_grad_args* args) {
     range(a.N <= kOperandLd && a.K <= kOperandLd, "N, K over 2^20");
     range(a.M <= kMaxOut / 2 / (a.N > a.K ? a.N : a.K), "M x N or M x K over 2^41");
     const bool products = a.dx || a.dw_gate;
-    w.lddz = ((int64_t)a.N + 7) / 8 * 8;  // rows of dz on 16-byte boundaries
+    // Rows of dz on 16-byte boundaries, and in whole steps of dx's sum (128 bytes) where
+    // that is at most an eighth more.
+    const int64_t step = 128 / (int64_t)size_of(a.x_type), whole = (a.N + step - 1) / step * step;
+    w.lddz = whole <= a.N + a.N / 8 ? whole : ((int64_t)a.N + 7) / 8 * 8;
     if (products) w.dz_bytes = round_up(2 * (size_t)a.M * (size_t)w.lddz * size_of(a.x_type));
-    w.row_blocks = vcsr::dz_row_blocks(a.M, a.N, a.y_type);
+    w.row_blocks = vcsr::gated_row_blocks(a.M, w.lddz, a.y_type);
     // A single block of rows writes dbias itself.
     if (w.row_blocks > 1) w.bias_bytes = round_up((size_t)w.row_blocks * (size_t)a.N * 4);
     char* const base = (char*)a.workspace;
@@ -499,6 +502,7 @@ GatedGrad grad_of(const vcsr_gated_grad_args* args) {
     x.ldq = a.ldwg;
     x.q2 = a.w_up;
     x.ldq2 = a.ldwu;
+    x.whole = w.lddz == whole;
     x.q_cols = true;
     x.out = a.dx;
     x.ldo = a.lddx;

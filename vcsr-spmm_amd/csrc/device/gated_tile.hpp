@@ -167,6 +167,8 @@ hipError_t launch_gated_tiles(const GatedGemm& g, const GemmPlan& p, hipStream_t
 }
 
 // ------------------------------------------------------------------ gradients
+struct HalfGemm : Gemm {};  // one of dw's products
+
 // dw's two products, from multiples of 8 on so that all keep their XCDs (dw_part's
 // blocks are one's), then dx, then the sums of dbias' partial rows.  DW, DX: which of
 // them there are.
@@ -195,7 +197,8 @@ __global__ __launch_bounds__(kThreads<TILE>) void gated_grad_kernel(TwinGemm dw,
         const bool second = b >= half;
         if (second) b -= half;
         if (b >= dw_part.blocks) return;
-        Gemm g = dw;
+        HalfGemm g;
+        static_cast<Gemm&>(g) = dw;
         g.p = second ? dw.p2 : dw.p;
         g.out = second ? dw.out2 : dw.out;
         g.ldo = second ? dw.ldo2 : dw.ldo;
@@ -223,14 +226,8 @@ hipError_t launch_grad_parts(const TwinGemm& dw, const GemmPlan& p, const TwiceG
             <<<blocks, kThreads<256>, 0, st>>>(dw, a, dx, b, bias[0], bias[1]);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && DX) e = launch_join(dx, q.splits, st);
-    if (e != hipSuccess || !DW || p.splits <= 1) return e;
-    Gemm one = dw;
-    e = launch_join(one, p.splits, st);
-    if (e != hipSuccess) return e;
-    one.out = dw.out2;
-    one.ldo = dw.ldo2;
-    one.part = dw.part + (int64_t)p.splits * dw.I * part_ld(dw.J);
-    return launch_join(one, p.splits, st);
+    if (e == hipSuccess && DW) e = launch_join(dw, p.splits, st, dw.out2, dw.ldo2);
+    return e;
 }
 template <class T>
 hipError_t launch_grad_of(const TwinGemm& dw, const GemmPlan& p, const TwiceGemm& dx,

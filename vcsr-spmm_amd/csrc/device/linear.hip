@@ -289,6 +289,11 @@ PairPlan plan_grad(const TwinGemm& dw, const TwiceGemm& dx) {
         p.dw = plan_of(w, nullptr, false);
     else
         p.dx = plan_of(x, nullptr, false);
+    // Whole products in tiles of one size are one launch: 8192 x 2048 x 4096 bf16 565 us,
+    // 574 in two.
+    if (dw.out && dx.out && !forced.plan.tile && p.dw.tile == p.dx.tile && p.dw.splits == 1 &&
+        p.dx.splits == 1)
+        p.together = true;
     p.dw.rows = dw.I;
     p.dx.rows = dx.I;
     return p;

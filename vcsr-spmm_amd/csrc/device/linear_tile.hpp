@@ -475,14 +475,17 @@ struct Place {
     int64_t i0, j0;
     uint32_t split;
 };
-template <int TI, int TJ>
+template <int TI, int TJ, bool PCOLS>
 __device__ __forceinline__ Place place_of(const Gemm& g, uint32_t block, uint32_t blocks,
                                           uint32_t splits) {
     constexpr uint32_t kBand = 4;
     const uint32_t ti = (uint32_t)((g.I + TI - 1) / TI);
     const uint32_t tj = (uint32_t)(((int64_t)g.J + TJ - 1) / TJ);
     const uint32_t b = xcd_remap(block, blocks);
-    const uint32_t split = b % splits, t = b / splits;
+    // dw's parts of the sum are many and its tiles few: the tiles of one part, which read
+    // the same rows of both operands, go together.
+    const uint32_t split = PCOLS ? b / (ti * tj) : b % splits;
+    const uint32_t t = PCOLS ? b % (ti * tj) : b / splits;
     const uint32_t band = t / (kBand * ti), in_band = t - band * (kBand * ti);
     const uint32_t width = tj - band * kBand < kBand ? tj - band * kBand : kBand;
     return Place{(int64_t)(in_band / width) * TI, (int64_t)(band * kBand + in_band % width) * TJ,
@@ -724,6 +727,10 @@ struct Sides {
                        extent<T>(g.I, g.R, g.ldp, PCOLS)};
         q[0] = Operand{(const uint8_t*)g.q, g.ldq * size, J, j0, extent<T>(J, g.R, g.ldq, QCOLS)};
         if constexpr (TWICE) {
+            if (g.whole) {  // the zeros behind the last row too
+                constexpr int64_t BK = kStepBytes / size;
+                p[0].bytes = extent<T>(g.I, (g.R + BK - 1) / BK * BK, g.ldp, false);
+            }
             p[1] = p[0];
             p[1].p = (const uint8_t*)g.p2;
         }
@@ -758,7 +765,13 @@ struct Steps {
             return;
         }
         const int64_t all = (g.R + BK - 1) / BK;
-        const bool ragged = ragged_end<T>(g, g.R, p_cols, q_cols);
+        // Where P has zeros behind R, so has Q: what lies past its last row is past the
+        // descriptor's range, which is told dword by dword.  Only a last row that ends
+        // inside one would lose its last value.
+        bool ragged;
+        if constexpr (TWICE)
+            ragged = g.whole ? sizeof(T) == 2 && g.J % 2 != 0
+                             : ragged_end<T>(g, g.R, p_cols, q_cols);
         const int64_t whole = ragged ? all - 1 : all;
         const int64_t b = (int64_t)split * steps, e = b + steps < 2 * all ? b + steps : 2 * all;
         auto clamp = [&](int64_t t) { return t < 0 ? 0 : t < whole ? t : whole; };
@@ -791,9 +804,10 @@ struct Part {
 // where there are too few blocks to hide a trip to memory otherwise.
 template <int TILE, int STAGES>
 constexpr int kLds = STAGES * 2 * TILE * kStepBytes;
-template <class T, int TI, int TJ, int WI, int WJ, int STAGES, bool PCOLS, bool QCOLS, class G>
-__device__ __forceinline__ void gemm_shared(const G& g, const Part& part, uint32_t block,
-                                            uint8_t* lds0) {
+template <class T, int TI, int TJ, int WI, int WJ, int STAGES, bool PCOLS, bool QCOLS, bool ALL,
+          class G>
+__device__ __forceinline__ void gemm_shared(const G& g, const Part& part, const Place& at, int role,
+                                            int nx, int ny, uint8_t* lds0) {
     constexpr bool GATED = std::is_same<G, GatedGemm>::value;
     constexpr bool TWICE = std::is_same<G, TwiceGemm>::value;
     constexpr int NT = 64 * WI * WJ;
@@ -806,12 +820,11 @@ __device__ __forceinline__ void gemm_shared(const G& g, const Part& part, uint32
     using RQ = Reader<T, TJ, QCOLS, true>;
     constexpr int kStage = (TI + TJ) * kStepBytes;
     const int splits = part.splits;
-    const Place at = place_of<TI, TJ>(g, block, part.blocks, (uint32_t)splits);
     const Sides<T, G, PCOLS, QCOLS> o(g, at);
     const Steps<T, G> steps(g, part.steps, at.split, PCOLS, QCOLS);
 
     const int wave = uniform((int)(threadIdx.x >> 6));
-    const int ri = (wave / WJ) * (TI / WI), rj = (wave % WJ) * (TJ / WJ);
+    const int ri = (role / WJ) * (TI / WI), rj = (role % WJ) * (TJ / WJ);
     f32x4 acc[FI][FJ];
 #pragma unroll
     for (int x = 0; x < FI; ++x)
@@ -819,17 +832,21 @@ __device__ __forceinline__ void gemm_shared(const G& g, const Part& part, uint32
         for (int y = 0; y < FJ; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     auto multiply = [&](const uint8_t* lp, const uint8_t* lq) {
+        if (!ALL && nx == 0) return;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             Frag<T> p[FI];
 #pragma unroll
-            for (int x = 0; x < FI; ++x) p[x].set(RP::get(lp, ri, x, s));
+            for (int x = 0; x < FI; ++x)
+                if (ALL || x < nx) p[x].set(RP::get(lp, ri, x, s));
 #pragma unroll
             for (int y = 0; y < FJ; ++y) {
+                if (!ALL && y >= ny) break;
                 Frag<T> q;
                 q.set(RQ::get(lq, rj, y, s));
 #pragma unroll
-                for (int x = 0; x < FI; ++x) acc[x][y] = mma<T>(q, p[x], acc[x][y]);
+                for (int x = 0; x < FI; ++x)
+                    if (ALL || x < nx) acc[x][y] = mma<T>(q, p[x], acc[x][y]);
             }
         }
     };
@@ -904,6 +921,37 @@ __device__ __forceinline__ void gemm_shared(const G& g, const Part& part, uint32
                                     at.j0 + rj, splits, at.split);
 }
 
+// The gated products in FP32, which the matrix units bound, leave out a tile's blocks past
+// out's last row or column (ALL: there are none); which wave has which part goes round
+// with the block, so that the idle ones are not always the same SIMD's.  (The gradients
+// of 30011 x 130 x 257 156 us, 164 with all blocks.)  A block's waves may differ in ALL:
+// they meet at the same number of barriers.
+template <class T, int TI, int TJ, int WI, int WJ, int STAGES, bool PCOLS, bool QCOLS, class G>
+__device__ __forceinline__ void gemm_tile(const G& g, const Part& part, uint32_t block,
+                                          uint8_t* lds) {
+    constexpr bool GATED = std::is_same<G, GatedGemm>::value;
+    constexpr int FI = TI / WI / 16, FJ = TJ / WJ / 16;
+    const Place at = place_of<TI, TJ, PCOLS>(g, block, part.blocks, (uint32_t)part.splits);
+    const int wave = uniform((int)(threadIdx.x >> 6));
+    if constexpr (sizeof(T) < 4 || std::is_same<G, Gemm>::value) {
+        gemm_shared<T, TI, TJ, WI, WJ, STAGES, PCOLS, QCOLS, true>(g, part, at, wave, FI, FJ, lds);
+    } else {
+        const int role = (wave + (int)block) & (WI * WJ - 1);
+        // Blocks of the wave's part that out has: of 16 rows, and of 32 columns in two (a
+        // gated projection's 64 are 32).
+        const int64_t rows = g.I - at.i0 - role / WJ * (TI / WI);
+        const int64_t cols = g.J - at.j0 - role % WJ * (TJ / WJ);
+        const int nx = rows <= 0 || cols <= 0 ? 0 : rows < FI * 16 ? (int)((rows + 15) / 16) : FI;
+        const int ny = GATED || cols >= FJ * 16 ? FJ : (int)((cols + 31) / 32) * 2;
+        if (nx == FI && ny == FJ)
+            gemm_shared<T, TI, TJ, WI, WJ, STAGES, PCOLS, QCOLS, true>(g, part, at, role, nx, ny,
+                                                                      lds);
+        else
+            gemm_shared<T, TI, TJ, WI, WJ, STAGES, PCOLS, QCOLS, false>(g, part, at, role, nx, ny,
+                                                                       lds);
+    }
+}
+
 // 256 x 256 tiles, eight waves of 128 x 64, one block a compute unit.
 //
 // Two waves a SIMD take turns: while one multiplies, the other brings its next
@@ -934,7 +982,7 @@ __device__ __forceinline__ void gemm_turns(const G& g, const Part& part, uint32_
     using RQ = Reader<T, TJ, QCOLS, true>;
     static_assert(LQ::GR + 2 * LP::GR == kAhead, "loads of a step");
     const int splits = part.splits;
-    const Place at = place_of<TI, TJ>(g, block, part.blocks, (uint32_t)splits);
+    const Place at = place_of<TI, TJ, PCOLS>(g, block, part.blocks, (uint32_t)splits);
     const Sides<T, G, PCOLS, QCOLS> o(g, at);
     const Steps<T, G> steps(g, part.steps, at.split, PCOLS, QCOLS);
     const int n = steps.n;
@@ -1072,9 +1120,9 @@ __device__ __forceinline__ void gemm_block(const G& g, const Part& part, uint32_
         gemm_turns<T, PCOLS, QCOLS>(g, part, block, lds);
     else if constexpr (TILE == 64 && std::is_same<G, GatedGemm>::value)
         // A wave has 32 columns of each weight.
-        gemm_shared<T, TILE, TILE, 4, 1, STAGES, PCOLS, QCOLS>(g, part, block, lds);
+        gemm_tile<T, TILE, TILE, 4, 1, STAGES, PCOLS, QCOLS>(g, part, block, lds);
     else
-        gemm_shared<T, TILE, TILE, 2, 2, STAGES, PCOLS, QCOLS>(g, part, block, lds);
+        gemm_tile<T, TILE, TILE, 2, 2, STAGES, PCOLS, QCOLS>(g, part, block, lds);
 }
 template <int TILE>
 constexpr int kThreads = TILE == 256 ? 512 : 256;
@@ -1124,9 +1172,16 @@ __global__ __launch_bounds__(kThreads<TILE>) void gemm_pair_kernel(Gemm dw, Part
 }
 
 // The partial sums of a split product and the epilogue, for few parts: a thread
-// adds those of 8 columns in order.
+// adds those of 8 columns in order.  blockIdx.y: of two products of one size, the first
+// or the one whose sums begin `next` behind its own and whose out is out2.
 template <class O>
-__global__ __launch_bounds__(256) void gemm_join_few_kernel(Gemm g, int splits) {
+__global__ __launch_bounds__(256) void gemm_join_few_kernel(Gemm g, int splits, void* out2,
+                                                            int64_t ldo2, int64_t next) {
+    if (blockIdx.y) {
+        g.part += next;
+        g.out = out2;
+        g.ldo = ldo2;
+    }
     const int64_t ld = part_ld(g.J);
     const uint32_t per_row = (uint32_t)(ld / 8);
     const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -1156,8 +1211,14 @@ __global__ __launch_bounds__(256) void gemm_join_few_kernel(Gemm g, int splits) 
 // eight in order: with few columns of out the parts' loads are what there is to
 // run at once.
 template <class O>
-__global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits) {
+__global__ __launch_bounds__(256) void gemm_join_kernel(Gemm g, int splits, void* out2, int64_t ldo2,
+                                                        int64_t next) {
     __shared__ float lds[8][32][9];
+    if (blockIdx.y) {
+        g.part += next;
+        g.out = out2;
+        g.ldo = ldo2;
+    }
     const int64_t ld = part_ld(g.J);
     const uint32_t per_row = (uint32_t)(ld / 8);
     const int at = threadIdx.x & 31, grp = threadIdx.x >> 5;
@@ -1305,20 +1366,24 @@ inline Part part_of(const Gemm& g, const GemmPlan& p) {
     return Part{p.splits, p.steps, (uint32_t)(tiles * p.splits)};
 }
 
-inline hipError_t launch_join(const Gemm& g, int splits, hipStream_t st) {
+// out2: of the second of two products, whose partial sums lie behind the first's.
+inline hipError_t launch_join(const Gemm& g, int splits, hipStream_t st, void* out2 = nullptr,
+                              int64_t ldo2 = 0) {
     if (splits <= 1) return hipSuccess;
+    const unsigned pair = out2 ? 2 : 1;
+    const int64_t next = (int64_t)splits * g.I * part_ld(g.J);
     const int64_t vectors = g.I * (part_ld(g.J) / 8);
     const unsigned few = (unsigned)((vectors + 255) / 256), many = (unsigned)((vectors + 31) / 32);
     if (g.out_type == VCSR_BF16) {
         if (splits < 8)
-            gemm_join_few_kernel<bf16><<<few, 256, 0, st>>>(g, splits);
+            gemm_join_few_kernel<bf16><<<dim3(few, pair), 256, 0, st>>>(g, splits, out2, ldo2, next);
         else
-            gemm_join_kernel<bf16><<<many, 256, 0, st>>>(g, splits);
+            gemm_join_kernel<bf16><<<dim3(many, pair), 256, 0, st>>>(g, splits, out2, ldo2, next);
     } else {
         if (splits < 8)
-            gemm_join_few_kernel<float><<<few, 256, 0, st>>>(g, splits);
+            gemm_join_few_kernel<float><<<dim3(few, pair), 256, 0, st>>>(g, splits, out2, ldo2, next);
         else
-            gemm_join_kernel<float><<<many, 256, 0, st>>>(g, splits);
+            gemm_join_kernel<float><<<dim3(many, pair), 256, 0, st>>>(g, splits, out2, ldo2, next);
     }
     return hipGetLastError();
 }
