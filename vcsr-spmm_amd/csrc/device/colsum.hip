@@ -1,5 +1,6 @@
 // colsum.hip - what the gradients sum over rows, in a fixed order: the partial
 // rows of dweight and dbias, and dz = dy * act'(z) with the sums of its rows.
+#include "common.hpp"
 #include "dense.hpp"
 
 namespace vcsr {
@@ -17,7 +18,8 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* part, int32
         out = out2;
     }
     const int col = threadIdx.x & 15, grp = threadIdx.x >> 4;
-    const int64_t c = (int64_t)blockIdx.x * 16 + col;
+    // Neighbouring blocks, which share lines, on one XCD.
+    const int64_t c = (int64_t)xcd_remap(blockIdx.x, gridDim.x) * 16 + col;
     float t = 0.f;
     if (c < C) {
 #pragma unroll 8

@@ -117,6 +117,46 @@ __device__ __forceinline__ void store_row(T* row, int lane, int stride, int C,
     }
 }
 
+// The same as it lies in memory, so that a row can be under way while the one before it is
+// worked on.
+template <class T, int NV, int V>
+struct RawRow {
+    Mem<T, V> m[NV];
+    __device__ __forceinline__ static int back_of(int lane, int stride, int C) {
+        const int c = ((NV - 1) * stride + lane) * V;
+        return c + V > C ? c + V - C : 0;
+    }
+    __device__ __forceinline__ void load(const T* row, int lane, int stride, int C) {
+#pragma unroll
+        for (int k = 0; k + 1 < NV; ++k) m[k] = *(const Mem<T, V>*)(row + (k * stride + lane) * V);
+        const int back = back_of(lane, stride, C);
+        m[NV - 1] = *(const Mem<T, V>*)(row +
+                                        (back < V ? ((NV - 1) * stride + lane) * V - back : 0));
+    }
+    // Its values, zeros past the row's end.
+    __device__ __forceinline__ void get(int lane, int stride, int C, float (&v)[NV][V]) const {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[k][i] = to_f32(m[k].v[i]);
+        const int back = back_of(lane, stride, C);
+        if (C % V == 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[NV - 1][i] = back ? 0.f : v[NV - 1][i];
+            return;
+        }
+#pragma unroll
+        for (int s = 1; s < V; s <<= 1)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float next = i + s < V ? v[NV - 1][i + s < V ? i + s : i] : 0.f;
+                v[NV - 1][i] = back & s ? next : v[NV - 1][i];
+            }
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[NV - 1][i] = back >= V ? 0.f : v[NV - 1][i];
+    }
+};
+
 // A launch has fewer than 2^32 threads: more rows than that, at `threads` each, go
 // in several.  launch(first, count) takes whole blocks of at most 256 rows.
 template <class F>
