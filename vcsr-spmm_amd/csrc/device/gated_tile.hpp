@@ -124,12 +124,12 @@ template <class T, class O>
 hipError_t launch_gated_rows(const GatedGemm& g, hipStream_t st) {
     const unsigned blocks = (unsigned)(((int64_t)g.J / 2 + 7) / 8);
     const int64_t lines = (g.R * (int64_t)sizeof(T) + 127) / 128;
+    // Two blocks of four lines a unit rather than one of eight: 1 x 4096 x 8192 bf16 25.3
+    // us (5.3 TB/s) against 30.7, 1 x 4096 x 1024 7.4 against 7.1.
     if (lines <= 16)
         gated_rows_kernel<T, O, 2><<<blocks, 512, 0, st>>>(g);
-    else if (lines <= 32)
-        gated_rows_kernel<T, O, 4><<<blocks, 512, 0, st>>>(g);
     else
-        gated_rows_kernel<T, O, 8><<<blocks, 512, 0, st>>>(g);
+        gated_rows_kernel<T, O, 4><<<blocks, 512, 0, st>>>(g);
     return hipGetLastError();
 }
 
