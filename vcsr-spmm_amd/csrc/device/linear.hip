@@ -142,7 +142,7 @@ GemmPlan plan_of(const Gemm& g, float* us_out = nullptr, bool may_divide = true)
     // few blocks would read long rows alone, past what a wave asks for at once: 512 x
     // 8000 bf16 16 us against 10.
     if (g.I <= 8 && !g.p_cols && !g.q_cols && (g.J >= 2048 || g.R * size <= 64 * 128) &&
-        g.J < 1 << 27) {  // 32 threads a column, and fewer than 2^32 a launch
+        g.J <= (1 << 27) - 16) {  // blocks of 16 columns, fewer than 2^23 of 512 threads
         if (us_out) *us_out = 7.f;
         return GemmPlan{16, 1, 1, steps_of(g), g.I};
     }
