@@ -424,7 +424,7 @@ typedef struct {
     void* y;             int64_t ldy;   /* may be x or residual itself, if of
                                            one type                          */
     float* y_scale;      /* M, for VCSR_FP8 (NULL otherwise)                 */
-    float* mean;         /* NULL, or M: mean(t)                              */
+    float* mean;         /* NULL, or M: mean(t); another vector than rstd    */
     float* rstd;         /* NULL, or M: 1 / sqrt(variance + eps)             */
 } vcsr_layernorm_args;
 int vcsr_layernorm(const vcsr_layernorm_args* args, void* stream, float* ms);

@@ -22,6 +22,7 @@ NORM = {
     "misaligned bias": dict(bias=mat(8, ptr=4098)),
     "short mean": dict(mean=mat(3)),
     "misaligned mean": dict(mean=mat(4, ptr=4097)),
+    "mean over rstd": dict(mean=mat(4, ptr=A), rstd=mat(4, ptr=A)),
     "misaligned rstd": dict(rstd=mat(4, ptr=4097)),
     "stride under the row": dict(x=mat(4, 8, ld=6, nbytes=4096)),
     "x too short for its stride": dict(x=mat(4, 8, ld=64, nbytes=128)),

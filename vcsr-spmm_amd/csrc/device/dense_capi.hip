@@ -98,6 +98,8 @@ vcsr_layernorm_args checked(const vcsr_layernorm_args* args) {
     check_norm(a);
     check_vector(a.bias, "bias: alignment", true);
     check_vector(a.mean, "mean: alignment", true);
+    need(!a.mean || (a.mean != a.rstd && a.mean != a.y_scale),
+         "mean: another vector than rstd and y_scale");
     return a;
 }
 
