@@ -289,10 +289,16 @@ PairPlan plan_grad(const TwinGemm& dw, const TwiceGemm& dx) {
         p.dw = plan_of(w, nullptr, false);
     else
         p.dx = plan_of(x, nullptr, false);
+    // Room for the sums of dbias and for dw's halves rounded up, which come to fewer blocks.
+    auto room = [](int64_t blocks, int tile) { return launches(blocks + (1 << 18), tile); };
+    const int64_t blocks_w = p.dw.splits > 0 ? tiles_of(w, p.dw.tile) * p.dw.splits : 0;
+    const int64_t blocks_x = p.dx.splits > 0 ? tiles_of(x, p.dx.tile) * p.dx.splits : 0;
+    if (!p.together && !room(blocks_w, p.dw.tile)) p.dw.splits = 0;
+    if (!p.together && !room(blocks_x, p.dx.tile)) p.dx.splits = 0;
     // Whole products in tiles of one size are one launch: 8192 x 2048 x 4096 bf16 565 us,
     // 574 in two.
-    if (dw.out && dx.out && !forced.plan.tile && p.dw.tile == p.dx.tile && p.dw.splits == 1 &&
-        p.dx.splits == 1)
+    if (!forced.plan.tile && p.dw.tile == p.dx.tile && p.dw.splits == 1 && p.dx.splits == 1 &&
+        room(blocks_w + blocks_x, p.dw.tile))
         p.together = true;
     p.dw.rows = dw.I;
     p.dx.rows = dx.I;
@@ -321,7 +327,7 @@ size_t gated_grad_workspace(const TwinGemm& dw, const TwiceGemm& dx) {
 }
 hipError_t launch_gated_grad(const TwinGemm& dw, const TwiceGemm& dx, const RowSum (&bias)[2],
                              hipStream_t st) {
-    PairPlan p = plan_grad(dw, dx);
+    const PairPlan p = plan_grad(dw, dx);
     const RowSum none[2] = {};
     auto go = [&](bool w, bool x, const RowSum(&sums)[2]) {
         GemmPlan a = p.dw, b = p.dx;
