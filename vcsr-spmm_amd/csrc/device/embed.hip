@@ -9,6 +9,11 @@
 // are the work of the chunk they start in, also past its end; longer ones (a few
 // tokens make up much of a text) are added chunk by chunk, and their partial rows by
 // another launch, in order.
+// Memory bounds the lookup (65536 tokens of 2048 bf16 60 us: 5.6 TB/s with each row of the
+// table that has a token read once) and most of the gradient (32768 tokens of 2048 bf16
+// to 32768 x 2048 FP32 107 us: the sort 23 in four launches, the sums with the zeros 81,
+// the join 5).  5001 tokens of 257 FP32, added, are three launches one after the other, 19.8 us:
+// rank 7, sums 9, join 4.
 #include "common.hpp"
 #include "dense.hpp"
 #include "launch.hpp"
@@ -175,6 +180,8 @@ void launch_ends(const vcsr_embed_args& a, hipStream_t st) {
                 embed_kernel<X, Y, ENDS, NV, U, false><<<grid, 256, 0, st>>>(b, lanes);
         }
     };
+    // Loads of a lane: of long rows (2048 bf16, 65536 tokens) four of one row 58 us, two of
+    // two 70, one of four 65; of short ones (256) 12, 9.6 and 9.2.
     if (nv > 128)
         go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
     else if (nv > 64)
@@ -247,7 +254,8 @@ __device__ __forceinline__ void zero_rows(const Zeros& z, int64_t wave, int64_t 
 }
 // Few tokens: each one's place is the number of tokens before it.  All keys go to LDS; a
 // block takes 16 tokens, a lane one of them and a thirty-second of the keys, and LDS adds
-// the parts.
+// the parts.  Comparisons bound it, n * n of them: the whole gradient of 4000 tokens of 512
+// bf16 is 16 us (by digits, below, 31), of 12000 33 (41), of 16000 more than by digits.
 constexpr int kMostRanked = 12288;
 __global__ __launch_bounds__(512) void rank_kernel(const int32_t* __restrict__ ids, int32_t n,
                                                    int32_t V, int32_t* __restrict__ keys,
@@ -641,7 +649,8 @@ Shape shape_of(const vcsr_embed_grad_args& a) {
     s.runs.width = (int)((nv + slabs - 1) / slabs);
     s.runs.E = 64;
     s.runs.ldp = nv * v;
-    // Enough waves to have the chip's loads under way.
+    // Enough waves to have the chip's loads under way: 4000 tokens of 512 bf16 with E = 8
+    // 16 us, 16 20, 64 40; of 130000 E = 32 and 64 are alike.
     while (s.runs.E > 8 && a.M / s.runs.E * slabs < 2048) s.runs.E /= 2;
     s.runs.chunks = (a.M + s.runs.E - 1) / s.runs.E;
     if (a.M <= 64) return s;

@@ -9,7 +9,7 @@
 // over the rows a block takes in registers, then over the blocks (colsum.hip),
 // in a fixed order.  All of it is bound by memory: 32768 x 4096 bf16 with a residual
 // to e4m3 163 us (5.8 TB/s), 62451 x 128 FP32 28 us (4.6 TB/s), the gradient of
-// 16384 x 2050 bf16 68 us (3.9 TB/s), of 32768 x 4096 217 us (4.9 TB/s).
+// 16384 x 2050 bf16 67 us (4.0 TB/s), of 32768 x 4096 217 us (4.9 TB/s).
 #include "dense.hpp"
 #include "norm_rows.hpp"
 
