@@ -288,6 +288,19 @@ def test_gated_gradient_sizes(gpu, size):
     grad_once(gpu, gpu.Stream(), np.random.default_rng(8), M, N, K, kind, kind, "gelu")
 
 
+# Few rows: dx's long sum is split, dw is whole, and both are one launch.
+FEW_ROWS = [(1, 2752, 64, "bf16"), (9, 1551, 384, "f32"), (10, 603, 1780, "f32"),
+            (84, 6272, 64, "bf16"), (239, 1536, 64, "f32")]
+
+
+@pytest.mark.parametrize("size", FEW_ROWS, ids=lambda s: "x".join(map(str, s)))
+def test_gated_gradient_of_few_rows(gpu, size):
+    M, N, K, kind = size
+    together, tile_w, splits_w, tile_x, splits_x = gated_grad_plan(gpu, M, N, K, kind)
+    assert together and tile_w == tile_x and splits_w == 1 and splits_x > 1
+    grad_once(gpu, gpu.Stream(), np.random.default_rng(23), M, N, K, kind, kind, "gelu")
+
+
 def test_gated_grad_against_differences(gpu):
     """The directional derivative of <dy, y> along a random direction of all inputs."""
     vs, st = gpu, gpu.Stream()

@@ -295,9 +295,12 @@ PairPlan plan_grad(const TwinGemm& dw, const TwiceGemm& dx) {
     const int64_t blocks_x = p.dx.splits > 0 ? tiles_of(x, p.dx.tile) * p.dx.splits : 0;
     if (!p.together && !room(blocks_w, p.dw.tile)) p.dw.splits = 0;
     if (!p.together && !room(blocks_x, p.dx.tile)) p.dx.splits = 0;
-    // Whole products in tiles of one size are one launch: 8192 x 2048 x 4096 bf16 565 us,
-    // 574 in two.
-    if (!forced.plan.tile && p.dw.tile == p.dx.tile && p.dw.splits == 1 && p.dx.splits == 1 &&
+    // Products in tiles of one size, of which one at most is split (the partial sums share
+    // the workspace), are one launch: 8192 x 2048 x 4096 bf16 565 us, 574 in two; 9 x 384 x
+    // 1551 FP32 with dx split 17, 21 in two; 500 x 1000 x 1500 bf16 42 and 46.
+    const bool shared = (p.dw.splits == 1 && p.dx.splits > 0) ||
+                        (p.dx.splits == 1 && p.dw.splits > 0);
+    if (!forced.plan.tile && p.dw.tile == p.dx.tile && shared &&
         room(blocks_w + blocks_x, p.dw.tile))
         p.together = true;
     p.dw.rows = dw.I;
