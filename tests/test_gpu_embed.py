@@ -165,6 +165,19 @@ def test_embed_grad_distributions(gpu, kind, M):
         assert one.tobytes() == two.tobytes()
 
 
+@pytest.mark.parametrize("C", [1, 3, 7, 8, 9, 40, 63, 64, 65, 255, 256, 500, 511, 513, 4100])
+@pytest.mark.parametrize("tk", ["f32", "bf16"])
+def test_embed_grad_clears_rows(gpu, tk, C):
+    """Rows shorter and longer than a wave's pieces, most of them without a token, in
+    whole groups and a last one of fewer."""
+    st, rng = gpu.Stream(), np.random.default_rng(C)
+    for n, (M, V) in enumerate([(20, 1000), (90, 1024), (13000, 641), (3, 63), (66, 65)]):
+        pad, off = ((0, 0), (8, 0), (3, 1))[n % 3]
+        print(f"embed grad clears {tk} C={C} M={M} V={V} pad={pad}", flush=True)
+        ids = rng.choice(np.array([0, 1, V // 2, V - 1, V, -1]), M).astype(np.int32)
+        grad_once(gpu, st, rng, M, V, C, "bf16", tk, ids, False, pad, off)
+
+
 @pytest.mark.parametrize("V", [1, 2, 255, 256, 511, 512, 513, 1023, 1024, 262143, 262144, 300000])
 def test_embed_grad_digits(gpu, V):
     """Tables of one, two and three digits' rows, at both ends of each."""
