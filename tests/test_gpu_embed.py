@@ -66,6 +66,46 @@ def test_embed(gpu, kinds, C):
         assert not Y.values()[~inside].any()
 
 
+@pytest.mark.parametrize("C", [2, 4, 5, 6, 7, 9, 12, 13, 20, 31])
+@pytest.mark.parametrize("kinds", FORWARD)
+def test_embed_of_narrow_rows(gpu, kinds, C):
+    """Around the vectors of 4, 8 and 16 values that the pairs of types have."""
+    xk, yk = kinds.split()
+    vs, st, rng = gpu, gpu.Stream(), np.random.default_rng(C)
+    for M, V, pad, off in ((3, 2, 0, 0), (300, 50, 1, 1), (65, 7, 4, 3)):
+        table, ids = values(rng, (V, C), xk), tokens(rng, M, V, "uniform")
+        ts = np.full(V, 0.5, np.float32) if xk == "fp8" else None
+        T, Y = Mat(vs, st, table, xk, pad, off), Mat(vs, st, None, yk, pad, 2 * off, (M, C))
+        vs.run_embed_gpu(T.view, ints(vs, st, ids), Y.view, scale=2.0,
+                         table_scale=vector(vs, st, ts) if ts is not None else None, stream=st)
+        st.sync()
+        want = table * (1 if ts is not None else 2)  # exact in FP32
+        inside = (ids >= 0) & (ids < V)
+        want = np.where(inside[:, None], want[np.where(inside, ids, 0)], 0)
+        close(Y.values(), want, rounding(want, yk), f"{kinds} {M}x{C}")
+
+
+@pytest.mark.parametrize("kinds", FORWARD)
+def test_embed_of_a_large_result(gpu, kinds):
+    """128 MB of y and more, which go past the caches; whole rows and others."""
+    xk, yk = kinds.split()
+    vs, st, rng = gpu, gpu.Stream(), np.random.default_rng(6)
+    V, M = 3000, 1 << 17
+    for C in (512, 516, 509) if yk == "bf16" else (256, 260, 253):
+        table = values(rng, (V, C), "fp8" if xk == "fp8" else "bf16")  # exact in y's type
+        ids = tokens(rng, M, V, "uniform")
+        ts = np.ones(V, np.float32) if xk == "fp8" else None
+        y = vs.DeviceArray((M, C), vs.BF16 if yk == "bf16" else np.float32)
+        print(f"embed {kinds} of {M} x {C}", flush=True)
+        vs.run_embed_gpu(Mat(vs, st, table, xk).view, ints(vs, st, ids), y,
+                         table_scale=vector(vs, st, ts) if ts is not None else None, stream=st)
+        st.sync()
+        inside = (ids >= 0) & (ids < V)
+        rows = np.vstack([table, np.zeros((1, C))]).astype(np.float32)
+        want = (vs.to_bf16(rows) if yk == "bf16" else rows)[np.where(inside, ids, V)]
+        assert np.array_equal(y.numpy(st), want)
+
+
 def test_embed_keeps_what_is_not_finite(gpu):
     """NaN and infinities in the table's rows; a row of zeros for padding whatever row 0
     holds."""
