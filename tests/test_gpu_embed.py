@@ -205,6 +205,16 @@ def test_embed_grad_distributions(gpu, kind, M):
         assert one.tobytes() == two.tobytes()
 
 
+@pytest.mark.parametrize("M", [12288, 12289, 12800, 12801, 16384, 16385, 65536, 65537, 131072,
+                               131073, 262145, 524288, 524289])
+def test_embed_grad_tiles(gpu, M):
+    """Numbers of tokens at both ends of the sort's tiles and of their number."""
+    st, rng = gpu.Stream(), np.random.default_rng(M)
+    for V, kind in ((40, "runs"), (70000, "frequent")):
+        print(f"embed grad tiles M={M} V={V}", flush=True)
+        grad_once(gpu, st, rng, M, V, 4, "f32", "f32", tokens(rng, M, V, kind), False)
+
+
 @pytest.mark.parametrize("C", [1, 3, 7, 8, 9, 40, 63, 64, 65, 255, 256, 500, 511, 513, 4100])
 @pytest.mark.parametrize("tk", ["f32", "bf16"])
 def test_embed_grad_clears_rows(gpu, tk, C):

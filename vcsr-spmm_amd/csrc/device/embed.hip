@@ -11,7 +11,7 @@
 // another launch, in order.
 // Memory bounds the lookup (65536 tokens of 2048 bf16 60 us: 5.6 TB/s with each row of the
 // table that has a token read once) and most of the gradient (32768 tokens of 2048 bf16
-// to 32768 x 2048 FP32 107 us: the sort 23 in four launches, the sums with the zeros 81,
+// to 32768 x 2048 FP32 105 us: the sort 20 in four launches, the sums with the zeros 80,
 // the join 5).  5001 tokens of 257 FP32, added, are three launches one after the other, 19.8 us:
 // rank 7, sums 9, join 4.
 #include "common.hpp"
@@ -271,9 +271,9 @@ __device__ __forceinline__ void zero_piece(uint8_t* p, int64_t bytes, int64_t i)
 // which: the first launch writes to owner[v] some token of id v, so that a row has one if
 // its owner is a token of its id; what else lies there does not matter, and nothing has
 // to be cleared first.  They are cleared beside the sums, past the caches where they are
-// many (`large`): 32768 tokens and 32768 x 2048 FP32 take 107 us, 120 through the caches
-// (with dy's loads past them too 123); clearing every row beside the sort and writing
-// some again 131.
+// many (`large`): 32768 tokens and 32768 x 2048 FP32 take 105 us, 13 more with the zeros
+// through the caches, 11 more with dy's loads through them, 24 more with every row cleared
+// beside the sort and some written again.
 struct Zeros {
     uint8_t* p;
     int64_t ld, bytes;  // of a row
@@ -288,7 +288,7 @@ __host__ __device__ constexpr int64_t zero_group(int64_t bytes) {
 }
 // Waves take groups of up to 64 rows, a lane a row to see which have a token (`met`).  Of
 // rows that are shorter than 64 pieces the lanes take several at a time: 13307 tokens of 33
-// FP32 to 32517 rows of bf16 are 38 us, 72 one row after the other.
+// FP32 to 32517 rows of bf16 are 30 us, 34 more one row after the other.
 template <bool LARGE, class F>
 __device__ __forceinline__ void zero_rows(const Zeros& z, int64_t wave, int64_t waves, F&& met) {
     const int lane = threadIdx.x & 63;
@@ -319,7 +319,7 @@ __device__ __forceinline__ void zero_rows(const Zeros& z, int64_t wave, int64_t 
 // Few tokens: each one's place is the number of tokens before it.  All keys go to LDS; a
 // block takes 16 tokens, a lane one of them and a thirty-second of the keys, and LDS adds
 // the parts.  Comparisons bound it, n * n of them: the whole gradient of 4000 tokens of 512
-// bf16 is 16 us (by digits, below, 31), of 12000 33 (41), of 16000 more than by digits.
+// bf16 is 16 us (by digits, below, 30), of 12000 33 (by digits 34 at 12500).
 constexpr int kMostRanked = 12288;
 __global__ __launch_bounds__(512) void rank_kernel(const int32_t* __restrict__ ids, int32_t n,
                                                    int32_t V, int32_t* __restrict__ keys,
@@ -373,7 +373,10 @@ __global__ __launch_bounds__(512) void rank_kernel(const int32_t* __restrict__ i
 // More: by digits of up to 9 bits, the lowest first, two launches each.  A block takes a
 // tile of `tile` keys in a row, each of its 4 waves a quarter; `pos` is null for the
 // first digit, whose keys are the ids themselves.
-constexpr int kDigits = 512;
+// The blocks' counts are read kTogether at a time, all under way together: rows of zeros
+// go up to a multiple of them (13 blocks: 39 us a gradient, 43 with a loop of its own for
+// those).
+constexpr int kDigits = 512, kTogether = 16;
 struct Radix {
     const int32_t *keys, *pos;
     int32_t n, V, tile, shift, digits;
@@ -398,6 +401,9 @@ __global__ __launch_bounds__(256) void digit_count_kernel(Radix r, int32_t* coun
     __syncthreads();
     for (int d = threadIdx.x; d < r.digits; d += 256)
         counts[(int64_t)blockIdx.x * r.digits + d] = lds[d];
+    if (blockIdx.x + 1 < gridDim.x) return;
+    for (int32_t b = gridDim.x; b % kTogether; ++b)
+        for (int d = threadIdx.x; d < r.digits; d += 256) counts[(int64_t)b * r.digits + d] = 0;
 }
 __global__ __launch_bounds__(256) void digit_place_kernel(Radix r, const int32_t* counts,
                                                           int32_t* keys, int32_t* pos) {
@@ -409,14 +415,15 @@ __global__ __launch_bounds__(256) void digit_place_kernel(Radix r, const int32_t
     // Digits [2 tid, 2 tid + 2): how many keys of them there are, and in blocks before.
     int32_t all[2] = {0, 0}, before[2] = {0, 0};
     if (2 * tid < r.digits) {
-#pragma unroll 16
-        for (int32_t b = 0; b < (int32_t)gridDim.x; ++b) {
-            const int2 c = *(const int2*)(counts + (int64_t)b * r.digits + 2 * tid);
-            all[0] += c.x;
-            all[1] += c.y;
-            before[0] += b < (int32_t)blockIdx.x ? c.x : 0;
-            before[1] += b < (int32_t)blockIdx.x ? c.y : 0;
-        }
+        for (int32_t b0 = 0; b0 < (int32_t)gridDim.x; b0 += kTogether)
+#pragma unroll
+            for (int32_t b = b0; b < b0 + kTogether; ++b) {
+                const int2 c = *(const int2*)(counts + (int64_t)b * r.digits + 2 * tid);
+                all[0] += c.x;
+                all[1] += c.y;
+                before[0] += b < (int32_t)blockIdx.x ? c.x : 0;
+                before[1] += b < (int32_t)blockIdx.x ? c.y : 0;
+            }
     }
     const int32_t two = all[0] + all[1], scan = wave_inclusive_scan(two, lane);
     if (lane == 63) sums[wave] = scan;
@@ -728,10 +735,13 @@ Shape shape_of(const vcsr_embed_grad_args& a) {
     s.passes = (bits + 8) / 9;
     s.bits = (bits + s.passes - 1) / s.passes;
     if (s.passes > 1) s.arrays = 4;
-    s.tile = 1024;
-    while ((a.M + s.tile - 1) / s.tile > 128) s.tile *= 2;
+    // A short tile's 64 keys a turn against as many counts to read: 24000 tokens 41.8 us,
+    // 45 with tiles from 1024; 130000 90, 94 with 256 blocks; 400000 171, 181 with 128.
+    s.tile = 512;
+    while ((a.M + s.tile - 1) / s.tile > (s.tile < 2048 ? 128 : 256)) s.tile *= 2;
     s.tiles = (a.M + s.tile - 1) / s.tile;
-    s.counts = round_up((size_t)s.tiles << s.bits << 2);
+    const int64_t rows = (s.tiles + kTogether - 1) / kTogether * kTogether;
+    s.counts = round_up((size_t)rows << s.bits << 2);
     return s;
 }
 
