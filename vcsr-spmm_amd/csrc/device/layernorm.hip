@@ -336,7 +336,9 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void layernorm_grad_kerne
             const float* const w = w_lds + (k * stride + lane) * V;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                s[k][i] = (s[k][i] - mean) * rstd;  // h
+                // h, past the row's end zero: -mean * rstd may be infinite there.
+                const bool in = k + 1 < NV || (k * stride + lane) * V + i < a.C;
+                s[k][i] = in ? (s[k][i] - mean) * rstd : 0.f;
                 if (WPR == 1 && !live) s[k][i] = d[k][i] = 0.f;
                 dw[k][i] = __builtin_fmaf(d[k][i], s[k][i], dw[k][i]);
                 db[k][i] += d[k][i];
