@@ -295,7 +295,9 @@ __device__ __forceinline__ void zero_rows(const Zeros& z, int64_t wave, int64_t 
     const int64_t most = zero_group(z.bytes), pieces = (z.bytes + 15) / 16;
     for (int64_t r0 = wave * most; r0 < z.rows; r0 += waves * most) {
         const int rows = z.rows - r0 < most ? (int)(z.rows - r0) : (int)most;
-        const uint64_t kept = __ballot(lane < rows && met(lane < rows ? r0 + lane : r0));
+        // With all lanes: met reads other lanes' tokens.
+        const bool has = met(lane < rows ? r0 + lane : r0);
+        const uint64_t kept = __ballot(lane < rows && has);
         if (!kept && z.ld == z.bytes) {
             for (int64_t i = lane; 16 * i < rows * z.bytes; i += 64)
                 zero_piece<LARGE>(z.p + r0 * z.ld, rows * z.bytes, i);
@@ -574,7 +576,8 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, 
         k.key = __builtin_amdgcn_ds_permute(rank * 4, mine);
         pos = __builtin_amdgcn_ds_permute(rank * 4, lane);
         const int valid = __popcll(__ballot(k.key < a.V)), first = (int)chunk * r.E;
-        const uint64_t starts = __ballot(lane < valid && (lane == 0 || __shfl_up(k.key, 1) != k.key));
+        const int32_t previous = __shfl_up(k.key, 1);  // with all lanes, lane 1 reads lane 0
+        const uint64_t starts = __ballot(lane < valid && (lane == 0 || previous != k.key));
         // The first run that begins in a token from `at` on.
         auto start_from = [&](int at) {
             const uint64_t later = at < 64 ? starts >> at << at : 0;
