@@ -207,7 +207,10 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(vcsr_gated_grad_args a, X
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float z = g[u][i];
-                    g[u][i] = d[u][i] * w[u][i] * act_grad_f32<ACT>(z);
+                    // Where dy * z_up passes FP32's range both are over 1, and what act' (1.13
+                    // at most) brings back into it is formed by taking act' first.
+                    const float slope = act_grad_f32<ACT>(z), both = d[u][i] * w[u][i];
+                    g[u][i] = __builtin_isinf(both) ? d[u][i] * slope * w[u][i] : both * slope;
                     w[u][i] = d[u][i] * act_f32<ACT>(z);
                     if (ENDS == 0 || i < n) {
                         sum[0][i] += g[u][i];
