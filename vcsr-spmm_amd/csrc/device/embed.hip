@@ -35,15 +35,6 @@ __device__ __forceinline__ void widen(const u32x4& r, float (&v)[8], bf16) {
         v[2 * i + 1] = __builtin_bit_cast(float, r[i] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void widen(const u32x4& r, float (&v)[16], fp8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[4 * i] = fp8_to_f32<0>(r[i]);
-        v[4 * i + 1] = fp8_to_f32<1>(r[i]);
-        v[4 * i + 2] = fp8_to_f32<2>(r[i]);
-        v[4 * i + 3] = fp8_to_f32<3>(r[i]);
-    }
-}
 
 // Of 4 and 8 bytes.
 __device__ __forceinline__ void widen(uint32_t r, float (&v)[4], fp8) {
@@ -134,30 +125,19 @@ __device__ __forceinline__ auto load_bits(const T* row, int64_t c, int64_t C) {
 template <class X, class Y>
 constexpr int kForward = 16 / (int)(sizeof(X) > sizeof(Y) ? sizeof(X) : sizeof(Y));
 
-// Stores past the caches, of whole 16 bytes.
-template <int V>
-__device__ __forceinline__ void store_large(float* p, const float (&v)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4)
-        __builtin_nontemporal_store(
-            __builtin_bit_cast(u32x4, f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]}), (Any16*)(p + i));
+// Stores past the caches, of whole 16 bytes; of bf16's 8 (rows of FP32) through them.
+__device__ __forceinline__ void store_large(float* p, const float (&v)[4]) {
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}), (Any16*)p);
 }
-template <int V>
-__device__ __forceinline__ void store_large(bf16* p, const float (&v)[V]) {
-    if constexpr (V < 8) {
-        store_vec(p, V, v);
-    } else {
+__device__ __forceinline__ void store_large(bf16* p, const float (&v)[8]) {
+    Mem<bf16, 8> m;
 #pragma unroll
-        for (int i = 0; i < V; i += 8) {
-            Mem<bf16, 8> m;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) m.v[k] = (bf16)v[i + k];
-            u32x4 q;
-            __builtin_memcpy(&q, &m, 16);
-            __builtin_nontemporal_store(q, (Any16*)(p + i));
-        }
-    }
+    for (int k = 0; k < 8; ++k) m.v[k] = (bf16)v[k];
+    u32x4 q;
+    __builtin_memcpy(&q, &m, 16);
+    __builtin_nontemporal_store(q, (Any16*)p);
 }
+__device__ __forceinline__ void store_large(bf16* p, const float (&v)[4]) { store_vec(p, 4, v); }
 
 // Groups of `lanes` (a power of two <= 64) lanes take U rows each, of them NV vectors
 // a lane from blockIdx.y's slab on; all loads go out together.  The table's rows stay
