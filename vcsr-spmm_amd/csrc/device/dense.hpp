@@ -190,6 +190,12 @@ size_t layernorm_grad_workspace(const vcsr_layernorm_grad_args& a);
 hipError_t launch_embed(const vcsr_embed_args& a, hipStream_t st);
 hipError_t launch_embed_grad(const vcsr_embed_grad_args& a, hipStream_t st);
 size_t embed_grad_workspace(const vcsr_embed_grad_args& a);
+// How its tokens are sorted (0: in each wave, 1: by ranks, 2: by digits), the digits and
+// their bits, the keys of a tile, and the sorted tokens of a chunk.
+struct EmbedGradPlan {
+    int32_t sort, digits, bits, tile, chunk;
+};
+EmbedGradPlan embed_grad_plan(const vcsr_embed_grad_args& a);
 
 // -------------------------------------------------------------- colsum.hip
 // out[c] = sum over p < P of part[p * ld + c] for c < C, in a fixed order.

@@ -891,6 +891,14 @@ int vcsr_test_gated_grad_plan(const vcsr_gated_grad_args* args, int64_t* out) {
         std::copy(v, v + 5, out);
     });
 }
+// {sort, digits, bits, tile, chunk}
+int vcsr_test_embed_grad_plan(const vcsr_embed_grad_args* args, int64_t* out) {
+    return guarded([&] {
+        const vcsr::EmbedGradPlan p = vcsr::embed_grad_plan(checked_sizes(args));
+        const int64_t v[5] = {p.sort, p.digits, p.bits, p.tile, p.chunk};
+        std::copy(v, v + 5, out);
+    });
+}
 // {together, dw's tile and splits, dx's}
 int vcsr_test_linear_grad_plan(const vcsr_linear_grad_args* args, int64_t* out) {
     return guarded([&] {

@@ -783,6 +783,13 @@ hipError_t launch_embed(const vcsr_embed_args& a, hipStream_t st) {
                                 : launch_forward<fp8, bf16>(a, st);
 }
 
+EmbedGradPlan embed_grad_plan(const vcsr_embed_grad_args& a) {
+    if (a.M <= 0) return EmbedGradPlan{};
+    const Shape s = shape_of(a);
+    return EmbedGradPlan{a.M <= 64 ? 0 : a.M <= kMostRanked ? 1 : 2, s.passes, s.bits, s.tile,
+                         s.runs.E};
+}
+
 size_t embed_grad_workspace(const vcsr_embed_grad_args& a) {
     return a.M > 0 ? shape_of(a).bytes() : 0;
 }
