@@ -404,6 +404,10 @@ typedef struct {
 int vcsr_rmsnorm_grad_workspace(const vcsr_rmsnorm_grad_args* args, size_t* bytes);
 int vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args* args, void* stream, float* ms);
 
+/* Of the embedding, layer norm, the gated projection and their gradients below an output
+ * or the workspace that is the buffer of an input or of another output is VCSR_EINVAL,
+ * but for those that a comment allows. */
+
 /* t = x + residual;  y = (t - mean(t)) / sqrt(mean((t - mean(t))^2) + eps) * weight +
  * bias, row by row, in FP32; the variance is that of the centred values.  y of
  * VCSR_FP8 as vcsr_rmsnorm has it.  A row with a NaN or an infinity gives NaN for all of
@@ -424,7 +428,7 @@ typedef struct {
     void* y;             int64_t ldy;   /* may be x or residual itself, if of
                                            one type                          */
     float* y_scale;      /* M, for VCSR_FP8 (NULL otherwise)                 */
-    float* mean;         /* NULL, or M: mean(t); another vector than rstd    */
+    float* mean;         /* NULL, or M: mean(t)                              */
     float* rstd;         /* NULL, or M: 1 / sqrt(variance + eps)             */
 } vcsr_layernorm_args;
 int vcsr_layernorm(const vcsr_layernorm_args* args, void* stream, float* ms);
@@ -465,7 +469,7 @@ typedef struct {
     const void* table;   int64_t ldt;
     const float* table_scale; /* V, for VCSR_FP8 (NULL otherwise)            */
     const int32_t* ids;  /* M                                                */
-    void* y;             int64_t ldy;   /* another matrix than the table     */
+    void* y;             int64_t ldy;
 } vcsr_embed_args;
 int vcsr_embed(const vcsr_embed_args* args, void* stream, float* ms);
 
@@ -482,7 +486,7 @@ typedef struct {
     float scale;
     const void* dy;      int64_t lddy;
     const int32_t* ids;  /* M                                                */
-    void* dtable;        int64_t lddt;  /* V x C, another matrix than dy     */
+    void* dtable;        int64_t lddt;  /* V x C                             */
     void* workspace;     size_t workspace_bytes;
 } vcsr_embed_grad_args;
 /* As vcsr_rmsnorm_grad_workspace. */
@@ -544,8 +548,7 @@ int vcsr_linear_grad(const vcsr_linear_grad_args* args, void* stream, float* ms)
 /* A gated projection: z_gate = x Wg^T + gate_bias, z_up = x Wu^T + up_bias,
  * y = act(z_gate) * z_up, in one pass over x (the first half of a gated feed-forward
  * block; vcsr_linear is the second).  Types, scales and sums as vcsr_linear has them; y
- * is formed from the unrounded z.  The outputs are other matrices than x and the
- * weights, and than each other. */
+ * is formed from the unrounded z. */
 typedef struct {
     int64_t M;           /* rows of x and y; 0 is no work                    */
     int32_t N, K;        /* outputs and inputs of a row, >= 1; N <= 2^29     */
@@ -573,8 +576,8 @@ int vcsr_gated(const vcsr_gated_args* args, void* stream, float* ms);
  * act'(z_gate), dz_up = dy * act(z_gate), dx = dz_gate Wg + dz_up Wu, dw_gate =
  * dz_gate^T x, dw_up = dz_up^T x, each bias' the sum over rows of its dz.  For VCSR_BF16
  * operands both dz are rounded to bf16 before the products, as vcsr_linear_grad has it.
- * dx and the dw are other matrices than those their products read (the weights for dx,
- * x for the dw, and each other's operands where both are asked for). */
+ * dx and the dw may lie over dy and both z, and over the operand that no product asked
+ * for reads (x for dx alone, the weights for the dw alone). */
 typedef struct {
     int64_t M;
     int32_t N, K;

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <memory>
 #include <string>
 #include <vector>
@@ -61,6 +62,16 @@ void check_workspace(const void* p, size_t have, size_t want) {
     need((uintptr_t)p % 16 == 0, "workspace: not 16-byte aligned");
 }
 
+// Outputs lie over none of what else a call reads or writes (`others`), nor over each other.
+using Buffers = std::initializer_list<const void*>;
+void check_apart(Buffers outputs, Buffers others, const char* what) {
+    for (const void* const* o = outputs.begin(); o != outputs.end(); ++o) {
+        if (!*o) continue;
+        for (const void* const* p = o + 1; p != outputs.end(); ++p) need(*o != *p, what);
+        for (const void* p : others) need(*o != p, what);
+    }
+}
+
 // What the two norms check alike.
 template <class Args>
 void check_norm(Args& a) {
@@ -98,8 +109,12 @@ vcsr_layernorm_args checked(const vcsr_layernorm_args* args) {
     check_norm(a);
     check_vector(a.bias, "bias: alignment", true);
     check_vector(a.mean, "mean: alignment", true);
-    need(!a.mean || (a.mean != a.rstd && a.mean != a.y_scale),
-         "mean: another vector than rstd and y_scale");
+    if (a.M > 0) {
+        check_apart({a.mean, a.rstd, a.y_scale},
+                    {a.x, a.residual, a.sum, a.y, a.weight, a.bias},
+                    "mean, rstd, y_scale: other buffers than each other, the matrices and vectors");
+        check_apart({a.sum, a.y}, {a.weight, a.bias}, "sum, y: other buffers than weight and bias");
+    }
     return a;
 }
 
@@ -141,7 +156,14 @@ vcsr_layernorm_grad_args checked(const vcsr_layernorm_grad_args* args) {
     check_vector(a.mean, "mean: pointer or alignment", a.M == 0);
     check_vector(a.dbias, "dbias: alignment", true);
     need(!a.dbias || a.dbias != a.dweight, "dbias: another vector than dweight");
-    check_workspace(a.workspace, a.workspace_bytes, vcsr::layernorm_grad_workspace(a));
+    const size_t want = vcsr::layernorm_grad_workspace(a);
+    check_workspace(a.workspace, a.workspace_bytes, want);
+    if (a.M > 0) {
+        check_apart({a.dx}, {a.weight, a.mean, a.rstd}, "dx: another buffer than weight, mean and rstd");
+        check_apart({a.dweight, a.dbias, want ? a.workspace : nullptr},
+                    {a.dy, a.s, a.weight, a.mean, a.rstd, a.dsum, a.dx},
+                    "dweight, dbias, workspace: other buffers than each other and all others");
+    }
     return a;
 }
 
@@ -167,7 +189,9 @@ vcsr_embed_args checked(const vcsr_embed_args* args) {
     need((a.table_scale != nullptr) == (a.table_type == VCSR_FP8) || a.M == 0,
          "table_scale: given for VCSR_FP8 and only then");
     check_vector(a.table_scale, "table_scale: alignment", true);
-    need(a.y != a.table || a.M == 0, "y: another matrix than the table");
+    if (a.M > 0)
+        check_apart({a.y}, {a.table, a.table_scale, a.ids},
+                    "y: another buffer than the table, its scales and ids");
     return a;
 }
 vcsr_embed_grad_args checked_sizes(const vcsr_embed_grad_args* args) {
@@ -185,8 +209,11 @@ vcsr_embed_grad_args checked(const vcsr_embed_grad_args* args) {
     check_vector(a.ids, "ids: pointer or alignment", a.M == 0);
     check_matrix(a.dtable, a.lddt, a.C, a.table_type, "dtable: pointer, alignment or stride", false,
                  a.V);
-    need(a.dtable != a.dy || a.M == 0, "dtable: another matrix than dy");
-    check_workspace(a.workspace, a.workspace_bytes, vcsr::embed_grad_workspace(a));
+    const size_t want = vcsr::embed_grad_workspace(a);
+    check_workspace(a.workspace, a.workspace_bytes, want);
+    if (a.M > 0)
+        check_apart({a.dtable, want ? a.workspace : nullptr}, {a.dy, a.ids},
+                    "dtable, workspace: other buffers than each other, dy and ids");
     return a;
 }
 
@@ -323,11 +350,13 @@ vcsr_gated_args checked(const vcsr_gated_args* args) {
     check_matrix(a.y, a.ldy, a.N, a.y_type, "y: pointer, alignment or stride", false, a.M);
     need(!a.z_gate || (a.z_gate != a.z_up && a.z_gate != a.y && a.z_up != a.y),
          "y, z_gate, z_up: three matrices");
+    const size_t want = vcsr::gated_workspace(gemm_of(a));
+    check_workspace(a.workspace, a.workspace_bytes, want);
     if (a.M > 0)
-        for (const void* out : {(const void*)a.y, (const void*)a.z_gate, (const void*)a.z_up})
-            need(!out || (out != a.x && out != a.w_gate && out != a.w_up),
-                 "y, z_gate, z_up: other matrices than x, w_gate and w_up");
-    check_workspace(a.workspace, a.workspace_bytes, vcsr::gated_workspace(gemm_of(a)));
+        check_apart({a.y, a.z_gate, a.z_up, want ? a.workspace : nullptr},
+                    {a.x, a.w_gate, a.w_up, a.x_scale, a.gate_scale, a.up_scale, a.gate_bias,
+                     a.up_bias},
+                    "y, z_gate, z_up, workspace: other buffers than each other and all inputs");
     return a;
 }
 
@@ -560,6 +589,19 @@ GatedGrad checked(const vcsr_gated_grad_args* args) {
                  "dw_gate, dw_up: over a weight, which dx's product reads");
         }
     check_workspace(a.workspace, a.workspace_bytes, w.bytes());
+    if (a.M > 0) {
+        // dx and the dw may lie over dy and both z, which are read before.
+        check_apart({a.dgate_bias, a.dup_bias},
+                    {a.dy, a.z_gate, a.z_up, a.dx, a.dw_gate, a.dw_up, a.dw_gate ? a.x : nullptr,
+                     a.dx ? a.w_gate : nullptr, a.dx ? a.w_up : nullptr},
+                    "dgate_bias, dup_bias: other buffers than all others");
+        if (w.bytes())
+            check_apart({a.workspace},
+                        {a.dy, a.z_gate, a.z_up, a.dx, a.dw_gate, a.dw_up, a.dgate_bias, a.dup_bias,
+                         a.dw_gate ? a.x : nullptr, a.dx ? a.w_gate : nullptr,
+                         a.dx ? a.w_up : nullptr},
+                        "workspace: another buffer than all others");
+    }
     return w;
 }
 
