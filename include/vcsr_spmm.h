@@ -412,7 +412,9 @@ int vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args* args, void* stream, float* m
  * bias, row by row, in FP32; the variance is that of the centred values.  y of
  * VCSR_FP8 as vcsr_rmsnorm has it.  A row with a NaN or an infinity gives NaN for all of
  * y, and no other row does.  The row's sums are FP32's too: where that of t passes
- * 3.4e38 y is NaN, where that of the squares does rstd is zero and y the bias. */
+ * 3.4e38 y is NaN, where that of the squares does rstd is zero and y the bias.  Squares
+ * under 1e-38 (deviations under 1e-19) lose bits and in the end are zero: with eps = 0
+ * such a row, as one whose values are all the same, gives infinities or NaN. */
 typedef struct {
     int64_t M;           /* rows; 0 is no work                               */
     int32_t C;           /* columns, >= 1                                    */

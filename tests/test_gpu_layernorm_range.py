@@ -48,3 +48,35 @@ def test_layernorm_grad_of_constant_rows_far_from_zero(gpu, kinds, C):
     close(dweight.numpy(st), (dy * h).sum(0), (M + 8) * EPS * (np.abs(dy) * ah).sum(0) + 1e-30,
           f"dweight {kinds} {C}")
     close(dbias.numpy(st), dy.sum(0), (M + 4) * EPS * np.abs(dy).sum(0) + 1e-30, f"dbias {kinds} {C}")
+
+
+@pytest.mark.parametrize("yk", ["f32", "bf16", "fp8"])
+@pytest.mark.parametrize("C", [2, 64, 100, 700, 9001])
+def test_layernorm_of_squares_below_fp32(gpu, C, yk):
+    """Deviations of 2^-80, whose squares are zero in FP32: beside eps they count for nothing,
+    without it rstd is infinite and y infinite or NaN, in that row alone."""
+    vs, st, rng = gpu, gpu.Stream(), np.random.default_rng(C)
+    x = values(rng, (3, C), "f32")
+    x[1] = 2.0 ** -80 * np.where(np.arange(C) % 2, 1, -1)
+    b = (0.3 * rng.standard_normal(C)).astype(np.float32)
+    for eps in (1e-5, 1e-12, 0.0):
+        Y, rstd = Mat(vs, st, None, yk, shape=(3, C)), vector(vs, st, np.zeros(3))
+        scale = vector(vs, st, np.zeros(3)) if yk == "fp8" else None
+        print(f"layernorm tiny {yk} C={C} eps={eps}", flush=True)
+        vs.run_layernorm_gpu(Mat(vs, st, x, "f32").view, vector(vs, st, np.ones(C)), Y.view,
+                             bias=vector(vs, st, b), rstd=rstd, y_scale=scale, eps=eps, stream=st)
+        st.sync()
+        y, r = Y.values(), rstd.numpy(st)
+        if yk == "fp8":
+            with np.errstate(invalid="ignore"):
+                y = y * scale.numpy(st).astype(np.float64)[:, None]
+        assert np.isfinite(y[[0, 2]]).all() and np.isfinite(r[[0, 2]]).all()
+        if eps:
+            # (t - mean) * rstd is at most 2^-80 * 1e6, less than any bias' rounding.
+            want = b.astype(np.float64)
+            tol = 2 * EPS * np.abs(want) + 2.0 ** -59 + rounding(want, "f32" if yk == "fp8" else yk)
+            if yk == "fp8":  # codes of b / scale, the scale from the largest
+                tol += np.maximum(2.0 ** -4 * np.abs(want), 2.0 ** -10 * np.abs(want).max() / 448)
+            close(y[1], want, tol * 1.01, f"{yk} {C} {eps}")
+        else:
+            assert np.isinf(r[1]) and not np.isfinite(y[1]).any()
