@@ -639,7 +639,9 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(vcsr_embed_grad_args a, 
 }
 
 // The partial rows of the long run that begins in chunk blockIdx.x, 256 columns a
-// block: each wave adds every fourth one, then LDS adds the waves, in order.
+// block: each wave adds every fourth one, then LDS adds the waves, in order.  A run of very
+// many tokens is a chain of loads in a few blocks: 65536 tokens of 512 bf16, all of one id, 98
+// us (63 with ids as text has them), 2^20 of 128 608 (180).
 template <class X>
 __global__ __launch_bounds__(256) void embed_join_kernel(vcsr_embed_grad_args a, Runs r) {
     __shared__ float lds[4][64][5];

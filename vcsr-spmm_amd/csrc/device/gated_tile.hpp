@@ -9,12 +9,17 @@
 // dwu = dzu^T x two halves of one launch.
 //
 // What bounds them, for rows x inputs x outputs: few rows the weights' read (1 x 4096 x
-// 8192 bf16 25.3 us, 5.3 TB/s), large bf16 ones the chip's power (8192 x 4096 x 8192 867 to
-// 930 us, 1.18 to 1.27 PFLOP/s, the matrix units busy 57% at 2.0 GHz), e4m3 ones
-// widening (5001 x 4096 x 4096 236 to 251 us, 1.34 to 1.42 PFLOP/s, 4096 rows of it in tiles
-// of 256 and the rest in 128).  Gradients of 8192 x 2048 x 4096 bf16: the products 500 us,
-// 1.1 PFLOP/s, busy 46% at 2.2 GHz (transposing reads; keys without LDS conflicts change
-// nothing); of 30011 x 130 x 257 FP32 the products 117 us, busy 57%.
+// 8192 bf16 25.3 us, 5.3 TB/s; FP32 53.6, 5.0 TB/s; e4m3 16.5, 4.1 TB/s), large FP32 ones
+// the matrix units (4096^3 1981 us, 139 TFLOP/s), large bf16 ones the chip's power (8192 x
+// 4096 x 8192 867 to 930 us, 1.18 to 1.27 PFLOP/s, the matrix units busy 57% at 2.0 GHz),
+// e4m3 ones widening (5001 x 4096 x 4096 236 to 251 us, 1.34 to 1.42 PFLOP/s, 4096 rows of it
+// in tiles of 256 and the rest in 128).  Gradients of 8192 x 2048 x 4096 bf16: the products some 500
+// us of a pass' 558 (520 to 527 by themselves under a profiler), 1.1 PFLOP/s, busy 46% at 2.2
+// GHz (transposing reads; keys without LDS conflicts change nothing); of 30011 x 130 x 257
+// FP32 some 112 of 153 (128 under a profiler), busy 57%.  Farthest off are gradients with a
+// narrow side, which write and read both dz for few products: 12102 x 66 x 3628 FP32 539 us,
+// 7416 x 64 x 7913 bf16 222 to 239, where the bytes and products that cannot be done without
+// are 150 and 68.
 #pragma once
 
 #include "linear_tile.hpp"
@@ -133,7 +138,9 @@ hipError_t launch_gated_rows(const GatedGemm& g, hipStream_t st) {
     const unsigned blocks = (unsigned)(((int64_t)g.J / 2 + 7) / 8);
     const int64_t lines = (g.R * (int64_t)sizeof(T) + 127) / 128;
     // Two blocks of four lines a unit rather than one of eight: 1 x 4096 x 8192 bf16 25.3
-    // us (5.3 TB/s) against 30.7, 1 x 4096 x 1024 7.4 against 7.1.
+    // us (5.3 TB/s) against 30.7, FP32 53.6 and 62.9, 1 x 8192 x 8192 e4m3 24.5 and 29.2
+    // (two sets of weights in turn, which the last cache helps); with fewer outputs (1 x 4096
+    // x 1024) bf16 7.4 against 7.1, FP32 14.5 and 13.8.
     if (lines <= 16)
         gated_rows_kernel<T, O, 2><<<blocks, 512, 0, st>>>(g);
     else

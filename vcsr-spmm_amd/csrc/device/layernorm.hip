@@ -10,7 +10,8 @@
 // registers, then over the blocks (colsum.hip), in a fixed order.
 // Memory bounds both: 62451 x 128 FP32 28 us (4.6 TB/s), 32768 x 4096 bf16 188 us, to
 // e4m3 187; the gradient of 16384 x 2050 bf16 68 us (4.0 TB/s; 62 and, for the sums over
-// the blocks, 6), of 32768 x 4096 209 us (5.1 TB/s), of 62451 x 128 FP32 30.  A single
+// the blocks, 6), of 32768 x 4096 208 us (5.2 TB/s), of 62451 x 128 FP32 27 to 30; of few
+// long rows (822 x 4154 FP32) 21 to 22 us, 7 of them for both sums.  A single
 // row of 4096 bf16 to e4m3 is a kernel of 4.2 us: two trips to memory and three sums.
 #include "dense.hpp"
 #include "norm_rows.hpp"
@@ -296,8 +297,8 @@ __global__ __launch_bounds__(WPR > 1 ? 64 * WPR : 256) void layernorm_grad_kerne
 #pragma unroll
         for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
     const float inv_c = 1.f / (float)a.C;
-    // The next row's loads are under way while a row is worked on (16384 x 2050 bf16 71 us,
-    // 77 without, both with 9 for the sums over the blocks), unless registers are short.
+    // The next row's loads are under way while a row is worked on (16384 x 2050 bf16 67.5 us,
+    // 70.3 without; 822 x 4154 FP32 21.1 and 22.6), unless registers are short.
     constexpr bool AHEAD = NV < 4;
     RawRow<X, NV, V> rs, ro;
     RawRow<D, NV, V> rd;

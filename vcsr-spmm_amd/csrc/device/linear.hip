@@ -19,7 +19,10 @@ constexpr int64_t kCus = tile::kCus;
 //
 // The times are of operands by rows.  Gradients, whose operands lie by columns, are
 // estimated with the same ones, which is too little for them (8192 x 2048 x 4096 bf16: dx
-// 103 us by the table, 124 to 131 measured; dw in 128 tiles 121, 158 to 178).
+// 103 us by the table, 124 to 131 measured; dw in 128 tiles 121, 158 to 178).  So are gated
+// projections, whose tile of 64 has other waves and another loader: of 9 to 512 rows the
+// choice is up to a quarter slower than the best (359 x 4360 x 2078 bf16 42.9 us in tiles of
+// 64, 33.8 in tiles of 128 and four parts).
 struct TileCost {
     int tile, stages, room;
     float step[5], rest[5];
