@@ -1,5 +1,5 @@
-"""The layer norm's gradient where a factor of a row leaves FP32's range, on the GPU: what
-lies behind a row's end must not reach its sums."""
+"""Layer norm and its gradient where a factor of a row leaves FP32's range, on the GPU: what
+lies behind a row's end must not reach its sums, nor a row another one."""
 from __future__ import annotations
 
 import numpy as np
